@@ -29,7 +29,9 @@
 extern "C" {
 #endif
 
-#define SIGATTN_ABI_VERSION 2
+#define SIGATTN_ABI_VERSION 3
+/* A problem with abi_version 2 is taken too: it ends before kv_heads. */
+#define SIGATTN_ABI_VERSION_MIN 2
 
 /* Element type of Q, K, V, dO and of every output. */
 enum sigattn_dtype {
@@ -47,12 +49,14 @@ enum sigattn_status {
   SIGATTN_ERR_SHAPE = -4,         /* negative size, or B*H / T too large */
   SIGATTN_ERR_STRIDE = -5,        /* negative stride */
   SIGATTN_ERR_DENSE_LENGTHS = -6, /* dense call (no seq_lens) with Tq != Tk */
-  SIGATTN_ERR_ABI_VERSION = -7,   /* problem.abi_version != SIGATTN_ABI_VERSION */
+  SIGATTN_ERR_ABI_VERSION = -7,   /* problem.abi_version is none the library takes */
   SIGATTN_ERR_LAUNCH = -8,        /* hipGetLastError() reported a failure */
   SIGATTN_ERR_LAYOUT = -9,        /* seq_lens and cu_seqlens both set for one axis */
   SIGATTN_ERR_WORKSPACE = -10,    /* workspace too small for the call, or misaligned */
-  SIGATTN_ERR_SCRATCH = -11       /* sigattn_fwd_noalloc: scratch need above
+  SIGATTN_ERR_SCRATCH = -11,      /* sigattn_fwd_noalloc: scratch need above
                                      SIGATTN_NOALLOC_SCRATCH_BYTES */
+  SIGATTN_ERR_KV_HEADS = -12      /* kv_heads does not divide H, or is set to
+                                     another number in a layout that is not packed */
 };
 
 /*
@@ -62,7 +66,7 @@ enum sigattn_status {
  * every kernel: sigmoid_triton_dense.py:505-506).
  */
 typedef struct sigattn_problem {
-  int32_t abi_version;    /* must be SIGATTN_ABI_VERSION */
+  int32_t abi_version;    /* SIGATTN_ABI_VERSION (or 2, without kv_heads) */
   int32_t dtype;          /* enum sigattn_dtype */
   int64_t B, Tq, Tk, H, D;
   int64_t q_stride_b, q_stride_t, q_stride_h;
@@ -91,6 +95,14 @@ typedef struct sigattn_problem {
   const int32_t *cu_seqlens_q; /* [B+1] int32 or NULL */
   const int32_t *cu_seqlens_k; /* [B+1] int32 or NULL */
   int64_t rows_q, rows_k;      /* packed row counts (used with cu_seqlens_*) */
+  /*
+   * Grouped heads (ABI version 3; no counterpart in the reference, whose
+   * heads all have keys and values of their own): K, V, dK and dV have
+   * kv_heads heads, H a multiple of it, and query head h reads K / V head
+   * h / (H / kv_heads); dK and dV of a head are the sums over its query heads.
+   * 0 means H.  Fewer than H need both axes packed.
+   */
+  int64_t kv_heads;
 } sigattn_problem;
 
 /* ABI version compiled into the library. */

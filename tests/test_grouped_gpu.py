@@ -1,0 +1,260 @@
+"""Grouped heads in packed sequences (sigmoid_attention_varlen with fewer
+key/value heads than query heads) against the formulas in 64 bits."""
+
+import os
+
+import pytest
+import torch
+
+import triton_sigmoid as ts
+from reference64 import assert_within, packed
+from triton_sigmoid import _capi
+
+pytestmark = pytest.mark.gpu
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def offsets(lens, first=0):
+    at = [first]
+    for n in lens:
+        at.append(at[-1] + n)
+    return at
+
+
+def make(rows_q, rows_k, H, Hkv, D, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(rows, heads):
+        return torch.randn(rows, heads, D, generator=g).to(dtype).cuda()
+
+    return normal(rows_q, H), normal(rows_k, Hkv), normal(rows_k, Hkv), normal(rows_q, H)
+
+
+def run(q, k, v, do, cu_q, cu_k, **kw):
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    cq, ck = (torch.tensor(c, dtype=torch.int32, device="cuda") for c in (cu_q, cu_k))
+    o = ts.sigmoid_attention_varlen(q, k, v, cq, ck, **kw)
+    return dict(zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, (q, k, v), do))))
+
+
+def check(q, k, v, do, cu_q, cu_k, causal, mod=None, **kw):
+    got = run(q, k, v, do, cu_q, cu_k, is_causal=causal, score_mod=mod, **kw)
+    want = packed(q, k, v, do, cu_q, cu_k, causal, mod)
+    for x in got:
+        assert_within(got[x], want[x], x)
+    return got
+
+
+LENS = {
+    "one": [1],
+    "short": [1, 0, 31, 32, 33],
+    "odd": [63, 200, 0, 129, 1, 64],
+    "block": [128, 256],
+    "long": [515, 1, 1030],
+}
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("heads", [(4, 2), (6, 2), (8, 1), (7, 7)], ids=lambda h: f"{h[0]}x{h[1]}")
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("lens", ["one", "short", "odd", "long"])
+def test_against_64_bits(lens, dtype, D, heads, causal):
+    n = LENS[lens]
+    if lens == "long" and (D in (16, 32) or heads == (7, 7)):
+        n = [515]
+    cu = offsets(n)
+    q, k, v, do = make(cu[-1], cu[-1], *heads, D, DT[dtype])
+    check(q, k, v, do, cu, cu, causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_score_mod_and_other_key_lengths(dtype, D):
+    """Queries and keys of different lengths, a sequence without keys, a term
+    per key with -inf (a masked key) in it."""
+    nq, nk = [40, 3, 0, 130], [77, 0, 5, 300]
+    cq, ck = offsets(nq), offsets(nk)
+    q, k, v, do = make(cq[-1], ck[-1], 6, 3, D, DT[dtype], 1)
+    mod = torch.randn(ck[-1], generator=torch.Generator().manual_seed(2)).cuda()
+    mod[5], mod[-1] = -torch.inf, -torch.inf
+    for causal in (False, True):
+        check(q, k, v, do, cq, ck, causal, mod)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_outside_every_sequence_are_zero(D):
+    cu = offsets([70, 0, 33], first=5)
+    q, k, v, do = make(cu[-1] + 9, cu[-1] + 9, 4, 2, D, torch.bfloat16, 3)
+    got = check(q, k, v, do, cu, cu, True)
+    for x in got.values():
+        assert not x[:5].any() and not x[cu[-1]:].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_sequences_than_the_ordered_batches(dtype):
+    n = [(7 * i) % 41 for i in range(90)]
+    cu = offsets(n)
+    q, k, v, do = make(cu[-1], cu[-1], 8, 2, 64, DT[dtype], 4)
+    check(q, k, v, do, cu, cu, True)
+    q, k, v, do = make(cu[-1], cu[-1], 4, 1, 128, DT[dtype], 5)
+    check(q, k, v, do, cu, cu, True)
+
+
+@pytest.mark.parametrize("D", [32, 128])
+def test_rows_off_16_bytes(D):
+    """Tensors that start off a 16-byte boundary take the portable kernels."""
+    cu = offsets([33, 0, 70])
+    q, k, v, do = make(cu[-1], cu[-1], 6, 2, D, torch.float16, 6)
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+
+    check(off(q), off(k), off(v), off(do), cu, cu, True)
+
+
+def test_strided_inputs():
+    cu = offsets([50, 90])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, 64, torch.bfloat16, 7)
+    wide = torch.cat([q, k, v], dim=1)  # a fused projection's output
+    got = run(wide[:, :4], wide[:, 4:6], wide[:, 6:], do, cu, cu, is_causal=True)
+    same = run(q, k, v, do, cu, cu, is_causal=True)
+    for x in got:
+        assert torch.equal(got[x], same[x])
+
+
+@pytest.mark.parametrize("binding", ["node", "python"])
+@pytest.mark.parametrize("mb", ["0", "1", "2048"])
+def test_backward_workspace_limits(monkeypatch, mb, binding):
+    """The two-pass backward in whole groups of heads, and without a workspace."""
+    monkeypatch.setenv("SIGATTN_BWD_WORKSPACE_MB", mb)
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    cu = offsets([300, 700])
+    q, k, v, do = make(cu[-1], cu[-1], 6, 2, 128, torch.bfloat16, 8)
+    check(q, k, v, do, cu, cu, True)
+
+
+def test_workspace_of_one_head_runs_without_it():
+    """A dS workspace below one group of heads: the library recomputes."""
+    cu = offsets([256, 256])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, 128, torch.bfloat16, 9)
+    cut = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    scale = torch.tensor(128 ** -0.5, device="cuda")
+    bias = -torch.log(torch.full((2,), 256.0, device="cuda"))
+    pr = _capi._problem(q, k, v, bias, None, scale, None, None, True, packed=(cut, cut, 256, 256))
+    lib = _capi.load_library()
+    import ctypes
+    full = lib.sigattn_bwd_workspace_bytes(ctypes.byref(pr))
+    want = packed(q, k, v, do, cu, cu, True)
+    stream = torch.cuda.current_stream().cuda_stream
+    for share in (4, 3, 2, 1):  # of four heads: one, one, one group, two groups
+        n = full // share
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+        g = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+        rc = lib.sigattn_bwd_ws(ctypes.byref(pr), do.data_ptr(), *(t.data_ptr() for t in g), ws.data_ptr(), n, stream)
+        assert rc == 0
+        for x, t in zip(("dq", "dk", "dv"), g):
+            assert_within(t, want[x], f"{x}, workspace of {n}")
+
+
+def test_equals_repeated_heads():
+    """The same as each query head with a copy of its key/value head: O and dQ
+    bit for bit, dK and dV within the bounds of the sum."""
+    cu = offsets([100, 400])
+    q, k, v, do = make(cu[-1], cu[-1], 8, 2, 128, torch.bfloat16, 10)
+    got = run(q, k, v, do, cu, cu, is_causal=True)
+    rep = run(q, k.repeat_interleave(4, 1), v.repeat_interleave(4, 1), do, cu, cu, is_causal=True)
+    assert torch.equal(got["o"], rep["o"]) and torch.equal(got["dq"], rep["dq"])
+
+
+def test_deterministic_and_on_another_stream():
+    cu = offsets([333, 5, 600])
+    q, k, v, do = make(cu[-1], cu[-1], 8, 2, 64, torch.float16, 11)
+    one = run(q, k, v, do, cu, cu, is_causal=True)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        two = run(q, k, v, do, cu, cu, is_causal=True)
+    side.synchronize()
+    for x in one:
+        assert torch.equal(one[x], two[x])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_captured_forward_and_backward(D):
+    cu = offsets([130, 77])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, D, torch.bfloat16, 12)
+    cut = torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+    def step():
+        a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+        o = ts.sigmoid_attention_varlen(a, b, c, cut, cut, 130, 130, is_causal=True)
+        return (o.detach(), *torch.autograd.grad(o, (a, b, c), do))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        for t, new in zip((q, k, v, do), make(cu[-1], cu[-1], 4, 2, D, torch.bfloat16, 20 + seed)):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+
+
+def test_gradients_against_differences():
+    """fp32 gradients against central differences of the 64-bit forward."""
+    cu = offsets([9, 14])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, 32, torch.float32, 13)
+    got = run(q, k, v, do, cu, cu, is_causal=True)
+    step = 1e-4
+
+    def loss(a, b, c):
+        return (packed_value(a, b, c) * do.double()).sum()
+
+    def packed_value(a, b, c):
+        from reference64 import one_head
+        o = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+        import math
+        for x, y in zip(cu[:-1], cu[1:]):
+            for h in range(4):
+                o[x:y, h] = one_head(a[x:y, h], b[x:y, h // 2], c[x:y, h // 2], None, -math.log(y - x),
+                                     torch.float32, 0)["o"][0]
+        return o
+
+    args = [t.double() for t in (q, k, v)]
+    g = torch.Generator().manual_seed(14)
+    for i, x in enumerate(("dq", "dk", "dv")):
+        d = torch.randn(args[i].shape, generator=g, dtype=torch.float64).cuda()
+        hi, lo = list(args), list(args)
+        hi[i], lo[i] = args[i] + step * d, args[i] - step * d
+        want = (loss(*hi) - loss(*lo)) / (2 * step)
+        have = (got[x].double() * d).sum()
+        # fp32 sums of a few thousand terms of size one; the differences' own
+        # error is step^2 of the third derivative.
+        size = (got[x].double() * d).abs().sum()
+        assert abs(have - want) <= 1e-5 * size + 1e-6
+
+
+def test_compiled_forward_and_backward():
+    cu = offsets([60, 100])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, 64, torch.bfloat16, 15)
+    cut = torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+    def fn(a, b, c):
+        return ts.sigmoid_attention_varlen(a, b, c, cut, cut, 100, 100, is_causal=True)
+
+    want = run(q, k, v, do, cu, cu, is_causal=True)
+    a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+    o = torch.compile(fn, fullgraph=True)(a, b, c)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, (a, b, c), do))))
+    for x in got:
+        assert torch.equal(got[x], want[x])

@@ -281,10 +281,41 @@ __global__ __launch_bounds__(256, 2) void bwd_dq_kernel(const KParams p) {
 // (causal diagonal, seq_lens_q, pipeline fill) are applied to the packed
 // words of the few blocks that need them.
 // ---------------------------------------------------------------------------
+// The queries that a dK/dV item streams, as tiles t and 32-query blocks g
+// counted through: those of one query head, or (GROUPED) of the qgroup heads
+// that share the item's K / V head, one head after another without a break in
+// the pipeline.  dK and dV of a shared head are the sums over its query heads,
+// so they stay in the same accumulators.  Tiles and blocks are visited in
+// order, so their places within a head are counters, not divisions.
+template <bool GROUPED> struct HeadStream {
+  int nb = 0;                                      // blocks of one head
+  int t1 = 0, th = 0;                              // next tile to copy: place in its head, head
+  int g[3] = {0, -1, -2}, h[3] = {0, 0, 0};        // blocks r, r - 1, r - 2: the same
+  __device__ __forceinline__ explicit HeadStream(int blocks) {
+    if constexpr (GROUPED) nb = blocks;
+  }
+  __device__ __forceinline__ int tile(int t) const { return GROUPED ? t1 : t; }
+  __device__ __forceinline__ int64_t head_of_tile(int) const { return GROUPED ? th : 0; }
+  __device__ __forceinline__ void next_tile() {
+    if constexpr (GROUPED) {
+      if (2 * ++t1 == nb) t1 = 0, ++th;
+    }
+  }
+  // Block r - back of region r within its head (negative: pipeline fill).
+  __device__ __forceinline__ int block(int r, int back) const { return GROUPED ? g[back] : r - back; }
+  __device__ __forceinline__ int head(int back) const { return GROUPED ? h[back] : 0; }
+  __device__ __forceinline__ void next_block() {
+    if constexpr (GROUPED) {
+      g[2] = g[1], h[2] = h[1], g[1] = g[0], h[1] = h[0];
+      if (++g[0] == nb) g[0] = 0, ++h[0];
+    }
+  }
+};
+
 template <int D> struct DkdvLds {
   uint16_t q[4][64 * D], o[4][64 * D];
 };
-template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT>
+template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPED>
 __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, DkdvLds<D> &lds) {
   constexpr int BN = 128;                 // keys per workgroup (32 per wave)
   constexpr int BMQ = 64;                 // queries per LDS tile (two 32-query blocks)
@@ -339,7 +370,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   const int l32 = lane & 31, hi = lane >> 5;
   const int k0 = kblk * BN, kw = k0 + w * 32, my_k = kw + l32;
 
-  const int64_t qoff = p.q_base(b, h);
+  const int hq = GROUPED ? p.first_q_head(h) : h;
+  const int64_t qoff = p.q_base(b, hq);
   const int64_t koff = p.k_base(b, h);
   const uint16_t *Qb = (const uint16_t *)p.q + qoff;
   const uint16_t *dOb = (const uint16_t *)p.dout + qoff;
@@ -357,8 +389,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
     mstart = split_tile(rchunk, p.rsplit, ntq) * BMQ;
     mend = min(Lq, split_tile(rchunk + 1, p.rsplit, ntq) * BMQ);
   }
-  const int ntiles = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;
+  const int ntiles1 = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;  // of one query head
+  const int ntiles = GROUPED ? p.qgroup * ntiles1 : ntiles1;
   const int NB = 2 * ntiles;
+  HeadStream<GROUPED> hs(2 * ntiles1);
 
   const float scale = *p.scale;
   const float bias = p.bias[b];
@@ -393,8 +427,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   dma.init(w, lane, half);
   const int q_stride_bytes = (int)(p.sq_t * 2);
   auto issue = [&](int st, int t) SIGATTN_INLINE {
-    dma.issue(sQ[st], Qb + (int64_t)mstart * p.sq_t, q_stride_bytes, t * BMQ, mend - mstart);
-    dma.issue(sO[st], dOb + (int64_t)mstart * p.sq_t, q_stride_bytes, t * BMQ, mend - mstart);
+    const int64_t at = (int64_t)mstart * p.sq_t + hs.head_of_tile(t) * p.sq_h;
+    dma.issue(sQ[st], Qb + at, q_stride_bytes, hs.tile(t) * BMQ, mend - mstart);
+    dma.issue(sO[st], dOb + at, q_stride_bytes, hs.tile(t) * BMQ, mend - mstart);
+    hs.next_tile();
   };
 
   f32x16 sacc[2], pacc[2];       // S and dP accumulators, by block parity
@@ -445,17 +481,19 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   const int kbw = kw / 32;
   uint16_t *ds_bh = nullptr;
   if constexpr (DSOUT)
-    ds_bh = p.ds + ((int64_t)b * p.H + h) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
+    ds_bh = p.ds + ((int64_t)b * p.H * p.q_heads() + hq) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
                        DsLayout::kTileElems;
   // Every region issues exactly two store instructions, so the tile
   // barrier can wait for its copies with a fixed vmcnt while the stores are
   // still in flight: a skipped tile is a store through a buffer resource of
   // zero bytes, which the hardware drops.
-  auto store_ds = [&](int slot, int g) SIGATTN_INLINE {
+  auto store_ds = [&](int slot, int g, int head) SIGATTN_INLINE {
     const int qb = mstart / 32 + g;
     const bool ok = g >= 0 && 32 * qb < Lq && kw < Lk && (!CAUSAL || qb >= kbw);
     // Buffer over this wave's tile (or over nothing).
-    const uint16_t *tp = ds_bh + (ok ? DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
+    const int64_t skip = GROUPED ? head * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) : 0;
+    const uint16_t *tp =
+        ds_bh + (ok ? skip + DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
     const __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc((void *)tp, (short)0, ok ? 2048 : 0, kBufferWord3);
     const int off = 16 * lane;
@@ -502,7 +540,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
       // VALU work), stored where the next vmcnt(0) is furthest away: at the
       // start of even regions, after the tile barrier in odd ones.
       if constexpr (DSOUT) {
-        if (((U % 2) == 0 && win == 0) || ((U % 2) == 1 && win * 4 == BAR)) store_ds(SL, r - 2);
+        if (((U % 2) == 0 && win == 0) || ((U % 2) == 1 && win * 4 == BAR)) store_ds(SL, hs.block(r, 2), hs.head(2));
       }
       // One wait for the window's four operands instead of one per MFMA.
       asm volatile("" ::"v"(opq[(win * 4) % LA]), "v"(opq[(win * 4 + 1) % LA]),
@@ -567,7 +605,9 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (r == 0 || needs_mask(r - 1)) mask_words(1 - SL, r - 1);
+    const int done = hs.block(r, 1);
+    if (r == 0 || needs_mask(done)) mask_words(1 - SL, done);
+    hs.next_block();
   };
 
   // Pipeline fill: blocks -2 and -1 contribute P = dS = 0; their gradient
@@ -634,10 +674,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   }
 }
 
-template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT>
+template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPED>
 __global__ __launch_bounds__(256, (D <= 64 ? 2 : 1)) void bwd_dkdv_kernel(const KParams p) {
   __shared__ __attribute__((aligned(16))) DkdvLds<D> lds;
-  bwd_dkdv_body<T, D, CAUSAL, SCOREMOD, DSOUT>(p, blockIdx.x, lds);
+  bwd_dkdv_body<T, D, CAUSAL, SCOREMOD, DSOUT, GROUPED>(p, blockIdx.x, lds);
 }
 
 // The recompute backward's two kernels in one launch: the first nkv workgroups
@@ -653,7 +693,7 @@ __global__ __launch_bounds__(256, WK) void bwd_fused_kernel(const KParams pq, co
     DqLds<D, SCOREMOD> dq;
     DkdvLds<D> dkdv;
   } lds;
-  if ((int)blockIdx.x < nkv) bwd_dkdv_body<T, D, CAUSAL, SCOREMOD, false>(pk, blockIdx.x, lds.dkdv);
+  if ((int)blockIdx.x < nkv) bwd_dkdv_body<T, D, CAUSAL, SCOREMOD, false, false>(pk, blockIdx.x, lds.dkdv);
   else bwd_dq_body<T, D, WK, CAUSAL, SCOREMOD>(pq, (int)blockIdx.x - nkv, lds.dq);
 }
 
@@ -695,7 +735,7 @@ __global__ __launch_bounds__(256, WK) void bwd_fused_kernel(const KParams pq, co
 #endif
 constexpr bool kDkdvGrouped = SIGATTN_DKDV_GROUPED != 0;
 
-template <typename T, bool CAUSAL, bool SCOREMOD, bool DSOUT>
+template <typename T, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPED>
 __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) {
   constexpr int D = 128;
   constexpr int BN = 128;                 // keys per workgroup (32 per wave pair)
@@ -762,7 +802,8 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
     const int l32 = lane & 31, hi = lane >> 5;
     const int k0 = kblk * BN, kw = k0 + pair * 32, my_k = kw + l32;
 
-    const int64_t qoff = p.q_base(b, h);
+    const int hq = GROUPED ? p.first_q_head(h) : h;
+    const int64_t qoff = p.q_base(b, hq);
     const int64_t koff = p.k_base(b, h);
     const uint16_t *Qb = (const uint16_t *)p.q + qoff;
     const uint16_t *dOb = (const uint16_t *)p.dout + qoff;
@@ -770,8 +811,10 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
     // Causal: queries before the workgroup's first key see none of its keys.
     const int mstart = CAUSAL ? (k0 / BMQ) * BMQ : 0;
     const int mend = (k0 >= Lk) ? mstart : Lq;
-    const int ntiles = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;
+    const int ntiles1 = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;  // of one query head
+    const int ntiles = GROUPED ? p.qgroup * ntiles1 : ntiles1;
     const int NB = 2 * ntiles;
+    HeadStream<GROUPED> hs(2 * ntiles1);
 
     const float scale = *p.scale;
     const bool kok = my_k < Lk;
@@ -782,8 +825,10 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
     dma.init(pair, lane);
     const int q_stride_bytes = (int)(p.sq_t * 2);
     auto issue = [&](int st, int t) SIGATTN_INLINE {
-      dma.issue(sQ[st], Qb + (int64_t)mstart * p.sq_t, q_stride_bytes, t * BMQ, mend - mstart);
-      dma.issue(sO[st], dOb + (int64_t)mstart * p.sq_t, q_stride_bytes, t * BMQ, mend - mstart);
+      const int64_t at = (int64_t)mstart * p.sq_t + hs.head_of_tile(t) * p.sq_h;
+      dma.issue(sQ[st], Qb + at, q_stride_bytes, hs.tile(t) * BMQ, mend - mstart);
+      dma.issue(sO[st], dOb + at, q_stride_bytes, hs.tile(t) * BMQ, mend - mstart);
+      hs.next_tile();
     };
 
     // Zeroes the packed words of block g whose query lies before the block
@@ -925,7 +970,9 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
             }
           }
         }
-        if (r == 0 || needs_mask(r - 1)) mask_words(pw[1 - SL], r - 1);
+        const int done = hs.block(r, 1);
+        if (r == 0 || needs_mask(done)) mask_words(pw[1 - SL], done);
+        hs.next_block();
       };
 
       for (int r0 = 0; r0 < NB + 2; r0 += 8) {
@@ -980,12 +1027,14 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
       const int kbw = kw / 32;
       uint16_t *ds_bh = nullptr;
       if constexpr (DSOUT)
-        ds_bh = p.ds + ((int64_t)b * p.H + h) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
+        ds_bh = p.ds + ((int64_t)b * p.H * p.q_heads() + hq) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
                            DsLayout::kTileElems;
-      auto store_ds = [&](int g) SIGATTN_INLINE {
+      auto store_ds = [&](int g, int head) SIGATTN_INLINE {
         const int qb = mstart / 32 + g;
         const bool ok = g >= 0 && 32 * qb < Lq && kw < Lk && (!CAUSAL || qb >= kbw);
-        const uint16_t *tp = ds_bh + (ok ? DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
+        const int64_t skip = GROUPED ? head * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) : 0;
+        const uint16_t *tp =
+            ds_bh + (ok ? skip + DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc((void *)tp, (short)0, ok ? 2048 : 0, kBufferWord3);
         const int off = 16 * lane;
@@ -1022,8 +1071,10 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
             const float t0 = pr0 * pacc[SL][2 * e], t1 = pr1 * pacc[SL][2 * e + 1];
             dw[e] = Elem<T>::pack(__builtin_fmaf(-pr0, t0, t0), __builtin_fmaf(-pr1, t1, t1));
           }
-          if (r < 2 || needs_mask(r - 2)) mask_words(dw, r - 2);
-          if constexpr (DSOUT) store_ds(r - 2);
+          const int done = hs.block(r, 2);
+          if (r < 2 || needs_mask(done)) mask_words(dw, done);
+          if constexpr (DSOUT) store_ds(done, hs.head(2));
+          hs.next_block();
         }
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
@@ -1346,6 +1397,20 @@ static void bwd_dq_t(const KParams &kp, bool causal, bool sm, hipStream_t st) {
   bwd_dq_w<T, D, 1>(kp, causal, sm, st);
 }
 
+// f(bool constants) of the run-time flags.
+template <class F> static void by_flags(bool a, bool b, bool c, F &&f) {
+  const auto last = [&](auto x, auto y) {
+    if (c) f(x, y, std::true_type{});
+    else f(x, y, std::false_type{});
+  };
+  const auto next = [&](auto x) {
+    if (b) last(x, std::true_type{});
+    else last(x, std::false_type{});
+  };
+  if (a) next(std::true_type{});
+  else next(std::false_type{});
+}
+
 template <typename T, int D, bool DSOUT>
 static void bwd_dkdv_t(const KParams &kp, bool causal, bool sm, hipStream_t st) {
   launch_rows<128>(kp, kp.Tk, [&](const KParams &p, dim3 grid) {
@@ -1357,24 +1422,16 @@ static void bwd_dkdv_t(const KParams &kp, bool causal, bool sm, hipStream_t st) 
         const bool one_block = !causal && paired < device_compute_units();
         grid = dim3((unsigned)(one_block ? (int64_t)p.nblk * p.B * p.H : paired));
       }
-      if (causal) {
-        if (sm) bwd_dkdv_pair_kernel<T, true, true, DSOUT><<<grid, 512, 0, st>>>(p);
-        else bwd_dkdv_pair_kernel<T, true, false, DSOUT><<<grid, 512, 0, st>>>(p);
-      } else {
-        if (sm) bwd_dkdv_pair_kernel<T, false, true, DSOUT><<<grid, 512, 0, st>>>(p);
-        else bwd_dkdv_pair_kernel<T, false, false, DSOUT><<<grid, 512, 0, st>>>(p);
-      }
+      by_flags(causal, sm, p.qgroup > 1, [&](auto c, auto m, auto g) {
+        bwd_dkdv_pair_kernel<T, c.value, m.value, DSOUT, g.value><<<grid, 512, 0, st>>>(p);
+      });
       return;
     }
     // Range split (dense non-causal recompute backward): rsplit workgroups per item.
     if (!causal && !DSOUT && p.rsplit > 1) grid.x *= (unsigned)p.rsplit;
-    if (causal) {
-      if (sm) bwd_dkdv_kernel<T, D, true, true, DSOUT><<<grid, 256, 0, st>>>(p);
-      else bwd_dkdv_kernel<T, D, true, false, DSOUT><<<grid, 256, 0, st>>>(p);
-    } else {
-      if (sm) bwd_dkdv_kernel<T, D, false, true, DSOUT><<<grid, 256, 0, st>>>(p);
-      else bwd_dkdv_kernel<T, D, false, false, DSOUT><<<grid, 256, 0, st>>>(p);
-    }
+    by_flags(causal, sm, p.qgroup > 1, [&](auto c, auto m, auto g) {
+      bwd_dkdv_kernel<T, D, c.value, m.value, DSOUT, g.value><<<grid, 256, 0, st>>>(p);
+    });
   });
 }
 

@@ -27,8 +27,18 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool aligned16(const void *ptr) { return ((uintptr_t)ptr & 15u) == 0; }
 
+// K / V heads (version 2 of the struct ends before the field).
+int64_t kv_heads(const sigattn_problem *p) {
+  return p->abi_version >= 3 && p->kv_heads != 0 ? p->kv_heads : p->H;
+}
+
+// Query heads per K / V head.
+int64_t head_group(const sigattn_problem *p) { return p->H > 0 ? p->H / kv_heads(p) : 1; }
+
 KParams make_params(const sigattn_problem *p) {
   KParams k{};
+  k.hgroup = (int)head_group(p);
+  k.qgroup = 1;
   k.ncu = sigattn::device_compute_units();
   k.q = p->q;
   k.k = p->k;
@@ -413,12 +423,12 @@ int64_t ds_bytes_per_head(const sigattn_problem *p) {
   return p->B * tiles * 2048;
 }
 
-// The sub-problem of heads [h0, h0 + nh): every tensor is [.., H, D] with
-// its own head stride, so the heads are a pointer offset away; bias,
+// The sub-problem of heads [h0, h0 + nh), whole groups: every tensor is
+// [.., H, D] with its own head stride, so the heads are a pointer offset away; bias,
 // score_mod and the sequence lengths are per batch and stay as they are.
 KParams head_slice(const KParams &k, int64_t h0, int64_t nh, int64_t esize) {
   KParams s = k;
-  const int64_t qo = h0 * k.sq_h * esize, ko = h0 * k.sk_h * esize;
+  const int64_t qo = h0 * k.sq_h * esize, ko = h0 / k.hgroup * k.sk_h * esize;
   auto adv = [](const void *ptr, int64_t off) -> const char * {
     return ptr == nullptr ? nullptr : (const char *)ptr + off;
   };
@@ -430,6 +440,14 @@ KParams head_slice(const KParams &k, int64_t h0, int64_t nh, int64_t esize) {
   s.dk = (void *)adv(k.dk, ko);
   s.dv = (void *)adv(k.dv, ko);
   s.H = (int)nh;
+  return s;
+}
+
+// The dK/dV kernels' view of a problem: its items are K / V heads, each of
+// which streams the queries of its group (KParams::qgroup).
+KParams kv_items(const KParams &k) {
+  KParams s = k;
+  if (k.hgroup > 1) s.H = k.H / k.hgroup, s.qgroup = k.hgroup, s.hgroup = 1;
   return s;
 }
 
@@ -452,7 +470,7 @@ void gap_axes(const sigattn_problem *p, void *q_out, void *k_out0, void *k_out1,
   }
   if (p->cu_seqlens_k != nullptr && (k_out0 != nullptr || k_out1 != nullptr) && p->rows_k > 0) {
     b.cu = p->cu_seqlens_k;
-    b.B = (int)p->B, b.T = (int)p->Tk, b.H = (int)p->H, b.D = (int)p->D;
+    b.B = (int)p->B, b.T = (int)p->Tk, b.H = (int)kv_heads(p), b.D = (int)p->D;
     b.rows = p->rows_k, b.st = p->k_stride_t, b.sh = p->k_stride_h;
     b.out[0] = k_out0, b.out[1] = k_out1;
   }
@@ -517,6 +535,7 @@ const char *sigattn_strerror(int status) {
       return "seq_lens and cu_seqlens cannot both be given for the same sequence axis";
     case SIGATTN_ERR_WORKSPACE:
       return "workspace too small for the call or not 16-byte aligned";
+    case SIGATTN_ERR_KV_HEADS: return "kv_heads must divide H, and fewer than H need packed sequences";
     case SIGATTN_ERR_SCRATCH:
       return "problem needs more than the fixed scratch buffer of sigattn_fwd_noalloc";
     default: return "unknown sigattn status";
@@ -525,7 +544,7 @@ const char *sigattn_strerror(int status) {
 
 int sigattn_check(const sigattn_problem *p) {
   if (p == nullptr) return SIGATTN_ERR_NULL_ARG;
-  if (p->abi_version != SIGATTN_ABI_VERSION) return SIGATTN_ERR_ABI_VERSION;
+  if (p->abi_version < SIGATTN_ABI_VERSION_MIN || p->abi_version > SIGATTN_ABI_VERSION) return SIGATTN_ERR_ABI_VERSION;
   if (p->dtype != SIGATTN_F16 && p->dtype != SIGATTN_BF16 && p->dtype != SIGATTN_F32)
     return SIGATTN_ERR_DTYPE;
   if (!is_pow2_head_dim(p->D)) return SIGATTN_ERR_HEAD_DIM;
@@ -536,6 +555,10 @@ int sigattn_check(const sigattn_problem *p) {
     return SIGATTN_ERR_LAYOUT;
   if (p->Tq > (INT_MAX / 2) || p->Tk > (INT_MAX / 2) || p->B > INT_MAX || p->H > INT_MAX)
     return SIGATTN_ERR_SHAPE;
+  if (p->abi_version >= 3 && p->kv_heads != 0 && p->kv_heads != p->H &&
+      (p->kv_heads < 0 || p->kv_heads > p->H || p->H % p->kv_heads != 0 || p->cu_seqlens_q == nullptr ||
+       p->cu_seqlens_k == nullptr))
+    return SIGATTN_ERR_KV_HEADS;
   // Largest grid any kernel launches: ceil(T / 64) row blocks per (b, h).
   const int64_t rows = p->Tq > p->Tk ? p->Tq : p->Tk;
   if (p->B * p->H > 0 && cdiv(rows, 64) > (int64_t)INT_MAX / (p->B * p->H)) return SIGATTN_ERR_SHAPE;
@@ -706,6 +729,7 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   if (workspace != nullptr && mfma && wide_head(p) && p->Tq > 0 && p->Tk > 0) {
     heads_per_pass = (int64_t)workspace_bytes / ds_bytes_per_head(p);
     if (heads_per_pass > p->H) heads_per_pass = p->H;
+    heads_per_pass -= heads_per_pass % head_group(p);  // whole groups: dK / dV are sums over them
   }
   if (parts != kBwdAll && workspace != nullptr) {
     if (!mfma || !wide_head(p)) return SIGATTN_ERR_WORKSPACE;  // no two-pass kernels for this problem
@@ -748,7 +772,7 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
     for (int64_t h0 = 0; h0 < p->H; h0 += heads_per_pass) {
       const int64_t nh = p->H - h0 < heads_per_pass ? p->H - h0 : heads_per_pass;
       KParams s = head_slice(k, h0, nh, 2);
-      if (parts != kBwdDq) sigattn::launch_bwd_dkdv_mfma(s, dt, D, causal, sm, true, st);
+      if (parts != kBwdDq) sigattn::launch_bwd_dkdv_mfma(kv_items(s), dt, D, causal, sm, true, st);
       if (h0 == 0 && dq_gaps) use_gaps(s, gq, gk);  // the first group's dQ launch
       if (parts != kBwdDkdv) sigattn::launch_bwd_dq_ds_mfma(s, dt, D, causal, st);
     }
@@ -768,7 +792,7 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   // side stream, then the dQ kernel on the caller's.
   hipStream_t side = nullptr;
   if (need_dq && need_dkdv && mfma && concurrent_backward(p)) side = t_side.fork(st);
-  if (side != nullptr) sigattn::launch_bwd_dkdv_mfma(k, dt, D, causal, sm, false, side);
+  if (side != nullptr) sigattn::launch_bwd_dkdv_mfma(kv_items(k), dt, D, causal, sm, false, side);
   KParams kq = k;
   if (dq_gaps) use_gaps(kq, gq, gk);
   if (need_dq) {
@@ -777,9 +801,10 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
     else sigattn::launch_bwd_dq_generic(k, dt, D, causal, st);
   }
   if (need_dkdv && side == nullptr) {
-    if (mfma) sigattn::launch_bwd_dkdv_mfma(k, dt, D, causal, sm, false, st);
-    else if (f32mma) sigattn::launch_bwd_dkdv_f32(k, D, causal, sm, st);
-    else sigattn::launch_bwd_dkdv_generic(k, dt, D, causal, st);
+    const KParams kk = kv_items(k);
+    if (mfma) sigattn::launch_bwd_dkdv_mfma(kk, dt, D, causal, sm, false, st);
+    else if (f32mma) sigattn::launch_bwd_dkdv_f32(kk, D, causal, sm, st);
+    else sigattn::launch_bwd_dkdv_generic(kk, dt, D, causal, st);
   }
   if (side != nullptr && !t_side.join(st, side)) return SIGATTN_ERR_LAUNCH;
   return launch_status();

@@ -132,6 +132,13 @@ struct KParams {
   // The D = 32 kernels computing head_dim 16 (see dmem).
   __device__ __forceinline__ bool half_head(int D) const { return D == 32 && dmem == 16; }
 
+  // Grouped heads: hgroup query heads in a row read one K / V head (0 or 1:
+  // each its own).  Kernels whose items are query heads (forward, dQ) take the
+  // K / V head of item head h from hgroup; the dK/dV kernels run with H = the
+  // K / V heads and qgroup = the query heads of each, whose queries an item
+  // streams one head after another (hgroup is then 1).
+  int hgroup, qgroup;
+
   // Valid query / key rows of batch b.
   __device__ __forceinline__ int len_q(int b) const {
     return cu_q != nullptr ? packed_len(cu_q, rows_q, b, Tq) : clamp_len(seq_q, b, Tq);
@@ -146,8 +153,11 @@ struct KParams {
   }
   __device__ __forceinline__ int64_t k_base(int b, int h) const {
     const int64_t r = cu_k != nullptr ? packed_first(cu_k, rows_k, b) * sk_t : (int64_t)b * sk_b;
-    return r + (int64_t)h * sk_h;
+    return r + (int64_t)(hgroup > 1 ? h / hgroup : h) * sk_h;
   }
+  // First query head of the dK/dV item head h, and the query heads it streams.
+  __device__ __forceinline__ int first_q_head(int h) const { return qgroup > 1 ? h * qgroup : h; }
+  __device__ __forceinline__ int q_heads() const { return qgroup > 1 ? qgroup : 1; }
   // score_mod entry of key 0 of batch b.
   __device__ __forceinline__ int64_t mod_base(int b) const {
     return cu_k != nullptr ? packed_first(cu_k, rows_k, b) : (int64_t)b * Tk;

@@ -254,7 +254,7 @@ __device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, floa
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
   const int kw = k0 + 32 * w, myk = kw + l32;
-  const int64_t qoff = p.q_base(b, h), koff = p.k_base(b, h);
+  const int64_t koff = p.k_base(b, h);
 
   // Causal: queries before the workgroup's first key see none of its keys.
   const int mstart = CAUSAL ? min(k0, Lq) : 0;
@@ -277,30 +277,33 @@ __device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, floa
   F32RowReads<D> rr;
   rr.init(l32, hi);
   const int stride_bytes = (int)(p.sq_t * 4);
-  const float *Qm = (const float *)p.q + qoff + (int64_t)mstart * p.sq_t;
-  const float *dOm = (const float *)p.dout + qoff + (int64_t)mstart * p.sq_t;
-  for (int t = 0; t < ntiles; ++t) {
-    float *tQ = lds + (t & 1) * 2 * FB * D, *tO = tQ + FB * D;
-    dma.issue((uint16_t *)tQ, (const uint16_t *)Qm, stride_bytes, t * FB, Lq - mstart);
-    dma.issue((uint16_t *)tO, (const uint16_t *)dOm, stride_bytes, t * FB, Lq - mstart);
-    wait_dma();
-    __syncthreads();
-    const int m0 = mstart + t * FB;
-    if (kw >= rows || (CAUSAL && m0 + FB <= kw)) continue;
-    f32x16 s = zero16(), dp = zero16();
-    float pr[16], ds[16];
-    head_product<D>(s, tQ, kv, l32, hi);
-    head_product<D>(dp, tO, vv, l32, hi);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int q = m0 + 8 * (i / 4) + 4 * hi + i % 4;
-      pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
-      const float u = pr[i] * dp[i];
-      ds[i] = __builtin_fmaf(-pr[i], u, u);
-      if (q >= Lq || (CAUSAL && q < myk)) pr[i] = ds[i] = 0.0f;
+  // u: tiles since the start, over the query heads of this K / V head.
+  for (int g = 0, u = 0; g < p.q_heads(); ++g) {
+    const int64_t qoff = p.q_base(b, p.first_q_head(h) + g) + (int64_t)mstart * p.sq_t;
+    const float *Qm = (const float *)p.q + qoff, *dOm = (const float *)p.dout + qoff;
+    for (int t = 0; t < ntiles; ++t, ++u) {
+      float *tQ = lds + (u & 1) * 2 * FB * D, *tO = tQ + FB * D;
+      dma.issue((uint16_t *)tQ, (const uint16_t *)Qm, stride_bytes, t * FB, Lq - mstart);
+      dma.issue((uint16_t *)tO, (const uint16_t *)dOm, stride_bytes, t * FB, Lq - mstart);
+      wait_dma();
+      __syncthreads();
+      const int m0 = mstart + t * FB;
+      if (kw >= rows || (CAUSAL && m0 + FB <= kw)) continue;
+      f32x16 s = zero16(), dp = zero16();
+      float pr[16], ds[16];
+      head_product<D>(s, tQ, kv, l32, hi);
+      head_product<D>(dp, tO, vv, l32, hi);
+  #pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int q = m0 + 8 * (i / 4) + 4 * hi + i % 4;
+        pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
+        const float u = pr[i] * dp[i];
+        ds[i] = __builtin_fmaf(-pr[i], u, u);
+        if (q >= Lq || (CAUSAL && q < myk)) pr[i] = ds[i] = 0.0f;
+      }
+      row_product<D>(dva, tO, pr, rr);
+      row_product<D>(dka, tQ, ds, rr);
     }
-    row_product<D>(dva, tO, pr, rr);
-    row_product<D>(dka, tQ, ds, rr);
   }
   if (myk < min(w_.row_end, p.k_rows_out(Lk))) {
     store_row<D>((float *)p.dk + koff + (int64_t)myk * p.sk_t, dka, scale, myk < Lk, hi, half);
@@ -768,8 +771,7 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
   const int l32 = lane & 31, hi = lane >> 5;
   const int k0 = it.row0, kw = k0 + 32 * (w / WK), myk = kw + l32, wt = w % WK;
 
-  const int64_t qoff = p.q_base(b, h), koff = p.k_base(b, h);
-  const float *Qb = (const float *)p.q + qoff, *dOb = (const float *)p.dout + qoff;
+  const int64_t koff = p.k_base(b, h);
   // Queries of the workgroup: causal ones before its first key see none of its keys.
   const int mstart = CAUSAL ? min(k0, Lq) : 0;
   const int nsteps = k0 < Lk ? (Lq - mstart + TR - 1) / TR : 0;
@@ -789,39 +791,43 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
   TileOffsets<D> to;
   to.init(lane);
   Tiles st;
-  auto load = [&](int t) SIGATTN_INLINE { st.load(Qb, dOb, p.sq_t, mstart + t * TR, Lq, half); };
-  if (nsteps > 0) load(0);
-  for (int t = 0; t < nsteps; ++t) {
-    __syncthreads();
-    st.store(tiles, rg);
-    if (t + 1 < nsteps) load(t + 1);
-    __syncthreads();
-    const int m0 = mstart + t * TR + FB * wt;
-    // Nothing for keys past Lk, queries past Lq, or (causal) queries that all
-    // precede the wave's first key.
-    if (kw >= Lk || m0 >= Lq || (CAUSAL && m0 + FB <= kw)) continue;
-    const uint16_t *tQ = tiles, *tO = Tiles::part(tiles, 1, 0);
-    const f32x16 s = head3<D, Tiles::PART>(tQ, to, FB * wt, kf);
-    const f32x16 dp = head3<D, Tiles::PART>(tO, to, FB * wt, vf);
-    float pr[16], ds[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
-      const float u = pr[i] * dp[i];
-      ds[i] = __builtin_fmaf(-pr[i], u, u);
-    }
-    // Queries at or past seq_lens_q, or (causal) before the lane's key.
-    if (m0 + FB > Lq || (CAUSAL && m0 < kw + 31)) {
-      const int e_end = Lq - m0 - 4 * hi;               // query m0 + 4hi + e valid iff
-      const int e_lo = CAUSAL ? myk - m0 - 4 * hi : 0;  // e_lo <= e < e_end
-#pragma unroll
+  for (int g = 0; g < p.q_heads(); ++g) {  // the query heads of this K / V head
+    const int64_t qoff = p.q_base(b, p.first_q_head(h) + g);
+    const float *Qb = (const float *)p.q + qoff, *dOb = (const float *)p.dout + qoff;
+    auto load = [&](int t) SIGATTN_INLINE { st.load(Qb, dOb, p.sq_t, mstart + t * TR, Lq, half); };
+    if (nsteps > 0) load(0);
+    for (int t = 0; t < nsteps; ++t) {
+      __syncthreads();
+      st.store(tiles, rg);
+      if (t + 1 < nsteps) load(t + 1);
+      __syncthreads();
+      const int m0 = mstart + t * TR + FB * wt;
+      // Nothing for keys past Lk, queries past Lq, or (causal) queries that all
+      // precede the wave's first key.
+      if (kw >= Lk || m0 >= Lq || (CAUSAL && m0 + FB <= kw)) continue;
+      const uint16_t *tQ = tiles, *tO = Tiles::part(tiles, 1, 0);
+      const f32x16 s = head3<D, Tiles::PART>(tQ, to, FB * wt, kf);
+      const f32x16 dp = head3<D, Tiles::PART>(tO, to, FB * wt, vf);
+      float pr[16], ds[16];
+  #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int e = 8 * (i / 4) + i % 4;
-        if (e >= e_end || e < e_lo) pr[i] = ds[i] = 0.0f;
+        pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
+        const float u = pr[i] * dp[i];
+        ds[i] = __builtin_fmaf(-pr[i], u, u);
       }
+      // Queries at or past seq_lens_q, or (causal) before the lane's key.
+      if (m0 + FB > Lq || (CAUSAL && m0 < kw + 31)) {
+        const int e_end = Lq - m0 - 4 * hi;               // query m0 + 4hi + e valid iff
+        const int e_lo = CAUSAL ? myk - m0 - 4 * hi : 0;  // e_lo <= e < e_end
+  #pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = 8 * (i / 4) + i % 4;
+          if (e >= e_end || e < e_lo) pr[i] = ds[i] = 0.0f;
+        }
+      }
+      row3<D, Tiles::PART>(dva, tO, to, 2 * wt, pr);
+      row3<D, Tiles::PART>(dka, tQ, to, 2 * wt, ds);
     }
-    row3<D, Tiles::PART>(dva, tO, to, 2 * wt, pr);
-    row3<D, Tiles::PART>(dka, tQ, to, 2 * wt, ds);
   }
   add_waves<NDB, WK>(dva, lds, w, lane);
   add_waves<NDB, WK>(dka, lds, w, lane);

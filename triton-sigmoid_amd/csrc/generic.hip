@@ -157,7 +157,6 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
   const int b = bh / p.H, h = bh % p.H;
   const int Lq = p.len_q(b), Lk = p.len_k(b);
   const int key = kb * GB + threadIdx.x;
-  const int64_t qbase = p.q_base(b, h);
   const int64_t kbase = p.k_base(b, h);
   const float scale = *p.scale, bias = p.bias[b];
   const bool kok = key < Lk;
@@ -173,36 +172,39 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
   }
   const int mstart = CAUSAL ? (kb * GB) / GT * GT : 0;
   const int mend = (kb * GB >= Lk) ? 0 : Lq;
-  for (int m0 = mstart; m0 < mend; m0 += GT) {
-    for (int e = threadIdx.x; e < GT * D; e += GB) {
-      const int r = e / D, d = e % D, q = m0 + r;
-      const bool ok = q < Lq;
-      sQ[r][d] = ok ? ld<T>(p.q, qbase + (int64_t)q * p.sq_t + d) : 0.0f;
-      sO[r][d] = ok ? ld<T>(p.dout, qbase + (int64_t)q * p.sq_t + d) : 0.0f;
-    }
-    __syncthreads();
-    const int jn = min(GT, mend - m0);
-    for (int j = 0; j < jn; ++j) {
-      const int q = m0 + j;
-      float s = 0.0f, dp = 0.0f;
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        s = __builtin_fmaf(sQ[j][d], kv[d], s);
-        dp = __builtin_fmaf(sO[j][d], vv[d], dp);
+  for (int g = 0; g < p.q_heads(); ++g) {  // the query heads of this K / V head
+    const int64_t qbase = p.q_base(b, p.first_q_head(h) + g);
+    for (int m0 = mstart; m0 < mend; m0 += GT) {
+      for (int e = threadIdx.x; e < GT * D; e += GB) {
+        const int r = e / D, d = e % D, q = m0 + r;
+        const bool ok = q < Lq;
+        sQ[r][d] = ok ? ld<T>(p.q, qbase + (int64_t)q * p.sq_t + d) : 0.0f;
+        sO[r][d] = ok ? ld<T>(p.dout, qbase + (int64_t)q * p.sq_t + d) : 0.0f;
       }
-      float pr = sigmoid_of(s, scale, c);
-      const float t = pr * dp;
-      float ds = __builtin_fmaf(-pr, t, t);
-      if (CAUSAL && key > q) { pr = 0.0f; ds = 0.0f; }
-      pr = round_to<T>(pr);
-      ds = round_to<T>(ds);
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        dv[d] = __builtin_fmaf(pr, sO[j][d], dv[d]);
-        dk[d] = __builtin_fmaf(ds, sQ[j][d], dk[d]);
+      __syncthreads();
+      const int jn = min(GT, mend - m0);
+      for (int j = 0; j < jn; ++j) {
+        const int q = m0 + j;
+        float s = 0.0f, dp = 0.0f;
+  #pragma unroll
+        for (int d = 0; d < D; ++d) {
+          s = __builtin_fmaf(sQ[j][d], kv[d], s);
+          dp = __builtin_fmaf(sO[j][d], vv[d], dp);
+        }
+        float pr = sigmoid_of(s, scale, c);
+        const float t = pr * dp;
+        float ds = __builtin_fmaf(-pr, t, t);
+        if (CAUSAL && key > q) { pr = 0.0f; ds = 0.0f; }
+        pr = round_to<T>(pr);
+        ds = round_to<T>(ds);
+  #pragma unroll
+        for (int d = 0; d < D; ++d) {
+          dv[d] = __builtin_fmaf(pr, sO[j][d], dv[d]);
+          dk[d] = __builtin_fmaf(ds, sQ[j][d], dk[d]);
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
   if (key < p.k_rows_out(Lk)) {
 #pragma unroll

@@ -112,6 +112,7 @@ sigattn_problem make_problem(const Tensor &q, const Tensor &k, const Tensor &v, 
     p.cu_seqlens_k = static_cast<const int32_t *>(lay.cuk.data_ptr());
     p.rows_q = q.size(0);
     p.rows_k = k.size(0);
+    p.kv_heads = k.size(1);
   } else {
     p.B = q.size(0);
     p.Tq = q.size(1);
@@ -168,7 +169,8 @@ int64_t two_pass_bytes(const sigattn_problem &p, int64_t limit, int dev) {
   const int64_t full = (int64_t)g_api.bwd_workspace_bytes(&p);
   if (full <= limit) return full;
   const int64_t per_head = full / p.H;
-  const int64_t heads = limit / per_head;
+  const int64_t group = p.kv_heads > 0 ? p.H / p.kv_heads : 1;
+  const int64_t heads = limit / per_head / group * group;
   const int64_t grid = heads * p.B * ((p.Tq + g_dq_ds_rows - 1) / g_dq_ds_rows);
   if (heads == 0 || grid < compute_units(dev)) return 0;
   return heads * per_head;

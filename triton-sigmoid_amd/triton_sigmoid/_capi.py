@@ -21,7 +21,7 @@ import torch
 # SIGATTN_LIBRARY may name another build of the same sources (a tile-
 # configuration variant from _build.py --out ... -D...).
 LIB_PATH = Path(os.environ.get("SIGATTN_LIBRARY") or Path(__file__).resolve().parent / "libsigattn.so")
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 F16, BF16, F32 = 0, 1, 2
 _DTYPE_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
@@ -59,6 +59,7 @@ class SigattnProblem(ctypes.Structure):
         ("cu_seqlens_k", _c_vp),
         ("rows_q", _c_i64),
         ("rows_k", _c_i64),
+        ("kv_heads", _c_i64),
     ]
 
 
@@ -215,6 +216,7 @@ def _problem(Q, K, V, bias, score_mod, sm_scale, seq_lens_q, seq_lens_k, causal,
         qs, ks = (0,) + Q.stride(), (0,) + K.stride()
         pr.cu_seqlens_q, pr.cu_seqlens_k = _ptr(cu_q), _ptr(cu_k)
         pr.rows_q, pr.rows_k = Q.shape[0], K.shape[0]
+        pr.kv_heads = K.shape[1]
     pr.abi_version = ABI_VERSION
     pr.dtype = _DTYPE_CODE[Q.dtype]
     pr.B, pr.Tq, pr.Tk, pr.H, pr.D = B, Tq, Tk, H, D
@@ -342,7 +344,8 @@ def bwd_workspace_bytes(lib, pr: SigattnProblem, device: torch.device) -> int:
     if full <= limit:
         return full
     per_head = full // pr.H
-    heads = limit // per_head
+    group = pr.H // pr.kv_heads if pr.kv_heads else 1  # the library's groups are whole K / V heads
+    heads = limit // per_head // group * group
     grid = heads * pr.B * -(-pr.Tq // _DQ_DS_ROWS)
     if heads == 0 or grid < _compute_units(device):
         return 0

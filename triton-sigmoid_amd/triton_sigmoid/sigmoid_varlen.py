@@ -160,7 +160,10 @@ def sigmoid_attention_varlen(
     each sequence.
 
     Args:
-        query: [total_q, H, D]; key, value: [total_k, H, D].
+        query: [total_q, H, D]; key, value: [total_k, H_kv, D] with H a
+            multiple of H_kv: query head h reads key / value head
+            h // (H // H_kv), whose gradients are the sums over its query
+            heads.
         cu_seqlens_q / cu_seqlens_k: [B + 1] non-decreasing offsets (any integer
             dtype, converted to int32) with cu[0] = 0 and cu[B] = total rows;
             sequence b is rows cu[b] .. cu[b+1]-1.
@@ -190,7 +193,7 @@ def sigmoid_attention_varlen(
     _, H, D = query.shape
     N_k, H_k, D_k = key.shape
     N_v, H_v, D_v = value.shape
-    if H != H_k or H != H_v:
+    if H_k != H_v or H != H_k and (H_k == 0 or H % H_k):
         raise ValueError(f"Number of heads mismatch: Q={H}, K={H_k}, V={H_v}")
     if D != D_k or D != D_v:
         raise ValueError(f"Head dimension mismatch: Q={D}, K={D_k}, V={D_v}")
