@@ -281,6 +281,91 @@ int sigattn_bwd_dkdv_ws(const sigattn_problem *p, const void *dout, void *dk, vo
 int sigattn_bwd_dq_ws(const sigattn_problem *p, void *dq, const void *workspace,
                       size_t workspace_bytes, void *stream);
 
+/*
+ * Paged key/value cache (no counterpart in the reference).  K and V of every
+ * sequence live in pages of page_size tokens, anywhere in two caches of
+ * num_pages pages: token j of sequence b is row j % page_size of page
+ * block_table[b, j / page_size].  page_size is a power of two, 16 at least.
+ * A slot is page * page_size + row; num_pages * page_size < 2^31.
+ */
+
+/*
+ * The bookkeeping of one serving step, on the device: request b has
+ * context_lens[b] tokens in the cache and adds new_lens[b] (negative lengths
+ * count as 0).  Its new pages, those of its tokens past the pages it already
+ * holds, are taken from free_pages in request order and entered into
+ * block_table (int32 [B, max_pages], row stride table_stride); other entries
+ * stay.  Further outputs, int32:
+ *   cu_seqlens [B + 1]      offsets of the requests' new tokens, packed
+ *   seq_lens [B]            context_lens + new_lens
+ *   slot_mapping            slot of each of num_tokens packed token rows; -1
+ *                           for rows past the last request's and for tokens
+ *                           without a page
+ *   pages_needed [1]        pages the step takes: more than num_free means that
+ *                           pages were missing.  Entries of missing pages are -1.
+ * Pages past max_pages are not entered and count as missing for their tokens
+ * alone.  B <= SIGATTN_PLAN_MAX_BATCH; sums of tokens and pages fit 31 bits.
+ * One launch.
+ */
+#define SIGATTN_PLAN_MAX_BATCH 8192
+int sigattn_paged_plan(int64_t B, const int32_t *context_lens, const int32_t *new_lens, int32_t *block_table,
+                       int64_t table_stride, int64_t max_pages, const int32_t *free_pages, int64_t num_free,
+                       int64_t page_size, int64_t num_tokens, int32_t *slot_mapping, int32_t *cu_seqlens,
+                       int32_t *seq_lens, int32_t *pages_needed, void *stream);
+
+/*
+ * Writes packed K and V rows [rows, kv_heads, D] into the caches: row t goes to
+ * slot_mapping[t].  Rows with a slot outside [0, num_pages * page_size) are not
+ * written.  Strides in elements; k and v share theirs, and so do the caches.
+ * Slots within a call are distinct: which of two rows with one slot stays is
+ * not defined.  esize: bytes of an element, 2 or 4.
+ */
+typedef struct sigattn_paged_rows {
+  int32_t esize, reserved;
+  int64_t rows, kv_heads, D;
+  int64_t src_stride_t, src_stride_h;
+  int64_t cache_stride_p, cache_stride_t, cache_stride_h; /* page, token, head */
+  int64_t num_pages, page_size;
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  const int32_t *slot_mapping;
+} sigattn_paged_rows;
+int sigattn_paged_write(const sigattn_paged_rows *r, void *stream);
+
+/*
+ * Sigmoid attention of new tokens over a paged cache that holds them already.
+ * Queries are packed [rows_q, H, D]: those of sequence b, at most max_seqlen_q,
+ * are rows cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1 (clamped to rows_q), and are
+ * the last of its seq_lens_k[b] tokens (clamped to [0, max_pages * page_size]):
+ * query i of n sits at position L - n + i, and under the causal mask sees keys
+ * up to that one (none where it is negative: the row is zeros).  Query head h
+ * reads K / V head h / (H / kv_heads).  Pages outside [0, num_pages) hold no
+ * keys: their positions add nothing.  Rows of `out` that no sequence covers
+ * are zeros.  bias: added to every score; own_bias 0 means -log(L).
+ */
+typedef struct sigattn_paged_problem {
+  int32_t abi_version;    /* SIGATTN_ABI_VERSION, 3 at least */
+  int32_t dtype;          /* enum sigattn_dtype */
+  int64_t B, H, kv_heads, D, rows_q, max_seqlen_q;
+  int64_t num_pages, page_size, max_pages;
+  int64_t q_stride_t, q_stride_h;                 /* q; out is contiguous [rows_q, H, D] */
+  int64_t k_stride_p, k_stride_t, k_stride_h;     /* both caches: page, token, head */
+  int64_t table_stride, mod_stride;               /* rows of block_table and score_mod */
+  const void *q, *k_cache, *v_cache;
+  const int32_t *block_table;  /* [B, max_pages] */
+  const int32_t *seq_lens_k;   /* [B] */
+  const int32_t *cu_seqlens_q; /* [B + 1] */
+  const float *score_mod;      /* [B, max_pages * page_size] fp32, or NULL */
+  float scale, bias;
+  int32_t own_bias, causal;
+} sigattn_paged_problem;
+
+int sigattn_paged_check(const sigattn_paged_problem *p);
+/* Device memory (16-byte aligned) that sigattn_paged_fwd works in; 0: none. */
+size_t sigattn_paged_fwd_workspace_bytes(const sigattn_paged_problem *p);
+int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

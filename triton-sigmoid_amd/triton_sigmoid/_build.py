@@ -26,7 +26,8 @@ INCLUDE = ROOT.parent / "include"
 LIB_PATH = PKG_DIR / "libsigattn.so"
 BUILD_DIR = ROOT / "_build"
 
-SOURCES = ["fwd.hip", "bwd.hip", "decode.hip", "f32.hip", "generic.hip", "bias.hip", "capi.cpp"]
+SOURCES = ["fwd.hip", "bwd.hip", "decode.hip", "f32.hip", "generic.hip", "bias.hip", "paged.hip",
+           "capi.cpp", "paged_capi.cpp"]
 SOURCE_FLAGS = {"bias.hip": ["-ffp-contract=off"]}  # see the file
 ARCH = "gfx950"
 AUTOGRAD_SOURCE = "torch_autograd.cpp"

@@ -63,6 +63,69 @@ class SigattnProblem(ctypes.Structure):
     ]
 
 
+class SigattnPagedRows(ctypes.Structure):
+    """Mirror of `struct sigattn_paged_rows` (include/sigattn.h)."""
+
+    _fields_ = [
+        ("esize", _c_i32),
+        ("reserved", _c_i32),
+        ("rows", _c_i64),
+        ("kv_heads", _c_i64),
+        ("D", _c_i64),
+        ("src_stride_t", _c_i64),
+        ("src_stride_h", _c_i64),
+        ("cache_stride_p", _c_i64),
+        ("cache_stride_t", _c_i64),
+        ("cache_stride_h", _c_i64),
+        ("num_pages", _c_i64),
+        ("page_size", _c_i64),
+        ("k", _c_vp),
+        ("v", _c_vp),
+        ("k_cache", _c_vp),
+        ("v_cache", _c_vp),
+        ("slot_mapping", _c_vp),
+    ]
+
+
+class SigattnPagedProblem(ctypes.Structure):
+    """Mirror of `struct sigattn_paged_problem` (include/sigattn.h)."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("dtype", _c_i32),
+        ("B", _c_i64),
+        ("H", _c_i64),
+        ("kv_heads", _c_i64),
+        ("D", _c_i64),
+        ("rows_q", _c_i64),
+        ("max_seqlen_q", _c_i64),
+        ("num_pages", _c_i64),
+        ("page_size", _c_i64),
+        ("max_pages", _c_i64),
+        ("q_stride_t", _c_i64),
+        ("q_stride_h", _c_i64),
+        ("k_stride_p", _c_i64),
+        ("k_stride_t", _c_i64),
+        ("k_stride_h", _c_i64),
+        ("table_stride", _c_i64),
+        ("mod_stride", _c_i64),
+        ("q", _c_vp),
+        ("k_cache", _c_vp),
+        ("v_cache", _c_vp),
+        ("block_table", _c_vp),
+        ("seq_lens_k", _c_vp),
+        ("cu_seqlens_q", _c_vp),
+        ("score_mod", _c_vp),
+        ("scale", ctypes.c_float),
+        ("bias", ctypes.c_float),
+        ("own_bias", _c_i32),
+        ("causal", _c_i32),
+    ]
+
+
+# Largest batch of sigattn_paged_plan (SIGATTN_PLAN_MAX_BATCH).
+PLAN_MAX_BATCH = 8192
+
 # Exported symbols and their signatures (every function in include/sigattn.h).
 SIGNATURES = {
     "sigattn_abi_version": ([], _c_i32),
@@ -87,6 +150,12 @@ SIGNATURES = {
     "sigattn_bwd_split_workspace_bytes": ([ctypes.POINTER(SigattnProblem)], ctypes.c_size_t),
     "sigattn_bwd_split": ([ctypes.POINTER(SigattnProblem), _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_size_t,
                            _c_vp], _c_i32),
+    "sigattn_paged_plan": ([_c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp,
+                            _c_vp, _c_vp, _c_vp], _c_i32),
+    "sigattn_paged_write": ([ctypes.POINTER(SigattnPagedRows), _c_vp], _c_i32),
+    "sigattn_paged_check": ([ctypes.POINTER(SigattnPagedProblem)], _c_i32),
+    "sigattn_paged_fwd_workspace_bytes": ([ctypes.POINTER(SigattnPagedProblem)], ctypes.c_size_t),
+    "sigattn_paged_fwd": ([ctypes.POINTER(SigattnPagedProblem), _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
 }
 
 _lib = None
