@@ -258,9 +258,9 @@ int sigattn_bwd_dkdv(const sigattn_problem *p, const void *dout, void *dk, void 
  * workspace holds 2 bytes per (query, key) pair of every 32x32 block that has
  * a visible pair (causal: the lower triangle), per batch and head:
  * sigattn_bwd_workspace_bytes(p) for the whole problem, or 0 when the
- * problem has no two-pass form (fp32, D other than 64 or 128, misaligned
- * rows).  sigattn_bwd_ws with a smaller workspace runs the
- * heads in groups that fit, one group after another on `stream`; with room
+ * problem has no two-pass form (fp32, D other than 64 or 128, grouped heads
+ * at D = 64, misaligned rows).  sigattn_bwd_ws with a smaller workspace runs the
+ * heads in groups that fit (whole K / V heads), one group after another on `stream`; with room
  * for less than one head, or workspace NULL, it runs sigattn_bwd.  Results
  * equal sigattn_bwd's within fp32 summation order; the workspace must be
  * 16-byte aligned and is only used until the call's kernels finish.
@@ -361,7 +361,13 @@ typedef struct sigattn_paged_problem {
 } sigattn_paged_problem;
 
 int sigattn_paged_check(const sigattn_paged_problem *p);
-/* Device memory (16-byte aligned) that sigattn_paged_fwd works in; 0: none. */
+/*
+ * Device memory (16-byte aligned) that sigattn_paged_fwd works in, only until
+ * its kernels finish: fp32 sums of sequences whose keys are cut into chunks that
+ * run beside each other, added in chunk order by a kernel of their own
+ * (deterministic).  0: none.  With workspace NULL no sequence is cut; one that
+ * is too small is SIGATTN_ERR_WORKSPACE.
+ */
 size_t sigattn_paged_fwd_workspace_bytes(const sigattn_paged_problem *p);
 int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace, size_t workspace_bytes,
                       void *stream);

@@ -317,6 +317,7 @@ template <int D> struct DkdvLds {
 };
 template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPED>
 __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, DkdvLds<D> &lds) {
+  static_assert(!(DSOUT && GROUPED), "two-pass backward of grouped heads: D = 128 only");
   constexpr int BN = 128;                 // keys per workgroup (32 per wave)
   constexpr int BMQ = 64;                 // queries per LDS tile (two 32-query blocks)
   constexpr int NST = 4;                  // LDS ring stages
@@ -481,19 +482,17 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   const int kbw = kw / 32;
   uint16_t *ds_bh = nullptr;
   if constexpr (DSOUT)
-    ds_bh = p.ds + ((int64_t)b * p.H * p.q_heads() + hq) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
+    ds_bh = p.ds + ((int64_t)b * p.H + h) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) *
                        DsLayout::kTileElems;
   // Every region issues exactly two store instructions, so the tile
   // barrier can wait for its copies with a fixed vmcnt while the stores are
   // still in flight: a skipped tile is a store through a buffer resource of
   // zero bytes, which the hardware drops.
-  auto store_ds = [&](int slot, int g, int head) SIGATTN_INLINE {
+  auto store_ds = [&](int slot, int g) SIGATTN_INLINE {
     const int qb = mstart / 32 + g;
     const bool ok = g >= 0 && 32 * qb < Lq && kw < Lk && (!CAUSAL || qb >= kbw);
     // Buffer over this wave's tile (or over nothing).
-    const int64_t skip = GROUPED ? head * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) : 0;
-    const uint16_t *tp =
-        ds_bh + (ok ? skip + DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
+    const uint16_t *tp = ds_bh + (ok ? DsLayout::tile(qb, kbw, p.ds_nqb, CAUSAL) : 0) * DsLayout::kTileElems;
     const __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc((void *)tp, (short)0, ok ? 2048 : 0, kBufferWord3);
     const int off = 16 * lane;
@@ -540,7 +539,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
       // VALU work), stored where the next vmcnt(0) is furthest away: at the
       // start of even regions, after the tile barrier in odd ones.
       if constexpr (DSOUT) {
-        if (((U % 2) == 0 && win == 0) || ((U % 2) == 1 && win * 4 == BAR)) store_ds(SL, hs.block(r, 2), hs.head(2));
+        if (((U % 2) == 0 && win == 0) || ((U % 2) == 1 && win * 4 == BAR)) store_ds(SL, r - 2);
       }
       // One wait for the window's four operands instead of one per MFMA.
       asm volatile("" ::"v"(opq[(win * 4) % LA]), "v"(opq[(win * 4 + 1) % LA]),
@@ -1430,7 +1429,8 @@ static void bwd_dkdv_t(const KParams &kp, bool causal, bool sm, hipStream_t st) 
     // Range split (dense non-causal recompute backward): rsplit workgroups per item.
     if (!causal && !DSOUT && p.rsplit > 1) grid.x *= (unsigned)p.rsplit;
     by_flags(causal, sm, p.qgroup > 1, [&](auto c, auto m, auto g) {
-      bwd_dkdv_kernel<T, D, c.value, m.value, DSOUT, g.value><<<grid, 256, 0, st>>>(p);
+      // The two-pass backward of grouped heads is D = 128's alone.
+      if constexpr (!(DSOUT && g.value)) bwd_dkdv_kernel<T, D, c.value, m.value, DSOUT, g.value><<<grid, 256, 0, st>>>(p);
     });
   });
 }
@@ -1517,8 +1517,11 @@ void launch_bwd_dkdv_mfma(const KParams &p, int dtype, int D, bool causal, bool 
                           hipStream_t st) {
   by_type(dtype, D, [&](auto *t, auto d) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (dsout) bwd_dkdv_t<T, decltype(d)::value, true>(p, causal, sm, st);
-    else bwd_dkdv_t<T, decltype(d)::value, false>(p, causal, sm, st);
+    constexpr int DD = decltype(d)::value;
+    if constexpr (DD > 32) {  // no two-pass form below
+      if (dsout) return bwd_dkdv_t<T, DD, true>(p, causal, sm, st);
+    }
+    bwd_dkdv_t<T, DD, false>(p, causal, sm, st);
   });
 }
 

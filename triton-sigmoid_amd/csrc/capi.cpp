@@ -119,6 +119,9 @@ struct SplitPlan {
 // D = 16 and 32 the main forward and the recompute backward serve every shape.
 bool wide_head(const sigattn_problem *p) { return p->D == 64 || p->D == 128; }
 
+// ... and with grouped heads at D = 128 alone (below it the recompute kernels are faster).
+bool two_pass_head(const sigattn_problem *p) { return wide_head(p) && (p->D == 128 || head_group(p) == 1); }
+
 // Head dim of the MFMA kernel instance: head_dim 16 runs in the D = 32
 // kernels (KParams::dmem = 16).
 int mfma_head_dim(const sigattn_problem *p) { return p->D == 16 ? 32 : (int)p->D; }
@@ -726,13 +729,13 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   // The halves (kBwdDq, kBwdDkdv) need the whole problem's dS at once: the
   // dQ half reads what a dK/dV half with the same workspace stored.
   int64_t heads_per_pass = 0;
-  if (workspace != nullptr && mfma && wide_head(p) && p->Tq > 0 && p->Tk > 0) {
+  if (workspace != nullptr && mfma && two_pass_head(p) && p->Tq > 0 && p->Tk > 0) {
     heads_per_pass = (int64_t)workspace_bytes / ds_bytes_per_head(p);
     if (heads_per_pass > p->H) heads_per_pass = p->H;
     heads_per_pass -= heads_per_pass % head_group(p);  // whole groups: dK / dV are sums over them
   }
   if (parts != kBwdAll && workspace != nullptr) {
-    if (!mfma || !wide_head(p)) return SIGATTN_ERR_WORKSPACE;  // no two-pass kernels for this problem
+    if (!mfma || !two_pass_head(p)) return SIGATTN_ERR_WORKSPACE;  // no two-pass kernels for this problem
     if (p->Tq > 0 && p->Tk > 0 && heads_per_pass < p->H) return SIGATTN_ERR_WORKSPACE;
   }
   const bool twopass = heads_per_pass > 0;
@@ -813,7 +816,7 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
 size_t sigattn_bwd_workspace_bytes(const sigattn_problem *p) {
   if (sigattn_check(p) != SIGATTN_OK || p->B == 0 || p->H == 0 || p->Tq == 0 || p->Tk == 0) return 0;
   const void *none[1] = {nullptr};
-  if (!use_mfma(p, none, 0) || !wide_head(p)) return 0;
+  if (!use_mfma(p, none, 0) || !two_pass_head(p)) return 0;
   return (size_t)(ds_bytes_per_head(p) * p->H);
 }
 

@@ -1,4 +1,5 @@
-// Paged key/value cache: parameters and launchers of the kernels that read it.
+// Paged key/value cache: parameters, work units and tile copies of the kernels
+// that read it.
 #pragma once
 
 #include "common.h"
@@ -8,8 +9,17 @@ namespace sigattn {
 // Attention over a paged cache.  The base's q, out, k, v, score_mod, cu_q,
 // rows_q, sq_*, sk_t, sk_h, B, H, Tq (longest query sequence), Tk (tokens a
 // block-table row can hold) and dmem mean what they do there; H counts query
-// heads.
+// heads, and `out` is contiguous [rows_q, H, dmem].
+//
+// A kernel's work unit is (sequence, block of query columns, K / V head, chunk
+// of the keys); the columns of a sequence are its tokens times the G query
+// heads of a K / V head, column c = token c / G of head c % G.  A kernel takes
+// the sequences of more than cols_lo and at most cols_hi columns.  split_units
+// > 0: sequences are cut into chunks of at least min_chunk keys, so that there
+// are about that many units; a unit of a cut sequence leaves its fp32 sums in
+// `ws`, and cut[b] where they begin, for the reduction.
 struct PagedParams : KParams {
+  static constexpr bool kPaged = true;
   const int32_t *table;  // [B, max_pages], row stride table_stride
   const int32_t *lens;   // [B] keys
   int64_t table_stride, mod_stride, sk_p;
@@ -17,11 +27,213 @@ struct PagedParams : KParams {
   int lp, num_pages;     // log2 of the page size
   float fscale, fbias;
   int own_bias;          // 0: the bias is -log(keys)
+  int cols_lo, cols_hi;
+  int split_units, min_chunk;
+  int2 *cut;             // [B] (first unit / Hkv, chunks)
 
   __device__ __forceinline__ int keys(int b) const { return clamp_len(lens, b, Tk); }
   __device__ __forceinline__ float bias_of(int Lk) const { return own_bias ? fbias : -logf((float)Lk); }
+  // Blocks of `block` columns that this kernel runs of a sequence of n tokens.
+  __device__ __forceinline__ int blocks_of(int n, int block) const {
+    const int cols = n * G;
+    return cols > cols_lo && cols <= cols_hi ? (cols + block - 1) / block : 0;
+  }
 };
 
+struct PagedUnit {
+  int b, hk, qb;      // sequence, K / V head, column block
+  int Lq, Lk;         // its tokens and keys
+  int k0, k1;         // keys of the chunk
+  int nck = 0;        // chunks of the sequence (0: no such unit)
+};
+
+// Sum over the wave's lanes, in a fixed order.
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+
+// Unit u of the kernel with column blocks of `block`, from the lengths on the
+// device (no host synchronisation): sequences in order, their blocks last
+// (under the causal mask longest) first, chunks, K / V heads fastest.  Every wave computes it
+// alike, 64 sequences at a time.  Chunks: with work W = sum of blocks times
+// keys, C = W Hkv / split_units keys (min_chunk at least), ceil(keys / C) chunks
+// of equal length: at most split_units + the units of an uncut batch.
+__device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
+  const int lane = __lane_id();
+  int C = 1 << 30;  // more than any length
+  if (p.split_units > 0) {
+    float work = 0.0f;
+    for (int b = lane; b < p.B; b += 64) work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
+    const float c = wave_sum(work) * (float)p.Hkv / (float)p.split_units;
+    C = __builtin_amdgcn_readfirstlane(max(p.min_chunk, (int)fminf(c, 1e9f) + 1));
+  }
+  PagedUnit un;
+  const int row = u / p.Hkv;
+  un.hk = u - row * p.Hkv;
+  for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int Lq = b < p.B ? p.len_q(b) : 0, Lk = b < p.B ? p.keys(b) : 0;
+    const int nqb = p.blocks_of(Lq, block), nck = max((Lk + C - 1) / C, 1);
+    int sum = nqb * nck;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(sum, d);
+      if (lane >= d) sum += x;
+    }
+    const int first = base + sum - nqb * nck;
+    const uint64_t m = __ballot(row >= first && row < base + sum);
+    if (m != 0) {
+      const int at = __builtin_ctzll(m);
+      un.b = b0 + at;
+      un.Lq = __builtin_amdgcn_readlane(Lq, at), un.Lk = __builtin_amdgcn_readlane(Lk, at);
+      un.nck = __builtin_amdgcn_readlane(nck, at);
+      const int r = row - __builtin_amdgcn_readlane(first, at), q = r / un.nck, chunk = r - q * un.nck;
+      un.qb = __builtin_amdgcn_readlane(nqb, at) - 1 - q;
+      const int len = ((un.Lk + un.nck - 1) / un.nck + 63) & ~63;
+      un.k0 = min(chunk * len, un.Lk), un.k1 = min(un.k0 + len, un.Lk);
+      if (p.split_units > 0 && r == 0 && un.hk == 0 && lane == at)
+        p.cut[b] = make_int2(first, nck);
+      break;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return un;
+}
+
+// fp32 sums of unit u: [block columns][D] at u * block * D floats of ws.
+// (a: column block's 16-row accumulators; col: this lane's column of the
+// sequence, cc: of the unit; further column blocks 32 columns on.)
+template <typename T, int D, int NCB, class Acc>
+__device__ __forceinline__ void paged_store(const PagedParams &p, const PagedUnit &un, const Acc &acc, int col, int cc,
+                                            int block, int unit, int hi, bool half) {
+  constexpr int NDB = D / 32;
+  const int d = half ? 16 : D;
+  const int64_t row0 = packed_first(p.cu_q, p.rows_q, un.b);
+#pragma unroll
+  for (int c = 0; c < NCB; ++c) {
+    const int q = col + 32 * c;
+    if (q >= un.Lq * p.G) continue;
+    const int tok = q / p.G;
+    uint16_t *orow = (uint16_t *)p.out + ((row0 + tok) * p.H + un.hk * p.G + q - tok * p.G) * d;
+    float *part = p.ws + ((int64_t)unit * block + cc + 32 * c) * D;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (half && g >= 2) break;  // columns 16..31: not in the tensor
+        const int d0 = db * 32 + 8 * g + 4 * hi;
+        const f32x16 &a = acc[c][db];
+        const f32x4 v = {a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+        if (un.nck == 1) *(u32x2 *)(orow + d0) = (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
+        else *(f32x4 *)(part + d0) = v;
+      }
+    }
+  }
+}
+
+// A 16-byte source of zeros.
+static __device__ const uint32_t kZeroPiece[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+
+// DmaPlan for tiles of a paged cache: ROWS keys from a key that is a multiple
+// of 16, copied by NWAVES waves, each a run of rows that begins at a multiple of
+// its length.  Pages hold a power of two of rows, 16 at least, so 16 rows of a
+// tile lie on one page: their table entry is a scalar load (made one tile
+// ahead of its use) and the page's address scalar arithmetic in 64 bits; the
+// lanes keep 32-bit offsets within 16 rows.  Rows past the chunk and rows on a
+// page outside the cache come from kZeroPiece: every instruction still issues,
+// so counted waits hold.
+template <int ROWS, int D, int NWAVES> struct PagedDma {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR;
+  static constexpr int RPW = ROWS / NWAVES, NI = RPW / RPI;  // rows, instructions per wave
+  static constexpr int NE = RPW > 16 ? RPW / 16 : 1;         // table entries per wave and tile
+  static_assert(NI >= 1 && RPW % RPI == 0 && (RPW <= 16 ? 16 % RPW == 0 : RPW % 16 == 0), "tile shape");
+  typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
+
+  uint32_t voff[NI];  // byte offset of this lane's piece from the wave's first row of 16
+  uint32_t cbyte[NI];
+  ScalarInts row;     // the sequence's table row
+  int ent[NE];        // pages of the next tile
+  int key0, keys, r0, lrow, lp, pages;  // chunk's first key and length; the wave's first row; the lane's row of an instruction
+  int64_t page_bytes;
+  uint32_t row_bytes;
+
+  __device__ __forceinline__ void init(const PagedParams &p, int b, int first, int n, int wave, int lane, bool half) {
+    const int cmask = half ? CPR / 2 - 1 : CPR - 1;
+    key0 = first, keys = n, lp = p.lp, pages = p.num_pages;
+    r0 = wave * RPW;
+    lrow = lane / CPR;
+    // (Uniform to the compiler, so that the entries are scalar loads: a vector
+    // load would count among the tile copies that the kernels wait for.)
+    const uint64_t at = (uint64_t)(uintptr_t)(p.table + (int64_t)b * p.table_stride);
+    row = (ScalarInts)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at));
+    page_bytes = p.sk_p * 2, row_bytes = (uint32_t)(p.sk_t * 2);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int in_tile = r0 + i * RPI + lrow;
+      cbyte[i] = 16 * (((lane % CPR) ^ swz<D>(in_tile)) & cmask);
+      voff[i] = (uint32_t)((i * RPI) % 16 + lrow) * row_bytes + cbyte[i];
+    }
+  }
+  // Entries of the tile whose first key is `tile` of the chunk.
+  __device__ __forceinline__ void load(int tile) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int key = key0 + min(tile + r0 + 16 * e, keys - 1);
+      ent[e] = row[__builtin_amdgcn_readfirstlane(key >> lp)];
+    }
+  }
+  static __device__ __forceinline__ void copy(uint16_t *lds, const char *base, uint32_t off) {
+    const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
+  }
+  static __device__ __forceinline__ void copy_at(uint16_t *lds, const char *at) {
+    const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(at), "{m0}"(dst) : "memory");
+  }
+  // Copies one tensor's tile whose entries are in `ent` (head: the head's
+  // element 0 of page 0).
+  __device__ __forceinline__ void issue_one(uint16_t *lds, const uint16_t *head, int tile) const {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int first = tile + r0 + 16 * e;  // of the chunk
+      const int id = ent[e], n = keys - first;
+      const bool there = id >= 0 && id < pages;
+      const int in_page = (key0 + first) & ((1 << lp) - 1);
+      const char *base = (const char *)head + (there ? id : 0) * page_bytes + (int64_t)in_page * row_bytes;
+      constexpr int PER = NI / NE;
+      if (there && n >= (RPW < 16 ? RPW : 16)) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) copy(lds + (r0 + (e * PER + i) * RPI) * D, base, voff[e * PER + i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const bool in = there && i * RPI + lrow < n;
+          copy_at(lds + (r0 + (e * PER + i) * RPI) * D, in ? base + voff[e * PER + i] : (const char *)kZeroPiece);
+        }
+      }
+    }
+  }
+  // The same, for a tile that is followed by the one from key `next` on.
+  __device__ __forceinline__ void issue_last(uint16_t *lds, const uint16_t *head, int tile, int next) {
+    issue_one(lds, head, tile);
+    if (next < keys) load(next);
+  }
+};
+
+// Attention of every sequence: any dtype, alignment and strides.
 void launch_paged_generic(const PagedParams &p, int dtype, int D, bool causal, hipStream_t st);
+// MFMA kernels, dtype in {kF16, kBF16}, D in {32, 64, 128} (16 as 32 with
+// dmem = 16), 16-byte aligned rows: blocks of paged_block(D) columns; a wave
+// or workgroup per chunk for sequences of up to 32 columns; and the
+// sums of cut sequences.  ngap leading workgroups of the first two zero the
+// rows outside every sequence.
+int paged_block(int D);
+void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
+void launch_paged_decode(const PagedParams &p, int units, bool wave_units, int dtype, int D, bool causal,
+                         hipStream_t st);
+void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int dtype, int D, hipStream_t st);
 
 }  // namespace sigattn

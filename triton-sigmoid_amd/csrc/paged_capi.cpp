@@ -36,6 +36,92 @@ PagedParams make_params(const sigattn_paged_problem *p, void *out) {
   return k;
 }
 
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool aligned16(const void *ptr) { return ((uintptr_t)ptr & 15u) == 0; }
+
+// The MFMA kernels take f16 / bf16 whose rows start on 16-byte boundaries (and
+// whose 16 rows of a tile lie within 2^31 bytes).
+bool use_mfma(const sigattn_paged_problem *p, const void *out) {
+  if (p->dtype == SIGATTN_F32) return false;
+  const int64_t strides[5] = {p->q_stride_t, p->q_stride_h, p->k_stride_p, p->k_stride_t, p->k_stride_h};
+  for (int64_t s : strides)
+    if (s % 8 != 0) return false;
+  return p->k_stride_t < (int64_t)1 << 26 && aligned16(p->q) && aligned16(p->k_cache) && aligned16(p->v_cache) &&
+         aligned16(out);
+}
+
+// Head dim of the kernel instance: head_dim 16 runs in the D = 32 kernels.
+int kernel_dim(const sigattn_paged_problem *p) { return p->D == 16 ? 32 : (int)p->D; }
+
+// What one kernel runs: its units at most (the device finds out how many there
+// are), how it cuts sequences (PagedParams) and the partials that takes.
+struct Part {
+  int64_t units = 0;
+  int split_units = 0, min_chunk = 0, block = 0;
+  bool wave_units = false;
+  size_t partial_bytes = 0;
+};
+
+// Sequences of up to kDecodeCols columns run in the decode kernel, longer ones
+// in the forward's; a batch of one, whose length the host knows to be a long
+// one or does not know, runs in the forward's alone.
+constexpr int kDecodeCols = 32;
+struct Plan {
+  Part fwd, decode;
+  int cols_lo = 0;  // columns that are not the forward kernel's
+  size_t cut_bytes = 0, bytes = 0;
+};
+
+// Units of `t` workgroups (waves) in flight: sequences are cut so that a part
+// has about as many, where its uncut units may be fewer.
+void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const PagedParams &k, int D) {
+  part.units = uncut;
+  if (k.Tk <= min_chunk || t <= 0) return;
+  const int64_t most = uncut * cdiv(k.Tk, min_chunk);
+  int64_t extra = t - uncut > t / 2 ? t - uncut : t / 2;
+  if (extra > most) extra = most;
+  part.split_units = (int)extra;
+  part.min_chunk = (int)min_chunk;
+  // One more unit per K / V head than the sums say: their rounding.
+  part.units = uncut + extra + k.Hkv;
+  part.partial_bytes = (size_t)part.units * part.block * D * sizeof(float);
+}
+
+Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
+  Plan pl;
+  const int64_t cols = (int64_t)k.Tq * k.G, all = p->rows_q * k.G, cus = k.ncu;
+  const bool decode = cols <= kDecodeCols || k.B > 1, fwd = cols > kDecodeCols;
+  pl.fwd.block = sigattn::paged_block(D), pl.decode.block = 32;
+  if (decode) {
+    const int64_t pairs = (int64_t)k.B * k.Hkv;
+    pl.decode.wave_units = pairs >= cus;
+    cut_part(pl.decode, pairs, (pl.decode.wave_units ? 8 : 2) * cus, 256, k, D);
+  }
+  if (fwd) {
+    if (decode) pl.cols_lo = kDecodeCols;
+    // Blocks: whole ones of all columns, and one that is not whole for each
+    // sequence of the kernel's.
+    const int64_t seqs = all / (pl.cols_lo + 1) < k.B ? all / (pl.cols_lo + 1) : k.B;
+    const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = D == 128 ? 1 : (D == 64 ? 3 : 4);
+    const int64_t full = cdiv(all, pl.fwd.block) * k.Hkv;
+    cut_part(pl.fwd, uncut, full < 2 * per_cu * cus ? 2 * per_cu * cus : 0, 512, k, D);
+  }
+  const bool cut = pl.fwd.split_units > 0 || pl.decode.split_units > 0;
+  pl.cut_bytes = cut ? cdiv((int64_t)k.B * 2 * (int64_t)sizeof(int2), 256) * 256 : 0;
+  pl.bytes = pl.cut_bytes + pl.fwd.partial_bytes + pl.decode.partial_bytes;
+  return pl;
+}
+
+// k's fields for one part of a plan (part.split_units 0: nothing is cut).
+PagedParams of_part(const PagedParams &k, const Part &part, int lo, int hi, int2 *cut, float *ws) {
+  PagedParams s = k;
+  s.cols_lo = lo, s.cols_hi = hi;
+  s.split_units = part.split_units, s.min_chunk = part.min_chunk;
+  s.cut = cut, s.ws = ws;
+  return s;
+}
+
 int launch_status() { return hipGetLastError() == hipSuccess ? SIGATTN_OK : SIGATTN_ERR_LAUNCH; }
 
 }  // namespace
@@ -68,7 +154,11 @@ int sigattn_paged_check(const sigattn_paged_problem *p) {
   return SIGATTN_OK;
 }
 
-size_t sigattn_paged_fwd_workspace_bytes(const sigattn_paged_problem *) { return 0; }
+size_t sigattn_paged_fwd_workspace_bytes(const sigattn_paged_problem *p) {
+  if (sigattn_paged_check(p) != SIGATTN_OK || p->rows_q == 0 || p->H == 0 || p->B == 0) return 0;
+  const PagedParams k = make_params(p, nullptr);
+  return use_mfma(p, nullptr) ? make_plan(p, k, kernel_dim(p)).bytes : 0;
+}
 
 int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace, size_t workspace_bytes,
                       void *stream) {
@@ -76,17 +166,50 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
   if (rc != SIGATTN_OK) return rc;
   if (p->rows_q == 0 || p->H == 0) return SIGATTN_OK;
   if (out == nullptr) return SIGATTN_ERR_NULL_ARG;
-  (void)workspace, (void)workspace_bytes;
   const hipStream_t st = (hipStream_t)stream;
-  const PagedParams k = make_params(p, out);
+  PagedParams k = make_params(p, out);
+  const bool mfma = p->B > 0 && use_mfma(p, out), causal = p->causal != 0;
+  const int D = kernel_dim(p), dt = p->dtype;
+  Plan pl;
+  if (mfma) pl = make_plan(p, k, D);
+  if (workspace != nullptr && pl.bytes > 0 && (workspace_bytes < pl.bytes || !aligned16(workspace)))
+    return SIGATTN_ERR_WORKSPACE;
+  if (workspace == nullptr) {  // nothing is cut
+    pl.fwd.split_units = pl.decode.split_units = 0;
+  }
   (void)hipGetLastError();
+  sigattn::GapAxis gap;
+  gap.cu = p->cu_seqlens_q, gap.B = k.B, gap.T = k.Tq, gap.H = k.H, gap.D = (int)p->D;
+  gap.rows = p->rows_q, gap.st = p->H * p->D, gap.sh = p->D, gap.out[0] = out;
   if (p->B == 0) {  // no sequence: every row is outside
-    sigattn::GapAxis a;
-    a.H = k.H, a.D = (int)p->D, a.rows = p->rows_q, a.st = p->H * p->D, a.sh = p->D, a.out[0] = out;
-    sigattn::launch_zero_gaps(a, sigattn::GapAxis{}, p->dtype == SIGATTN_F32 ? 4 : 2, st);
+    sigattn::launch_zero_gaps(gap, sigattn::GapAxis{}, dt == SIGATTN_F32 ? 4 : 2, st);
     return launch_status();
   }
-  sigattn::launch_paged_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
+  if (!mfma) {
+    sigattn::launch_paged_generic(k, dt, (int)p->D, causal, st);
+    return launch_status();
+  }
+  char *ws = (char *)workspace;
+  int2 *cuts = (int2 *)ws;
+  float *partials = (float *)(ws + pl.cut_bytes);
+  k.gap[0] = gap;
+  // The first kernel also zeroes the rows outside every sequence (workgroups in
+  // a multiple of 8, so that its items keep their XCDs).
+  const int gaps = (int)(cdiv(cdiv(p->rows_q, 64), 8) * 8);
+  const PagedParams kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, cuts, partials);
+  const PagedParams kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0, cuts + p->B,
+                                 partials + pl.fwd.partial_bytes / sizeof(float));
+  if (pl.fwd.units > 0) {
+    PagedParams s = kf;
+    s.ngap[0] = gaps;
+    sigattn::launch_paged_fwd(s, (int)pl.fwd.units, dt, D, causal, st);
+  }
+  if (pl.decode.units > 0) {
+    PagedParams s = kd;
+    s.ngap[0] = pl.fwd.units > 0 ? 0 : gaps;
+    sigattn::launch_paged_decode(s, (int)pl.decode.units, pl.decode.wave_units, dt, D, causal, st);
+  }
+  if (kf.split_units > 0 || kd.split_units > 0) sigattn::launch_paged_reduce(kf, kd, dt, D, st);
   return launch_status();
 }
 

@@ -1,0 +1,130 @@
+// Attention over a paged cache: prompts and chunks of them, and the sums of
+// sequences whose keys were cut.
+//
+// The kernel is the forward's (fwd_kernel.h) on PagedParams: its tiles come
+// through the block table, its columns are tokens times the query heads of a
+// K / V head, and a unit's keys may be a chunk of the sequence's, whose fp32
+// sums the reduction adds in chunk order (sigmoid attention has no row
+// normalisation, so O is the plain sum over the chunks).
+#include "fwd_kernel.h"
+#include "launch.h"
+
+namespace sigattn {
+namespace {
+
+// D = 128: eight waves, one workgroup per CU; below, four, three and four per
+// CU (fwd_kernel.h).
+constexpr int waves_of(int D) { return D == 128 ? 8 : 4; }
+
+template <typename T, int D> void fwd_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
+  constexpr int NWV = waves_of(D);
+  const dim3 grid((unsigned)(units + p.ngap[0])), block(64 * NWV);
+  if (causal) {
+    if (p.score_mod) fwd_mfma_kernel<T, D, NWV, 1, 1, true, true, PagedParams><<<grid, block, 0, st>>>(p);
+    else fwd_mfma_kernel<T, D, NWV, 1, 1, true, false, PagedParams><<<grid, block, 0, st>>>(p);
+  } else {
+    if (p.score_mod) fwd_mfma_kernel<T, D, NWV, 1, 1, false, true, PagedParams><<<grid, block, 0, st>>>(p);
+    else fwd_mfma_kernel<T, D, NWV, 1, 1, false, false, PagedParams><<<grid, block, 0, st>>>(p);
+  }
+}
+
+// Output rows (token, query head) of cut sequences: the sum of the chunks'
+// partials in chunk order.  D / 4 threads add one row, four columns each; the
+// 256 / (D / 4) groups of a workgroup take rows of their own (many rows), or
+// (ROWS = false) every group a share of one row's chunks, added in group order
+// (few rows of many chunks).
+struct ReduceArgs {
+  PagedParams p;
+  const float *ws[2];   // blocks of more than / up to `cols` columns
+  const int2 *cut[2];   // nullptr: no sequence was cut there
+  int block[2], cols;
+};
+
+template <typename T, int D, bool ROWS>
+__global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
+  constexpr int CG = D / 4, NG = 256 / CG;
+  __shared__ f32x4 part[ROWS ? 1 : NG][CG];
+  const PagedParams &p = a.p;
+  const int c = threadIdx.x % CG, g = threadIdx.x / CG;
+  const int64_t item = ROWS ? (int64_t)blockIdx.x * NG + g : (int64_t)blockIdx.x;
+  const int64_t r = item / p.H;
+  const int h = (int)(item - r * p.H);
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  int nck = 0;
+  if (r < p.rows_q) {
+    int lo = 0, hi = p.B - 1;  // the last sequence that begins at or before row r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (packed_first(p.cu_q, p.rows_q, mid) <= r) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t tok = r - packed_first(p.cu_q, p.rows_q, lo);
+    const int Lq = p.len_q(lo), few = Lq * p.G <= a.cols;
+    if (tok < Lq && a.cut[few] != nullptr) {
+      const int2 cut = a.cut[few][lo];
+      nck = cut.y;
+      if (nck > 1) {
+        const int block = a.block[few], hk = h / p.G, col = (int)tok * p.G + h - hk * p.G;
+        const int nqb = (Lq * p.G + block - 1) / block, qb = col / block;
+        const int64_t unit = (cut.x + (int64_t)(nqb - 1 - qb) * nck) * p.Hkv + hk;
+        const float *src = a.ws[few] + (unit * block + col - qb * block) * D + 4 * c;
+        const int64_t step = (int64_t)p.Hkv * block * D;
+#pragma unroll 8
+        for (int j = ROWS ? 0 : g; j < nck; j += ROWS ? 1 : NG) v += *(const f32x4 *)(src + j * step);
+      }
+    }
+  }
+  if constexpr (!ROWS) {
+    if (nck <= 1) return;  // the whole workgroup
+    part[g][c] = v;
+    __syncthreads();
+    if (g != 0) return;
+#pragma unroll
+    for (int x = 1; x < NG; ++x) v += part[x][c];
+  }
+  if (nck > 1 && 4 * c < p.dmem)
+    *(u32x2 *)((uint16_t *)p.out + (r * p.H + h) * p.dmem + 4 * c) =
+        (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
+}
+
+template <typename T, int D> void reduce_t(const ReduceArgs &a, hipStream_t st) {
+  constexpr int NG = 256 / (D / 4);
+  const int64_t rows = a.p.rows_q * a.p.H;
+  // One row per workgroup where that is few workgroups a CU.
+  if (rows <= 8 * (int64_t)a.p.ncu) paged_reduce_kernel<T, D, false><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
+  else paged_reduce_kernel<T, D, true><<<dim3((unsigned)((rows + NG - 1) / NG)), dim3(256), 0, st>>>(a);
+}
+
+template <class F> void by_type(int dtype, int D, F &&f) {
+  const auto d = [&](auto *t) {
+    if (D == 128) f(t, std::integral_constant<int, 128>{});
+    else if (D == 64) f(t, std::integral_constant<int, 64>{});
+    else f(t, std::integral_constant<int, 32>{});
+  };
+  if (dtype == kBF16) d((__bf16 *)nullptr);
+  else d((_Float16 *)nullptr);
+}
+
+}  // namespace
+
+int paged_block(int D) { return 32 * waves_of(D); }
+
+void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st) {
+  by_type(dtype, D, [&](auto *t, auto d) {
+    fwd_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(p, units, causal, st);
+  });
+}
+
+void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int dtype, int D, hipStream_t st) {
+  ReduceArgs a{};
+  a.p = fwd;
+  a.ws[0] = fwd.ws, a.ws[1] = decode.ws;
+  a.cut[0] = fwd.split_units > 0 ? fwd.cut : nullptr;
+  a.cut[1] = decode.split_units > 0 ? decode.cut : nullptr;
+  a.block[0] = paged_block(D), a.block[1] = 32, a.cols = decode.cols_hi;
+  by_type(dtype, D, [&](auto *t, auto d) {
+    reduce_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(a, st);
+  });
+}
+
+}  // namespace sigattn

@@ -27,6 +27,7 @@ LIB_PATH = PKG_DIR / "libsigattn.so"
 BUILD_DIR = ROOT / "_build"
 
 SOURCES = ["fwd.hip", "bwd.hip", "decode.hip", "f32.hip", "generic.hip", "bias.hip", "paged.hip",
+           "paged_fwd.hip", "paged_decode.hip",
            "capi.cpp", "paged_capi.cpp"]
 SOURCE_FLAGS = {"bias.hip": ["-ffp-contract=off"]}  # see the file
 ARCH = "gfx950"
