@@ -57,12 +57,24 @@ def test_check(kw, rc):
 
 
 def test_workspace_policy_takes_whole_groups(monkeypatch):
-    """The Python layer's two-pass workspace is a whole number of groups."""
+    """The Python layer's two-pass workspace: the whole problem's within the
+    limit, else passes of whole K / V heads of one size that fill the GPU."""
     lib = _capi.load_library()
     p = _problem(D=128, Tq=4096, Tk=4096, H=24, kv_heads=4, rows_q=8192, rows_k=8192)
     full = lib.sigattn_bwd_workspace_bytes(ctypes.byref(p))
     per_head = full // 24
     monkeypatch.setattr(_capi, "_compute_units", lambda dev: 8)
-    for heads, want in ((5, 0), (6, 6), (11, 6), (12, 12), (23, 18), (24, 24)):
-        monkeypatch.setattr(_capi, "bwd_workspace_limit", lambda: heads * per_head)
+    for heads, want in ((5, 0), (6, 6), (11, 6), (12, 12), (17, 12), (18, 12), (23, 12), (24, 24)):
+        monkeypatch.setattr(_capi, "bwd_workspace_limit", lambda grouped: heads * per_head)
         assert _capi.bwd_workspace_bytes(lib, p, torch.device("cuda:0")) == want * per_head
+    monkeypatch.setattr(_capi, "_compute_units", lambda dev: 64)  # 64 key blocks a K / V head
+    for heads, want in ((6, 0), (12, 12)):
+        monkeypatch.setattr(_capi, "bwd_workspace_limit", lambda grouped: heads * per_head)
+        assert _capi.bwd_workspace_bytes(lib, p, torch.device("cuda:0")) == want * per_head
+
+
+def test_workspace_limit(monkeypatch):
+    monkeypatch.delenv("SIGATTN_BWD_WORKSPACE_MB", raising=False)
+    assert _capi.bwd_workspace_limit() == 2048 << 20 and _capi.bwd_workspace_limit(True) == 8192 << 20
+    monkeypatch.setenv("SIGATTN_BWD_WORKSPACE_MB", "64")
+    assert _capi.bwd_workspace_limit() == _capi.bwd_workspace_limit(True) == 64 << 20

@@ -258,3 +258,49 @@ def test_compiled_forward_and_backward():
     got = dict(zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, (a, b, c), do))))
     for x in got:
         assert torch.equal(got[x], want[x])
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads", [(6, 2), (10, 2), (16, 1)], ids=lambda h: f"{h[0]}x{h[1]}")
+def test_head_split_parts(heads, D, causal):
+    """Few K / V heads: their groups run in parts whose sums are added; rows
+    outside every sequence stay zero, and the parts' workspace may hold anything."""
+    cu = offsets([140, 0, 300], first=3)
+    q, k, v, do = make(cu[-1] + 7, cu[-1] + 7, *heads, D, torch.bfloat16, 16)
+    junk = torch.full((64 << 20,), float("nan"), device="cuda")
+    del junk  # the allocator hands it out again
+    got = check(q, k, v, do, cu, cu, causal)
+    for x in got.values():
+        assert not x[:3].any() and not x[cu[-1]:].any()
+    same = run(q, k, v, do, cu, cu, is_causal=causal)
+    for x in got:
+        assert torch.equal(got[x], same[x])
+
+
+def test_head_split_asks_for_its_workspace():
+    import ctypes
+    cut = torch.tensor([0, 256, 400], dtype=torch.int32, device="cuda")
+    lib = _capi.load_library()
+    for D, entry in ((64, "split"), (128, "ws")):
+        q, k, v, do = make(400, 400, 8, 2, D, torch.float16, 17)
+        scale, bias = torch.tensor(0.1, device="cuda"), torch.zeros(2, device="cuda")
+        pr = _capi._problem(q, k, v, bias, None, scale, None, None, True, packed=(cut, cut, 256, 256))
+        size = lib.sigattn_bwd_split_workspace_bytes if entry == "split" else lib.sigattn_bwd_workspace_bytes
+        call = lib.sigattn_bwd_split if entry == "split" else lib.sigattn_bwd_ws
+        n = size(ctypes.byref(pr))
+        parts = 4 * 2 * 400 * 2 * D * 4  # a head each
+        assert n > parts if entry == "ws" else n == parts
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        g = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+        args = (ctypes.byref(pr), do.data_ptr(), *(t.data_ptr() for t in g), ws.data_ptr())
+        stream = torch.cuda.current_stream().cuda_stream
+        want = packed(q, k, v, do, cut.tolist(), cut.tolist(), True, bias=0.0, scale=float(scale))
+        for nbytes in (n, n - 16):
+            rc = call(*args, nbytes, stream)
+            if entry == "split" and nbytes < n:
+                assert rc == -10
+                continue
+            assert rc == 0  # ws: without room for the parts the groups run whole
+            for x, t in zip(("dq", "dk", "dv"), g):
+                assert_within(t, want[x], x)

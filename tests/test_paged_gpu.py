@@ -491,3 +491,49 @@ def test_serving_equals_the_prompt_at_once(D, dtype):
             val[at[b]:at[b + 1], h], err[at[b]:at[b + 1], h] = o
     assert_within(got, (val, err), "served")
     assert_within(whole, (val, err), "at once")
+
+
+@pytest.mark.parametrize("B", [3, 64, 65, 200])
+def test_cuts_of_ragged_batches(B):
+    """Long and short contexts in one batch, with and without the candidates of
+    small batches: every unit finds its chunk, every row its sums."""
+    r = random.Random(B)
+    top = {3: 6000, 64: 1500, 65: 1500, 200: 700}[B]
+    ctx = [r.choice((0, 3, r.randint(0, 300), r.randint(0, top))) for _ in range(B)]
+    ctx[r.randrange(B)] = 2 * top
+    check(ctx, [1] * B, 16, 4, 2, 64, torch.bfloat16)
+    new = [r.choice((1, 1, 0, 5, 40)) for _ in range(B)]
+    check([min(c, 1500) for c in ctx], new, 32, 4, 2, 128, torch.bfloat16)
+
+
+def test_workspace_of_other_calls_does_not_matter():
+    """The same with a workspace full of NaN, and without one (nothing is cut)."""
+    import ctypes
+
+    from triton_sigmoid import _capi
+    q, kc, vc, table, lens, cu, rows = make([3000, 10, 900, 500], [1, 1, 50, 33], 16, 8, 2, 128, torch.bfloat16)
+    new = [1, 1, 50, 33]
+    want = ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 50, is_causal=True)
+    lib = _capi.load_library()
+    p = _capi.SigattnPagedProblem()
+    p.abi_version, p.dtype = _capi.ABI_VERSION, _capi.BF16
+    p.B, p.H, p.kv_heads, p.D, p.rows_q, p.max_seqlen_q = 4, 8, 2, 128, q.shape[0], 50
+    p.num_pages, p.page_size, p.max_pages = kc.shape[0], 16, table.shape[1]
+    p.q_stride_t, p.q_stride_h = 1024, 128
+    p.k_stride_p, p.k_stride_t, p.k_stride_h = kc.stride()[:3]
+    p.table_stride = table.stride(0)
+    p.q, p.k_cache, p.v_cache = q.data_ptr(), kc.data_ptr(), vc.data_ptr()
+    p.block_table, p.seq_lens_k, p.cu_seqlens_q = table.data_ptr(), lens.data_ptr(), cu.data_ptr()
+    p.scale, p.causal = 128 ** -0.5, 1
+    n = lib.sigattn_paged_fwd_workspace_bytes(ctypes.byref(p))
+    assert n > 0
+    ws = torch.full((n // 4 + 4,), float("nan"), device="cuda")
+    out = torch.full_like(q, float("nan"))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), ws.data_ptr(), n, stream) == 0
+    assert torch.equal(out, want)
+    assert lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), ws.data_ptr(), n - 1, stream) == -10
+    assert lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), ws.data_ptr() + 4, n, stream) == -10
+    out.fill_(float("nan"))
+    assert lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), None, 0, stream) == 0
+    assert_within(out, reference(q, rows, new, True), "uncut")

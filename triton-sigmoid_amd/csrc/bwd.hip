@@ -312,11 +312,58 @@ template <bool GROUPED> struct HeadStream {
   }
 };
 
+// A lane's row of fp32 dK (t = 0) or dV (t = 1) of a head-split item, times `f`.
+template <int NDB>
+__device__ __forceinline__ void store_part(const KParams &p, int part, int b, int key, int h, const f32x16 (&acc)[NDB],
+                                           int t, float f, int hi, bool half) {
+  float *row = p.part_row(part, t, packed_first(p.cu_k, p.rows_k, b) + key, h);
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (half && g >= 2) break;  // columns 16..31: not in the tensor
+      const f32x16 &a = acc[db];
+      *(f32x4 *)(row + db * 32 + 8 * g + 4 * hi) = (f32x4){a[4 * g] * f, a[4 * g + 1] * f, a[4 * g + 2] * f,
+                                                           a[4 * g + 3] * f};
+    }
+}
+
+// dK and dV of head-split items: the sum of the parts' fp32 rows in their
+// order, rounded once.  Rows that no sequence covers are left to the dQ launch,
+// which zeroes them.  Eight elements a thread; bound by memory.
+template <typename T> __global__ __launch_bounds__(256) void add_parts_kernel(const KParams p) {
+  const int64_t per_row = (int64_t)p.H * p.dmem / 8, n = p.rows_k * per_row;
+  const int64_t tensor = p.rows_k * p.H * p.dmem;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per_row, c = 8 * (i - row * per_row);
+    int lo = 0, hi = p.B - 1;  // the last sequence that begins at or before the row
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (packed_first(p.cu_k, p.rows_k, mid) <= row) lo = mid;
+      else hi = mid - 1;
+    }
+    if (row - packed_first(p.cu_k, p.rows_k, lo) >= p.len_k(lo) || row < packed_first(p.cu_k, p.rows_k, lo)) continue;
+    const int h = (int)(c / p.dmem), d = (int)(c - (int64_t)h * p.dmem);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 v[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      const float *src = p.kv_part + t * tensor + row * p.H * p.dmem + c;
+      for (int s = 0; s < p.qsplit; ++s, src += 2 * tensor) {
+        v[0] += *(const f32x4 *)src;
+        v[1] += *(const f32x4 *)(src + 4);
+      }
+      *(u32x4 *)((uint16_t *)(t == 0 ? p.dk : p.dv) + row * p.sk_t + h * p.sk_h + d) =
+          (u32x4){Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[0].z, v[0].w), Elem<T>::pack(v[1].x, v[1].y),
+                  Elem<T>::pack(v[1].z, v[1].w)};
+    }
+  }
+}
+
 template <int D> struct DkdvLds {
   uint16_t q[4][64 * D], o[4][64 * D];
 };
 template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPED>
-__device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, DkdvLds<D> &lds) {
+__device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int id, DkdvLds<D> &lds) {
   static_assert(!(DSOUT && GROUPED), "two-pass backward of grouped heads: D = 128 only");
   constexpr int BN = 128;                 // keys per workgroup (32 per wave)
   constexpr int BMQ = 64;                 // queries per LDS tile (two 32-query blocks)
@@ -335,6 +382,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   auto &sQ = lds.q;
   auto &sO = lds.o;
 
+  const int nparts = GROUPED && p.qsplit > 1 ? p.qsplit : 1, wg = GROUPED ? id / nparts : id;
+  const int part = GROUPED ? id - wg * nparts : 0;
   int b, h, kblk;
   int ritem = 0, rchunk = 0;  // range split: the item and this workgroup's chunk of its queries
   if (!CAUSAL && !DSOUT && p.rsplit > 1) {
@@ -371,7 +420,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
   const int l32 = lane & 31, hi = lane >> 5;
   const int k0 = kblk * BN, kw = k0 + w * 32, my_k = kw + l32;
 
-  const int hq = GROUPED ? p.first_q_head(h) : h;
+  const int head0 = GROUPED ? p.part_head(part) : 0, nheads = GROUPED ? p.part_head(part + 1) - head0 : 1;
+  const int hq = GROUPED ? p.first_q_head(h) + head0 : h;
   const int64_t qoff = p.q_base(b, hq);
   const int64_t koff = p.k_base(b, h);
   const uint16_t *Qb = (const uint16_t *)p.q + qoff;
@@ -391,7 +441,7 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
     mend = min(Lq, split_tile(rchunk + 1, p.rsplit, ntq) * BMQ);
   }
   const int ntiles1 = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;  // of one query head
-  const int ntiles = GROUPED ? p.qgroup * ntiles1 : ntiles1;
+  const int ntiles = GROUPED ? nheads * ntiles1 : ntiles1;
   const int NB = 2 * ntiles;
   HeadStream<GROUPED> hs(2 * ntiles1);
 
@@ -651,6 +701,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const KParams &p, const int wg, Dk
           p.rs_part + (int64_t)ritem * p.rsplit * (2 * BN * D), p.rs_cnt + ritem, rchunk, p.rsplit, w, lane))
     return;
 
+  if (GROUPED && nparts > 1) {
+    if (kok) store_part<NDB>(p, part, b, my_k, h, dka, 0, scale, hi, half), store_part<NDB>(p, part, b, my_k, h, dva, 1, 1.0f, hi, half);
+    return;
+  }
   if (my_k < p.k_rows_out(Lk)) {
     uint16_t *kr = dKb + (int64_t)my_k * p.sk_t;
     uint16_t *vr = dVb + (int64_t)my_k * p.sk_t;
@@ -763,18 +817,21 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
   // the grid has half as many workgroup starts.  A dense non-causal grid
   // that would not fill the GPU paired runs one key block per workgroup
   // (grid = nblk per (batch, head)).
+  const int nparts = GROUPED && p.qsplit > 1 ? p.qsplit : 1, wg = (int)blockIdx.x / nparts;
+  const int part = (int)blockIdx.x - wg * nparts;
   int b, h, kblk0, nitems;
   if (p.ragged() && p.B <= 64) {
     const auto lq = [&](int i) SIGATTN_INLINE { return p.len_q(i); };
     const auto lk = [&](int i) SIGATTN_INLINE { return p.len_k(i); };
-    const WorkItem it = CAUSAL ? WorkOrder::by_level(blockIdx.x, p.B, p.H, lk, BN, p.nblk, false, p.ncu, 1)
-                               : WorkOrder::by_stream(blockIdx.x, p.B, p.H, lk, BN, p.nblk, lq);
+    const WorkItem it = CAUSAL ? WorkOrder::by_level(wg, p.B, p.H, lk, BN, p.nblk, false, p.ncu, 1)
+                               : WorkOrder::by_stream(wg, p.B, p.H, lk, BN, p.nblk, lq);
     b = it.b, h = it.h, kblk0 = it.blk, nitems = 1;
   } else {
     const int BH = p.B * p.H;
     int bh;
-    dense_item(blockIdx.x, BH, (int)(gridDim.x / BH), !CAUSAL || kDkdvGrouped, bh, kblk0);
-    const bool paired = (int)(gridDim.x / BH) < p.nblk;
+    const int nper = (int)(gridDim.x / nparts / BH);
+    dense_item(wg, BH, nper, !CAUSAL || kDkdvGrouped, bh, kblk0);
+    const bool paired = nper < p.nblk;
     nitems = paired && p.nblk - 1 - kblk0 > kblk0 ? 2 : 1;
     b = bh / p.H, h = bh % p.H;
   }
@@ -801,7 +858,8 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
     const int l32 = lane & 31, hi = lane >> 5;
     const int k0 = kblk * BN, kw = k0 + pair * 32, my_k = kw + l32;
 
-    const int hq = GROUPED ? p.first_q_head(h) : h;
+    const int head0 = GROUPED ? p.part_head(part) : 0, nheads = GROUPED ? p.part_head(part + 1) - head0 : 1;
+    const int hq = GROUPED ? p.first_q_head(h) + head0 : h;
     const int64_t qoff = p.q_base(b, hq);
     const int64_t koff = p.k_base(b, h);
     const uint16_t *Qb = (const uint16_t *)p.q + qoff;
@@ -811,7 +869,7 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
     const int mstart = CAUSAL ? (k0 / BMQ) * BMQ : 0;
     const int mend = (k0 >= Lk) ? mstart : Lq;
     const int ntiles1 = mend > mstart ? (mend - mstart + BMQ - 1) / BMQ : 0;  // of one query head
-    const int ntiles = GROUPED ? p.qgroup * ntiles1 : ntiles1;
+    const int ntiles = GROUPED ? nheads * ntiles1 : ntiles1;
     const int NB = 2 * ntiles;
     HeadStream<GROUPED> hs(2 * ntiles1);
 
@@ -985,7 +1043,9 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
         if (r0 + 7 < NB + 2) region(r0 + 7, std::integral_constant<int, 7>{});
       }
 
-      if (my_k < kmax) {
+      if (GROUPED && nparts > 1) {
+        if (kok) store_part<NDB>(p, part, b, my_k, h, dva, 1, 1.0f, hi, false);
+      } else if (my_k < kmax) {
         uint16_t *vr = (uint16_t *)p.dv + koff + (int64_t)my_k * p.sk_t;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
@@ -1106,7 +1166,9 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
         if (r0 + 7 < NB + 2) region(r0 + 7, std::integral_constant<int, 7>{});
       }
 
-      if (my_k < kmax) {
+      if (GROUPED && nparts > 1) {
+        if (kok) store_part<NDB>(p, part, b, my_k, h, dka, 0, scale, hi, false);
+      } else if (my_k < kmax) {
         uint16_t *kr = (uint16_t *)p.dk + koff + (int64_t)my_k * p.sk_t;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
@@ -1421,6 +1483,7 @@ static void bwd_dkdv_t(const KParams &kp, bool causal, bool sm, hipStream_t st) 
         const bool one_block = !causal && paired < device_compute_units();
         grid = dim3((unsigned)(one_block ? (int64_t)p.nblk * p.B * p.H : paired));
       }
+      if (p.qgroup > 1 && p.qsplit > 1) grid.x *= (unsigned)p.qsplit;
       by_flags(causal, sm, p.qgroup > 1, [&](auto c, auto m, auto g) {
         bwd_dkdv_pair_kernel<T, c.value, m.value, DSOUT, g.value><<<grid, 512, 0, st>>>(p);
       });
@@ -1428,6 +1491,7 @@ static void bwd_dkdv_t(const KParams &kp, bool causal, bool sm, hipStream_t st) 
     }
     // Range split (dense non-causal recompute backward): rsplit workgroups per item.
     if (!causal && !DSOUT && p.rsplit > 1) grid.x *= (unsigned)p.rsplit;
+    if (p.qgroup > 1 && p.qsplit > 1) grid.x *= (unsigned)p.qsplit;
     by_flags(causal, sm, p.qgroup > 1, [&](auto c, auto m, auto g) {
       // The two-pass backward of grouped heads is D = 128's alone.
       if constexpr (!(DSOUT && g.value)) bwd_dkdv_kernel<T, D, c.value, m.value, DSOUT, g.value><<<grid, 256, 0, st>>>(p);
@@ -1519,9 +1583,13 @@ void launch_bwd_dkdv_mfma(const KParams &p, int dtype, int D, bool causal, bool 
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int DD = decltype(d)::value;
     if constexpr (DD > 32) {  // no two-pass form below
-      if (dsout) return bwd_dkdv_t<T, DD, true>(p, causal, sm, st);
+      if (dsout) bwd_dkdv_t<T, DD, true>(p, causal, sm, st);
     }
-    bwd_dkdv_t<T, DD, false>(p, causal, sm, st);
+    if (!dsout) bwd_dkdv_t<T, DD, false>(p, causal, sm, st);
+    if (p.qgroup > 1 && p.qsplit > 1) {
+      const int64_t n = (p.rows_k * p.H * p.dmem / 8 + 255) / 256;
+      add_parts_kernel<T><<<dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st>>>(p);
+    }
   });
 }
 

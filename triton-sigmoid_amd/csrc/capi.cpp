@@ -411,6 +411,37 @@ BwdSplit bwd_range_split(const sigattn_problem *p, bool mfma) {
   return s;
 }
 
+// Head split of grouped dK/dV items (KParams::qsplit).  Items are K / V heads
+// times key blocks, a group's queries long each: with few of them the GPU
+// waits for the last.  The fewest parts, up to a head each, that make two
+// workgroups per CU of them; the parts' fp32 sums are written and read again.
+// Forward and backward, us, by workgroups per CU aimed at, none / 1 / 2 / 3 / 6:
+// fp16 B=8 T=2048 lengths 512..2048 D=64 H=16 Hkv=2 443 / 264 / 263 / - / 262,
+// Hkv=8 236 / 236 / 236 / - / 261; bf16 B=9 T=3001 lengths 67..3001 D=128 H=12
+// Hkv=4 664 / 686 / 682 / 771 / -, Hkv=2 - / 793 / 695 / 707 / -, B=2 Hkv=4 - /
+// 333 / 305 / 306 / -.
+constexpr int64_t kHeadSplitPerCu = 2;
+struct HeadSplit {
+  int n = 1;
+  int64_t bytes = 0;
+};
+
+HeadSplit head_split(const sigattn_problem *p, bool mfma) {
+  HeadSplit s;
+  const int64_t G = head_group(p), cus = sigattn::device_compute_units();
+  if (!mfma || G <= 1 || p->cu_seqlens_k == nullptr || p->Tq <= 0 || p->Tk <= 0 || cus <= 0) return s;
+  // Key blocks: whole ones of all rows, and a part of one for each sequence
+  // (half of which are counted).
+  const int64_t rows = p->rows_k < p->B * p->Tk ? p->rows_k : p->B * p->Tk;
+  const int64_t items = (rows / 128 + (p->B + 1) / 2) * kv_heads(p);
+  int64_t n = items > 0 ? cdiv(kHeadSplitPerCu * cus, items) : 1;
+  if (n > G) n = G;
+  if (n < 2) return s;
+  s.n = (int)n;
+  s.bytes = n * 2 * p->rows_k * kv_heads(p) * p->D * (int64_t)sizeof(float);
+  return s;
+}
+
 // Sets k's range-split fields for `r` over the workspace at `ws`; the caller
 // clears the counters (launch_rs_clear) before k's kernel runs.
 void use_range_split(KParams &k, const RangeSplit &r, void *ws) {
@@ -447,7 +478,7 @@ KParams head_slice(const KParams &k, int64_t h0, int64_t nh, int64_t esize) {
 }
 
 // The dK/dV kernels' view of a problem: its items are K / V heads, each of
-// which streams the queries of its group (KParams::qgroup).
+// which streams the queries of its group (KParams::qgroup), in k.qsplit parts.
 KParams kv_items(const KParams &k) {
   KParams s = k;
   if (k.hgroup > 1) s.H = k.H / k.hgroup, s.qgroup = k.hgroup, s.hgroup = 1;
@@ -703,7 +734,8 @@ int sigattn_fwd_noalloc(const sigattn_problem *p, void *out, void *stream) {
 enum BwdParts { kBwdAll, kBwdDq, kBwdDkdv };
 
 static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *dk, void *dv,
-                    void *workspace, size_t workspace_bytes, void *stream, BwdParts parts) {
+                    void *workspace, size_t workspace_bytes, void *stream, BwdParts parts, int qsplit = 1,
+                    float *kv_part = nullptr) {
   const int rc = sigattn_check(p);
   if (rc != SIGATTN_OK) return rc;
   if (workspace != nullptr && !aligned16(workspace)) return SIGATTN_ERR_WORKSPACE;
@@ -728,11 +760,21 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   // Two-pass backward when a workspace holds the dS of at least one head.
   // The halves (kBwdDq, kBwdDkdv) need the whole problem's dS at once: the
   // dQ half reads what a dK/dV half with the same workspace stored.
+  // Behind the whole problem's dS, the workspace may hold the parts of a head
+  // split.
   int64_t heads_per_pass = 0;
+  HeadSplit hs;
   if (workspace != nullptr && mfma && two_pass_head(p) && p->Tq > 0 && p->Tk > 0) {
     heads_per_pass = (int64_t)workspace_bytes / ds_bytes_per_head(p);
     if (heads_per_pass > p->H) heads_per_pass = p->H;
     heads_per_pass -= heads_per_pass % head_group(p);  // whole groups: dK / dV are sums over them
+    // Passes of one size: a last one of few K / V heads would not fill the GPU.
+    if (heads_per_pass > 0 && head_group(p) > 1) {
+      const int64_t groups = kv_heads(p), per = heads_per_pass / head_group(p);
+      heads_per_pass = cdiv(groups, cdiv(groups, per)) * head_group(p);
+    }
+    hs = head_split(p, mfma);
+    if (heads_per_pass < p->H || (int64_t)workspace_bytes < ds_bytes_per_head(p) * p->H + hs.bytes) hs = HeadSplit{};
   }
   if (parts != kBwdAll && workspace != nullptr) {
     if (!mfma || !two_pass_head(p)) return SIGATTN_ERR_WORKSPACE;  // no two-pass kernels for this problem
@@ -751,6 +793,8 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   k.dq = dq;
   k.dk = dk;
   k.dv = dv;
+  k.qsplit = qsplit;
+  k.kv_part = kv_part;
   const hipStream_t st = (hipStream_t)stream;
   const bool causal = p->causal != 0, sm = p->score_mod != nullptr;
   const int dt = p->dtype, D = mfma || f32mma ? mfma_head_dim(p) : (int)p->D;
@@ -767,6 +811,8 @@ static int bwd_impl(const sigattn_problem *p, const void *dout, void *dq, void *
   if (!dq_gaps) sigattn::launch_zero_gaps(gq, gk, dt == SIGATTN_F32 ? 4 : 2, st);
   if (twopass) {
     k.ds = (uint16_t *)workspace;
+    k.qsplit = hs.n;
+    k.kv_part = (float *)((char *)workspace + ds_bytes_per_head(p) * p->H);
     k.ds_nqb = (int)cdiv(p->Tq, 32);
     k.ds_nkb = (int)cdiv(p->Tk, 32);
     // Per head group: dK/dV (storing dS), then dQ from dS, on one stream, so
@@ -817,7 +863,7 @@ size_t sigattn_bwd_workspace_bytes(const sigattn_problem *p) {
   if (sigattn_check(p) != SIGATTN_OK || p->B == 0 || p->H == 0 || p->Tq == 0 || p->Tk == 0) return 0;
   const void *none[1] = {nullptr};
   if (!use_mfma(p, none, 0) || !two_pass_head(p)) return 0;
-  return (size_t)(ds_bytes_per_head(p) * p->H);
+  return (size_t)(ds_bytes_per_head(p) * p->H + head_split(p, true).bytes);
 }
 
 int sigattn_bwd_ws(const sigattn_problem *p, const void *dout, void *dq, void *dk, void *dv,
@@ -833,7 +879,10 @@ int sigattn_bwd(const sigattn_problem *p, const void *dout, void *dq, void *dk, 
 size_t sigattn_bwd_split_workspace_bytes(const sigattn_problem *p) {
   if (sigattn_check(p) != SIGATTN_OK || p->B == 0 || p->H == 0) return 0;
   const void *none[1] = {nullptr};
-  return (size_t)bwd_range_split(p, use_mfma(p, none, 0)).bytes;
+  const bool mfma = use_mfma(p, none, 0);
+  // At D = 128 the parts go with the dS of sigattn_bwd_ws.
+  if (head_group(p) > 1) return p->D == 128 ? 0 : (size_t)head_split(p, mfma).bytes;
+  return (size_t)bwd_range_split(p, mfma).bytes;
 }
 
 int sigattn_bwd_split(const sigattn_problem *p, const void *dout, void *dq, void *dk, void *dv,
@@ -847,6 +896,11 @@ int sigattn_bwd_split(const sigattn_problem *p, const void *dout, void *dq, void
   if (want_kv && (dk == nullptr || dv == nullptr)) return SIGATTN_ERR_NULL_ARG;
   const BwdParts parts = want_dq && want_kv ? kBwdAll : (want_dq ? kBwdDq : kBwdDkdv);
   const void *ptrs[7] = {p->q, p->k, p->v, dout, dq, dk, dv};
+  if (head_group(p) > 1 && p->D != 128 && workspace != nullptr) {
+    const HeadSplit hs = head_split(p, use_mfma(p, ptrs, 7));
+    if (hs.n > 1 && ((size_t)hs.bytes > workspace_bytes || !aligned16(workspace))) return SIGATTN_ERR_WORKSPACE;
+    return bwd_impl(p, dout, dq, dk, dv, nullptr, 0, stream, parts, hs.n, (float *)workspace);
+  }
   const BwdSplit bs = workspace != nullptr ? bwd_range_split(p, use_mfma(p, ptrs, 7)) : BwdSplit{};
   if (bs.bytes == 0) return bwd_impl(p, dout, dq, dk, dv, nullptr, 0, stream, parts);
   if ((size_t)bs.bytes > workspace_bytes || !aligned16(workspace)) return SIGATTN_ERR_WORKSPACE;

@@ -139,6 +139,12 @@ struct KParams {
   // K / V heads and qgroup = the query heads of each, whose queries an item
   // streams one head after another (hgroup is then 1).
   int hgroup, qgroup;
+  // Head split of grouped dK/dV items (qsplit <= 1: off): an item runs as
+  // qsplit workgroups, each with as even a share of its query heads, whose
+  // fp32 dK and dV go to kv_part: [qsplit][2][rows_k][H][dmem], added in that
+  // order by a kernel of their own (packed layouts).
+  int qsplit;
+  float *kv_part;
 
   // Valid query / key rows of batch b.
   __device__ __forceinline__ int len_q(int b) const {
@@ -159,6 +165,12 @@ struct KParams {
   // First query head of the dK/dV item head h, and the query heads it streams.
   __device__ __forceinline__ int first_q_head(int h) const { return qgroup > 1 ? h * qgroup : h; }
   __device__ __forceinline__ int q_heads() const { return qgroup > 1 ? qgroup : 1; }
+  // First of an item's query heads that part `i` of qsplit takes.
+  __device__ __forceinline__ int part_head(int i) const { return qsplit > 1 ? i * qgroup / qsplit : i * qgroup; }
+  // Row `row` (of the tensor) of part i's dK (t = 0) or dV (t = 1).
+  __device__ __forceinline__ float *part_row(int i, int t, int64_t row, int h) const {
+    return kv_part + (((2 * i + t) * rows_k + row) * H + h) * dmem;
+  }
   // score_mod entry of key 0 of batch b.
   __device__ __forceinline__ int64_t mod_base(int b) const {
     return cu_k != nullptr ? packed_first(cu_k, rows_k, b) : (int64_t)b * Tk;

@@ -15,8 +15,8 @@ namespace sigattn {
 // of the keys); the columns of a sequence are its tokens times the G query
 // heads of a K / V head, column c = token c / G of head c % G.  A kernel takes
 // the sequences of more than cols_lo and at most cols_hi columns.  split_units
-// > 0: sequences are cut into chunks of at least min_chunk keys, so that there
-// are about that many units; a unit of a cut sequence leaves its fp32 sums in
+// > 0: sequences are cut into chunks of at least min_chunk keys, total_units
+// (split_units more than the uncut batch can have) at most; a unit of a cut sequence leaves its fp32 sums in
 // `ws`, and cut[b] where they begin, for the reduction.
 struct PagedParams : KParams {
   static constexpr bool kPaged = true;
@@ -28,7 +28,7 @@ struct PagedParams : KParams {
   float fscale, fbias;
   int own_bias;          // 0: the bias is -log(keys)
   int cols_lo, cols_hi;
-  int split_units, min_chunk;
+  int split_units, total_units, min_chunk;
   int2 *cut;             // [B] (first unit / Hkv, chunks)
 
   __device__ __forceinline__ int keys(int b) const { return clamp_len(lens, b, Tk); }
@@ -41,10 +41,10 @@ struct PagedParams : KParams {
 };
 
 struct PagedUnit {
-  int b, hk, qb;      // sequence, K / V head, column block
-  int Lq, Lk;         // its tokens and keys
-  int k0, k1;         // keys of the chunk
-  int nck = 0;        // chunks of the sequence (0: no such unit)
+  int b = 0, hk = 0, qb = 0;  // sequence, K / V head, column block
+  int Lq = 0, Lk = 0;         // its tokens and keys
+  int k0 = 0, k1 = 0;         // keys of the chunk
+  int nck = 0;                // chunks of the sequence (0: no such unit)
 };
 
 // Sum over the wave's lanes, in a fixed order.
@@ -59,22 +59,40 @@ __device__ __forceinline__ float wave_sum(float x) {
 // (under the causal mask longest) first, chunks, K / V heads fastest.  Every wave computes it
 // alike, 64 sequences at a time.  Chunks: with work W = sum of blocks times
 // keys, C = W Hkv / split_units keys (min_chunk at least), ceil(keys / C) chunks
-// of equal length: at most split_units + the units of an uncut batch.
+// of equal length: at most split_units + the units of an uncut batch.  Batches
+// of up to 64 sequences take a shorter C where that many units allow it.
 __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
   const int lane = __lane_id();
+  const int Lq0 = lane < p.B ? p.len_q(lane) : 0, Lk0 = lane < p.B ? p.keys(lane) : 0;
   int C = 1 << 30;  // more than any length
   if (p.split_units > 0) {
-    float work = 0.0f;
-    for (int b = lane; b < p.B; b += 64) work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
-    const float c = wave_sum(work) * (float)p.Hkv / (float)p.split_units;
-    C = __builtin_amdgcn_readfirstlane(max(p.min_chunk, (int)fminf(c, 1e9f) + 1));
+    const int nqb0 = p.blocks_of(Lq0, block);
+    float work = (float)nqb0 * (float)Lk0;
+    for (int b = lane + 64; b < p.B; b += 64) work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
+    work = wave_sum(work) * (float)p.Hkv;
+    const float c = work / (float)p.split_units;
+    C = max(p.min_chunk, (int)fminf(c, 1e9f) + 1);
+    if (p.B <= 64) {
+      // The smallest of 64 lengths, one a lane, that gives no more units than
+      // fit: from the work's share of all of them up to C, which does.
+      const float least = work / (float)p.total_units;
+      const int mine = lane == 63 ? C : max(p.min_chunk, (int)fminf(least + (c - least) * lane / 63.0f, 1e9f) + 1);
+      int rows = 0;
+      for (int b = 0; b < p.B; ++b) {
+        const int n = __builtin_amdgcn_readlane(nqb0, b), L = __builtin_amdgcn_readlane(Lk0, b);
+        rows += n * max((int)ceilf((float)L / (float)mine), 1);
+      }
+      const uint64_t fits = __ballot(rows * (int64_t)p.Hkv <= p.total_units) | (1ull << 63);
+      C = __builtin_amdgcn_readlane(mine, __builtin_ctzll(fits));
+    }
+    C = __builtin_amdgcn_readfirstlane(C);
   }
   PagedUnit un;
   const int row = u / p.Hkv;
   un.hk = u - row * p.Hkv;
   for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
     const int b = b0 + lane;
-    const int Lq = b < p.B ? p.len_q(b) : 0, Lk = b < p.B ? p.keys(b) : 0;
+    const int Lq = b0 == 0 ? Lq0 : b < p.B ? p.len_q(b) : 0, Lk = b0 == 0 ? Lk0 : b < p.B ? p.keys(b) : 0;
     const int nqb = p.blocks_of(Lq, block), nck = max((Lk + C - 1) / C, 1);
     int sum = nqb * nck;
 #pragma unroll
@@ -99,6 +117,9 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     }
     base += __builtin_amdgcn_readlane(sum, 63);
   }
+  // Wave-uniform as they are; the compiler is told so (scalar addresses).
+  for (int *x : {&un.b, &un.hk, &un.qb, &un.Lq, &un.Lk, &un.k0, &un.k1, &un.nck})
+    *x = __builtin_amdgcn_readfirstlane(*x);
   return un;
 }
 
@@ -118,18 +139,22 @@ __device__ __forceinline__ void paged_store(const PagedParams &p, const PagedUni
     const int tok = q / p.G;
     uint16_t *orow = (uint16_t *)p.out + ((row0 + tok) * p.H + un.hk * p.G + q - tok * p.G) * d;
     float *part = p.ws + ((int64_t)unit * block + cc + 32 * c) * D;
+const auto store = [&](auto &&put) SIGATTN_INLINE {
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) {
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (half && g >= 2) break;  // columns 16..31: not in the tensor
-        const int d0 = db * 32 + 8 * g + 4 * hi;
-        const f32x16 &a = acc[c][db];
-        const f32x4 v = {a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-        if (un.nck == 1) *(u32x2 *)(orow + d0) = (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
-        else *(f32x4 *)(part + d0) = v;
-      }
-    }
+        for (int g = 0; g < 4; ++g) {
+          if (half && g >= 2) break;  // columns 16..31: not in the tensor
+          const f32x16 &a = acc[c][db];
+          put(db * 32 + 8 * g + 4 * hi, (f32x4){a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]});
+        }
+    };
+    if (un.nck == 1)
+      store([&](int d0, f32x4 v) SIGATTN_INLINE {
+        *(u32x2 *)(orow + d0) = (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
+      });
+    else
+      store([&](int d0, f32x4 v) SIGATTN_INLINE { *(f32x4 *)(part + d0) = v; });
   }
 }
 
@@ -143,8 +168,8 @@ static __device__ const uint32_t kZeroPiece[4] __attribute__((aligned(16))) = {0
 // ahead of its use) and the page's address scalar arithmetic in 64 bits; the
 // lanes keep 32-bit offsets within 16 rows.  Rows past the chunk and rows on a
 // page outside the cache come from kZeroPiece: every instruction still issues,
-// so counted waits hold.
-template <int ROWS, int D, int NWAVES> struct PagedDma {
+// so counted waits hold.  NT: non-temporal loads, for rows that are read once.
+template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
   static constexpr int CPR = D / 8, RPI = 64 / CPR;
   static constexpr int RPW = ROWS / NWAVES, NI = RPW / RPI;  // rows, instructions per wave
   static constexpr int NE = RPW > 16 ? RPW / 16 : 1;         // table entries per wave and tile
@@ -187,7 +212,10 @@ template <int ROWS, int D, int NWAVES> struct PagedDma {
   }
   static __device__ __forceinline__ void copy(uint16_t *lds, const char *base, uint32_t off) {
     const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
+    if constexpr (NT)
+      asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
+    else
+      asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
   }
   static __device__ __forceinline__ void copy_at(uint16_t *lds, const char *at) {
     const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
@@ -227,13 +255,11 @@ template <int ROWS, int D, int NWAVES> struct PagedDma {
 void launch_paged_generic(const PagedParams &p, int dtype, int D, bool causal, hipStream_t st);
 // MFMA kernels, dtype in {kF16, kBF16}, D in {32, 64, 128} (16 as 32 with
 // dmem = 16), 16-byte aligned rows: blocks of paged_block(D) columns; a wave
-// or workgroup per chunk for sequences of up to 32 columns; and the
-// sums of cut sequences.  ngap leading workgroups of the first two zero the
+// per chunk for sequences of up to 32 columns; and the sums of cut sequences.  ngap leading workgroups of the first two zero the
 // rows outside every sequence.
 int paged_block(int D);
 void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
-void launch_paged_decode(const PagedParams &p, int units, bool wave_units, int dtype, int D, bool causal,
-                         hipStream_t st);
+void launch_paged_decode(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
 void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int dtype, int D, hipStream_t st);
 
 }  // namespace sigattn

@@ -58,15 +58,20 @@ int kernel_dim(const sigattn_paged_problem *p) { return p->D == 16 ? 32 : (int)p
 // are), how it cuts sequences (PagedParams) and the partials that takes.
 struct Part {
   int64_t units = 0;
-  int split_units = 0, min_chunk = 0, block = 0;
-  bool wave_units = false;
+  int split_units = 0, total_units = 0, min_chunk = 0, block = 0;
   size_t partial_bytes = 0;
 };
 
 // Sequences of up to kDecodeCols columns run in the decode kernel, longer ones
 // in the forward's; a batch of one, whose length the host knows to be a long
 // one or does not know, runs in the forward's alone.
+// The decode kernel's chunks: a round of the waves that the GPU runs at a time
+// at D = 128 (four per CU), of 256 keys at least.  Whole call, us, bf16 H=32 Hkv=8
+// D=128 contexts 1024..8191: waves per CU 4 / 8, B=16 49 / 55, B=64 up to 3000
+// 100 / 101, B=200 up to 900 83 / 81, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s);
+// chunks of 128 / 256 / 512 keys, B=1 65536 keys H=16 Hkv=2 27 / 23 / 31.
 constexpr int kDecodeCols = 32;
+constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 256;
 struct Plan {
   Part fwd, decode;
   int cols_lo = 0;  // columns that are not the forward kernel's
@@ -83,6 +88,7 @@ void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const Pag
   if (extra > most) extra = most;
   part.split_units = (int)extra;
   part.min_chunk = (int)min_chunk;
+  part.total_units = (int)(uncut + extra);
   // One more unit per K / V head than the sums say: their rounding.
   part.units = uncut + extra + k.Hkv;
   part.partial_bytes = (size_t)part.units * part.block * D * sizeof(float);
@@ -95,8 +101,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
   pl.fwd.block = sigattn::paged_block(D), pl.decode.block = 32;
   if (decode) {
     const int64_t pairs = (int64_t)k.B * k.Hkv;
-    pl.decode.wave_units = pairs >= cus;
-    cut_part(pl.decode, pairs, (pl.decode.wave_units ? 8 : 2) * cus, 256, k, D);
+    cut_part(pl.decode, pairs, kDecodeWaves * cus, kDecodeChunk, k, D);
   }
   if (fwd) {
     if (decode) pl.cols_lo = kDecodeCols;
@@ -117,7 +122,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
 PagedParams of_part(const PagedParams &k, const Part &part, int lo, int hi, int2 *cut, float *ws) {
   PagedParams s = k;
   s.cols_lo = lo, s.cols_hi = hi;
-  s.split_units = part.split_units, s.min_chunk = part.min_chunk;
+  s.split_units = part.split_units, s.total_units = part.total_units, s.min_chunk = part.min_chunk;
   s.cut = cut, s.ws = ws;
   return s;
 }
@@ -207,7 +212,7 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
   if (pl.decode.units > 0) {
     PagedParams s = kd;
     s.ngap[0] = pl.fwd.units > 0 ? 0 : gaps;
-    sigattn::launch_paged_decode(s, (int)pl.decode.units, pl.decode.wave_units, dt, D, causal, st);
+    sigattn::launch_paged_decode(s, (int)pl.decode.units, dt, D, causal, st);
   }
   if (kf.split_units > 0 || kd.split_units > 0) sigattn::launch_paged_reduce(kf, kd, dt, D, st);
   return launch_status();

@@ -7,15 +7,12 @@
 // K / V head is read once for all of them.  A unit is (sequence, K / V head,
 // chunk of keys), chunks so that the GPU is full (PagedUnit); units of
 // one chunk write O themselves, the others leave fp32 sums for the reduction.
-//   * WPU = 1: every wave has a unit of its own, the units of one key range in
-//     head order, so the four waves of a workgroup read the rows of
-//     neighbouring K / V heads and never wait for each other;
-//   * WPU = 4: the waves of a workgroup take every fourth 32-key block of a unit
-//     and add their sums through LDS: a quarter of the partials, for batches
-//     with few (sequence, K / V head) pairs.
-// Each wave streams its 32-key blocks through a private two-stage LDS ring with
-// direct, non-temporal global->LDS copies (PagedDma) that it waits for with its
-// own vmcnt: Sᵀ = K·Qᵀ, P = sigmoid(Sᵀ) on packed words, Oᵀ += Vᵀ·Pᵀ.
+// Every wave has a unit of its own, the units of one key range in head order,
+// so the waves of a workgroup read the rows of neighbouring K / V heads and never
+// wait for each other.  A wave streams its 32-key blocks through a private
+// two-stage LDS ring with direct, non-temporal global->LDS copies (PagedDma) that
+// it waits for with its own vmcnt: Sᵀ = K·Qᵀ, P = sigmoid(Sᵀ) on packed words,
+// Oᵀ += Vᵀ·Pᵀ.
 #include <type_traits>
 
 #include "launch.h"
@@ -25,29 +22,30 @@ namespace sigattn {
 namespace {
 
 constexpr int kCols = 32;
+// Waves per workgroup.  1 / 2 / 4, us (as the caller's figures): B=16 contexts
+// 1024..8191 61 / 48 / 49, B=64 8000..9000 438 / 333 / 338, D=64 35 / 34 / 29.
+constexpr int kWaves = 4;
 
-template <typename T, int D, int WPU, bool CAUSAL, bool SCOREMOD>
-__global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams p) {
-  constexpr int NW = 4, KB = 32;  // waves, keys per block
+template <typename T, int D, bool CAUSAL, bool SCOREMOD>
+__global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(const PagedParams p) {
+  constexpr int NW = kWaves, KB = 32;  // waves, keys per block
   constexpr int NKS = D / 16, NDB = D / 32;
-  using Dma = PagedDma<KB, D, 1>;
+  using Dma = PagedDma<KB, D, 1, true>;
   constexpr int NI = Dma::NI;                  // copy instructions per block of V
   constexpr int NK = NI + (SCOREMOD ? 1 : 0);  // ... of K, with its keys' score_mod
 
   __shared__ __attribute__((aligned(16))) uint16_t sK[NW][2][KB * D];
   __shared__ __attribute__((aligned(16))) uint16_t sV[NW][2][KB * D];
   __shared__ __attribute__((aligned(16))) float sM[SCOREMOD ? NW : 1][2][64];
-  static_assert(WPU == 1 || sizeof(sK) >= NW * 32 * D * sizeof(float), "reduction buffer");
 
   const int wg = gap_prologue<2>(p, sK);
   if (wg < 0) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
-  const int unit = WPU == 1 ? wg * NW + w : wg;
+  const int unit = wg * NW + w;
   const PagedUnit un = paged_unit(p, unit, kCols);
-  if (un.nck == 0) return;  // (WPU = 4: the whole workgroup)
-  const int wu = WPU == 1 ? 0 : w;  // the wave's place in its unit
+  if (un.nck == 0) return;
   const bool half = p.half_head(D);
   const int cols = un.Lq * p.G, keys = un.k1 - un.k0;
 
@@ -76,33 +74,31 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams 
   to.init(lane);
   Dma dma;
   dma.init(p, un.b, un.k0, keys, 0, lane, half);
-  const int nb = (keys + KB - 1) / KB;                      // blocks of the unit
-  const int nbw = nb > wu ? (nb - wu + WPU - 1) / WPU : 0;  // ... of this wave
-  auto first_key = [&](int i) SIGATTN_INLINE { return KB * (wu + WPU * i); };  // of the chunk
+  const int nb = (keys + KB - 1) / KB;
   const float *mod = SCOREMOD ? p.score_mod + un.b * p.mod_stride + un.k0 : nullptr;
   auto issue_k = [&](int i) SIGATTN_INLINE {
-    dma.issue_one(sK[w][i & 1], Kb, first_key(i));
+    dma.issue_one(sK[w][i & 1], Kb, KB * i);
     if constexpr (SCOREMOD) {
-      const uint32_t off = 4u * (uint32_t)min(first_key(i) + lane, keys - 1);
+      const uint32_t off = 4u * (uint32_t)min(KB * i + lane, keys - 1);
       const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)sM[w][i & 1]);
       asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(mod), "{m0}"(dst) : "memory");
     }
   };
-  auto issue_v = [&](int i) SIGATTN_INLINE { dma.issue_last(sV[w][i & 1], Vb, first_key(i), first_key(i + 1)); };
+  auto issue_v = [&](int i) SIGATTN_INLINE { dma.issue_last(sV[w][i & 1], Vb, KB * i, KB * (i + 1)); };
 
-  // The wait for Q comes before the copies, which the kernel counts.
-#pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) asm volatile("" ::"v"(qf[ks]));
-  if (nbw > 0) dma.load(first_key(0));
+  if (nb > 0) dma.load(0);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (i < nbw) {
+    if (i < nb) {
       issue_k(i);
       issue_v(i);
     }
-  for (int i = 0; i < nbw; ++i) {
+  // The wait for Q (which also waits for the copies above) stays out of the loop.
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) asm volatile("" ::"v"(qf[ks]));
+  for (int i = 0; i < nb; ++i) {
     // Copies in issue order: K(i) V(i) K(i+1) V(i+1) K(i+2) ...
-    if (i + 1 < nbw) wait_vm<2 * NI + NK>();
+    if (i + 1 < nb) wait_vm<2 * NI + NK>();
     else wait_vm<NI>();
     const uint16_t *tK = sK[w][i & 1], *tV = sV[w][i & 1];
     f32x16 sc = zero16();
@@ -120,7 +116,7 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams 
     }
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) sc = Elem<T>::mfma(ld_row<D>(tK, to, 0, ks), qf[ks], sc);
-    if (i + 2 < nbw) {
+    if (i + 2 < nb) {
       // Every read of K(i) has returned before the copy that replaces it.
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       issue_k(i + 2);
@@ -128,7 +124,7 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams 
 
     // P words: accumulator element e of lane (l32, hi) is key
     // kb + 8(e/4) + 4hi + e%4 of column l32.  Keys past the chunk have zero V rows.
-    const int kb = first_key(i);
+    const int kb = KB * i;
     uint32_t pk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -141,8 +137,8 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams 
         pk[e] &= (key < lim ? 0x0000ffffu : 0u) | (key + 1 < lim ? 0xffff0000u : 0u);
       }
     }
-    if (i + 2 < nbw) wait_vm<NI + 2 * NK>();
-    else if (i + 1 < nbw) wait_vm<NI + NK>();
+    if (i + 2 < nb) wait_vm<NI + 2 * NK>();
+    else if (i + 1 < nb) wait_vm<NI + NK>();
     else wait_vm<0>();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -150,70 +146,37 @@ __global__ __launch_bounds__(256, 1) void paged_decode_kernel(const PagedParams 
 #pragma unroll
       for (int db = 0; db < NDB; ++db) acc[0][db] = Elem<T>::mfma(ld_tr<D>(tV, to, j, db), bp, acc[0][db]);
     }
-    if (i + 2 < nbw) {
+    if (i + 2 < nb) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       issue_v(i + 2);
     }
   }
 
-  if constexpr (WPU == 4) {
-    // Waves 1..3 hand their sums to wave 0, which adds them in wave order.
-    float *red = (float *)&sK[0][0][0];
-    __syncthreads();  // every wave has read its last tile
-    if (w > 0) {
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x16 &a = acc[0][db];
-          *(f32x4 *)(red + ((w - 1) * NDB * 4 + 4 * db + g) * 256 + 4 * lane) =
-              (f32x4){a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-        }
-    }
-    __syncthreads();
-    if (w > 0) return;
-#pragma unroll
-    for (int x = 0; x < NW - 1; ++x)
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          f32x16 &a = acc[0][db];
-          const f32x4 v = *(const f32x4 *)(red + (x * NDB * 4 + 4 * db + g) * 256 + 4 * lane);
-          a[4 * g] += v.x, a[4 * g + 1] += v.y, a[4 * g + 2] += v.z, a[4 * g + 3] += v.w;
-        }
-  }
   paged_store<T, D, 1>(p, un, acc, l32, l32, kCols, unit, hi, half);
 }
 
-template <typename T, int D, int WPU> void decode_w(const PagedParams &p, int units, bool causal, hipStream_t st) {
-  const dim3 grid((unsigned)((WPU == 1 ? (units + 3) / 4 : units) + p.ngap[0])), block(256);
+template <typename T, int D> void decode_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
+  const dim3 grid((unsigned)((units + kWaves - 1) / kWaves + p.ngap[0])), block(64 * kWaves);
   if (causal) {
-    if (p.score_mod) paged_decode_kernel<T, D, WPU, true, true><<<grid, block, 0, st>>>(p);
-    else paged_decode_kernel<T, D, WPU, true, false><<<grid, block, 0, st>>>(p);
+    if (p.score_mod) paged_decode_kernel<T, D, true, true><<<grid, block, 0, st>>>(p);
+    else paged_decode_kernel<T, D, true, false><<<grid, block, 0, st>>>(p);
   } else {
-    if (p.score_mod) paged_decode_kernel<T, D, WPU, false, true><<<grid, block, 0, st>>>(p);
-    else paged_decode_kernel<T, D, WPU, false, false><<<grid, block, 0, st>>>(p);
+    if (p.score_mod) paged_decode_kernel<T, D, false, true><<<grid, block, 0, st>>>(p);
+    else paged_decode_kernel<T, D, false, false><<<grid, block, 0, st>>>(p);
   }
 }
 
-template <typename T>
-void decode_t(const PagedParams &p, int units, bool wave_units, int D, bool causal, hipStream_t st) {
-  const auto go = [&](auto d) {
-    if (wave_units) decode_w<T, decltype(d)::value, 1>(p, units, causal, st);
-    else decode_w<T, decltype(d)::value, 4>(p, units, causal, st);
-  };
-  if (D == 128) go(std::integral_constant<int, 128>{});
-  else if (D == 64) go(std::integral_constant<int, 64>{});
-  else go(std::integral_constant<int, 32>{});
+template <typename T> void decode_d(const PagedParams &p, int units, int D, bool causal, hipStream_t st) {
+  if (D == 128) decode_t<T, 128>(p, units, causal, st);
+  else if (D == 64) decode_t<T, 64>(p, units, causal, st);
+  else decode_t<T, 32>(p, units, causal, st);
 }
 
 }  // namespace
 
-void launch_paged_decode(const PagedParams &p, int units, bool wave_units, int dtype, int D, bool causal,
-                         hipStream_t st) {
-  if (dtype == kBF16) decode_t<__bf16>(p, units, wave_units, D, causal, st);
-  else decode_t<_Float16>(p, units, wave_units, D, causal, st);
+void launch_paged_decode(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st) {
+  if (dtype == kBF16) decode_d<__bf16>(p, units, D, causal, st);
+  else decode_d<_Float16>(p, units, D, causal, st);
 }
 
 }  // namespace sigattn

@@ -169,8 +169,13 @@ int64_t two_pass_bytes(const sigattn_problem &p, int64_t limit, int dev) {
   const int64_t full = (int64_t)g_api.bwd_workspace_bytes(&p);
   if (full <= limit) return full;
   const int64_t per_head = full / p.H;
-  const int64_t group = p.kv_heads > 0 ? p.H / p.kv_heads : 1;
-  const int64_t heads = limit / per_head / group * group;
+  if (p.kv_heads != 0 && p.kv_heads != p.H) {
+    const int64_t group = p.H / p.kv_heads, most = limit / per_head / group;
+    if (most == 0) return 0;
+    const int64_t passes = (p.kv_heads + most - 1) / most, per = (p.kv_heads + passes - 1) / passes;
+    return per * (p.rows_k / 128) >= 2 * compute_units(dev) ? per * group * per_head : 0;
+  }
+  const int64_t heads = limit / per_head;
   const int64_t grid = heads * p.B * ((p.Tq + g_dq_ds_rows - 1) / g_dq_ds_rows);
   if (heads == 0 || grid < compute_units(dev)) return 0;
   return heads * per_head;
