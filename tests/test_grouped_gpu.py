@@ -304,3 +304,36 @@ def test_head_split_asks_for_its_workspace():
             assert rc == 0  # ws: without room for the parts the groups run whole
             for x, t in zip(("dq", "dk", "dv"), g):
                 assert_within(t, want[x], x)
+
+
+def test_short_way_of_eager_calls(monkeypatch):
+    """Canonical eager calls go straight to the C++ node, with the same results
+    and refusals as the Python layer's."""
+    assert _capi.autograd_node() is not None
+    cu = offsets([30, 0, 70])
+    q, k, v, do = make(cu[-1], cu[-1], 4, 2, 64, torch.bfloat16, 18)
+    whole, took = _capi.quick_module.quick_varlen, []
+
+    def spy(*args):
+        got = whole(*args)
+        took.append(got is not None)
+        return got
+
+    monkeypatch.setattr(_capi.quick_module, "quick_varlen", spy)
+    mod = torch.randn(cu[-1], device="cuda")
+    for kw in (dict(), dict(score_mod=mod), dict(scale=0.3, sigmoid_bias=-2.0)):
+        given = run(q, k, v, do, cu, cu, max_seqlen_q=70, max_seqlen_k=70, is_causal=True, **kw)
+        assert took.pop()
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+        same = run(q, k, v, do, cu, cu, max_seqlen_q=70, max_seqlen_k=70, is_causal=True, **kw)
+        monkeypatch.delenv("SIGATTN_EAGER_BINDING")
+        assert not took.pop()
+        for x in given:
+            assert torch.equal(given[x], same[x])
+    cut = torch.tensor(cu, device="cuda", dtype=torch.int32)
+    with pytest.raises(ValueError, match="heads mismatch"):
+        ts.sigmoid_attention_varlen(q[:, :3].contiguous(), k, v, cut, cut, 70, 70)
+    with pytest.raises(ValueError, match="non-negative"):
+        ts.sigmoid_attention_varlen(q, k, v, cut, cut, -1, 70)
+    run(q.float(), k.float(), v.float(), do.float(), cu, cu)  # no longest lengths: the Python layer reads them
+    assert not took.pop()

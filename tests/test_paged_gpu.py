@@ -537,3 +537,37 @@ def test_workspace_of_other_calls_does_not_matter():
     out.fill_(float("nan"))
     assert lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), None, 0, stream) == 0
     assert_within(out, reference(q, rows, new, True), "uncut")
+
+
+def test_python_binding(monkeypatch):
+    """The Python layer's own calls equal the C++ module's."""
+    from triton_sigmoid import _capi
+    ctx, new = [100, 33, 900], [1, 40, 1]
+    q, kc, vc, table, lens, cu, _ = make(ctx, new, 16, 6, 2, 64, torch.float16)
+    k, v = (torch.randn(42, 2, 64, device="cuda").half() for _ in range(2))
+
+    def step():
+        t, a, b = table.clone(), kc.clone(), vc.clone()
+        plan = ts.paged_plan(ints(ctx), ints(new), t, ints([1, 2, 3, 4]), 16, 44)
+        ts.paged_cache_write(k, v, a, b, plan.slot_mapping[:42].contiguous())
+        return (*plan, a, b, ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 40, is_causal=True))
+
+    assert _capi.autograd_node() is not None
+    calls = []
+    for name in ("quick_plan", "quick_write", "quick_paged"):
+        whole = getattr(_capi.quick_module, name)
+
+        def spy(*args, whole=whole, name=name):
+            got = whole(*args)
+            calls.append((name, got is not None and got is not False))
+            return got
+
+        monkeypatch.setattr(_capi.quick_module, name, spy)
+    one = step()
+    assert calls == [("quick_plan", True), ("quick_write", True), ("quick_paged", True)]
+    monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    two = step()
+    assert [took for _, took in calls[3:]] == [False] * 3
+    for a, b in zip(one, two):
+        assert torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a,
+                           b.nan_to_num(7.0) if b.is_floating_point() else b)

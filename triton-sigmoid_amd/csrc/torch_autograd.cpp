@@ -1,5 +1,6 @@
 // Eager autograd node of the public APIs (sigmoid_attention,
-// sigmoid_attention_padded, sigmoid_attention_varlen), in C++.
+// sigmoid_attention_padded, sigmoid_attention_varlen), in C++, and the short
+// ways of eager calls with canonical arguments into the library.
 //
 // The reference builds its eager path from torch.autograd.Function-style
 // registrations in Python (src/triton_sigmoid/sigmoid_triton_dense.py:696-753,
@@ -59,6 +60,10 @@ struct Api {
   decltype(&sigattn_bwd_ws) bwd_ws = nullptr;
   decltype(&sigattn_bwd_split_workspace_bytes) bwd_split_workspace_bytes = nullptr;
   decltype(&sigattn_bwd_split) bwd_split = nullptr;
+  decltype(&sigattn_paged_plan) paged_plan = nullptr;
+  decltype(&sigattn_paged_write) paged_write = nullptr;
+  decltype(&sigattn_paged_fwd_workspace_bytes) paged_fwd_workspace_bytes = nullptr;
+  decltype(&sigattn_paged_fwd) paged_fwd = nullptr;
 };
 Api g_api;
 bool g_bound = false;
@@ -312,10 +317,33 @@ struct Quick {
     return at::impl::torch_function_mode_enabled() || c10::impl::dispatch_mode_enabled() ||
            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
   }
-  static bool tensor(const py::object &o, Tensor &t) {
+  static bool usable() { return g_bound && !observed() && std::getenv("SIGATTN_EAGER_BINDING") == nullptr; }
+  // A tensor of unit stride along its last dim.
+  static bool strided(const py::object &o, Tensor &t) {
     if (!THPVariable_CheckExact(o.ptr())) return false;
     t = THPVariable_Unpack(o.ptr());
-    return t.layout() == at::kStrided && !t.is_neg() && !t.is_conj() && t.is_contiguous();
+    return t.layout() == at::kStrided && !t.is_neg() && !t.is_conj() && t.dim() > 0 && t.stride(-1) == 1;
+  }
+  static bool tensor(const py::object &o, Tensor &t) { return strided(o, t) && t.is_contiguous(); }
+  // int32, contiguous, n dims, on `dev`.
+  static bool ints(const py::object &o, Tensor &t, int64_t dims, const at::Device &dev) {
+    return tensor(o, t) && t.scalar_type() == at::kInt && t.dim() == dims && t.device() == dev;
+  }
+  static bool integer(const py::object &o, int64_t &v) {
+    if (!PyLong_CheckExact(o.ptr())) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o.ptr(), &over);
+    return over == 0;
+  }
+  static bool float_type(const Tensor &t) {
+    const at::ScalarType type = t.scalar_type();
+    return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat;
+  }
+  static bool no_grad(std::initializer_list<const Tensor *> tensors) {
+    if (!at::GradMode::is_enabled()) return true;
+    for (const Tensor *t : tensors)
+      if (t->defined() && t->requires_grad()) return false;
+    return true;
   }
   static bool number(const py::object &o, double &v) {
     if (!PyFloat_CheckExact(o.ptr()) && !PyLong_CheckExact(o.ptr())) return false;
@@ -384,6 +412,174 @@ py::object quick(const py::object &query, const py::object &key, const py::objec
                                      std::nullopt, std::nullopt, 0, 0));
 }
 
+// sigmoid_attention_varlen on canonical arguments, or None.
+py::object quick_varlen(const py::object &query, const py::object &key, const py::object &value,
+                        const py::object &cu_seqlens_q, const py::object &cu_seqlens_k, const py::object &max_seqlen_q,
+                        const py::object &max_seqlen_k, const py::object &is_causal, const py::object &scale,
+                        const py::object &sigmoid_bias, const py::object &score_mod) {
+  const py::object no = py::none();
+  Tensor q, k, v, sm, cq, ck;
+  int64_t mq = 0, mk = 0;
+  if (!g_bound || Quick::observed() || std::getenv("SIGATTN_EAGER_BINDING") != nullptr ||
+      std::getenv("SIGATTN_BWD_WORKSPACE_MB") != nullptr || !Quick::tensor(query, q) || !Quick::tensor(key, k) ||
+      !Quick::tensor(value, v) || !PyBool_Check(is_causal.ptr()) || !Quick::integer(max_seqlen_q, mq) ||
+      !Quick::integer(max_seqlen_k, mk) || mq < 0 || mk < 0)
+    return no;
+  const at::Device dev = q.device();
+  if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || q.numel() == 0 || k.numel() == 0 ||
+      !Quick::float_type(q) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
+      !dev.is_cuda() || k.device() != dev || v.device() != dev || !Quick::gfx950(dev.index()))
+    return no;
+  const int64_t H = q.size(1), Hkv = k.size(1), D = q.size(2);
+  if (k.size(2) != D || H % Hkv != 0 || !Quick::ints(cu_seqlens_q, cq, 1, dev) ||
+      !Quick::ints(cu_seqlens_k, ck, 1, dev) || cq.numel() < 2 || ck.numel() != cq.numel())
+    return no;
+  if (!score_mod.is_none() && (!Quick::tensor(score_mod, sm) || sm.scalar_type() != at::kFloat || sm.device() != dev ||
+                               sm.dim() != 1 || sm.size(0) != k.size(0)))
+    return no;
+  double s = 1.0 / std::sqrt((double)D), bias_value = 0.0;
+  if (!scale.is_none() && !Quick::number(scale, s)) return no;
+  const bool own_bias = !sigmoid_bias.is_none();
+  if (own_bias && !Quick::number(sigmoid_bias, bias_value)) return no;
+  const c10::DeviceGuard guard(dev);
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return no;
+  const int64_t B = cq.numel() - 1;
+  const Tensor st = Quick::constant(-1, s, at::kFloat, dev);
+  if (!st.defined()) return no;
+  Tensor bias;
+  if (own_bias) {
+    bias = Quick::constant(B, bias_value, at::kFloat, dev);
+    if (!bias.defined()) return no;
+  } else {
+    bias = at::empty({B}, q.options().dtype(at::kFloat).requires_grad(false));
+    check_rc(g_api.default_bias(nullptr, static_cast<const int32_t *>(ck.data_ptr()), B,
+                                static_cast<float *>(bias.data_ptr()), stream),
+             "sigattn_default_bias");
+  }
+  const int64_t limit = (int64_t)(H == Hkv ? 2048 : 8192) << 20;  // _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB
+  return py::cast(SigattnNode::apply(q, k, v, bias, sm.defined() ? std::optional<Tensor>(sm) : std::nullopt, st,
+                                     std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
+}
+
+bool page_size_ok(int64_t n) { return n >= 16 && n <= (1 << 20) && (n & (n - 1)) == 0; }
+
+// The paged cache's calls on canonical arguments (int32 tensors of one gfx950
+// device, matching shapes, nothing that asks for a gradient), or None where the
+// Python layer has to take the call.
+py::object quick_plan(const py::object &context_lens, const py::object &new_lens, const py::object &block_table,
+                      const py::object &free_pages, const py::object &page_size, const py::object &num_tokens) {
+  const py::object no = py::none();
+  Tensor ctx, add, table, pages;
+  int64_t ps = 0, n = 0;
+  if (!Quick::usable() || !Quick::strided(block_table, table) || table.scalar_type() != at::kInt ||
+      table.dim() != 2 || !table.is_cuda() || !Quick::integer(page_size, ps) || !Quick::integer(num_tokens, n) ||
+      !page_size_ok(ps) || n < 0)
+    return no;
+  const at::Device dev = table.device();
+  const int64_t B = table.size(0);
+  if (!Quick::gfx950(dev.index()) || B > SIGATTN_PLAN_MAX_BATCH || (B > 1 && table.stride(0) < table.size(1)) ||
+      !Quick::ints(context_lens, ctx, 1, dev) || !Quick::ints(new_lens, add, 1, dev) ||
+      !Quick::ints(free_pages, pages, 1, dev) || ctx.size(0) != B || add.size(0) != B)
+    return no;
+  const c10::DeviceGuard guard(dev);
+  const auto opt = table.options();
+  const Tensor slots = at::empty({n}, opt), cu = at::empty({B + 1}, opt), lens = at::empty({B}, opt),
+               needed = at::empty({}, opt);
+  const auto p = [](const Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); };
+  check_rc(g_api.paged_plan(B, p(ctx), p(add), p(table), table.stride(0), table.size(1), p(pages), pages.numel(), ps, n,
+                            p(slots), p(cu), p(lens), p(needed),
+                            c10::hip::getCurrentHIPStream(dev.index()).stream()),
+           "sigattn_paged_plan");
+  return py::make_tuple(slots, cu, lens, needed);
+}
+
+// The caches: same shape, strides and type, pages the kernels take.
+bool quick_caches(const py::object &ko, const py::object &vo, Tensor &k, Tensor &v) {
+  return Quick::strided(ko, k) && Quick::strided(vo, v) && k.dim() == 4 && k.sizes() == v.sizes() &&
+         k.strides() == v.strides() && Quick::float_type(k) && v.scalar_type() == k.scalar_type() && k.is_cuda() &&
+         v.device() == k.device() && page_size_ok(k.size(1)) && Quick::gfx950(k.device().index());
+}
+
+bool quick_write(const py::object &key, const py::object &value, const py::object &key_cache,
+                 const py::object &value_cache, const py::object &slot_mapping) {
+  Tensor k, v, kc, vc, slots;
+  if (!Quick::usable() || !quick_caches(key_cache, value_cache, kc, vc) || !Quick::strided(key, k) ||
+      !Quick::strided(value, v))
+    return false;
+  const at::Device dev = kc.device();
+  if (k.dim() != 3 || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != kc.scalar_type() ||
+      v.scalar_type() != kc.scalar_type() || k.device() != dev || v.device() != dev || k.size(1) != kc.size(2) ||
+      k.size(2) != kc.size(3) || !Quick::ints(slot_mapping, slots, 1, dev) || slots.size(0) != k.size(0) ||
+      !Quick::no_grad({&k, &v, &kc, &vc}))
+    return false;
+  sigattn_paged_rows r;
+  std::memset(&r, 0, sizeof(r));
+  r.esize = (int32_t)k.element_size();
+  r.rows = k.size(0), r.kv_heads = k.size(1), r.D = k.size(2);
+  r.src_stride_t = k.stride(0), r.src_stride_h = k.stride(1);
+  r.cache_stride_p = kc.stride(0), r.cache_stride_t = kc.stride(1), r.cache_stride_h = kc.stride(2);
+  r.num_pages = kc.size(0), r.page_size = kc.size(1);
+  r.k = k.data_ptr(), r.v = v.data_ptr(), r.k_cache = kc.data_ptr(), r.v_cache = vc.data_ptr();
+  r.slot_mapping = static_cast<const int32_t *>(slots.data_ptr());
+  const c10::DeviceGuard guard(dev);
+  check_rc(g_api.paged_write(&r, c10::hip::getCurrentHIPStream(dev.index()).stream()), "sigattn_paged_write");
+  return true;
+}
+
+py::object quick_paged(const py::object &query, const py::object &key_cache, const py::object &value_cache,
+                       const py::object &block_table, const py::object &seq_lens_k, const py::object &cu_seqlens_q,
+                       const py::object &max_seqlen_q, const py::object &is_causal, const py::object &scale,
+                       const py::object &sigmoid_bias, const py::object &score_mod) {
+  const py::object no = py::none();
+  Tensor q, kc, vc, table, lens, cu, sm;
+  if (!Quick::usable() || !Quick::strided(query, q) || !quick_caches(key_cache, value_cache, kc, vc) ||
+      !Quick::strided(block_table, table) || !PyBool_Check(is_causal.ptr()))
+    return no;
+  const at::Device dev = q.device();
+  int64_t mq = q.size(0);
+  if (q.dim() != 3 || q.scalar_type() != kc.scalar_type() || kc.device() != dev || q.numel() == 0 ||
+      q.size(2) != kc.size(3) || kc.size(2) == 0 || q.size(1) % kc.size(2) != 0 || table.dim() != 2 ||
+      table.scalar_type() != at::kInt || table.device() != dev)
+    return no;
+  const int64_t B = table.size(0);
+  if (!Quick::ints(seq_lens_k, lens, 1, dev) || lens.size(0) != B || !Quick::ints(cu_seqlens_q, cu, 1, dev) ||
+      cu.size(0) != B + 1 || (!max_seqlen_q.is_none() && (!Quick::integer(max_seqlen_q, mq) || mq < 0)))
+    return no;
+  if (!score_mod.is_none() && (!Quick::tensor(score_mod, sm) || sm.scalar_type() != at::kFloat || sm.device() != dev ||
+                               sm.dim() != 2 || sm.size(0) != B || sm.size(1) != table.size(1) * kc.size(1)))
+    return no;
+  double s = 1.0 / std::sqrt((double)q.size(2)), bias = 0.0;
+  if (!scale.is_none() && !Quick::number(scale, s)) return no;
+  const bool own_bias = !sigmoid_bias.is_none();
+  if (own_bias && !Quick::number(sigmoid_bias, bias)) return no;
+  if (!Quick::no_grad({&q, &kc, &vc, &sm})) return no;
+  sigattn_paged_problem p;
+  std::memset(&p, 0, sizeof(p));
+  p.abi_version = SIGATTN_ABI_VERSION;
+  p.dtype = dtype_code(q);
+  p.B = B, p.H = q.size(1), p.kv_heads = kc.size(2), p.D = q.size(2), p.rows_q = q.size(0), p.max_seqlen_q = mq;
+  p.num_pages = kc.size(0), p.page_size = kc.size(1), p.max_pages = table.size(1);
+  p.q_stride_t = q.stride(0), p.q_stride_h = q.stride(1);
+  p.k_stride_p = kc.stride(0), p.k_stride_t = kc.stride(1), p.k_stride_h = kc.stride(2);
+  p.table_stride = table.stride(0);
+  p.q = q.data_ptr(), p.k_cache = kc.data_ptr(), p.v_cache = vc.data_ptr();
+  p.block_table = static_cast<const int32_t *>(table.data_ptr());
+  p.seq_lens_k = static_cast<const int32_t *>(lens.data_ptr());
+  p.cu_seqlens_q = static_cast<const int32_t *>(cu.data_ptr());
+  if (sm.defined()) p.score_mod = static_cast<const float *>(sm.data_ptr()), p.mod_stride = sm.stride(0);
+  p.scale = (float)s, p.bias = (float)bias;
+  p.own_bias = own_bias, p.causal = is_causal.ptr() == Py_True;
+  const c10::DeviceGuard guard(dev);
+  const Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  const Tensor ws = workspace((int64_t)g_api.paged_fwd_workspace_bytes(&p), q);  // without it: unsplit
+  check_rc(g_api.paged_fwd(&p, out.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
+                           c10::hip::getCurrentHIPStream(dev.index()).stream()),
+           "sigattn_paged_fwd");
+  return py::cast(out);
+}
+
 template <class F> void bind_one(F &dst, const py::dict &fns, const char *name) {
   TORCH_CHECK(fns.contains(name), "_sigattn_autograd.bind: missing ", name);
   dst = reinterpret_cast<F>(fns[name].cast<uintptr_t>());
@@ -401,6 +597,10 @@ void bind(const py::dict &fns, const std::vector<int64_t> &two_pass_dims, int64_
   bind_one(api.default_bias, fns, "sigattn_default_bias");
   bind_one(api.bwd_split_workspace_bytes, fns, "sigattn_bwd_split_workspace_bytes");
   bind_one(api.bwd_split, fns, "sigattn_bwd_split");
+  bind_one(api.paged_plan, fns, "sigattn_paged_plan");
+  bind_one(api.paged_write, fns, "sigattn_paged_write");
+  bind_one(api.paged_fwd_workspace_bytes, fns, "sigattn_paged_fwd_workspace_bytes");
+  bind_one(api.paged_fwd, fns, "sigattn_paged_fwd");
   TORCH_CHECK(dq_ds_rows > 0, "_sigattn_autograd.bind: dq_ds_rows must be positive");
   g_api = api;
   g_two_pass_dims = two_pass_dims;
@@ -419,6 +619,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Python layer has to take the call",
         py::arg("query"), py::arg("key"), py::arg("value"), py::arg("seq_lens_k"), py::arg("seq_lens_q"),
         py::arg("padded"), py::arg("is_causal"), py::arg("scale"), py::arg("sigmoid_bias"), py::arg("score_mod"));
+  m.def("quick_varlen", &quick_varlen, "sigmoid_attention_varlen on canonical arguments, or None");
+  m.def("quick_plan", &quick_plan, "paged_plan's new tensors on canonical arguments, or None");
+  m.def("quick_write", &quick_write, "paged_cache_write on canonical arguments: whether it took the call");
+  m.def("quick_paged", &quick_paged, "sigmoid_attention_paged on canonical arguments, or None");
   m.def("attention", &attention,
         "Forward with autograd; arguments are the canonical tensors of _capi._prepare (and _prepare_packed "
         "for the packed layout, with the longest sequences)",

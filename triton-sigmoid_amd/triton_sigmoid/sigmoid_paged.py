@@ -57,6 +57,22 @@ def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
+def _quick():
+    """The C++ module for eager calls on canonical arguments, or None."""
+    if torch.compiler.is_compiling():
+        return None
+    return _capi.quick_module if _capi.quick_module is not None else _bind()
+
+
+def _bind():
+    # The first call binds the module (which then serves every entry point);
+    # without the library the call fails with its own error further on.
+    if not _capi.LIB_PATH.exists():
+        return None
+    _capi.autograd_node()
+    return _capi.quick_module
+
+
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """t with unit stride along its last dim."""
     return t if t.stride(-1) == 1 else t.contiguous()
@@ -128,6 +144,11 @@ def paged_plan(
         gets no slots for the tokens past them.  Up to 8192 requests; sums of
         lengths have to fit 31 bits.
     """
+    quick = _quick()
+    if quick is not None:
+        got = quick.quick_plan(context_lens, new_lens, block_table, free_pages, page_size, num_tokens)
+        if got is not None:
+            return PagedPlan(block_table, *got)
     if block_table.dim() != 2:
         raise ValueError(f"block_table must have shape (B, max_pages), got {tuple(block_table.shape)}")
     B = block_table.shape[0]
@@ -227,6 +248,9 @@ def paged_cache_write(
             written.  The slots of one call have to be distinct: which of two
             rows with one slot stays is not defined.
     """
+    quick = _quick()
+    if quick is not None and quick.quick_write(key, value, key_cache, value_cache, slot_mapping):
+        return
     _check_caches(key_cache, value_cache)
     if key.dim() != 3 or value.dim() != 3:
         raise ValueError("Expected key and value to be 3D tensors (total_tokens, H_kv, D)")
@@ -367,6 +391,12 @@ def sigmoid_attention_paged(
         values of a sequence itself have to be finite.  Deterministic.
         Forward only.
     """
+    quick = _quick()
+    if quick is not None:
+        out = quick.quick_paged(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q,
+                                is_causal, scale, sigmoid_bias, score_mod)
+        if out is not None:
+            return out
     if query.dim() != 3:
         raise ValueError("Expected query to be a 3D tensor (total_tokens, H, D)")
     _check_caches(key_cache, value_cache)

@@ -188,6 +188,11 @@ def sigmoid_attention_varlen(
     the output and in dQ / dK / dV (they take no part in the attention), so
     no gradient row is left uninitialised.
     """
+    if not torch.compiler.is_compiling() and _capi.quick_module is not None:
+        out = _capi.quick_module.quick_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                                              is_causal, scale, sigmoid_bias, score_mod)
+        if out is not None:
+            return out
     if query.dim() != 3 or key.dim() != 3 or value.dim() != 3:
         raise ValueError("Expected query, key, and value to be 3D tensors (total_tokens, H, D)")
     _, H, D = query.shape
