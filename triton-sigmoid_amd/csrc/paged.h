@@ -47,11 +47,26 @@ struct PagedUnit {
   int nck = 0;                // chunks of the sequence (0: no such unit)
 };
 
-// Sum over the wave's lanes, in a fixed order.
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+// Inclusive sums over the lanes of the wave, by data-parallel-primitive adds (a
+// few cycles each, where a shuffle through LDS takes about a hundred): within
+// rows of 16 lanes, then rows 1 and 3 take row 0's and 2's total, then the upper
+// half the lower's.  Lane 63 has the sum.
+template <typename N> __device__ __forceinline__ N wave_scan(N x) {
+  const auto step = [&](auto ctrl, auto rows) SIGATTN_INLINE {
+    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                  decltype(rows)::value, 0xf, false);
+    x += __builtin_bit_cast(N, moved);
+  };
+  step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
   return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_scan(x)), 63));
 }
 
 // Unit u of the kernel with column blocks of `block`, from the lengths on the
@@ -94,13 +109,7 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     const int b = b0 + lane;
     const int Lq = b0 == 0 ? Lq0 : b < p.B ? p.len_q(b) : 0, Lk = b0 == 0 ? Lk0 : b < p.B ? p.keys(b) : 0;
     const int nqb = p.blocks_of(Lq, block), nck = max((Lk + C - 1) / C, 1);
-    int sum = nqb * nck;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(sum, d);
-      if (lane >= d) sum += x;
-    }
-    const int first = base + sum - nqb * nck;
+    const int sum = wave_scan(nqb * nck), first = base + sum - nqb * nck;
     const uint64_t m = __ballot(row >= first && row < base + sum);
     if (m != 0) {
       const int at = __builtin_ctzll(m);
@@ -202,14 +211,16 @@ template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
       voff[i] = (uint32_t)((i * RPI) % 16 + lrow) * row_bytes + cbyte[i];
     }
   }
-  // Entries of the tile whose first key is `tile` of the chunk.
-  __device__ __forceinline__ void load(int tile) {
+  // Entries of the tile whose first key is `tile` of the chunk (of its last
+  // key's page beyond; keys > 0).
+  __device__ __forceinline__ void entries(int tile, int (&to)[NE]) const {
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const int key = key0 + min(tile + r0 + 16 * e, keys - 1);
-      ent[e] = row[__builtin_amdgcn_readfirstlane(key >> lp)];
+      to[e] = row[__builtin_amdgcn_readfirstlane(key >> lp)];
     }
   }
+  __device__ __forceinline__ void load(int tile) { entries(tile, ent); }
   static __device__ __forceinline__ void copy(uint16_t *lds, const char *base, uint32_t off) {
     const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
     if constexpr (NT)
@@ -221,13 +232,16 @@ template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
     const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(at), "{m0}"(dst) : "memory");
   }
-  // Copies one tensor's tile whose entries are in `ent` (head: the head's
-  // element 0 of page 0).
+  // Copies one tensor's tile with the entries `at` (head: the head's element 0
+  // of page 0).
   __device__ __forceinline__ void issue_one(uint16_t *lds, const uint16_t *head, int tile) const {
+    issue_at(lds, head, tile, ent);
+  }
+  __device__ __forceinline__ void issue_at(uint16_t *lds, const uint16_t *head, int tile, const int (&at)[NE]) const {
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const int first = tile + r0 + 16 * e;  // of the chunk
-      const int id = ent[e], n = keys - first;
+      const int id = at[e], n = keys - first;
       const bool there = id >= 0 && id < pages;
       const int in_page = (key0 + first) & ((1 << lp) - 1);
       const char *base = (const char *)head + (there ? id : 0) * page_bytes + (int64_t)in_page * row_bytes;

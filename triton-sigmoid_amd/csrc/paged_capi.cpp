@@ -71,7 +71,17 @@ struct Part {
 // 100 / 101, B=200 up to 900 83 / 81, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s);
 // chunks of 128 / 256 / 512 keys, B=1 65536 keys H=16 Hkv=2 27 / 23 / 31.
 constexpr int kDecodeCols = 32;
-constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 256;
+#ifndef PD_MIN
+#define PD_MIN 256
+#endif
+constexpr int64_t kDecodeWaves = 4, kDecodeChunk = PD_MIN;
+// The forward kernel's chunks, where its blocks do not fill the GPU: a round of
+// its workgroups, of 1024 keys at least.  Whole call, us, one / two rounds: bf16
+// H=32 Hkv=8 D=128, 2 x 1024 tokens on up to 12000 keys 324 / 343, 256 on 12000
+// 57 / 77, 4 x 128 114 / 132, 2000 on none 59 / 89; chunks of 512 / 1024 / 2048
+// keys, 24 requests, 4 of up to 700 tokens on up to 4096 keys, H=12 Hkv=4 D=128
+// 87 / 69 / 83.
+constexpr int64_t kChunk = 1024;
 struct Plan {
   Part fwd, decode;
   int cols_lo = 0;  // columns that are not the forward kernel's
@@ -110,7 +120,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
     const int64_t seqs = all / (pl.cols_lo + 1) < k.B ? all / (pl.cols_lo + 1) : k.B;
     const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = D == 128 ? 1 : (D == 64 ? 3 : 4);
     const int64_t full = cdiv(all, pl.fwd.block) * k.Hkv;
-    cut_part(pl.fwd, uncut, full < 2 * per_cu * cus ? 2 * per_cu * cus : 0, 512, k, D);
+        cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, kChunk, k, D);
   }
   const bool cut = pl.fwd.split_units > 0 || pl.decode.split_units > 0;
   pl.cut_bytes = cut ? cdiv((int64_t)k.B * 2 * (int64_t)sizeof(int2), 256) * 256 : 0;

@@ -76,8 +76,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(const Page
   dma.init(p, un.b, un.k0, keys, 0, lane, half);
   const int nb = (keys + KB - 1) / KB;
   const float *mod = SCOREMOD ? p.score_mod + un.b * p.mod_stride + un.k0 : nullptr;
-  auto issue_k = [&](int i) SIGATTN_INLINE {
-    dma.issue_one(sK[w][i & 1], Kb, KB * i);
+  auto issue_k = [&](int i, const int (&at)[Dma::NE]) SIGATTN_INLINE {
+    dma.issue_at(sK[w][i & 1], Kb, KB * i, at);
     if constexpr (SCOREMOD) {
       const uint32_t off = 4u * (uint32_t)min(KB * i + lane, keys - 1);
       const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)sM[w][i & 1]);
@@ -86,13 +86,19 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(const Page
   };
   auto issue_v = [&](int i) SIGATTN_INLINE { dma.issue_last(sV[w][i & 1], Vb, KB * i, KB * (i + 1)); };
 
-  if (nb > 0) dma.load(0);
+  // The first three blocks' pages at once, then one block ahead.
+  if (nb > 0) {
+    int first[2][Dma::NE];
+    dma.entries(0, first[0]);
+    dma.entries(KB, first[1]);
+    dma.load(2 * KB);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (i < nb) {
-      issue_k(i);
-      issue_v(i);
-    }
+    for (int i = 0; i < 2; ++i)
+      if (i < nb) {
+        issue_k(i, first[i]);
+        dma.issue_at(sV[w][i], Vb, KB * i, first[i]);
+      }
+  }
   // The wait for Q (which also waits for the copies above) stays out of the loop.
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) asm volatile("" ::"v"(qf[ks]));
@@ -119,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(const Page
     if (i + 2 < nb) {
       // Every read of K(i) has returned before the copy that replaces it.
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue_k(i + 2);
+      issue_k(i + 2, dma.ent);
     }
 
     // P words: accumulator element e of lane (l32, hi) is key

@@ -29,10 +29,12 @@ template <typename T, int D> void fwd_t(const PagedParams &p, int units, bool ca
 }
 
 // Output rows (token, query head) of cut sequences: the sum of the chunks'
-// partials in chunk order.  D / 4 threads add one row, four columns each; the
-// 256 / (D / 4) groups of a workgroup take rows of their own (many rows), or
-// (ROWS = false) every group a share of one row's chunks, added in group order
-// (few rows of many chunks).
+// partials in chunk order.  CG threads add CG * 4 columns of one row.  Many rows
+// (ROWS): CG = D / 4, and every group of a workgroup takes a row of its own.
+// Few rows: CG = 8, a workgroup has 32 columns of a row, each of its 32 groups a
+// share of the chunks, whose sums are added in group order -- one or two loads
+// deep where a sequence has tens of chunks (B=1, 256 chunks, 16 rows D=128: 6.1 us
+// with a workgroup per row).
 struct ReduceArgs {
   PagedParams p;
   const float *ws[2];   // blocks of more than / up to `cols` columns
@@ -42,11 +44,11 @@ struct ReduceArgs {
 
 template <typename T, int D, bool ROWS>
 __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
-  constexpr int CG = D / 4, NG = 256 / CG;
+  constexpr int CG = ROWS ? D / 4 : 8, NG = 256 / CG;
   __shared__ f32x4 part[ROWS ? 1 : NG][CG];
   const PagedParams &p = a.p;
-  const int c = threadIdx.x % CG, g = threadIdx.x / CG;
-  const int64_t item = ROWS ? (int64_t)blockIdx.x * NG + g : (int64_t)blockIdx.x;
+  const int g = threadIdx.x / CG, c = threadIdx.x % CG + (ROWS ? 0 : CG * (int)(blockIdx.x % (D / 32)));
+  const int64_t item = ROWS ? (int64_t)blockIdx.x * NG + g : (int64_t)(blockIdx.x / (D / 32));
   const int64_t r = item / p.H;
   const int h = (int)(item - r * p.H);
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -76,11 +78,11 @@ __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
   }
   if constexpr (!ROWS) {
     if (nck <= 1) return;  // the whole workgroup
-    part[g][c] = v;
+    part[g][threadIdx.x % CG] = v;
     __syncthreads();
     if (g != 0) return;
 #pragma unroll
-    for (int x = 1; x < NG; ++x) v += part[x][c];
+    for (int x = 1; x < NG; ++x) v += part[x][threadIdx.x];
   }
   if (nck > 1 && 4 * c < p.dmem)
     *(u32x2 *)((uint16_t *)p.out + (r * p.H + h) * p.dmem + 4 * c) =
@@ -90,8 +92,9 @@ __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
 template <typename T, int D> void reduce_t(const ReduceArgs &a, hipStream_t st) {
   constexpr int NG = 256 / (D / 4);
   const int64_t rows = a.p.rows_q * a.p.H;
-  // One row per workgroup where that is few workgroups a CU.
-  if (rows <= 8 * (int64_t)a.p.ncu) paged_reduce_kernel<T, D, false><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
+  // A workgroup for 32 columns where that is few workgroups a CU.
+  const int64_t parts = rows * (D / 32);
+  if (parts <= 8 * (int64_t)a.p.ncu) paged_reduce_kernel<T, D, false><<<dim3((unsigned)parts), dim3(256), 0, st>>>(a);
   else paged_reduce_kernel<T, D, true><<<dim3((unsigned)((rows + NG - 1) / NG)), dim3(256), 0, st>>>(a);
 }
 
