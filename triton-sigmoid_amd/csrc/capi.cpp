@@ -436,6 +436,9 @@ HeadSplit head_split(const sigattn_problem *p, bool mfma) {
   const int64_t items = (rows / 128 + (p->B + 1) / 2) * kv_heads(p);
   int64_t n = items > 0 ? cdiv(kHeadSplitPerCu * cus, items) : 1;
   if (n > G) n = G;
+  // Four tiles of queries a part at least: shorter ones are all start and end.
+  const int64_t tiles = G * cdiv(p->Tq, 64);
+  if (n > tiles / 4) n = tiles / 4;
   if (n < 2) return s;
   s.n = (int)n;
   s.bytes = n * 2 * p->rows_k * kv_heads(p) * p->D * (int64_t)sizeof(float);

@@ -37,6 +37,7 @@
 
 #include "common.h"
 #include "launch.h"
+#include "paged.h"
 
 namespace sigattn {
 namespace {
@@ -935,7 +936,113 @@ template <int D> void dkdv_t(const KParams &kp, bool causal, bool scoremod, hipS
   });
 }
 
+// Forward over a paged cache (see paged.h), on the fp32 instruction: nothing to
+// split, and so no rows to find that the splits cannot hold.  Four waves of 32
+// columns share 32-key tiles of K and V in two stages, copied one tile ahead
+// through the block table; columns, key chunks and rows that are not there are
+// the 16-bit kernel's.  D MFMAs of 64 cycles a wave and tile bound it: 82 TFLOP/s
+// with full blocks (2 x 300 tokens on 1000 keys H=32 Hkv=8 D=128, 137 us), and in
+// decoding, where one wave of four has columns, 2.6 TB/s (16 requests, contexts
+// 1024..8191, 190 us).
+template <int D, bool CAUSAL, bool SCOREMOD>
+__global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const PagedParams p) {
+  constexpr int NDB = D / 32, BM = 32 * FW;
+  static_assert(BM == kPagedBlockF32, "columns per block");
+  __shared__ __attribute__((aligned(16))) float lds[4 * FB * D + (SCOREMOD ? 2 * FB : 0)];
+  const int wg = gap_prologue<4>(p, lds);
+  if (wg < 0) return;
+  const PagedUnit un = paged_unit(p, wg, BM);
+  if (un.nck == 0) return;
+  const bool half = p.half_head(D);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const int cols = un.Lq * p.G, keys = un.k1 - un.k0;
+  const int q0 = un.qb * BM, qw = q0 + 32 * w, myq = qw + l32;
+  // Keys of the chunk that column c sees.
+  const auto seen = [&](int c) SIGATTN_INLINE { return CAUSAL ? un.Lk - un.Lq + c / p.G + 1 - un.k0 : keys; };
+  const int nend = min(keys, max(seen(min(q0 + BM, cols) - 1), 0));
+  const int wend = qw < cols ? min(nend, seen(min(qw + 32, cols) - 1)) : 0;  // of this wave's columns
+  const int lim = seen(min(myq, cols - 1)), all_see = seen(min(qw, cols - 1));
+  const int ntiles = (nend + FB - 1) / FB;
+  const float bias = p.bias_of(un.Lk), nsl = -p.fscale * kLog2e, nbl = -bias * kLog2e;
+
+  const int64_t row0 = packed_first(p.cu_q, p.rows_q, un.b);
+  const int tok = myq / p.G, head = un.hk * p.G + myq - tok * p.G;
+  const uint16_t *Kb = (const uint16_t *)((const float *)p.k + (int64_t)un.hk * p.sk_h);
+  const uint16_t *Vb = (const uint16_t *)((const float *)p.v + (int64_t)un.hk * p.sk_h);
+  float qv[D / 2];
+  load_half_row<D>(qv, (const float *)p.q + (row0 + tok) * p.sq_t + (int64_t)head * p.sq_h, hi,
+                   myq < cols && !(half && hi));
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc[db] = zero16();
+  PagedDma<FB, 2 * D, FW, false, 4> dma;
+  dma.init(p, un.b, un.k0, keys, w, lane, half);
+  F32RowReads<D> rr;
+  rr.init(l32, hi);
+  float creg = 0.0f;
+  auto issue = [&](int t) SIGATTN_INLINE {
+    float *tK = lds + (t & 1) * 2 * FB * D;
+    if (SCOREMOD && tid < FB) {
+      const int key = t * FB + tid;
+      creg = key < keys ? -(bias + p.score_mod[un.b * p.mod_stride + un.k0 + key]) * kLog2e : 0.0f;
+    }
+    dma.issue_one((uint16_t *)tK, Kb, t * FB);
+    dma.issue_last((uint16_t *)(tK + FB * D), Vb, t * FB, (t + 1) * FB);
+  };
+  if (ntiles > 0) {
+    dma.load(0);
+    issue(0);
+  }
+  for (int t = 0; t < ntiles; ++t) {
+    const float *tK = lds + (t & 1) * 2 * FB * D, *tV = tK + FB * D;
+    float *tC = lds + 4 * FB * D + (t & 1) * FB;
+    wait_dma();
+    if (SCOREMOD && tid < FB) tC[tid] = creg;
+    // Tile t is there, and every wave is done with tile t - 1, whose stage the
+    // next copy fills.
+    __syncthreads();
+    if (t + 1 < ntiles) issue(t + 1);
+    const int k0 = t * FB;
+    if (k0 >= wend) continue;
+    f32x16 s = zero16();
+    head_product<D>(s, tK, qv, l32, hi);
+    float pr[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      pr[i] = sigmoid_from_neg_log2(
+          __builtin_fmaf(s[i], nsl, SCOREMOD ? tC[8 * (i / 4) + 4 * hi + i % 4] : nbl));
+    if (CAUSAL && k0 + FB > all_see) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + 8 * (i / 4) + 4 * hi + i % 4 >= lim) pr[i] = 0.0f;
+    }
+    row_product<D>(acc, tV, pr, rr);
+  }
+  if (myq >= cols) return;
+  if (un.nck == 1) store_row<D>((float *)p.out + ((row0 + tok) * p.H + head) * p.dmem, acc, 1.0f, true, hi, half);
+  else store_row<D>(p.ws + ((int64_t)wg * BM + myq - q0) * D, acc, 1.0f, true, hi, half);
+}
+
+template <int D> void paged_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
+  const dim3 grid((unsigned)(units + p.ngap[0])), block(64 * FW);
+  if (causal) {
+    if (p.score_mod) paged_f32_kernel<D, true, true><<<grid, block, 0, st>>>(p);
+    else paged_f32_kernel<D, true, false><<<grid, block, 0, st>>>(p);
+  } else {
+    if (p.score_mod) paged_f32_kernel<D, false, true><<<grid, block, 0, st>>>(p);
+    else paged_f32_kernel<D, false, false><<<grid, block, 0, st>>>(p);
+  }
+}
+
 }  // namespace
+
+void launch_paged_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st) {
+  if (D == 128) paged_t<128>(p, units, causal, st);
+  else if (D == 64) paged_t<64>(p, units, causal, st);
+  else paged_t<32>(p, units, causal, st);
+}
 
 void launch_fwd_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st) {
   if (D == 128) fwd_t<128>(p, causal, scoremod, st);

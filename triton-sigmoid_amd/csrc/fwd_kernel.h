@@ -76,8 +76,15 @@ template <int D, int WK = 1, int NCB = 1> constexpr int fwd_occupancy() {
 // the sequence's, and the causal limit of a column is its token's place among
 // them.  Tile rows past the keys and rows on pages that are not there are
 // zeros (PagedDma), so they add nothing whatever their P is.
+// The kernel's LDS, in arrays of their own: as members of one struct their
+// addresses took so many more registers that the D = 128 kernel spilled 100.
+template <int D, int WK> using FwdTiles = uint16_t[fwd_stages<D, WK>()][64 * D];
+template <int D, int WK, bool SCOREMOD> using FwdTerms = float[SCOREMOD ? fwd_stages<D, WK>() * 64 : 4];
+
+// Work item `wg` of the kernel's.
 template <typename T, int D, int NWV, int NCB, int WK, bool CAUSAL, bool SCOREMOD, class P>
-__global__ __launch_bounds__(64 * NWV, (fwd_occupancy<D, WK, NCB>())) void fwd_mfma_kernel(const P p) {
+__device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles<D, WK> &sK, FwdTiles<D, WK> &sV,
+                                              FwdTerms<D, WK, SCOREMOD> &sC) {
   constexpr bool PAGED = P::kPaged;
   static_assert(!PAGED || WK == 1, "pairs of waves: contiguous keys only");
   // NWV waves per workgroup (8: two per SIMD), NCB 32-query column blocks each.
@@ -103,12 +110,6 @@ __global__ __launch_bounds__(64 * NWV, (fwd_occupancy<D, WK, NCB>())) void fwd_m
   constexpr int BAR = NSTEP - LA;       // step of the tile barrier (in odd regions; WK = 2: in all)
   static_assert(NSTEP % LA == 0, "region shape");
 
-  __shared__ __attribute__((aligned(16))) uint16_t sK[NST][BN * D];
-  __shared__ __attribute__((aligned(16))) uint16_t sV[NST][BN * D];
-  __shared__ __attribute__((aligned(16))) float sC[SCOREMOD ? NST * BN : 4];
-
-  const int wg = gap_prologue<2>(p, sK);  // packed layouts: leading gap-zeroing workgroups
-  if (wg < 0) return;
   int b, h, qb0, nitems = 1;
   int ritem = 0, rchunk = 0;  // range split: the item and this workgroup's chunk of its keys
   [[maybe_unused]] PagedUnit un;
@@ -551,6 +552,15 @@ __global__ __launch_bounds__(64 * NWV, (fwd_occupancy<D, WK, NCB>())) void fwd_m
       }
     }
   }
+}
+
+template <typename T, int D, int NWV, int NCB, int WK, bool CAUSAL, bool SCOREMOD, class P>
+__global__ __launch_bounds__(64 * NWV, (fwd_occupancy<D, WK, NCB>())) void fwd_mfma_kernel(const P p) {
+  __shared__ __attribute__((aligned(16))) FwdTiles<D, WK> sK, sV;
+  __shared__ __attribute__((aligned(16))) FwdTerms<D, WK, SCOREMOD> sC;
+  const int wg = gap_prologue<2>(p, sK);  // packed layouts: leading gap-zeroing workgroups
+  if (wg < 0) return;
+  fwd_mfma_body<T, D, NWV, NCB, WK, CAUSAL, SCOREMOD, P>(p, wg, sK, sV, sC);
 }
 
 }  // namespace sigattn

@@ -178,7 +178,8 @@ static __device__ const uint32_t kZeroPiece[4] __attribute__((aligned(16))) = {0
 // lanes keep 32-bit offsets within 16 rows.  Rows past the chunk and rows on a
 // page outside the cache come from kZeroPiece: every instruction still issues,
 // so counted waits hold.  NT: non-temporal loads, for rows that are read once.
-template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
+// fp32 rows of D / 2 elements (ESIZE = 4) are the same bytes.
+template <int ROWS, int D, int NWAVES, bool NT = false, int ESIZE = 2> struct PagedDma {
   static constexpr int CPR = D / 8, RPI = 64 / CPR;
   static constexpr int RPW = ROWS / NWAVES, NI = RPW / RPI;  // rows, instructions per wave
   static constexpr int NE = RPW > 16 ? RPW / 16 : 1;         // table entries per wave and tile
@@ -203,7 +204,7 @@ template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
     const uint64_t at = (uint64_t)(uintptr_t)(p.table + (int64_t)b * p.table_stride);
     row = (ScalarInts)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32) |
                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at));
-    page_bytes = p.sk_p * 2, row_bytes = (uint32_t)(p.sk_t * 2);
+    page_bytes = p.sk_p * ESIZE, row_bytes = (uint32_t)(p.sk_t * ESIZE);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int in_tile = r0 + i * RPI + lrow;
@@ -269,11 +270,17 @@ template <int ROWS, int D, int NWAVES, bool NT = false> struct PagedDma {
 void launch_paged_generic(const PagedParams &p, int dtype, int D, bool causal, hipStream_t st);
 // MFMA kernels, dtype in {kF16, kBF16}, D in {32, 64, 128} (16 as 32 with
 // dmem = 16), 16-byte aligned rows: blocks of paged_block(D) columns; a wave
-// per chunk for sequences of up to 32 columns; and the sums of cut sequences.  ngap leading workgroups of the first two zero the
-// rows outside every sequence.
+// per chunk for sequences of up to 32 columns; and the sums of cut sequences.  ngap leading workgroups (pf's) zero the rows
+// outside every sequence.
 int paged_block(int D);
 void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
 void launch_paged_decode(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
+// Both in one launch (nf and nd units).
+void launch_paged_mixed(const PagedParams &pf, int nf, const PagedParams &pd, int nd, int dtype, int D, bool causal,
+                        hipStream_t st);
+// fp32, D in {32, 64, 128} (16 as above): blocks of kPagedBlockF32 columns.
+constexpr int kPagedBlockF32 = 128;
+void launch_paged_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st);
 void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int dtype, int D, hipStream_t st);
 
 }  // namespace sigattn

@@ -40,14 +40,13 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool aligned16(const void *ptr) { return ((uintptr_t)ptr & 15u) == 0; }
 
-// The MFMA kernels take f16 / bf16 whose rows start on 16-byte boundaries (and
-// whose 16 rows of a tile lie within 2^31 bytes).
+// The MFMA kernels take rows that start on 16-byte boundaries (and 16 of which
+// lie within 2^31 bytes).
 bool use_mfma(const sigattn_paged_problem *p, const void *out) {
-  if (p->dtype == SIGATTN_F32) return false;
   const int64_t strides[5] = {p->q_stride_t, p->q_stride_h, p->k_stride_p, p->k_stride_t, p->k_stride_h};
   for (int64_t s : strides)
-    if (s % 8 != 0) return false;
-  return p->k_stride_t < (int64_t)1 << 26 && aligned16(p->q) && aligned16(p->k_cache) && aligned16(p->v_cache) &&
+    if (s % (p->dtype == SIGATTN_F32 ? 4 : 8) != 0) return false;
+  return p->k_stride_t < (int64_t)1 << 25 && aligned16(p->q) && aligned16(p->k_cache) && aligned16(p->v_cache) &&
          aligned16(out);
 }
 
@@ -69,19 +68,17 @@ struct Part {
 // at D = 128 (four per CU), of 256 keys at least.  Whole call, us, bf16 H=32 Hkv=8
 // D=128 contexts 1024..8191: waves per CU 4 / 8, B=16 49 / 55, B=64 up to 3000
 // 100 / 101, B=200 up to 900 83 / 81, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s);
-// chunks of 128 / 256 / 512 keys, B=1 65536 keys H=16 Hkv=2 27 / 23 / 31.
+// chunks of 128 / 192 / 256 keys, B=1 65536 keys H=16 Hkv=2 23.2 / 21.1 / 21.5,
+// 2000 keys 15.5 / 17.2 / 19.5, B=4 up to 8191 20.3 / 20.2 / 21.7.
 constexpr int kDecodeCols = 32;
-#ifndef PD_MIN
-#define PD_MIN 256
-#endif
-constexpr int64_t kDecodeWaves = 4, kDecodeChunk = PD_MIN;
+constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 192;
 // The forward kernel's chunks, where its blocks do not fill the GPU: a round of
 // its workgroups, of 1024 keys at least.  Whole call, us, one / two rounds: bf16
 // H=32 Hkv=8 D=128, 2 x 1024 tokens on up to 12000 keys 324 / 343, 256 on 12000
 // 57 / 77, 4 x 128 114 / 132, 2000 on none 59 / 89; chunks of 512 / 1024 / 2048
 // keys, 24 requests, 4 of up to 700 tokens on up to 4096 keys, H=12 Hkv=4 D=128
 // 87 / 69 / 83.
-constexpr int64_t kChunk = 1024;
+constexpr int64_t kChunk = 1024, kChunkF32 = 256;
 struct Plan {
   Part fwd, decode;
   int cols_lo = 0;  // columns that are not the forward kernel's
@@ -107,8 +104,9 @@ void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const Pag
 Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
   Plan pl;
   const int64_t cols = (int64_t)k.Tq * k.G, all = p->rows_q * k.G, cus = k.ncu;
-  const bool decode = cols <= kDecodeCols || k.B > 1, fwd = cols > kDecodeCols;
-  pl.fwd.block = sigattn::paged_block(D), pl.decode.block = 32;
+  const bool f32 = p->dtype == SIGATTN_F32;  // one kernel for all
+  const bool decode = !f32 && (cols <= kDecodeCols || k.B > 1), fwd = f32 || cols > kDecodeCols;
+  pl.fwd.block = f32 ? sigattn::kPagedBlockF32 : sigattn::paged_block(D), pl.decode.block = 32;
   if (decode) {
     const int64_t pairs = (int64_t)k.B * k.Hkv;
     cut_part(pl.decode, pairs, kDecodeWaves * cus, kDecodeChunk, k, D);
@@ -118,9 +116,9 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
     // Blocks: whole ones of all columns, and one that is not whole for each
     // sequence of the kernel's.
     const int64_t seqs = all / (pl.cols_lo + 1) < k.B ? all / (pl.cols_lo + 1) : k.B;
-    const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = D == 128 ? 1 : (D == 64 ? 3 : 4);
+    const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = f32 ? 2 : D == 128 ? 1 : (D == 64 ? 3 : 4);
     const int64_t full = cdiv(all, pl.fwd.block) * k.Hkv;
-        cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, kChunk, k, D);
+        cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, f32 ? kChunkF32 : kChunk, k, D);
   }
   const bool cut = pl.fwd.split_units > 0 || pl.decode.split_units > 0;
   pl.cut_bytes = cut ? cdiv((int64_t)k.B * 2 * (int64_t)sizeof(int2), 256) * 256 : 0;
@@ -208,22 +206,19 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
   int2 *cuts = (int2 *)ws;
   float *partials = (float *)(ws + pl.cut_bytes);
   k.gap[0] = gap;
-  // The first kernel also zeroes the rows outside every sequence (workgroups in
+  // The kernel also zeroes the rows outside every sequence (workgroups in
   // a multiple of 8, so that its items keep their XCDs).
   const int gaps = (int)(cdiv(cdiv(p->rows_q, 64), 8) * 8);
   const PagedParams kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, cuts, partials);
   const PagedParams kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0, cuts + p->B,
                                  partials + pl.fwd.partial_bytes / sizeof(float));
-  if (pl.fwd.units > 0) {
-    PagedParams s = kf;
-    s.ngap[0] = gaps;
-    sigattn::launch_paged_fwd(s, (int)pl.fwd.units, dt, D, causal, st);
-  }
-  if (pl.decode.units > 0) {
-    PagedParams s = kd;
-    s.ngap[0] = pl.fwd.units > 0 ? 0 : gaps;
-    sigattn::launch_paged_decode(s, (int)pl.decode.units, dt, D, causal, st);
-  }
+  PagedParams first = pl.fwd.units > 0 ? kf : kd;
+  first.ngap[0] = gaps;
+  if (pl.fwd.units > 0 && pl.decode.units > 0)
+    sigattn::launch_paged_mixed(first, (int)pl.fwd.units, kd, (int)pl.decode.units, dt, D, causal, st);
+  else if (pl.decode.units > 0) sigattn::launch_paged_decode(first, (int)pl.decode.units, dt, D, causal, st);
+  else if (dt == SIGATTN_F32) sigattn::launch_paged_f32(first, (int)pl.fwd.units, D, causal, st);
+  else sigattn::launch_paged_fwd(first, (int)pl.fwd.units, dt, D, causal, st);
   if (kf.split_units > 0 || kd.split_units > 0) sigattn::launch_paged_reduce(kf, kd, dt, D, st);
   return launch_status();
 }

@@ -8,6 +8,7 @@
 // normalisation, so O is the plain sum over the chunks).
 #include "fwd_kernel.h"
 #include "launch.h"
+#include "paged_decode.h"
 
 namespace sigattn {
 namespace {
@@ -25,6 +26,42 @@ template <typename T, int D> void fwd_t(const PagedParams &p, int units, bool ca
   } else {
     if (p.score_mod) fwd_mfma_kernel<T, D, NWV, 1, 1, false, true, PagedParams><<<grid, block, 0, st>>>(p);
     else fwd_mfma_kernel<T, D, NWV, 1, 1, false, false, PagedParams><<<grid, block, 0, st>>>(p);
+  }
+}
+
+// Batches with sequences of both kernels: the first nf workgroups (after the gap
+// ones) run blocks of columns, the others decode, so that the longer part's
+// last workgroups run beside the shorter part's, and a launch less.  The parts
+// share their LDS; at D = 64 decoding takes three waves, which fit what three
+// workgroups of a CU leave each, and everywhere as many as the LDS holds.
+template <int D> constexpr int mixed_waves() { return D == 64 ? 3 : 4; }
+template <typename T, int D, bool CAUSAL, bool SCOREMOD>
+__global__ __launch_bounds__(64 * waves_of(D), (fwd_occupancy<D, 1, 1>())) void paged_mixed_kernel(
+    const PagedParams pf, const PagedParams pd, const int nf) {
+  constexpr int NW = mixed_waves<D>();
+  __shared__ __attribute__((aligned(16))) FwdTiles<D, 1> sK, sV;
+  __shared__ __attribute__((aligned(16))) FwdTerms<D, 1, SCOREMOD> sC;
+  __shared__ __attribute__((aligned(16))) DecodeTerms<NW, SCOREMOD> sM;
+  static_assert(sizeof(sK) == sizeof(DecodeTiles<D, NW>), "the parts share their tiles");
+  const int wg = gap_prologue<2>(pf, sK);
+  if (wg < 0) return;
+  if (wg < nf)
+    fwd_mfma_body<T, D, waves_of(D), 1, 1, CAUSAL, SCOREMOD, PagedParams>(pf, wg, sK, sV, sC);
+  else
+    paged_decode_body<T, D, NW, CAUSAL, SCOREMOD>(pd, wg - nf, reinterpret_cast<DecodeTiles<D, NW> &>(sK),
+                                                  reinterpret_cast<DecodeTiles<D, NW> &>(sV), sM);
+}
+
+template <typename T, int D>
+void mixed_t(const PagedParams &pf, int nf, const PagedParams &pd, int nd, bool causal, hipStream_t st) {
+  constexpr int NW = mixed_waves<D>();
+  const dim3 grid((unsigned)(nf + (nd + NW - 1) / NW + pf.ngap[0])), block(64 * waves_of(D));
+  if (causal) {
+    if (pf.score_mod) paged_mixed_kernel<T, D, true, true><<<grid, block, 0, st>>>(pf, pd, nf);
+    else paged_mixed_kernel<T, D, true, false><<<grid, block, 0, st>>>(pf, pd, nf);
+  } else {
+    if (pf.score_mod) paged_mixed_kernel<T, D, false, true><<<grid, block, 0, st>>>(pf, pd, nf);
+    else paged_mixed_kernel<T, D, false, false><<<grid, block, 0, st>>>(pf, pd, nf);
   }
 }
 
@@ -84,9 +121,10 @@ __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
 #pragma unroll
     for (int x = 1; x < NG; ++x) v += part[x][threadIdx.x];
   }
-  if (nck > 1 && 4 * c < p.dmem)
-    *(u32x2 *)((uint16_t *)p.out + (r * p.H + h) * p.dmem + 4 * c) =
-        (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
+  if (nck <= 1 || 4 * c >= p.dmem) return;
+  const int64_t at = (r * p.H + h) * p.dmem + 4 * c;
+  if constexpr (sizeof(T) == 4) *(f32x4 *)((float *)p.out + at) = v;
+  else *(u32x2 *)((uint16_t *)p.out + at) = (u32x2){Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w)};
 }
 
 template <typename T, int D> void reduce_t(const ReduceArgs &a, hipStream_t st) {
@@ -105,7 +143,8 @@ template <class F> void by_type(int dtype, int D, F &&f) {
     else f(t, std::integral_constant<int, 32>{});
   };
   if (dtype == kBF16) d((__bf16 *)nullptr);
-  else d((_Float16 *)nullptr);
+  else if (dtype == kF16) d((_Float16 *)nullptr);
+  else d((float *)nullptr);
 }
 
 }  // namespace
@@ -114,7 +153,16 @@ int paged_block(int D) { return 32 * waves_of(D); }
 
 void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st) {
   by_type(dtype, D, [&](auto *t, auto d) {
-    fwd_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(p, units, causal, st);
+    using T = std::remove_pointer_t<decltype(t)>;
+    if constexpr (sizeof(T) == 2) fwd_t<T, decltype(d)::value>(p, units, causal, st);
+  });
+}
+
+void launch_paged_mixed(const PagedParams &pf, int nf, const PagedParams &pd, int nd, int dtype, int D, bool causal,
+                        hipStream_t st) {
+  by_type(dtype, D, [&](auto *t, auto d) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if constexpr (sizeof(T) == 2) mixed_t<T, decltype(d)::value>(pf, nf, pd, nd, causal, st);
   });
 }
 
@@ -124,7 +172,7 @@ void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int 
   a.ws[0] = fwd.ws, a.ws[1] = decode.ws;
   a.cut[0] = fwd.split_units > 0 ? fwd.cut : nullptr;
   a.cut[1] = decode.split_units > 0 ? decode.cut : nullptr;
-  a.block[0] = paged_block(D), a.block[1] = 32, a.cols = decode.cols_hi;
+  a.block[0] = dtype == kF32 ? kPagedBlockF32 : paged_block(D), a.block[1] = 32, a.cols = decode.cols_hi;
   by_type(dtype, D, [&](auto *t, auto d) {
     reduce_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(a, st);
   });
