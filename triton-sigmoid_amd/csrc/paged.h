@@ -78,12 +78,23 @@ __device__ __forceinline__ float wave_sum(float x) {
 // of up to 64 sequences take a shorter C where that many units allow it.
 __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
   const int lane = __lane_id();
-  const int Lq0 = lane < p.B ? p.len_q(lane) : 0, Lk0 = lane < p.B ? p.keys(lane) : 0;
+  // The first 64 * kKeep sequences' lengths stay in registers, their loads in
+  // flight together.
+  constexpr int kKeep = 4;
+  int tokens[kKeep], keys[kKeep];
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int b = lane + 64 * i;
+    tokens[i] = b < p.B ? p.len_q(b) : 0, keys[i] = b < p.B ? p.keys(b) : 0;
+  }
   int C = 1 << 30;  // more than any length
   if (p.split_units > 0) {
-    const int nqb0 = p.blocks_of(Lq0, block);
-    float work = (float)nqb0 * (float)Lk0;
-    for (int b = lane + 64; b < p.B; b += 64) work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
+    const int nqb0 = p.blocks_of(tokens[0], block), Lk0 = keys[0];
+    float work = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) work += (float)p.blocks_of(tokens[i], block) * (float)keys[i];
+    for (int b = lane + 64 * kKeep; b < p.B; b += 64)
+      work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
     work = wave_sum(work) * (float)p.Hkv;
     const float c = work / (float)p.split_units;
     C = max(p.min_chunk, (int)fminf(c, 1e9f) + 1);
@@ -105,26 +116,32 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
   PagedUnit un;
   const int row = u / p.Hkv;
   un.hk = u - row * p.Hkv;
-  for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int Lq = b0 == 0 ? Lq0 : b < p.B ? p.len_q(b) : 0, Lk = b0 == 0 ? Lk0 : b < p.B ? p.keys(b) : 0;
+  int base = 0;
+  // Whether the unit is one of the 64 sequences' from b0 on (then `un` has it).
+  const auto among = [&](int b0, int Lq, int Lk) SIGATTN_INLINE {
     const int nqb = p.blocks_of(Lq, block), nck = max((Lk + C - 1) / C, 1);
     const int sum = wave_scan(nqb * nck), first = base + sum - nqb * nck;
     const uint64_t m = __ballot(row >= first && row < base + sum);
-    if (m != 0) {
-      const int at = __builtin_ctzll(m);
-      un.b = b0 + at;
-      un.Lq = __builtin_amdgcn_readlane(Lq, at), un.Lk = __builtin_amdgcn_readlane(Lk, at);
-      un.nck = __builtin_amdgcn_readlane(nck, at);
-      const int r = row - __builtin_amdgcn_readlane(first, at), q = r / un.nck, chunk = r - q * un.nck;
-      un.qb = __builtin_amdgcn_readlane(nqb, at) - 1 - q;
-      const int len = ((un.Lk + un.nck - 1) / un.nck + 63) & ~63;
-      un.k0 = min(chunk * len, un.Lk), un.k1 = min(un.k0 + len, un.Lk);
-      if (p.split_units > 0 && r == 0 && un.hk == 0 && lane == at)
-        p.cut[b] = make_int2(first, nck);
-      break;
-    }
     base += __builtin_amdgcn_readlane(sum, 63);
+    if (m == 0) return false;
+    const int at = __builtin_ctzll(m);
+    un.b = b0 + at;
+    un.Lq = __builtin_amdgcn_readlane(Lq, at), un.Lk = __builtin_amdgcn_readlane(Lk, at);
+    un.nck = __builtin_amdgcn_readlane(nck, at);
+    const int r = row - __builtin_amdgcn_readlane(first, at), q = r / un.nck, chunk = r - q * un.nck;
+    un.qb = __builtin_amdgcn_readlane(nqb, at) - 1 - q;
+    const int len = ((un.Lk + un.nck - 1) / un.nck + 63) & ~63;
+    un.k0 = min(chunk * len, un.Lk), un.k1 = min(un.k0 + len, un.Lk);
+    if (p.split_units > 0 && r == 0 && un.hk == 0 && lane == at) p.cut[un.b] = make_int2(first, nck);
+    return true;
+  };
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (!found && 64 * i < p.B) found = among(64 * i, tokens[i], keys[i]);
+  for (int b0 = 64 * kKeep; !found && b0 < p.B; b0 += 64) {
+    const int b = b0 + lane;
+    found = among(b0, b < p.B ? p.len_q(b) : 0, b < p.B ? p.keys(b) : 0);
   }
   // Wave-uniform as they are; the compiler is told so (scalar addresses).
   for (int *x : {&un.b, &un.hk, &un.qb, &un.Lq, &un.Lk, &un.k0, &un.k1, &un.nck})
