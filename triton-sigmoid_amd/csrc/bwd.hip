@@ -330,27 +330,31 @@ __device__ __forceinline__ void store_part(const KParams &p, int part, int b, in
 
 // dK and dV of head-split items: the sum of the parts' fp32 rows in their
 // order, rounded once.  Rows that no sequence covers are left to the dQ launch,
-// which zeroes them.  Eight elements a thread; bound by memory.
-template <typename T> __global__ __launch_bounds__(256) void add_parts_kernel(const KParams p) {
-  const int64_t per_row = (int64_t)p.H * p.dmem / 8, n = p.rows_k * per_row;
+// which zeroes them.  Eight elements a thread, per_row threads a row, as many
+// rows to a workgroup as it has threads for; bound by memory.
+template <typename T> __global__ __launch_bounds__(256) void add_parts_kernel(const KParams p, int per_row) {
+  const int rows = per_row < 256 ? 256 / per_row : 1, mine = (int)threadIdx.x / per_row;
+  const int64_t row = (int64_t)blockIdx.x * rows + mine;
+  if (mine >= rows || row >= p.rows_k) return;
+  int lo = 0, hi = p.B - 1;  // the last sequence that begins at or before the row
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (packed_first(p.cu_k, p.rows_k, mid) <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t first = packed_first(p.cu_k, p.rows_k, lo);
+  if (row < first || row - first >= p.len_k(lo)) return;
   const int64_t tensor = p.rows_k * p.H * p.dmem;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per_row, c = 8 * (i - row * per_row);
-    int lo = 0, hi = p.B - 1;  // the last sequence that begins at or before the row
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (packed_first(p.cu_k, p.rows_k, mid) <= row) lo = mid;
-      else hi = mid - 1;
-    }
-    if (row - packed_first(p.cu_k, p.rows_k, lo) >= p.len_k(lo) || row < packed_first(p.cu_k, p.rows_k, lo)) continue;
-    const int h = (int)(c / p.dmem), d = (int)(c - (int64_t)h * p.dmem);
+  for (int i = (int)threadIdx.x - mine * per_row; i < per_row; i += 256) {
+    const int c = 8 * i, h = c / p.dmem, d = c - h * p.dmem;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x4 v[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
       const float *src = p.kv_part + t * tensor + row * p.H * p.dmem + c;
-      for (int s = 0; s < p.qsplit; ++s, src += 2 * tensor) {
-        v[0] += *(const f32x4 *)src;
-        v[1] += *(const f32x4 *)(src + 4);
+#pragma unroll 4
+      for (int s = 0; s < p.qsplit; ++s) {
+        v[0] += *(const f32x4 *)(src + 2 * s * tensor);
+        v[1] += *(const f32x4 *)(src + 2 * s * tensor + 4);
       }
       *(u32x4 *)((uint16_t *)(t == 0 ? p.dk : p.dv) + row * p.sk_t + h * p.sk_h + d) =
           (u32x4){Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[0].z, v[0].w), Elem<T>::pack(v[1].x, v[1].y),
@@ -1587,8 +1591,8 @@ void launch_bwd_dkdv_mfma(const KParams &p, int dtype, int D, bool causal, bool 
     }
     if (!dsout) bwd_dkdv_t<T, DD, false>(p, causal, sm, st);
     if (p.qgroup > 1 && p.qsplit > 1) {
-      const int64_t n = (p.rows_k * p.H * p.dmem / 8 + 255) / 256;
-      add_parts_kernel<T><<<dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st>>>(p);
+      const int per_row = p.H * p.dmem / 8, rows = per_row < 256 ? 256 / per_row : 1;
+      add_parts_kernel<T><<<dim3((unsigned)((p.rows_k + rows - 1) / rows)), dim3(256), 0, st>>>(p, per_row);
     }
   });
 }

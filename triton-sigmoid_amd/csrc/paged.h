@@ -98,7 +98,7 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     work = wave_sum(work) * (float)p.Hkv;
     const float c = work / (float)p.split_units;
     C = max(p.min_chunk, (int)fminf(c, 1e9f) + 1);
-    if (p.B <= 64) {
+    if (p.B <= 64 && p.Tk < 1 << 23) {  // (where the quotients below are exact enough)
       // The smallest of 64 lengths, one a lane, that gives no more units than
       // fit: from the work's share of all of them up to C, which does.
       const float least = work / (float)p.total_units;
