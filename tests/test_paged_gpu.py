@@ -571,3 +571,74 @@ def test_python_binding(monkeypatch):
     for a, b in zip(one, two):
         assert torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a,
                            b.nan_to_num(7.0) if b.is_floating_point() else b)
+
+
+@pytest.mark.parametrize("heads", [(64, 1), (48, 1), (33, 1), (40, 2)], ids=lambda h: f"{h[0]}x{h[1]}")
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_groups_of_more_heads_than_a_block(heads, dtype):
+    for D in (64, 128):
+        check([0, 700, 40], [1, 1, 1], 16, *heads, D, DT[dtype])
+        check([100, 30], [5, 1], 16, *heads, D, DT[dtype])
+
+
+def test_wide_integers():
+    """int64 tables, slots and lengths; values past 32 bits are clamped: a slot
+    or page there is none, not another one."""
+    ctx, new = [40, 100], [1, 1]
+    q, kc, vc, table, lens, cu, rows = make(ctx, new, 16, 4, 2, 64, torch.bfloat16, fill=0.0)
+    wide = table.long()
+    wide[0, 0] = 2 ** 32 + int(table[0, 1])
+    got = ts.sigmoid_attention_paged(q, kc, vc, wide, lens.long(), cu.long(), 1)
+    assert_within(got, reference(q, rows, new, False, absent=[list(range(16)), []]), "o")
+    k = torch.ones(2, 2, 64, device="cuda").bfloat16()
+    before = kc.clone()
+    ts.paged_cache_write(k, k, kc, vc, torch.tensor([2 ** 32, -(2 ** 40)], device="cuda"))
+    assert torch.equal(kc, before)
+    plan = ts.paged_plan(ints([40, 100]).long(), ints(new).long(), table, ints([0]).long(), 16, 2)
+    assert plan.slot_mapping.dtype == I32
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_offsets_past_32_bits(dtype):
+    """A cache of more than 2^32 bytes a tensor (pages far apart): the last pages
+    are written and read."""
+    ps, Hkv, D, H = 16, 2, 64, 4
+    pages = 9
+    stride = 2 ** 29 // (1 if dtype == "bf16" else 2) + 64  # elements from page to page: 1 GiB
+    buf = torch.empty(2, (pages - 1) * stride + ps * Hkv * D, dtype=DT[dtype], device="cuda")
+    kc, vc = (t.as_strided((pages, ps, Hkv, D), (stride, Hkv * D, D, 1)) for t in buf)
+    g = torch.Generator().manual_seed(1)
+    lens, new = [70, 40], [1, 20]
+    rows = [torch.randn(2, n, Hkv, D, generator=g).to(DT[dtype]).cuda() for n in lens]
+    table = ints([[8, 0, 7, 5, 6], [4, 3, 1, -1, -1]])
+    pos = [torch.arange(n) for n in lens]
+    slots = torch.cat([table[b].cpu()[p // ps] * ps + p % ps for b, p in enumerate(pos)]).to(I32).cuda()
+    k, v = (torch.cat([r[i] for r in rows]) for i in range(2))
+    ts.paged_cache_write(k, v, kc, vc, slots)
+    assert torch.equal(kc[8, 3], rows[0][0][3]) and torch.equal(vc[6, 5], rows[0][1][69])
+    q = torch.randn(21, H, D, generator=g).to(DT[dtype]).cuda()
+    got = ts.sigmoid_attention_paged(q, kc, vc, table, ints(lens), ints(offsets(new)), 20, is_causal=True)
+    assert_within(got, reference(q, rows, new, True), "o")
+    got = ts.sigmoid_attention_paged(q[:2], kc, vc, table, ints(lens), ints([0, 1, 2]), 1)
+    assert_within(got, reference(q[:2], rows, [1, 1], False), "o")
+
+
+def test_two_calls_at_once_on_one_cache():
+    """Attention on two streams at once, of other sequences of one cache."""
+    ctx, new = [2000, 100, 900, 50], [1, 30, 1, 30]
+    q, kc, vc, table, lens, cu, rows = make(ctx, new, 16, 8, 2, 64, torch.bfloat16)
+    at = offsets(new)
+    halves = [(slice(0, 2), slice(0, at[2])), (slice(2, 4), slice(at[2], at[4]))]
+    want = [ts.sigmoid_attention_paged(q[r], kc, vc, table[b], lens[b], ints(offsets(new[b])), 30, is_causal=True)
+            for b, r in halves]
+    cus = [ints(offsets(new[b])) for b, _ in halves]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, (b, r), c in zip(streams, halves, cus):
+            with torch.cuda.stream(s):
+                got.append(ts.sigmoid_attention_paged(q[r], kc, vc, table[b], lens[b], c, 30, is_causal=True))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

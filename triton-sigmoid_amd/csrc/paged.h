@@ -29,6 +29,7 @@ struct PagedParams : KParams {
   int own_bias;          // 0: the bias is -log(keys)
   int cols_lo, cols_hi;
   int split_units, total_units, min_chunk;
+  int max_units;         // units that `ws` has room for
   int2 *cut;             // [B] (first unit / Hkv, chunks)
 
   __device__ __forceinline__ int keys(int b) const { return clamp_len(lens, b, Tk); }

@@ -135,6 +135,7 @@ PagedParams of_part(const PagedParams &k, const Part &part, int lo, int hi, int2
   PagedParams s = k;
   s.cols_lo = lo, s.cols_hi = hi;
   s.split_units = part.split_units, s.total_units = part.total_units, s.min_chunk = part.min_chunk;
+  s.max_units = (int)part.units;
   s.cut = cut, s.ws = ws;
   return s;
 }

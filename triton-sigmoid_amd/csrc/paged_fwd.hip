@@ -76,7 +76,7 @@ struct ReduceArgs {
   PagedParams p;
   const float *ws[2];   // blocks of more than / up to `cols` columns
   const int2 *cut[2];   // nullptr: no sequence was cut there
-  int block[2], cols;
+  int block[2], units[2], cols;
 };
 
 template <typename T, int D, bool ROWS>
@@ -106,6 +106,9 @@ __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
         const int block = a.block[few], hk = h / p.G, col = (int)tok * p.G + h - hk * p.G;
         const int nqb = (Lq * p.G + block - 1) / block, qb = col / block;
         const int64_t unit = (cut.x + (int64_t)(nqb - 1 - qb) * nck) * p.Hkv + hk;
+        // (Offsets that are out of order may leave a sequence without units and
+        // its cut unwritten: nothing is read past the partials.)
+        if (cut.x < 0 || nck > a.units[few] || unit + (int64_t)(nck - 1) * p.Hkv >= a.units[few]) nck = 0;
         const float *src = a.ws[few] + (unit * block + col - qb * block) * D + 4 * c;
         const int64_t step = (int64_t)p.Hkv * block * D;
 #pragma unroll 8
@@ -172,6 +175,7 @@ void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int 
   a.ws[0] = fwd.ws, a.ws[1] = decode.ws;
   a.cut[0] = fwd.split_units > 0 ? fwd.cut : nullptr;
   a.cut[1] = decode.split_units > 0 ? decode.cut : nullptr;
+  a.units[0] = fwd.max_units, a.units[1] = decode.max_units;
   a.block[0] = dtype == kF32 ? kPagedBlockF32 : paged_block(D), a.block[1] = 32, a.cols = decode.cols_hi;
   by_type(dtype, D, [&](auto *t, auto d) {
     reduce_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(a, st);

@@ -78,13 +78,20 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _ints(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """t as contiguous int32 on `dev`; wider integers are clamped, not wrapped."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
+    return _capi._as(t, torch.int32, dev)
+
+
 # --- plan -----------------------------------------------------------------------
 
 def _plan(context_lens, new_lens, block_table, free_pages, page_size, num_tokens):
     lib = _capi.load_library()
     _capi._check_device(block_table)
     dev = block_table.device
-    context_lens, new_lens, free_pages = (_capi._as(t, torch.int32, dev) for t in (context_lens, new_lens, free_pages))
+    context_lens, new_lens, free_pages = (_ints(t, dev) for t in (context_lens, new_lens, free_pages))
     B = block_table.shape[0]
     slots = torch.empty(num_tokens, dtype=torch.int32, device=dev)
     cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
@@ -185,7 +192,7 @@ def _write(key, value, key_cache, value_cache, slot_mapping):
     key, value = _unit(key), _unit(value)
     if key.stride() != value.stride():
         key, value = key.contiguous(), value.contiguous()
-    slot_mapping = _capi._as(slot_mapping, torch.int32, dev)
+    slot_mapping = _ints(slot_mapping, dev)
     r = _capi.SigattnPagedRows()
     r.esize = key.element_size()
     r.rows, r.kv_heads, r.D = key.shape
@@ -282,10 +289,10 @@ def _attend(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q
         if t.device != dev:
             raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
     query = _unit(query)
-    seq_lens_k, cu_seqlens_q = (_capi._as(t, torch.int32, dev) for t in (seq_lens_k, cu_seqlens_q))
+    seq_lens_k, cu_seqlens_q = (_ints(t, dev) for t in (seq_lens_k, cu_seqlens_q))
     if block_table.dtype != torch.int32 or block_table.device != dev or (
             block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        block_table = block_table.to(device=dev, dtype=torch.int32).contiguous()
+        block_table = _ints(block_table, dev)
     score_mod = _capi._as(score_mod, torch.float32, dev)
     out = torch.empty(query.shape, dtype=query.dtype, device=dev)
     if out.numel() == 0:
