@@ -600,6 +600,80 @@ def decode_bench(iters: int = 20):
     return rows
 
 
+# Serving steps over a paged cache (bench.py --serve): bf16, requests with
+# ~U[lo, hi] tokens in the cache, the first `ones` of which add one token and the
+# others `new`.
+SERVE_CONFIGS = [
+    dict(requests=64, ones=64, new=1, lo=1024, hi=8192, H=32, H_kv=8, D=128, page=16),
+    dict(requests=16, ones=16, new=1, lo=1024, hi=8192, H=32, H_kv=8, D=128, page=16),
+    dict(requests=1, ones=1, new=1, lo=65536, hi=65536, H=32, H_kv=8, D=128, page=64),
+    dict(requests=34, ones=32, new=512, lo=1024, hi=8192, H=32, H_kv=8, D=128, page=16),
+    dict(requests=2, ones=0, new=1024, lo=4096, hi=8192, H=32, H_kv=8, D=128, page=16),
+]
+
+
+def serve_bench(iters: int = 30):
+    """Serving steps through the public functions: paged_plan once a step, then
+    paged_cache_write and sigmoid_attention_paged for one layer, each timed
+    alone (events around `iters` calls) and the three together."""
+    import random
+
+    import torch
+    import triton_sigmoid as ts
+    dev = torch.device("cuda", 0)
+    rows = []
+    for cfg in SERVE_CONFIGS:
+        r, g = random.Random(cfg["requests"] + cfg["hi"]), torch.Generator(device=dev).manual_seed(1)
+        ps, H, Hkv, D = cfg["page"], cfg["H"], cfg["H_kv"], cfg["D"]
+        ctx = [r.randint(cfg["lo"], cfg["hi"]) for _ in range(cfg["requests"])]
+        new = [1 if b < cfg["ones"] else cfg["new"] for b in range(cfg["requests"])]
+        held, N = [-(-c // ps) for c in ctx], sum(new)
+        total = sum(-(-(c + n) // ps) for c, n in zip(ctx, new))
+        pool = torch.randperm(total, generator=g, device=dev).to(torch.int32)
+        width = max(-(-(c + n) // ps) for c, n in zip(ctx, new))
+        table, at = torch.full((len(ctx), width), -1, dtype=torch.int32, device=dev), 0
+        for b, n in enumerate(held):
+            table[b, :n] = pool[at:at + n]
+            at += n
+        free = pool[at:].contiguous()
+        normal = lambda *shape: torch.randn(shape, generator=g, device=dev, dtype=torch.bfloat16)
+        kc, vc = normal(total, ps, Hkv, D), normal(total, ps, Hkv, D)
+        q, k, v = normal(N, H, D), normal(N, Hkv, D), normal(N, Hkv, D)
+        ctx_t, new_t = (torch.tensor(x, dtype=torch.int32, device=dev) for x in (ctx, new))
+        plan = lambda: ts.paged_plan(ctx_t, new_t, table, free, ps, N)
+        p = plan()
+        write = lambda p=p: ts.paged_cache_write(k, v, kc, vc, p.slot_mapping)
+        attend = lambda p=p: ts.sigmoid_attention_paged(q, kc, vc, p.block_table, p.seq_lens, p.cu_seqlens, max(new),
+                                                        is_causal=True)
+
+        def step():
+            s = plan()
+            write(s)
+            return attend(s)
+
+        row = dict(cfg, tokens=N)
+        for name, fn in (("plan", plan), ("write", write), ("attention", attend), ("step", step)):
+            for _ in range(5):
+                fn()
+            torch.cuda.synchronize()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(iters):
+                fn()
+            b.record()
+            b.synchronize()
+            row[name + "_us"] = round(1e3 * a.elapsed_time(b) / iters, 2)
+        keys = sum(ctx) + N
+        pairs = sum(n * c + n * (n + 1) // 2 for c, n in zip(ctx, new))
+        row["attention_gbps"] = round((2 * keys * Hkv + 2 * N * H) * D * 2 / row["attention_us"] / 1e3, 1)
+        row["attention_tflops"] = round(4 * D * H * pairs / row["attention_us"] / 1e6, 2)
+        rows.append(row)
+        log(f"[serve] {row}")
+        del kc, vc, q, k, v
+        torch.cuda.empty_cache()
+    return rows
+
+
 def workload_name(name, cfg) -> str:
     shape = f"B={cfg['B']} L={cfg['L']} H={cfg['H']} D={cfg['D']} {cfg['dtype']} causal={cfg['causal']}"
     if cfg.get("padded"):
@@ -636,6 +710,8 @@ def main():
                     help="one point of that grid")
     ap.add_argument("--decode", action="store_true",
                     help="split-KV forward at decode shapes (HBM GB/s)")
+    ap.add_argument("--serve", action="store_true",
+                    help="serving steps over a paged cache: plan, cache write and attention (us)")
     ap.add_argument("--ceiling", action="store_true",
                     help="hipBLASLt bf16 GEMM TFLOPS on random and on zero operands (the box's practical MFMA rate)")
     ap.add_argument("--kernels", choices=("dense", "padded", "packed"),
@@ -657,6 +733,10 @@ def main():
         return
     if args.copy_calibration:
         copy_calibration()
+        return
+    if args.serve:
+        print(json.dumps({"metric": "serving steps over a paged cache, one layer: us per call", "unit": "us",
+                          "rows": serve_bench()}), flush=True)
         return
     if args.decode:
         rows = decode_bench()
