@@ -941,9 +941,7 @@ template <int D> void dkdv_t(const KParams &kp, bool causal, bool scoremod, hipS
 // columns share 32-key tiles of K and V in two stages, copied one tile ahead
 // through the block table; columns, key chunks and rows that are not there are
 // the 16-bit kernel's.  D MFMAs of 64 cycles a wave and tile bound it: 82 TFLOP/s
-// with full blocks (2 x 300 tokens on 1000 keys H=32 Hkv=8 D=128, 137 us), and in
-// decoding, where one wave of four has columns, 2.6 TB/s (16 requests, contexts
-// 1024..8191, 190 us).
+// with full blocks (2 x 300 tokens on 1000 keys H=32 Hkv=8 D=128, 137 us).
 template <int D, bool CAUSAL, bool SCOREMOD>
 __global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const PagedParams p) {
   constexpr int NDB = D / 32, BM = 32 * FW;
@@ -1025,6 +1023,109 @@ __global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const PagedParams
   else store_row<D>(p.ws + ((int64_t)wg * BM + myq - q0) * D, acc, 1.0f, true, hi, half);
 }
 
+// The same for batches of up to 32 columns a sequence (decoding): every wave has a
+// unit of its own (paged_decode.h), here with one 32-key stage each of K and V,
+// the next K block copied while P·V runs and the next V block while Q·Kᵀ does.
+// Four waves' D MFMAs of 64 cycles a tile keep up with memory, where the kernel
+// above has columns for one wave of four.  Whole call, us, there / here, H=32 Hkv=8
+// contexts 1024..8191: B=16 D=128 193 / 102 (4.9 TB/s), D=64 114 / 53, D=32 82 / 36;
+// B=64 D=128 988 / 442 (5.4 TB/s); B=1 23 / 21.
+template <int D, bool CAUSAL, bool SCOREMOD>
+__global__ __launch_bounds__(64 * FW, 1) void paged_f32_decode_kernel(const PagedParams p) {
+  constexpr int NDB = D / 32, NW = FW;
+  __shared__ __attribute__((aligned(16))) float sK[NW][FB * D], sV[NW][FB * D];
+  const int wg = gap_prologue<4>(p, sK);
+  if (wg < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const PagedUnit un = paged_unit(p, wg * NW + w, 32);
+  if (un.nck == 0) return;
+  const bool half = p.half_head(D);
+  const int cols = un.Lq * p.G, keys = un.k1 - un.k0, ntiles = (keys + FB - 1) / FB;
+  const int tok = l32 / p.G, head = un.hk * p.G + l32 - tok * p.G;
+  // Keys of the chunk that this lane's token sees, and that every token sees.
+  const int lim = un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0, all_see = un.Lk - un.Lq + 1 - un.k0;
+  const float bias = p.bias_of(un.Lk), nsl = -p.fscale * kLog2e, nbl = -bias * kLog2e;
+  const int64_t row0 = packed_first(p.cu_q, p.rows_q, un.b);
+  const uint16_t *Kb = (const uint16_t *)((const float *)p.k + (int64_t)un.hk * p.sk_h);
+  const uint16_t *Vb = (const uint16_t *)((const float *)p.v + (int64_t)un.hk * p.sk_h);
+  const float *mod = SCOREMOD ? p.score_mod + un.b * p.mod_stride + un.k0 : nullptr;
+  float qv[D / 2];
+  load_half_row<D>(qv, (const float *)p.q + (row0 + tok) * p.sq_t + (int64_t)head * p.sq_h, hi,
+                   l32 < cols && !(half && hi));
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc[db] = zero16();
+  using Dma = PagedDma<FB, 2 * D, 1, true, 4>;
+  Dma dma;
+  dma.init(p, un.b, un.k0, keys, 0, lane, half);
+  F32RowReads<D> rr;
+  rr.init(l32, hi);
+  uint16_t *tK = (uint16_t *)sK[w], *tV = (uint16_t *)sV[w];
+#pragma unroll
+  for (int s = 0; s < D / 2; ++s) asm volatile("" ::"v"(qv[s]));  // the copies are counted from here on
+  int now[Dma::NE];  // pages of the tile whose V block is copied next
+  if (ntiles > 0) {
+    dma.entries(0, now);
+    dma.load(FB);
+    dma.issue_at(tK, Kb, 0, now);
+    dma.issue_at(tV, Vb, 0, now);
+  }
+  for (int t = 0; t < ntiles; ++t) {
+    const int k0 = t * FB;
+    float c[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = nbl;
+    if (SCOREMOD) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[i] = -(bias + mod[min(k0 + 8 * (i / 4) + 4 * hi + i % 4, keys - 1)]) * kLog2e;
+      wait_dma();  // plain loads are not counted
+    } else {
+      wait_vm<Dma::NI>();  // K(t); V(t) may be in flight
+    }
+    f32x16 s = zero16();
+    head_product<D>(s, sK[w], qv, l32, hi);
+    const bool more = t + 1 < ntiles;
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of K(t) has returned
+#pragma unroll
+      for (int e = 0; e < Dma::NE; ++e) now[e] = dma.ent[e];
+      dma.issue_at(tK, Kb, k0 + FB, now);
+    }
+    float pr[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, c[i]));
+    if (CAUSAL && k0 + FB > all_see) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + 8 * (i / 4) + 4 * hi + i % 4 >= lim) pr[i] = 0.0f;
+    }
+    if (more) wait_vm<Dma::NI>();  // V(t); K(t + 1) may be in flight
+    else wait_dma();
+    row_product<D>(acc, sV[w], pr, rr);
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      dma.issue_at(tV, Vb, k0 + FB, now);
+      if (k0 + 2 * FB < keys) dma.load(k0 + 2 * FB);
+    }
+  }
+  if (l32 >= cols) return;
+  if (un.nck == 1) store_row<D>((float *)p.out + ((row0 + tok) * p.H + head) * p.dmem, acc, 1.0f, true, hi, half);
+  else store_row<D>(p.ws + ((int64_t)(wg * NW + w) * 32 + l32) * D, acc, 1.0f, true, hi, half);
+}
+
+template <int D> void paged_decode_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
+  const dim3 grid((unsigned)((units + FW - 1) / FW + p.ngap[0])), block(64 * FW);
+  if (causal) {
+    if (p.score_mod) paged_f32_decode_kernel<D, true, true><<<grid, block, 0, st>>>(p);
+    else paged_f32_decode_kernel<D, true, false><<<grid, block, 0, st>>>(p);
+  } else {
+    if (p.score_mod) paged_f32_decode_kernel<D, false, true><<<grid, block, 0, st>>>(p);
+    else paged_f32_decode_kernel<D, false, false><<<grid, block, 0, st>>>(p);
+  }
+}
+
 template <int D> void paged_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
   const dim3 grid((unsigned)(units + p.ngap[0])), block(64 * FW);
   if (causal) {
@@ -1037,6 +1138,12 @@ template <int D> void paged_t(const PagedParams &p, int units, bool causal, hipS
 }
 
 }  // namespace
+
+void launch_paged_decode_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st) {
+  if (D == 128) paged_decode_t<128>(p, units, causal, st);
+  else if (D == 64) paged_decode_t<64>(p, units, causal, st);
+  else paged_decode_t<32>(p, units, causal, st);
+}
 
 void launch_paged_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st) {
   if (D == 128) paged_t<128>(p, units, causal, st);

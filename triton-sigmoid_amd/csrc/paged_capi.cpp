@@ -65,20 +65,23 @@ struct Part {
 // in the forward's; a batch of one, whose length the host knows to be a long
 // one or does not know, runs in the forward's alone.
 // The decode kernel's chunks: a round of the waves that the GPU runs at a time
-// at D = 128 (four per CU), of 256 keys at least.  Whole call, us, bf16 H=32 Hkv=8
-// D=128 contexts 1024..8191: waves per CU 4 / 8, B=16 49 / 55, B=64 up to 3000
-// 100 / 101, B=200 up to 900 83 / 81, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s);
-// chunks of 128 / 192 / 256 keys, B=1 65536 keys H=16 Hkv=2 23.2 / 21.1 / 21.5,
-// 2000 keys 15.5 / 17.2 / 19.5, B=4 up to 8191 20.3 / 20.2 / 21.7.
+// at D = 128 (four per CU), of 64 keys at least.  Whole call, us, bf16 H=32 Hkv=8
+// D=128: waves per CU 4 / 8, B=16 contexts 1024..8191 49 / 55, B=64 1024..3000 100 /
+// 101, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s); chunks of 64 / 128 / 192 keys at
+// least, B=1 2000 keys 13.9 / 16.1 / 17.3, B=16 200..300 18.2 / 20.2 / 21.4, B=3
+// up to 8000 15.2 / 16.6 / 18.7, longer ones alike.
 constexpr int kDecodeCols = 32;
-constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 192;
+constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 64;
 // The forward kernel's chunks, where its blocks do not fill the GPU: a round of
 // its workgroups, of 1024 keys at least.  Whole call, us, one / two rounds: bf16
 // H=32 Hkv=8 D=128, 2 x 1024 tokens on up to 12000 keys 324 / 343, 256 on 12000
 // 57 / 77, 4 x 128 114 / 132, 2000 on none 59 / 89; chunks of 512 / 1024 / 2048
 // keys, 24 requests, 4 of up to 700 tokens on up to 4096 keys, H=12 Hkv=4 D=128
 // 87 / 69 / 83.
-constexpr int64_t kChunk = 1024, kChunkF32 = 256;
+constexpr int64_t kChunk = 1024;
+// (fp32 blocks: two rounds' worth of workgroups; chunks of 64 / 128 / 256 keys, us,
+// B=1 2000 keys 18 / 27 / 46.)
+constexpr int64_t kChunkF32 = 64;
 struct Plan {
   Part fwd, decode;
   int cols_lo = 0;  // columns that are not the forward kernel's
@@ -108,8 +111,9 @@ void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const Pag
 Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
   Plan pl;
   const int64_t cols = (int64_t)k.Tq * k.G, all = p->rows_q * k.G, cus = k.ncu;
-  const bool f32 = p->dtype == SIGATTN_F32;  // one kernel for all
-  const bool decode = !f32 && (cols <= kDecodeCols || k.B > 1), fwd = f32 || cols > kDecodeCols;
+  // (fp32: no launch for both, so one long sequence takes all to the blocks.)
+  const bool f32 = p->dtype == SIGATTN_F32;
+  const bool decode = cols <= kDecodeCols || (k.B > 1 && !f32), fwd = cols > kDecodeCols;
   pl.fwd.block = f32 ? sigattn::kPagedBlockF32 : sigattn::paged_block(D), pl.decode.block = 32;
   if (decode) {
     const int64_t pairs = (int64_t)k.B * k.Hkv;
@@ -122,7 +126,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
     const int64_t seqs = all / (pl.cols_lo + 1) < k.B ? all / (pl.cols_lo + 1) : k.B;
     const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = f32 ? 2 : D == 128 ? 1 : (D == 64 ? 3 : 4);
     const int64_t full = cdiv(all, pl.fwd.block) * k.Hkv;
-        cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, f32 ? kChunkF32 : kChunk, k, D);
+    cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, f32 ? kChunkF32 : kChunk, k, D);
   }
   const bool cut = pl.fwd.split_units > 0 || pl.decode.split_units > 0;
   pl.cut_bytes = cut ? cdiv((int64_t)k.B * 2 * (int64_t)sizeof(int2), 256) * 256 : 0;
@@ -221,6 +225,8 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
   first.ngap[0] = gaps;
   if (pl.fwd.units > 0 && pl.decode.units > 0)
     sigattn::launch_paged_mixed(first, (int)pl.fwd.units, kd, (int)pl.decode.units, dt, D, causal, st);
+  else if (pl.decode.units > 0 && dt == SIGATTN_F32)
+    sigattn::launch_paged_decode_f32(first, (int)pl.decode.units, D, causal, st);
   else if (pl.decode.units > 0) sigattn::launch_paged_decode(first, (int)pl.decode.units, dt, D, causal, st);
   else if (dt == SIGATTN_F32) sigattn::launch_paged_f32(first, (int)pl.fwd.units, D, causal, st);
   else sigattn::launch_paged_fwd(first, (int)pl.fwd.units, dt, D, causal, st);
