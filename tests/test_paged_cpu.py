@@ -62,6 +62,8 @@ def _write_args(**kw):
     (dict(key_cache=torch.zeros(4, 2, 16, 32, dtype=torch.bfloat16).transpose(1, 2)), ValueError, "same strides"),
     (dict(slot_mapping=torch.zeros(4, dtype=I32)), ValueError, r"slot_mapping must have shape \(3,\)"),
     (dict(key=torch.zeros(3, 2, 32)), RuntimeError, "share a dtype"),
+    (dict(zip(("key_cache", "value_cache"), (t[:, :, :1].expand(-1, -1, 2, -1) for t in _caches()))), ValueError,
+     "must not repeat rows"),
     (dict(key_cache=_caches(ps=24)[0], value_cache=_caches(ps=24)[0]), ValueError, "power of two"),
     (dict(zip(("key_cache", "value_cache"), _caches(dtype=torch.float64))), RuntimeError, "unsupported dtype"),
     (dict(zip(("key_cache", "value_cache"), _caches(D=48))), RuntimeError, "unsupported head dimension"),

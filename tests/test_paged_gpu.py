@@ -87,6 +87,37 @@ def test_plan_without_enough_pages_or_columns():
     check_plan([-3, 20], [5, -2], 16, 9)  # negative lengths count as none
 
 
+def test_plan_of_sums_past_32_bits_ends():
+    big, wide = (1 << 31) - 1, torch.full((4, 5), 99, dtype=I32, device="cuda")
+    table = wide[:3, 1:4]
+    ts.paged_plan(ints([big, 0, 5]), ints([big, 7, big]), table, ints([50, 51]), 1 << 20, 300)
+    torch.cuda.synchronize()
+    assert (wide[:, 0] == 99).all() and (wide[:, 4] == 99).all() and (wide[3] == 99).all()
+
+
+@pytest.mark.parametrize("binding", ["node", "python"])
+def test_autograd_sees_what_is_changed(monkeypatch, binding):
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    kc, vc = (torch.randn(4, 16, 2, 32, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table = torch.zeros(1, 2, dtype=I32, device="cuda")
+    at = table._version
+    plan = ts.paged_plan(ints([0]), ints([3]), table, ints([2, 1]), 16, 3)
+    assert table._version == at + 1
+    w = torch.ones((), device="cuda", requires_grad=True)
+    y = (w * kc).sum()
+    at = kc._version, vc._version
+    new = torch.randn(3, 2, 32, device="cuda", dtype=torch.bfloat16)
+    ts.paged_cache_write(new, new, kc, vc, plan.slot_mapping)
+    assert (kc._version, vc._version) == (at[0] + 1, at[1] + 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kc, vc = torch.zeros_like(kc), torch.zeros_like(vc)
+    ts.paged_cache_write(new, new, kc, vc, plan.slot_mapping)
+    assert torch.equal(kc[2, :3], new)
+
+
 def test_plan_keeps_other_entries_and_strides():
     wide = torch.full((3, 10), 99, dtype=I32, device="cuda")
     plan = ts.paged_plan(ints([17, 0, 3]), ints([16, 0, 1]), wide[:, 2:7], ints([50, 51, 52]), 16, 17)

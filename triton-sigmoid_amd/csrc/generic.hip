@@ -186,7 +186,7 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
       for (int j = 0; j < jn; ++j) {
         const int q = m0 + j;
         float s = 0.0f, dp = 0.0f;
-  #pragma unroll
+#pragma unroll
         for (int d = 0; d < D; ++d) {
           s = __builtin_fmaf(sQ[j][d], kv[d], s);
           dp = __builtin_fmaf(sO[j][d], vv[d], dp);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
         if (CAUSAL && key > q) { pr = 0.0f; ds = 0.0f; }
         pr = round_to<T>(pr);
         ds = round_to<T>(ds);
-  #pragma unroll
+#pragma unroll
         for (int d = 0; d < D; ++d) {
           dv[d] = __builtin_fmaf(pr, sO[j][d], dv[d]);
           dk[d] = __builtin_fmaf(ds, sQ[j][d], dk[d]);

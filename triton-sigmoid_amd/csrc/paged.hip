@@ -58,20 +58,20 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs a) {
   extern __shared__ int sums[];  // first token, then first free page, of each request and the end
   int *tok = sums, *page = sums + a.B + 1;
   const int tid = threadIdx.x, ps1 = (1 << a.lp) - 1;
-  const auto pages = [&](int tokens) { return (int)(((int64_t)tokens + ps1) >> a.lp); };
+  const auto pages = [&](int64_t tokens) { return (int)((tokens + ps1) >> a.lp); };
   // Each thread sums the requests of one contiguous piece.
   const int per = (a.B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int nt = 0, np = 0, all_t, all_p;
   for (int b = b0; b < b1; ++b) {
     const int c = plan_len(a.ctx, b), n = plan_len(a.add, b);
-    nt += n, np += pages(c + n) - pages(c);
+    nt += n, np += pages((int64_t)c + n) - pages(c);
   }
   scan2(nt, np, all_t, all_p);
   for (int b = b0; b < b1; ++b) {
     const int c = plan_len(a.ctx, b), n = plan_len(a.add, b);
     tok[b] = nt, page[b] = np;
     if (blockIdx.x == 0) a.cu[b] = nt, a.lens[b] = c + n;
-    nt += n, np += pages(c + n) - pages(c);
+    nt += n, np += pages((int64_t)c + n) - pages(c);
   }
   if (tid == 0) {
     tok[a.B] = all_t, page[a.B] = all_p;
@@ -88,21 +88,25 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs a) {
     }
     return lo;
   };
-  const auto fresh = [&](int i) { return (unsigned)i < (unsigned)a.num_free ? a.free_pages[i] : -1; };
+  const auto fresh = [&](int64_t i) { return i >= 0 && i < a.num_free ? a.free_pages[i] : -1; };
+  // (Positions and the loops' counters in 64 bits: lengths whose sums do not fit
+  // 32 give a useless plan, but an end and no access outside the tensors.)
   const int step = gridDim.x * kPlanThreads;
-  for (int i = blockIdx.x * kPlanThreads + tid; i < all_p; i += step) {
-    const int b = owner(page, i), j = pages(plan_len(a.ctx, b)) + i - page[b];
-    if ((unsigned)j < (unsigned)a.max_pages) a.table[b * a.table_stride + j] = fresh(i);
+  for (int64_t i = blockIdx.x * kPlanThreads + tid; i < all_p; i += step) {
+    const int b = owner(page, (int)i);
+    const int64_t j = pages(plan_len(a.ctx, b)) + i - page[b];
+    if (j >= 0 && j < a.max_pages) a.table[b * a.table_stride + j] = fresh(i);
   }
   for (int t = blockIdx.x * kPlanThreads + tid; t < a.num_tokens; t += step) {
     int slot = -1;
     if (t < all_t) {
-      const int b = owner(tok, t), c = plan_len(a.ctx, b), x = c + t - tok[b], j = x >> a.lp, held = pages(c);
-      if ((unsigned)j < (unsigned)a.max_pages) {
+      const int b = owner(tok, t), c = plan_len(a.ctx, b), held = pages(c);
+      const int64_t x = (int64_t)c + t - tok[b], j = x >> a.lp;
+      if (j >= 0 && j < a.max_pages) {
         // Pages of this step come from the free list itself: their table
         // entries may be another workgroup's to write.
         const int id = j < held ? a.table[b * a.table_stride + j] : fresh(page[b] + j - held);
-        if (id >= 0 && id <= INT32_MAX >> a.lp) slot = (id << a.lp) | (x & ps1);
+        if (id >= 0 && id <= INT32_MAX >> a.lp) slot = (id << a.lp) | (int)(x & ps1);
       }
     }
     a.slots[t] = slot;

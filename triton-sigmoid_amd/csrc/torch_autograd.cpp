@@ -463,6 +463,11 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
                                      std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
 }
 
+// Tells autograd of a tensor that was changed in place.
+void changed(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 bool page_size_ok(int64_t n) { return n >= 16 && n <= (1 << 20) && (n & (n - 1)) == 0; }
 
 // The paged cache's calls on canonical arguments (int32 tensors of one gfx950
@@ -492,6 +497,7 @@ py::object quick_plan(const py::object &context_lens, const py::object &new_lens
                             p(slots), p(cu), p(lens), p(needed),
                             c10::hip::getCurrentHIPStream(dev.index()).stream()),
            "sigattn_paged_plan");
+  changed(table);
   return py::make_tuple(slots, cu, lens, needed);
 }
 
@@ -514,6 +520,8 @@ bool quick_write(const py::object &key, const py::object &value, const py::objec
       k.size(2) != kc.size(3) || !Quick::ints(slot_mapping, slots, 1, dev) || slots.size(0) != k.size(0) ||
       !Quick::no_grad({&k, &v, &kc, &vc}))
     return false;
+  for (int i = 0; i < 3; ++i)
+    if (kc.size(i) > 1 && kc.stride(i) == 0) return false;
   sigattn_paged_rows r;
   std::memset(&r, 0, sizeof(r));
   r.esize = (int32_t)k.element_size();
@@ -525,6 +533,7 @@ bool quick_write(const py::object &key, const py::object &value, const py::objec
   r.slot_mapping = static_cast<const int32_t *>(slots.data_ptr());
   const c10::DeviceGuard guard(dev);
   check_rc(g_api.paged_write(&r, c10::hip::getCurrentHIPStream(dev.index()).stream()), "sigattn_paged_write");
+  changed(kc), changed(vc);
   return true;
 }
 

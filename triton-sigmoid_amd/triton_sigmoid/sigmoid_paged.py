@@ -85,6 +85,13 @@ def _ints(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     return _capi._as(t, torch.int32, dev)
 
 
+def _changed(*tensors: torch.Tensor) -> None:
+    """Tells autograd of tensors that were changed in place."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 # --- plan -----------------------------------------------------------------------
 
 def _plan(context_lens, new_lens, block_table, free_pages, page_size, num_tokens):
@@ -177,6 +184,7 @@ def paged_plan(
         got = paged_plan_op(context_lens, new_lens, block_table, free_pages, page_size, num_tokens)
     else:
         got = _plan(context_lens, new_lens, block_table, free_pages, page_size, num_tokens)
+        _changed(block_table)
     return PagedPlan(block_table, *got)
 
 
@@ -259,6 +267,9 @@ def paged_cache_write(
     if quick is not None and quick.quick_write(key, value, key_cache, value_cache, slot_mapping):
         return
     _check_caches(key_cache, value_cache)
+    if any(n > 1 and s == 0 for n, s in zip(key_cache.shape[:3], key_cache.stride())):
+        raise ValueError(f"the caches must not repeat rows (they are changed in place), got strides "
+                         f"{key_cache.stride()}")
     if key.dim() != 3 or value.dim() != 3:
         raise ValueError("Expected key and value to be 3D tensors (total_tokens, H_kv, D)")
     if key.shape != value.shape:
@@ -275,6 +286,7 @@ def paged_cache_write(
         paged_cache_write_op(key, value, key_cache, value_cache, slot_mapping)
     else:
         _write(key, value, key_cache, value_cache, slot_mapping)
+        _changed(key_cache, value_cache)
 
 
 # --- attention ----------------------------------------------------------------------
@@ -390,7 +402,8 @@ def sigmoid_attention_paged(
             row whose position is negative sees none and is zeros.
         scale: default 1/sqrt(D).
         sigmoid_bias: default -log(seq_lens_k[b]) per sequence.
-        score_mod: optional [B, max_pages * page_size] per-key term by position.
+        score_mod: optional [B, max_pages * page_size] per-key term by position
+            (no NaN below seq_lens_k).
 
     Returns:
         [N, H, D] output, contiguous.  Rows outside every sequence are zeros.
