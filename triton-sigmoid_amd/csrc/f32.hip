@@ -294,7 +294,7 @@ __device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, floa
       float pr[16], ds[16];
       head_product<D>(s, tQ, kv, l32, hi);
       head_product<D>(dp, tO, vv, l32, hi);
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int q = m0 + 8 * (i / 4) + 4 * hi + i % 4;
         pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
@@ -810,7 +810,7 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
       const f32x16 s = head3<D, Tiles::PART>(tQ, to, FB * wt, kf);
       const f32x16 dp = head3<D, Tiles::PART>(tO, to, FB * wt, vf);
       float pr[16], ds[16];
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
         pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, nc));
         const float u = pr[i] * dp[i];
@@ -820,7 +820,7 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
       if (m0 + FB > Lq || (CAUSAL && m0 < kw + 31)) {
         const int e_end = Lq - m0 - 4 * hi;               // query m0 + 4hi + e valid iff
         const int e_lo = CAUSAL ? myk - m0 - 4 * hi : 0;  // e_lo <= e < e_end
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int e = 8 * (i / 4) + i % 4;
           if (e >= e_end || e < e_lo) pr[i] = ds[i] = 0.0f;

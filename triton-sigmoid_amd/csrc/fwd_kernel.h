@@ -227,28 +227,28 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
 
     // This wave's query rows as B operands (k = d = 16s + 8h + j).
     u32x4 qf[NCB][NKS];
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < NCB; ++c) {
       const int q = myq0 + 32 * c;
       const bool ok = q < Lq;
       const uint16_t *qrow;
       if constexpr (PAGED) qrow = Qb + (int64_t)(q / p.G) * p.sq_t + (int64_t)(q % p.G) * p.sq_h + 8 * hi;
       else qrow = Qb + (int64_t)q * p.sq_t + 8 * hi;
-  #pragma unroll
+#pragma unroll
       for (int s = 0; s < NKS; ++s)
         qf[c][s] = ok && !(half && s > 0) ? *(const u32x4 *)(qrow + 16 * s) : zero4();
     }
     // Consume the Q loads here, so the compiler's wait for them is not placed
     // at the head of the key loop, where it would also wait for the tile copies.
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < NCB; ++c)
-  #pragma unroll
+#pragma unroll
       for (int s = 0; s < NKS; ++s) asm volatile("" ::"v"(qf[c][s]));
 
     f32x16 acc[NCB][NDB];
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < NCB; ++c)
-  #pragma unroll
+#pragma unroll
       for (int d = 0; d < NDB; ++d) acc[c][d] = zero16();
 
     TileOffsets<D> to;
@@ -265,7 +265,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     // Causal limits of this lane's columns and the keys that all of the wave's see.
     [[maybe_unused]] int lims[NCB], all_see = 0;
     if constexpr (PAGED && CAUSAL) {
-  #pragma unroll
+#pragma unroll
       for (int c = 0; c < NCB; ++c) lims[c] = max(min(Lk, seen(min(myq0 + 32 * c, Lq - 1))), 0);
       all_see = seen(min(qw, Lq - 1));
     }
@@ -312,11 +312,11 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     auto mask_words = [&](uint32_t (&pk)[NCB][8], int g) SIGATTN_INLINE {
       int kbase = 32 * g;
       asm volatile("" : "+s"(kbase));  // keeps this rare fix-up in its own branch
-  #pragma unroll
+#pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
         unsigned lim = CAUSAL ? (unsigned)min(Lk, myq0 + 32 * cb + 1) : (unsigned)Lk;
         if constexpr (PAGED && CAUSAL) lim = (unsigned)lims[cb];
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int i = 2 * e;
           const unsigned k0 = (unsigned)(kbase + 8 * (i / 4) + 4 * hi + (i % 4));
@@ -368,19 +368,19 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       float c[16];   // exp2 offsets of block r-1 (per key row)
       float cn[2];   // ... of block r's first word
       if constexpr (SCOREMOD) {
-  #pragma unroll
+#pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 cv = *(const float4 *)&sC[STVn * BN + KLn + cl + 8 * g + 4 * hi];
           c[4 * g + 0] = cv.x; c[4 * g + 1] = cv.y; c[4 * g + 2] = cv.z; c[4 * g + 3] = cv.w;
         }
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 2; ++i) cn[i] = sC[STC * BN + KL + cl + 4 * hi + i];
       } else {
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 16; ++i) c[i] = nbl;
         cn[0] = cn[1] = nbl;
       }
-  #pragma unroll
+#pragma unroll
       for (int step = 0; step < NSTEP; ++step) {
         if ((WK == 2 || (U % 2) == 1) && step == BAR) {
           const int u = (r + 1) / RPT;
@@ -401,11 +401,11 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
         asm volatile("" ::"v"(opq[step % LA]));
         const u32x4 a = opq[step % LA];
         if (step < NKS) {
-  #pragma unroll
+#pragma unroll
           for (int c2 = 0; c2 < NCB; ++c2) sc[c2] = Elem<T>::mfma(a, qf[c2][step], step == 0 ? zero16() : sc[c2]);
         } else {
           const int i = step - NKS, j = i / NDB, db = i % NDB;
-  #pragma unroll
+#pragma unroll
           for (int c2 = 0; c2 < NCB; ++c2) {
             const u32x4 bp = (u32x4){pp[c2][4 * j], pp[c2][4 * j + 1], pp[c2][4 * j + 2], pp[c2][4 * j + 3]};
             acc[c2][db] = Elem<T>::mfma(a, bp, acc[c2][db]);
@@ -416,7 +416,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
         // Sigmoid words of this step: stage B (reciprocal, packing) of word wd
         // from ea, then stage A (exp2) of the next word into ea -- in the last
         // word, of block r's first word (its Sᵀ chains are complete by then).
-  #pragma unroll
+#pragma unroll
         for (int wd = step * NWD / NSTEP; wd < (step + 1) * NWD / NSTEP; ++wd) {
           {
             const int cb = wd / 8, e = wd % 8;
@@ -434,7 +434,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
             ea[1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][1], nsl, cn[1]));
           }
         }
-  #pragma unroll
+#pragma unroll
         for (int c2 = 0; c2 < NCB; ++c2) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -450,12 +450,12 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     // (tile NST-1 is copied into it from the barrier of region 2·NST-5 on,
     // after every read of blocks -2 and -1), so 0 * operand stays 0.  WK = 2:
     // from stages NST-2 and NST-1, refilled in regions 0 and 1.
-  #pragma unroll
+#pragma unroll
     for (int x = 0; x < 2; ++x) {
-  #pragma unroll
+#pragma unroll
       for (int c2 = 0; c2 < NCB; ++c2) {
         sbuf[x][c2] = zero16();
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 8; ++e) pbuf[x][c2][e] = 0u;
       }
     }
@@ -473,7 +473,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     }
     __syncthreads();
     if (ntiles > 1) issue(1, 1);
-  #pragma unroll
+#pragma unroll
     for (int o = 0; o < LA; ++o) opq[o] = read_op(o, 0, NST - 1, 0);
 
     // This wave computes only up to its own last visible key block (causal) and
@@ -530,15 +530,15 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     }
 
     // Oᵀ accumulators -> O rows (4 consecutive d per 8-byte store).
-  #pragma unroll
+#pragma unroll
     for (int c = 0; c < NCB; ++c) {
       const int q = myq0 + 32 * c;
       if (q < p.q_rows_out(Lq)) {
         uint16_t *orow = Ob + (int64_t)q * p.sq_t;
         const bool valid = q < Lq;
-  #pragma unroll
+#pragma unroll
         for (int db = 0; db < NDB; ++db) {
-  #pragma unroll
+#pragma unroll
           for (int g = 0; g < 4; ++g) {
             if (half && g >= 2) break;  // columns 16..31: not in the tensor
             const int d0 = db * 32 + 8 * g + 4 * hi;
