@@ -354,6 +354,21 @@ def test_rows_outside_every_sequence_are_zero(new):
         assert not got[sum(new):].any()
 
 
+@pytest.mark.parametrize("B", [2, 70])
+@pytest.mark.parametrize("new", [1, 200], ids=["decode", "chunk"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_rows_before_the_first_sequence_are_zero(dtype, new, B):
+    # Contexts long enough to be cut: the sums of parts know the rows of no sequence too.
+    n = [new] + [1] * (B - 1)
+    q, kc, vc, table, lens, cu, _ = make([4000, 3000] + [5] * (B - 2), n, 16, 4, 2, 32, dtype)
+    want = ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, new, is_causal=True)
+    more = torch.cat([q, q, q])[:sum(n) + 60] if sum(n) > 60 else q.repeat(80, 1, 1)[:sum(n) + 60]
+    more[37:37 + sum(n)] = q
+    got = ts.sigmoid_attention_paged(more.contiguous(), kc, vc, table, lens, cu + 37, new, is_causal=True)
+    assert not got[:37].any() and not got[37 + sum(n):].any()
+    assert torch.equal(got[37:37 + sum(n)], want)
+
+
 def test_no_sequences_and_no_rows():
     q, kc, vc, table, lens, cu, _ = make([4], [3], 16, 4, 2, 64, torch.bfloat16)
     none = ts.sigmoid_attention_paged(q, kc, vc, table[:0], lens[:0], cu[:1])

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void paged_reduce_kernel(const ReduceArgs a) {
     }
     const int64_t tok = r - packed_first(p.cu_q, p.rows_q, lo);
     const int Lq = p.len_q(lo), few = Lq * p.G <= a.cols;
-    if (tok < Lq && a.cut[few] != nullptr) {
+    if (tok >= 0 && tok < Lq && a.cut[few] != nullptr) {
       const int2 cut = a.cut[few][lo];
       nck = cut.y;
       if (nck > 1) {
