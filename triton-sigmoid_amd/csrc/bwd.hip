@@ -286,7 +286,12 @@ __global__ __launch_bounds__(256, 2) void bwd_dq_kernel(const KParams p) {
 // that share the item's K / V head, one head after another without a break in
 // the pipeline.  dK and dV of a shared head are the sums over its query heads,
 // so they stay in the same accumulators.  Tiles and blocks are visited in
-// order, so their places within a head are counters, not divisions.
+// order, so their places within a head are counters, not divisions.  The rate is
+// that of heads with keys of their own where the items fill the GPU (bf16 causal
+// B=1 T=8192 H=32 D=128, dK/dV with dS: H_kv = 8 1.16 ms, 32 1.17 + 0.21 ms in the
+// two passes that its larger dS takes; B=9 lengths 67..3001 H=12: H_kv = 4 398 us,
+// 12 417), and 15 % less at D = 64, split (fp16 B=8 lengths 512..2048 H=16: H_kv =
+// 2 126 us and 9 for the parts, 16 110).
 template <bool GROUPED> struct HeadStream {
   int nb = 0;                                      // blocks of one head
   int t1 = 0, th = 0;                              // next tile to copy: place in its head, head
@@ -331,7 +336,8 @@ __device__ __forceinline__ void store_part(const KParams &p, int part, int b, in
 // dK and dV of head-split items: the sum of the parts' fp32 rows in their
 // order, rounded once.  Rows that no sequence covers are left to the dQ launch,
 // which zeroes them.  Eight elements a thread, per_row threads a row, as many
-// rows to a workgroup as it has threads for; bound by memory.
+// rows to a workgroup as it has threads for; bound by memory: 45 MB in 9.1 us,
+// 5.0 TB/s (four parts of 9945 rows H_kv=2 D=64).
 template <typename T> __global__ __launch_bounds__(256) void add_parts_kernel(const KParams p, int per_row) {
   const int rows = per_row < 256 ? 256 / per_row : 1, mine = (int)threadIdx.x / per_row;
   const int64_t row = (int64_t)blockIdx.x * rows + mine;

@@ -41,9 +41,10 @@ struct PagedParams : KParams {
   }
 };
 
-// Most chunks of a sequence: the reduction reads them all (B=1 65536 keys, chunks
-// of 128 / 192 keys, 512 / 342 of them, 23.2 / 21.1 us).
-constexpr int kMostChunks = 340;
+// Most chunks of a sequence: the reduction reads them all.  320 / 384 / 448, whole
+// call, us, bf16 B=1 H=16 Hkv=2 D=128: 32000 keys 18.9 / 16.8 / 16.8, 65535 21.9 /
+// 21.3 / 21.9 (512: 22.1), 131072 31.7 / 31.0 / 31.1.
+constexpr int kMostChunks = 384;
 
 struct PagedUnit {
   int b = 0, hk = 0, qb = 0;  // sequence, K / V head, column block
@@ -78,8 +79,8 @@ __device__ __forceinline__ float wave_sum(float x) {
 // device (no host synchronisation): sequences in order, their blocks last
 // (under the causal mask longest) first, chunks, K / V heads fastest.  Every wave computes it
 // alike, 64 sequences at a time.  Chunks: with work W = sum of blocks times
-// keys, C = W Hkv / split_units keys (min_chunk at least), ceil(keys / C) chunks
-// of equal length: at most split_units + the units of an uncut batch.  Batches
+// keys, C = W Hkv / split_units keys (min_chunk at least), ceil(keys / C) chunks at
+// most, of equal length: no more than split_units + the units of an uncut batch.  Batches
 // of up to 64 sequences take a shorter C where that many units allow it.
 __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
   const int lane = __lane_id();
@@ -124,7 +125,22 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
   int base = 0;
   // Whether the unit is one of the 64 sequences' from b0 on (then `un` has it).
   const auto among = [&](int b0, int Lq, int Lk) SIGATTN_INLINE {
-    const int nqb = p.blocks_of(Lq, block), nck = min(max((Lk + C - 1) / C, 1), kMostChunks);
+    const int nqb = p.blocks_of(Lq, block), most = min(max((Lk + C - 1) / C, 1), kMostChunks);
+    // Equal chunks of a multiple of `round` keys, as few as that takes.  Quotients
+    // in floats, corrected, where lengths are exact in them (0.5 to 1 us a call
+    // faster than by integer division).
+    const int round = block == 32 ? 32 : 64;
+    int len, nck;
+    if (p.Tk < 1 << 23) {
+      len = round * max((int)((float)Lk * __builtin_amdgcn_rcpf((float)(most * round))), 1);
+      if (len * most < Lk) len += round;
+      if (len * most < Lk) len += round;
+      nck = max((int)((float)Lk * __builtin_amdgcn_rcpf((float)len)), 1);
+      if (nck * len < Lk) ++nck;
+    } else {
+      len = max(((Lk + most - 1) / most + round - 1) & -round, round);
+      nck = max((Lk + len - 1) / len, 1);
+    }
     const int sum = wave_scan(nqb * nck), first = base + sum - nqb * nck;
     const uint64_t m = __ballot(row >= first && row < base + sum);
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -135,8 +151,8 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     un.nck = __builtin_amdgcn_readlane(nck, at);
     const int r = row - __builtin_amdgcn_readlane(first, at), q = r / un.nck, chunk = r - q * un.nck;
     un.qb = __builtin_amdgcn_readlane(nqb, at) - 1 - q;
-    const int len = ((un.Lk + un.nck - 1) / un.nck + 63) & ~63;
-    un.k0 = min(chunk * len, un.Lk), un.k1 = min(un.k0 + len, un.Lk);
+    const int size = __builtin_amdgcn_readlane(len, at);
+    un.k0 = chunk * size, un.k1 = min(un.k0 + size, un.Lk);
     if (p.split_units > 0 && r == 0 && un.hk == 0 && lane == at) p.cut[un.b] = make_int2(first, nck);
     return true;
   };
