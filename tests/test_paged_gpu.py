@@ -369,6 +369,28 @@ def test_rows_before_the_first_sequence_are_zero(dtype, new, B):
     assert torch.equal(got[37:37 + sum(n)], want)
 
 
+@pytest.mark.parametrize("chunk", [0, 40], ids=["decode", "mixed"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_thousand_sequences(dtype, chunk):
+    # Enough that nothing is cut and a unit is found without the other lengths.
+    r = random.Random(11)
+    ctx = [r.choice((0, 1, 15, 16, 40, 90)) for _ in range(1030)]
+    new = [r.choice((0, 1, 1, 1)) for _ in ctx]
+    ctx[700], new[3] = 400, chunk or 1
+    check(ctx, new, 16, 2, 1, 32, DT[dtype])
+
+
+def test_caches_and_tables_without_pages():
+    q = torch.randn(5, 4, 64, device="cuda", dtype=torch.bfloat16)
+    none = torch.empty(0, 16, 2, 64, device="cuda", dtype=torch.bfloat16)
+    some = torch.full((3, 16, 2, 64), float("nan"), device="cuda", dtype=torch.bfloat16)
+    cu = ints([0, 2, 5])
+    for cache, table in ((none, torch.zeros(2, 40, dtype=I32, device="cuda")), (some, ints([]).reshape(2, 0))):
+        got = ts.sigmoid_attention_paged(q, cache, cache.clone(), table, ints([600, 17]), cu, 3, is_causal=True)
+        assert got.shape == q.shape and not got.any()
+    ts.paged_cache_write(q[:, :2], q[:, 2:], none, none.clone(), ints([0, 1, 2, 3, 4]))
+
+
 def test_no_sequences_and_no_rows():
     q, kc, vc, table, lens, cu, _ = make([4], [3], 16, 4, 2, 64, torch.bfloat16)
     none = ts.sigmoid_attention_paged(q, kc, vc, table[:0], lens[:0], cu[:1])

@@ -84,6 +84,16 @@ __device__ __forceinline__ float wave_sum(float x) {
 // of up to 64 sequences take a shorter C where that many units allow it.
 __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
   const int lane = __lane_id();
+  if (block == 32 && p.split_units == 0) {
+    // Decoding, nothing cut: a unit is a sequence's K / V head.
+    PagedUnit un;
+    un.b = u / p.Hkv, un.hk = u - un.b * p.Hkv;
+    if (un.b >= p.B) return un;
+    un.Lq = p.len_q(un.b), un.Lk = un.k1 = p.keys(un.b);
+    un.nck = p.blocks_of(un.Lq, block);
+    for (int *x : {&un.b, &un.hk, &un.Lq, &un.Lk, &un.k1, &un.nck}) *x = __builtin_amdgcn_readfirstlane(*x);
+    return un;
+  }
   // The first 64 * kKeep sequences' lengths stay in registers, their loads in
   // flight together.
   constexpr int kKeep = 4;

@@ -94,9 +94,23 @@ struct Plan {
 // call, us, half a round more / two: bf16 H=32 Hkv=8 D=128, t = 1024: B=128
 // contexts 10..4000 194 / 181, B=300 10..2000 215 / 209, B=200 100..900 81 / 81;
 // fewer uncut units than t, B=64 8000..9000 H=8 338 / 357, 1024..3000 97 / 109.
-void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const PagedParams &k, int D) {
+//
+// Decoding stays uncut where a wave is through its sequence before the sums would
+// be added: in tables of few keys, or few for the rounds that the uncut units
+// take, and (the table may be longer than what is in it) in batches of four rounds
+// and of 1024 sequences, whose lengths every wave goes through to find a cut
+// unit.  Whole call, us, cut / not, bf16 H=32 Hkv=8 D=128: B=16 up to 160 keys 16.5
+// / 11.2, 300 17.5 / 16.9, 600 18.3 / 26.9; B=64 300 25.3 / 19.6, 600 32.0 / 31.1,
+// 1200 46 / 56; B=200 300 50 / 37, 1200 121 / 117, 50..4800 318 / 378; B=512 300 105 /
+// 75, 50..4000 737 / 726; B=4096 300 2042 / 563.  Hkv=1 H=8: B=1000 50..4000 217 /
+// 204, B=3000 642 / 552.  fp32: B=16 300 24.6 / 48.5, B=64 36 / 50, B=128 72 / 54, 600
+// 104 / 92.
+void cut_part(Part &part, int64_t uncut, int64_t t, int64_t min_chunk, const PagedParams &k, int D, bool decode,
+              bool f32) {
+  const int64_t few = f32 ? 0 : 320, per_round = f32 ? 500 : 1200;
   part.units = uncut;
   if (k.Tk <= min_chunk || t <= 0) return;
+  if (decode && (k.Tk <= few || k.Tk * t <= per_round * uncut || uncut >= 4 * t || k.B >= 1024)) return;
   const int64_t most = uncut * cdiv(k.Tk, min_chunk);
   int64_t extra = uncut >= t ? 2 * t : t - uncut > t / 2 ? t - uncut : t / 2;
   if (extra > most) extra = most;
@@ -117,7 +131,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
   pl.fwd.block = f32 ? sigattn::kPagedBlockF32 : sigattn::paged_block(D), pl.decode.block = 32;
   if (decode) {
     const int64_t pairs = (int64_t)k.B * k.Hkv;
-    cut_part(pl.decode, pairs, kDecodeWaves * cus, kDecodeChunk, k, D);
+    cut_part(pl.decode, pairs, kDecodeWaves * cus, kDecodeChunk, k, D, true, f32);
   }
   if (fwd) {
     if (decode) pl.cols_lo = kDecodeCols;
@@ -126,7 +140,7 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
     const int64_t seqs = all / (pl.cols_lo + 1) < k.B ? all / (pl.cols_lo + 1) : k.B;
     const int64_t uncut = (all / pl.fwd.block + seqs) * k.Hkv, per_cu = f32 ? 2 : D == 128 ? 1 : (D == 64 ? 3 : 4);
     const int64_t full = cdiv(all, pl.fwd.block) * k.Hkv;
-    cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, f32 ? kChunkF32 : kChunk, k, D);
+    cut_part(pl.fwd, uncut, full < per_cu * cus ? per_cu * cus : 0, f32 ? kChunkF32 : kChunk, k, D, false, f32);
   }
   const bool cut = pl.fwd.split_units > 0 || pl.decode.split_units > 0;
   pl.cut_bytes = cut ? cdiv((int64_t)k.B * 2 * (int64_t)sizeof(int2), 256) * 256 : 0;
