@@ -278,6 +278,27 @@ def test_head_split_parts(heads, D, causal):
         assert torch.equal(got[x], same[x])
 
 
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("heads", [(10, 2), (16, 1)], ids=lambda h: f"{h[0]}x{h[1]}")
+def test_head_split_parts_of_fp32(heads, D, causal):
+    """As above, on the fp32 kernels; values past what their splits hold take
+    the exact products, in parts too."""
+    cu = offsets([140, 0, 300], first=3)
+    q, k, v, do = make(cu[-1] + 7, cu[-1] + 7, *heads, D, torch.float32, 18)
+    junk = torch.full((64 << 20,), float("nan"), device="cuda")
+    del junk
+    got = check(q, k, v, do, cu, cu, causal)
+    for x in got.values():
+        assert not x[:3].any() and not x[cu[-1]:].any()
+    same = run(q, k, v, do, cu, cu, is_causal=causal)
+    for x in got:
+        assert torch.equal(got[x], same[x])
+    small = do.clone()
+    small[3:143] *= 1e-30
+    check(q, k, v, small, cu, cu, causal)
+
+
 def test_head_split_asks_for_its_workspace():
     import ctypes
     cut = torch.tensor([0, 256, 400], dtype=torch.int32, device="cuda")

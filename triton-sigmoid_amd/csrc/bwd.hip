@@ -362,9 +362,13 @@ template <typename T> __global__ __launch_bounds__(256) void add_parts_kernel(co
         v[0] += *(const f32x4 *)(src + 2 * s * tensor);
         v[1] += *(const f32x4 *)(src + 2 * s * tensor + 4);
       }
-      *(u32x4 *)((uint16_t *)(t == 0 ? p.dk : p.dv) + row * p.sk_t + h * p.sk_h + d) =
-          (u32x4){Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[0].z, v[0].w), Elem<T>::pack(v[1].x, v[1].y),
-                  Elem<T>::pack(v[1].z, v[1].w)};
+      T *to = (T *)(t == 0 ? p.dk : p.dv) + row * p.sk_t + h * p.sk_h + d;
+      if constexpr (sizeof(T) == 4) {
+        *(f32x4 *)to = v[0], *(f32x4 *)(to + 4) = v[1];
+      } else {
+        *(u32x4 *)to = (u32x4){Elem<T>::pack(v[0].x, v[0].y), Elem<T>::pack(v[0].z, v[0].w),
+                               Elem<T>::pack(v[1].x, v[1].y), Elem<T>::pack(v[1].z, v[1].w)};
+      }
     }
   }
 }
@@ -1596,11 +1600,17 @@ void launch_bwd_dkdv_mfma(const KParams &p, int dtype, int D, bool causal, bool 
       if (dsout) bwd_dkdv_t<T, DD, true>(p, causal, sm, st);
     }
     if (!dsout) bwd_dkdv_t<T, DD, false>(p, causal, sm, st);
-    if (p.qgroup > 1 && p.qsplit > 1) {
-      const int per_row = p.H * p.dmem / 8, rows = per_row < 256 ? 256 / per_row : 1;
-      add_parts_kernel<T><<<dim3((unsigned)((p.rows_k + rows - 1) / rows)), dim3(256), 0, st>>>(p, per_row);
-    }
   });
+  launch_add_parts(p, dtype, st);
+}
+
+void launch_add_parts(const KParams &p, int dtype, hipStream_t st) {
+  if (p.qgroup <= 1 || p.qsplit <= 1) return;
+  const int per_row = p.H * p.dmem / 8, rows = per_row < 256 ? 256 / per_row : 1;
+  const dim3 grid((unsigned)((p.rows_k + rows - 1) / rows)), block(256);
+  if (dtype == kBF16) add_parts_kernel<__bf16><<<grid, block, 0, st>>>(p, per_row);
+  else if (dtype == kF16) add_parts_kernel<_Float16><<<grid, block, 0, st>>>(p, per_row);
+  else add_parts_kernel<float><<<grid, block, 0, st>>>(p, per_row);
 }
 
 void launch_bwd_fused_mfma(const KParams &kp, int dtype, int D, bool causal, bool sm, hipStream_t st) {

@@ -419,7 +419,9 @@ BwdSplit bwd_range_split(const sigattn_problem *p, bool mfma) {
 // fp16 B=8 T=2048 lengths 512..2048 D=64 H=16 Hkv=2 443 / 264 / 263 / - / 262,
 // Hkv=8 236 / 236 / 236 / - / 261; bf16 B=9 T=3001 lengths 67..3001 D=128 H=12
 // Hkv=4 664 / 686 / 682 / 771 / -, Hkv=2 - / 793 / 695 / 707 / -, B=2 Hkv=4 - /
-// 333 / 305 / 306 / -.
+// 333 / 305 / 306 / -.  fp32, none / 2: B=1 H=16 Hkv=2 T=2048 D=128 1919 / 625, D=64
+// 642 / 336, T=512 D=128 558 / 182; T=4096 H=32 Hkv=8 3919 / 3435; B=8 lengths
+// 512..2048 D=64 H=16 Hkv=2 1698 / 1575; B=2 of 6 tokens H=48 Hkv=3 D=128 235 / 103.
 constexpr int64_t kHeadSplitPerCu = 2;
 struct HeadSplit {
   int n = 1;
@@ -434,11 +436,15 @@ HeadSplit head_split(const sigattn_problem *p, bool mfma) {
   // (half of which are counted).
   const int64_t rows = p->rows_k < p->B * p->Tk ? p->rows_k : p->B * p->Tk;
   const int64_t items = (rows / 128 + (p->B + 1) / 2) * kv_heads(p);
-  int64_t n = items > 0 ? cdiv(kHeadSplitPerCu * cus, items) : 1;
+  // (fp32: the nearest number, as its parts cost more.)
+  const bool f32 = p->dtype == SIGATTN_F32;
+  const int64_t aim = kHeadSplitPerCu * cus, up = f32 ? items / 2 : items - 1;
+  int64_t n = items > 0 ? (aim + up) / items : 1;
   if (n > G) n = G;
-  // Four tiles of queries a part at least: shorter ones are all start and end.
-  const int64_t tiles = G * cdiv(p->Tq, 64);
-  if (n > tiles / 4) n = tiles / 4;
+  // Four tiles of queries a part at least: shorter ones are all start and end
+  // (fp32: of D = 128, more of the shorter ones below).
+  const int64_t tiles = G * cdiv(p->Tq, 64), least = f32 ? 4 * 128 / p->D : 4;
+  if (n > tiles / least) n = tiles / least;
   if (n < 2) return s;
   s.n = (int)n;
   s.bytes = n * 2 * p->rows_k * kv_heads(p) * p->D * (int64_t)sizeof(float);
@@ -883,8 +889,9 @@ size_t sigattn_bwd_split_workspace_bytes(const sigattn_problem *p) {
   if (sigattn_check(p) != SIGATTN_OK || p->B == 0 || p->H == 0) return 0;
   const void *none[1] = {nullptr};
   const bool mfma = use_mfma(p, none, 0);
-  // At D = 128 the parts go with the dS of sigattn_bwd_ws.
-  if (head_group(p) > 1) return p->D == 128 ? 0 : (size_t)head_split(p, mfma).bytes;
+  // At D = 128 the 16-bit kernels' parts go with the dS of sigattn_bwd_ws.
+  if (head_group(p) > 1)
+    return mfma && p->D == 128 ? 0 : (size_t)head_split(p, mfma || use_f32_mfma(p, none, 0)).bytes;
   return (size_t)bwd_range_split(p, mfma).bytes;
 }
 
@@ -899,8 +906,9 @@ int sigattn_bwd_split(const sigattn_problem *p, const void *dout, void *dq, void
   if (want_kv && (dk == nullptr || dv == nullptr)) return SIGATTN_ERR_NULL_ARG;
   const BwdParts parts = want_dq && want_kv ? kBwdAll : (want_dq ? kBwdDq : kBwdDkdv);
   const void *ptrs[7] = {p->q, p->k, p->v, dout, dq, dk, dv};
-  if (head_group(p) > 1 && p->D != 128 && workspace != nullptr) {
-    const HeadSplit hs = head_split(p, use_mfma(p, ptrs, 7));
+  const bool f32mma = use_f32_mfma(p, ptrs, 7);
+  if (head_group(p) > 1 && (p->D != 128 || f32mma) && workspace != nullptr) {
+    const HeadSplit hs = head_split(p, f32mma || use_mfma(p, ptrs, 7));
     if (hs.n > 1 && ((size_t)hs.bytes > workspace_bytes || !aligned16(workspace))) return SIGATTN_ERR_WORKSPACE;
     return bwd_impl(p, dout, dq, dk, dv, nullptr, 0, stream, parts, hs.n, (float *)workspace);
   }

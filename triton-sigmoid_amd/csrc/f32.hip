@@ -245,8 +245,18 @@ __device__ __forceinline__ void dq_full(const KParams &p, const Item &w_, float 
     store_row<D>((float *)p.dq + qoff + (int64_t)myq * p.sq_t, acc, scale, myq < Lq, hi, half);
 }
 
+// A lane's rows of a head split's fp32 dK and dV (KParams::qsplit).
+template <int D>
+__device__ __forceinline__ void store_parts(const KParams &p, int part, int b, int key, int h,
+                                            const f32x16 (&dk)[D / 32], const f32x16 (&dv)[D / 32], float scale, int hi,
+                                            bool half) {
+  const int64_t row = packed_first(p.cu_k, p.rows_k, b) + key;
+  store_row<D>(p.part_row(part, 0, row, h), dk, scale, true, hi, half);
+  store_row<D>(p.part_row(part, 1, row, h), dv, 1.0f, true, hi, half);
+}
+
 template <int D, bool CAUSAL, bool SCOREMOD>
-__device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, float *lds) {
+__device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, int part, float *lds) {
   constexpr int NDB = D / 32;
   const int b = w_.b, h = w_.h, k0 = w_.row0;
   const int Lk = p.len_k(b), Lq = p.len_q(b), rows = min(Lk, w_.row_end);
@@ -279,7 +289,7 @@ __device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, floa
   rr.init(l32, hi);
   const int stride_bytes = (int)(p.sq_t * 4);
   // u: tiles since the start, over the query heads of this K / V head.
-  for (int g = 0, u = 0; g < p.q_heads(); ++g) {
+  for (int g = p.part_head(part), u = 0; g < p.part_head(part + 1); ++g) {
     const int64_t qoff = p.q_base(b, p.first_q_head(h) + g) + (int64_t)mstart * p.sq_t;
     const float *Qm = (const float *)p.q + qoff, *dOm = (const float *)p.dout + qoff;
     for (int t = 0; t < ntiles; ++t, ++u) {
@@ -305,6 +315,10 @@ __device__ __forceinline__ void dkdv_full(const KParams &p, const Item &w_, floa
       row_product<D>(dva, tO, pr, rr);
       row_product<D>(dka, tQ, ds, rr);
     }
+  }
+  if (p.qsplit > 1) {
+    if (kok) store_parts<D>(p, part, b, myk, h, dka, dva, scale, hi, half);
+    return;
   }
   if (myk < min(w_.row_end, p.k_rows_out(Lk))) {
     store_row<D>((float *)p.dk + koff + (int64_t)myk * p.sk_t, dka, scale, myk < Lk, hi, half);
@@ -763,7 +777,8 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
   __shared__ __attribute__((aligned(16))) float lds[lds_floats<D, WK>()];
   uint16_t *tiles = (uint16_t *)lds;
 
-  const Item it = item_of<WK, CAUSAL, false>(p, blockIdx.x, bwd_f32_occupancy<D, WK>());
+  const int nparts = p.qsplit > 1 ? p.qsplit : 1, wg = (int)blockIdx.x / nparts, part = (int)blockIdx.x - wg * nparts;
+  const Item it = item_of<WK, CAUSAL, false>(p, wg, bwd_f32_occupancy<D, WK>());
   const int b = it.b, h = it.h;
   const int Lq = p.len_q(b), Lk = p.len_k(b);
   const bool half = p.half_head(D);
@@ -792,7 +807,8 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
   TileOffsets<D> to;
   to.init(lane);
   Tiles st;
-  for (int g = 0; g < p.q_heads(); ++g) {  // the query heads of this K / V head
+  // The part's query heads of this K / V head.
+  for (int g = p.part_head(part); g < p.part_head(part + 1); ++g) {
     const int64_t qoff = p.q_base(b, p.first_q_head(h) + g);
     const float *Qb = (const float *)p.q + qoff, *dOb = (const float *)p.dout + qoff;
     auto load = [&](int t) SIGATTN_INLINE { st.load(Qb, dOb, p.sq_t, mstart + t * TR, Lq, half); };
@@ -840,9 +856,13 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
     const bool fits = doubt_below(rg, lds, least, zeros) && __builtin_fabsf(scale) < 0x1p32f;
     if (__syncthreads_or(!fits ||
                          (wt == 0 && kok && (in_doubt(dva, least, zeros) || in_doubt(dka, least, zeros))))) {
-      dkdv_full<D, CAUSAL, SCOREMOD>(p, it, lds);
+      dkdv_full<D, CAUSAL, SCOREMOD>(p, it, part, lds);
       return;
     }
+  }
+  if (nparts > 1) {
+    if (wt == 0 && kok) store_parts<D>(p, part, b, myk, h, dka, dva, scale, hi, half);
+    return;
   }
   if (wt == 0 && myk < p.k_rows_out(Lk)) {
     store_row<D>((float *)p.dk + koff + (int64_t)myk * p.sk_t, dka, scale, kok, hi, half);
@@ -867,7 +887,8 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
 // 0.76-1.0 (D = 64, from 1.25: 0.77-0.97 / 0.79-0.93), dense non-causal T=200 to
 // 512 0.71-1.00 / 0.75-1.08, causal T=512 1.04-1.55 / 0.89-1.27; T=33 0.9-1.2.
 template <int D> int f32_waves_per_rows(const KParams &p, int rows, int stream, bool causal) {
-  const int64_t bh = (int64_t)p.B * p.H, blocks = bh * ((rows + 127) / 128), cus = p.ncu;
+  const int parts = p.qgroup > 1 && p.qsplit > 1 ? p.qsplit : 1;
+  const int64_t bh = (int64_t)p.B * p.H * parts, blocks = bh * ((rows + 127) / 128), cus = p.ncu;
   if (D < 128 && bh * ((rows + 31) / 32) <= cus) return 4;
   if (D == 128 && stream <= 128 && blocks > cus) return 1;
   if (D >= 64 && stream > 64 && (D == 128 ? 2 : 1) * blocks > cus &&
@@ -925,7 +946,8 @@ template <int D> void dq_t(const KParams &kp, bool causal, bool scoremod, hipStr
 template <int D> void dkdv_t(const KParams &kp, bool causal, bool scoremod, hipStream_t st) {
   by_waves<D>(kp, kp.Tk, kp.Tq, causal, [&](auto wk, const KParams &p, int64_t n) {
     constexpr int WK = decltype(wk)::value;
-    const dim3 grid((unsigned)n), block(64 * FW);  // no gap rows here (the dQ launch's)
+    // (No gap rows here: the dQ launch's.)
+    const dim3 grid((unsigned)(n * (p.qsplit > 1 ? p.qsplit : 1))), block(64 * FW);
     if (causal) {
       if (scoremod) dkdv_f32_kernel<D, true, true, WK><<<grid, block, 0, st>>>(p);
       else dkdv_f32_kernel<D, true, false, WK><<<grid, block, 0, st>>>(p);
@@ -1167,6 +1189,7 @@ void launch_bwd_dkdv_f32(const KParams &p, int D, bool causal, bool scoremod, hi
   if (D == 128) dkdv_t<128>(p, causal, scoremod, st);
   else if (D == 64) dkdv_t<64>(p, causal, scoremod, st);
   else dkdv_t<32>(p, causal, scoremod, st);
+  launch_add_parts(p, kF32, st);
 }
 
 }  // namespace sigattn

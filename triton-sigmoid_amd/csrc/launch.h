@@ -102,6 +102,8 @@ void launch_zero_gaps(const GapAxis &a, const GapAxis &b, int esize, hipStream_t
 void launch_fwd_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);
 void launch_bwd_dq_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);
 void launch_bwd_dkdv_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);
+// dK and dV of a head split (KParams::qsplit) from its parts; nothing without one.
+void launch_add_parts(const KParams &p, int dtype, hipStream_t st);
 
 // Portable kernels: any dtype, D in {16, 32, 64, 128}, any alignment.
 void launch_fwd_generic(const KParams &p, int dtype, int D, bool causal, hipStream_t st);
