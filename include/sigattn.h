@@ -234,6 +234,10 @@ int sigattn_bwd(const sigattn_problem *p, const void *dout, void *dq, void *dk,
  * deterministic and equal sigattn_bwd's within fp32 summation order.  With
  * dq NULL (or dk and dv NULL) it runs only the other half, like
  * sigattn_bwd_dkdv (sigattn_bwd_dq), on the same workspace size.
+ * Grouped heads, below head_dim 128 and in fp32: where few K / V heads leave
+ * the GPU waiting, the query heads of a group run in parts whose fp32 dK and dV
+ * the workspace holds and a second kernel adds in order.  (f16 / bf16 at 128:
+ * sigattn_bwd_ws holds them behind the dS.)
  */
 size_t sigattn_bwd_split_workspace_bytes(const sigattn_problem *p);
 int sigattn_bwd_split(const sigattn_problem *p, const void *dout, void *dq, void *dk, void *dv,
