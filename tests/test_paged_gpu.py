@@ -369,14 +369,17 @@ def test_rows_before_the_first_sequence_are_zero(dtype, new, B):
     assert torch.equal(got[37:37 + sum(n)], want)
 
 
-@pytest.mark.parametrize("chunk", [0, 40], ids=["decode", "mixed"])
+@pytest.mark.parametrize("chunk, longest", [(0, 400), (40, 400), (40, 3000)], ids=["decode", "mixed", "chunk cut"])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_a_thousand_sequences(dtype, chunk):
-    # Enough that nothing is cut and a unit is found without the other lengths.
+def test_a_thousand_sequences(dtype, chunk, longest):
+    # Enough that decoding is not cut and its units are found without the other
+    # lengths; a chunk of new tokens on many keys is.
     r = random.Random(11)
     ctx = [r.choice((0, 1, 15, 16, 40, 90)) for _ in range(1030)]
     new = [r.choice((0, 1, 1, 1)) for _ in ctx]
-    ctx[700], new[3] = 400, chunk or 1
+    ctx[700], new[3] = longest, chunk or 1
+    if longest > 1024:
+        new[700] = chunk
     check(ctx, new, 16, 2, 1, 32, DT[dtype])
 
 

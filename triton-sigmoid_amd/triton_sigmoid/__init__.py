@@ -12,9 +12,9 @@ plus additions with no counterpart in the reference's API:
   * sigmoid_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k,
                              max_seqlen_q, max_seqlen_k, is_causal, scale,
                              sigmoid_bias, score_mod)
-    for packed [total_tokens, H, D] sequences (the layout the reference's
-    benchmark builds for flash_attn_varlen_func), whose keys and values may
-    have fewer heads than the queries.
+    for packed [total_tokens, H, D] sequences (the packed layout of the
+    reference's benchmark, benchmarks/benchmark_sigmoid.py:116-134), whose keys
+    and values may have fewer heads than the queries.
 and the paged key/value cache of a serving loop:
   * paged_plan(context_lens, new_lens, block_table, free_pages, page_size,
                num_tokens) pages and slots of a step's new tokens, on the GPU
