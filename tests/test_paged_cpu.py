@@ -7,6 +7,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import triton_sigmoid as ts
 from triton_sigmoid import _capi
@@ -206,3 +207,34 @@ def test_struct_layouts_match_the_header(tmp_path):
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
     got = {k: int(v) for k, v in (line.split() for line in out.splitlines())}
     assert got == want
+
+
+@pytest.mark.parametrize("name", ["query", "key_cache", "value_cache", "score_mod"])
+def test_tangents_are_refused(name):
+    """Forward mode has no rule here: a tangent is refused, not dropped."""
+    args = _attn_args(score_mod=torch.zeros(2, 48))
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        for call in (ts.sigmoid_attention_paged, torch.no_grad()(ts.sigmoid_attention_paged)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(**args)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.ops.myops.sigmoid_attn_paged_fwd(
+                args["query"], args["key_cache"], args["value_cache"], args["block_table"], args["seq_lens_k"],
+                args["cu_seqlens_q"], 2, args["score_mod"], 0.5, None, False)
+
+
+@pytest.mark.parametrize("name", ["key", "value", "key_cache", "value_cache"])
+def test_tangents_are_not_written(name):
+    args = _write_args()
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            ts.paged_cache_write(**args)
+
+
+def test_functional_forward_mode_is_refused():
+    args = _attn_args()
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda q: ts.sigmoid_attention_paged(**dict(args, query=q)), (args["query"],),
+                       (torch.ones_like(args["query"]),))

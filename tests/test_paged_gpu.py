@@ -6,6 +6,7 @@ import random
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import triton_sigmoid as ts
 from reference64 import assert_within, one_head
@@ -713,3 +714,30 @@ def test_two_calls_at_once_on_one_cache():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("binding", ["node", "python"])
+def test_tangents_are_refused(monkeypatch, binding):
+    """Canonical arguments too: the C++ module leaves a dual tensor to the
+    Python layer, which refuses it, also under no_grad."""
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    q, kc, vc, table, lens, cu, _ = make([20, 5], [1, 3], 16, 4, 2, 64, torch.bfloat16, fill=0.0)
+    mod = torch.zeros(2, table.shape[1] * 16, device="cuda")
+    rows = torch.randn(4, 2, 64, device="cuda").bfloat16()
+    before = kc.clone(), vc.clone()
+    with forward_ad.dual_level():
+        for i in range(4):
+            a = [q, kc, vc, mod]
+            a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i]))
+            for call in (ts.sigmoid_attention_paged, torch.no_grad()(ts.sigmoid_attention_paged)):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(a[0], a[1], a[2], table, lens, cu, 3, score_mod=a[3])
+            w = [rows, rows, kc, vc]
+            w[i] = forward_ad.make_dual(w[i], torch.ones_like(w[i]))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                ts.paged_cache_write(*w, ints([0, 1, 2, 3]))
+        # Without a tangent the calls run inside a dual level as outside.
+        got = ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 3, score_mod=mod)
+    assert torch.equal(got, ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 3, score_mod=mod))
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])

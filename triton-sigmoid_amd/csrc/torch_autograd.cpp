@@ -339,10 +339,11 @@ struct Quick {
     const at::ScalarType type = t.scalar_type();
     return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat;
   }
+  // No tensor asks for a gradient or carries a forward-mode tangent (level 0 is
+  // the only one; a mode that no_grad leaves on).
   static bool no_grad(std::initializer_list<const Tensor *> tensors) {
-    if (!at::GradMode::is_enabled()) return true;
     for (const Tensor *t : tensors)
-      if (t->defined() && t->requires_grad()) return false;
+      if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return false;
     return true;
   }
   static bool number(const py::object &o, double &v) {

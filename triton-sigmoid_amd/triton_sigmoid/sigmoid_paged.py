@@ -29,6 +29,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -55,6 +56,13 @@ def _check_page_size(page_size: int) -> None:
 def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+def _no_tangent(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    # Where the kernels are called, so that the custom ops refuse them too: a
+    # dual tensor's requires_grad is False, and no_grad does not stop forward mode.
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
 
 
 def _quick():
@@ -191,6 +199,7 @@ def paged_plan(
 # --- writer -----------------------------------------------------------------------
 
 def _write(key, value, key_cache, value_cache, slot_mapping):
+    _no_tangent("paged_cache_write", key, value, key_cache, value_cache)
     lib = _capi.load_library()
     _capi._check_device(key_cache)
     dev = key_cache.device
@@ -294,6 +303,7 @@ def paged_cache_write(
 def _attend(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, score_mod, scale,
             bias, is_causal):
     """bias None: -log(key length)."""
+    _no_tangent("sigmoid_attention_paged", query, key_cache, value_cache, score_mod)
     lib = _capi.load_library()
     _capi._check_device(query)
     dev = query.device
@@ -409,7 +419,8 @@ def sigmoid_attention_paged(
         [N, H, D] output, contiguous.  Rows outside every sequence are zeros.
         Slots of the cache past a sequence's length are never read; keys and
         values of a sequence itself have to be finite.  Deterministic.
-        Forward only.
+        Forward only: tensors that ask for a gradient (under grad mode) or
+        carry a forward-mode tangent are refused.
     """
     quick = _quick()
     if quick is not None:
