@@ -358,3 +358,103 @@ def test_short_way_of_eager_calls(monkeypatch):
         ts.sigmoid_attention_varlen(q, k, v, cut, cut, -1, 70)
     run(q.float(), k.float(), v.float(), do.float(), cu, cu)  # no longest lengths: the Python layer reads them
     assert not took.pop()
+
+
+# Few queries on many keys, not causal: the split-KV forward.  Its forms: waves
+# that share a chunk, with parts to add or one chunk each; a wave for each chunk,
+# with one each, cut by the lengths, or (more sequences than a wave has lanes)
+# of one length.  (lengths, heads, bytes of partials a call asks for: none or some)
+SHORT_QUERIES = {
+    "shared": ([1, 0, 17, 32], [900, 300, 0, 2000], (8, 2), True),
+    "shared, three to a head": ([5, 2], [700, 1500], (6, 2), True),
+    "shared, one chunk": ([3] * 40, [(37 * i) % 257 for i in range(39)] + [256], (16, 2), False),
+    "wave each, one chunk": ([1 + i % 2 for i in range(130)], [(53 * i) % 401 for i in range(129)] + [400], (16, 4),
+                             False),
+    "wave each, cut": ([1, 8, 0, 5], [16000, 17, 400, 9000], (16, 1), True),
+    "wave each, one length": ([1 + i % 3 for i in range(70)], [(97 * i) % 1031 for i in range(69)] + [1031], (6, 2),
+                              True),
+}
+
+
+@pytest.mark.parametrize("mod", [False, True], ids=["plain", "terms"])
+@pytest.mark.parametrize("dtype, D", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("shape", list(SHORT_QUERIES))
+def test_short_queries_on_long_keys(shape, dtype, D, mod):
+    import ctypes
+    nq, nk, heads, parts = SHORT_QUERIES[shape]
+    cq, ck = offsets(nq), offsets(nk)
+    q, k, v, do = make(cq[-1], ck[-1], *heads, D, DT[dtype], 30)
+    term = None
+    if mod:
+        term = torch.randn(ck[-1], generator=torch.Generator().manual_seed(31)).cuda()
+        term[5], term[-1] = -torch.inf, torch.finfo(torch.float32).min
+    check(q, k, v, do, cq, ck, False, term)
+    cut = [torch.tensor(c, dtype=torch.int32, device="cuda") for c in (cq, ck)]
+    pr = _capi._problem(q, k, v, torch.zeros(len(nq), device="cuda"), term, torch.tensor(1.0, device="cuda"), None, None,
+                        False, packed=(*cut, max(nq), max(nk)))
+    assert (_capi.load_library().sigattn_fwd_decode_workspace_bytes(ctypes.byref(pr)) > 0) == parts
+
+
+def test_gradients_of_repeated_heads_add_up():
+    """dK and dV of a shared head are the sums of those of its copies: within
+    the group's bound and those of the copies, each rounded once."""
+    cu = offsets([100, 400])
+    for D in (64, 128):
+        q, k, v, do = make(cu[-1], cu[-1], 8, 2, D, torch.bfloat16, 10)
+        got = run(q, k, v, do, cu, cu, is_causal=True)
+        rk, rv = k.repeat_interleave(4, 1), v.repeat_interleave(4, 1)
+        rep = run(q, rk, rv, do, cu, cu, is_causal=True)
+        bound, each = packed(q, k, v, do, cu, cu, True), packed(q, rk, rv, do, cu, cu, True)
+        for x in ("dk", "dv"):
+            total = rep[x].double().unflatten(1, (2, 4)).sum(2)
+            assert_within(got[x], (total, bound[x][1] + each[x][1].unflatten(1, (2, 4)).sum(2)), x)
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_two_pass_backward_in_several_passes(dtype, causal):
+    """The dS of some K / V heads at a time: workspaces of one query head (none:
+    recomputed), of one group, of two, of three (passes of two then), of all four,
+    and of all with the parts of a head split behind them."""
+    import ctypes
+    lens = [300, 77, 0, 513]
+    H, Hkv, D, G = 12, 4, 128, 3
+    cu = offsets(lens)
+    q, k, v, do = make(cu[-1], cu[-1], H, Hkv, D, DT[dtype], 32)
+    cut = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    bias = -torch.log(torch.tensor(lens, device="cuda").clamp(min=1).float())
+    scale = torch.tensor(D ** -0.5, device="cuda")  # (the problem holds addresses alone)
+    pr = _capi._problem(q, k, v, bias, None, scale, None, None, causal, packed=(cut, cut, 513, 513))
+    lib, blocks = _capi.load_library(), -(-513 // 32)
+    per_head = len(lens) * (blocks * (blocks + 1) // 2 if causal else blocks * blocks) * 2048
+    full = lib.sigattn_bwd_workspace_bytes(ctypes.byref(pr))
+    assert full > H * per_head
+    want = packed(q, k, v, do, cu, cu, causal)
+    stream = torch.cuda.current_stream().cuda_stream
+    for n in (per_head, G * per_head, 2 * G * per_head, 3 * G * per_head + 16, H * per_head, full):
+        ws = torch.full((n // 4,), float("nan"), device="cuda")
+        g = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+        rc = lib.sigattn_bwd_ws(ctypes.byref(pr), do.data_ptr(), *(t.data_ptr() for t in g), ws.data_ptr(), n, stream)
+        assert rc == 0
+        for x, t in zip(("dq", "dk", "dv"), g):
+            assert_within(t, want[x], f"{x}, workspace of {n / per_head:.2f} heads")
+
+
+@pytest.mark.parametrize("binding", ["node", "python"])
+def test_backward_past_the_workspace_limit(monkeypatch, binding):
+    """A training step whose dS is over the limit runs in passes of whole K / V
+    heads, through either binding."""
+    import ctypes
+    monkeypatch.setenv("SIGATTN_BWD_WORKSPACE_MB", "180")
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    lens = [1024 + (i % 5 - 2) * 38 for i in range(34)]
+    cu = offsets(lens)
+    q, k, v, do = make(cu[-1], cu[-1], 8, 4, 128, torch.bfloat16, 33)
+    cut = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    pr = _capi._problem(q, k, v, torch.zeros(len(lens), device="cuda"), None, torch.tensor(1.0, device="cuda"), None,
+                        None, True, packed=(cut, cut, max(lens), max(lens)))
+    lib = _capi.load_library()
+    full, size = lib.sigattn_bwd_workspace_bytes(ctypes.byref(pr)), _capi.bwd_workspace_bytes(lib, pr, q.device)
+    assert 0 < size <= 180 << 20 < full
+    check(q, k, v, do, cu, cu, True)
