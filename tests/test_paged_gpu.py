@@ -741,3 +741,64 @@ def test_tangents_are_refused(monkeypatch, binding):
         got = ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 3, score_mod=mod)
     assert torch.equal(got, ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 3, score_mod=mod))
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+@pytest.mark.parametrize("heads", [(4, 1), (4, 2)], ids=lambda h: f"{h[0]}x{h[1]}")
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_as_many_chunks_as_a_sequence_takes(dtype, heads):
+    """Contexts whose chunks of the least length would be more than are summed:
+    longer ones (24576 keys and more, for one sequence or two)."""
+    for ctx in ([29999], [65900], [40001, 27]):
+        check(ctx, [1] * len(ctx), 64, *heads, 64, DT[dtype])
+    check([26000], [5], 128, *heads, 128, DT[dtype], causal=False, mod=True)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 3]], ids=["decode", "chunk"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_tables_of_many_keys(dtype, new):
+    """A table row that can hold 2^23 keys (lengths that floats hold no longer
+    exactly), for short sequences and one that passes a page of 2^20."""
+    ps, H, Hkv, D = 1 << 20, 4, 1, 32
+    lens = [3000, 77, ps + 513]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda").to(DT[dtype])  # noqa: E731
+    rows = [normal(2, n, Hkv, D) for n in lens]
+    caches = torch.full((2, 5, ps, Hkv, D), float("nan"), dtype=DT[dtype], device="cuda")
+    pages = [[3], [0], [4, 2]]
+    for r, p in zip(rows, pages):
+        for j, page in enumerate(p):
+            part = r[:, j * ps:(j + 1) * ps]
+            caches[:, page, :part.shape[1]] = part
+    q = normal(sum(new), H, D)
+    for width in (2, 8, 13):
+        table = ints([p + [-1] * (width - len(p)) for p in pages])
+        got = ts.sigmoid_attention_paged(q, caches[0], caches[1], table, ints(lens), ints(offsets(new)), max(new),
+                                         is_causal=True)
+        assert_within(got, reference(q, rows, new, True), f"{width} pages a row")
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_rows_off_16_bytes(dtype, D, causal):
+    """Caches off a 16-byte boundary take the portable kernel: a term per key,
+    pages that are not there, rows of no sequence and a sequence without keys."""
+    ctx, new, ps = [100, 33, 0, 700], [1, 20, 3, 2], 32
+    q, kc, vc, table, lens, cu, rows = make(ctx, new, ps, 6, 2, D, DT[dtype], fill=0.0)
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+
+    table[0, 1], table[3, 0], table[3, 5] = -1, kc.shape[0], 2 ** 31 - 1
+    absent = [list(range(32, 64)), [], [], [*range(32), *range(160, 192)]]
+    mod = torch.randn(4, table.shape[1] * ps, generator=torch.Generator().manual_seed(7)).cuda()
+    mod[:, 3], mod[3, 100] = -torch.inf, torch.finfo(torch.float32).min
+    more = torch.cat([q, q[:9]])
+    for term in (None, mod):
+        got = ts.sigmoid_attention_paged(more, off(kc), off(vc), table, lens, cu, 20, is_causal=causal, score_mod=term)
+        assert_within(got[:sum(new)], reference(q, rows, new, causal, term, absent=absent), "o")
+        assert not got[sum(new):].any()
+    got = ts.sigmoid_attention_paged(q, off(kc), off(vc), table, ints([0, 53, 0, -5]), cu, 20, is_causal=causal)
+    assert got[1:21].any() and not got[:1].any() and not got[21:].any()
