@@ -225,16 +225,16 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
     sigattn::launch_paged_generic(k, dt, (int)p->D, causal, st);
     return launch_status();
   }
-  char *ws = (char *)workspace;
-  int2 *cuts = (int2 *)ws;
-  float *partials = (float *)(ws + pl.cut_bytes);
+  // The workspace: both parts' cuts, then their partials.
+  const auto at = [&](size_t bytes) -> void * { return workspace != nullptr ? (char *)workspace + bytes : nullptr; };
   k.gap[0] = gap;
   // The kernel also zeroes the rows outside every sequence (workgroups in
   // a multiple of 8, so that its items keep their XCDs).
   const int gaps = (int)(cdiv(cdiv(p->rows_q, 64), 8) * 8);
-  const PagedParams kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, cuts, partials);
-  const PagedParams kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0, cuts + p->B,
-                                 partials + pl.fwd.partial_bytes / sizeof(float));
+  const PagedParams kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, (int2 *)at(0), (float *)at(pl.cut_bytes));
+  const PagedParams kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0,
+                                 (int2 *)at((size_t)p->B * sizeof(int2)),
+                                 (float *)at(pl.cut_bytes + pl.fwd.partial_bytes));
   PagedParams first = pl.fwd.units > 0 ? kf : kd;
   first.ngap[0] = gaps;
   if (pl.fwd.units > 0 && pl.decode.units > 0)
