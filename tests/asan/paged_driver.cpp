@@ -7,6 +7,7 @@
 // fp32 sums of unit u at u * block * D floats and read max_units of them.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <random>
@@ -113,14 +114,65 @@ sigattn_paged_problem problem(int dtype, int64_t B, int64_t Hkv, int64_t G, int6
   return p;
 }
 
-// One part's partials lie in [from, to).
-void part(const PagedParams &p, int units, int block, int D, const char *from, const char *to) {
+// The units that paged_unit makes of a batch: the rule of its comment, in the
+// same floats (its sums may be added in another order).
+int64_t units_of(const PagedParams &p, int block, const std::vector<int> &tokens, const std::vector<int> &keys) {
+  const int B = (int)tokens.size();
+  const auto blocks = [&](int b) {
+    const int64_t cols = (int64_t)tokens[b] * p.G;
+    return (int)(cols > p.cols_lo && cols <= p.cols_hi ? (cols + block - 1) / block : 0);
+  };
+  if (block == 32 && p.split_units == 0) return (int64_t)B * p.Hkv;
+  int C = sigattn::kNoCut;
+  if (p.split_units > 0) {
+    float work = 0.0f;
+    for (int b = 0; b < B; ++b) work += (float)blocks(b) * (float)keys[b];
+    work *= (float)p.Hkv;
+    const float c = work / (float)p.split_units, least = work / (float)p.total_units;
+    C = sigattn::chunk_for(c, p.min_chunk);
+    if (B <= 64 && p.Tk < 1 << 23)
+      for (int lane = 0; lane < 63; ++lane) {
+        const int mine = sigattn::chunk_for(least + (c - least) * lane / 63.0f, p.min_chunk);
+        int64_t rows = 0;
+        for (int b = 0; b < B; ++b) rows += (int64_t)blocks(b) * std::max((int)std::ceil((float)keys[b] / (float)mine), 1);
+        if (rows * p.Hkv <= p.total_units) {
+          C = mine;
+          break;
+        }
+      }
+  }
+  int64_t units = 0;
+  for (int b = 0; b < B; ++b) {
+    const int64_t L = keys[b], round = block == 32 ? 32 : 64;
+    const int64_t most = std::min<int64_t>(std::max<int64_t>((L + C - 1) / C, 1), sigattn::kMostChunks);
+    const int64_t len = std::max<int64_t>(((L + most - 1) / most + round - 1) / round * round, round);
+    units += blocks(b) * std::max<int64_t>((L + len - 1) / len, 1) * p.Hkv;
+  }
+  return units;
+}
+
+// One part's partials lie in [from, to), and its units hold any lengths'.
+void part(const PagedParams &p, int units, int block, int D, const char *from, const char *to, std::mt19937 &rng,
+          int64_t rows) {
   EXPECT(units > 0 && p.max_units == units);
   EXPECT((int64_t)units + p.ngap[0] <= INT_MAX);
   if (p.split_units > 0) {
     EXPECT(p.min_chunk > 0 && p.total_units > p.split_units - 1 && p.total_units <= units);
     EXPECT((const char *)p.ws >= from && ((uintptr_t)p.ws & 15) == 0);
     EXPECT((const char *)(p.ws + (int64_t)units * block * D) <= to);
+  }
+  if (p.B > 3000) return;
+  for (int trial = 0; trial < 4; ++trial) {
+    std::vector<int> tokens(p.B), keys(p.B);
+    int64_t left = rows;
+    for (int b = 0; b < p.B; ++b) {
+      const int64_t most = std::min<int64_t>(left, p.Tq);
+      tokens[b] = trial == 0 ? (int)std::min<int64_t>(most, rows / p.B) : (int)(rng() % (uint64_t)(most + 1));
+      if (trial == 1 && b == 0) tokens[b] = (int)most;
+      left -= tokens[b];
+      keys[b] = trial < 2 ? p.Tk : (int)(rng() % (uint64_t)(p.Tk + 1)) >> (trial == 3 ? rng() % 20 : 0);
+    }
+    EXPECT(units_of(p, block, tokens, keys) <= units);
   }
 }
 
@@ -187,8 +239,8 @@ void sweep() {
       EXPECT(sigattn_paged_fwd(&p, kFake, nullptr, 0, nullptr) == SIGATTN_OK && g_calls.size() == 1);
       EXPECT(g_calls[0].f.split_units == 0 && g_calls[0].d.split_units == 0);
     }
-    if (c.nf > 0) part(c.f, c.nf, block, c.D, parts, end);
-    if (c.nd > 0) part(c.d, c.nd, 32, c.D, parts, end);
+    if (c.nf > 0) part(c.f, c.nf, block, c.D, parts, end, rng, p.rows_q);
+    if (c.nd > 0) part(c.d, c.nd, 32, c.D, parts, end, rng, p.rows_q);
   }
   EXPECT(valid > 10000 && cut > 2000 && mixed > 1000);
 }

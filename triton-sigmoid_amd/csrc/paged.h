@@ -46,6 +46,15 @@ struct PagedParams : KParams {
 // 21.3 / 21.9 (512: 22.1), 131072 31.7 / 31.0 / 31.1.
 constexpr int kMostChunks = 384;
 
+// The chunk length that gives every unit `keys` keys, `least` at least: one more,
+// and 2^30 + 1 at most.  A sequence has fewer than 2^30 keys, so a chunk of that
+// many never cuts it, and a length and a chunk together fit 31 bits.
+constexpr int kNoCut = 1 << 30;
+__host__ __device__ inline int chunk_for(float keys, int least) {
+  const int n = (int)(keys < (float)kNoCut ? keys : (float)kNoCut) + 1;
+  return n > least ? n : least;
+}
+
 struct PagedUnit {
   int b = 0, hk = 0, qb = 0;  // sequence, K / V head, column block
   int Lq = 0, Lk = 0;         // its tokens and keys
@@ -103,7 +112,7 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     const int b = lane + 64 * i;
     tokens[i] = b < p.B ? p.len_q(b) : 0, keys[i] = b < p.B ? p.keys(b) : 0;
   }
-  int C = 1 << 30;  // more than any length
+  int C = kNoCut;
   if (p.split_units > 0) {
     const int nqb0 = p.blocks_of(tokens[0], block), Lk0 = keys[0];
     float work = 0.0f;
@@ -113,12 +122,12 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
       work += (float)p.blocks_of(p.len_q(b), block) * (float)p.keys(b);
     work = wave_sum(work) * (float)p.Hkv;
     const float c = work / (float)p.split_units;
-    C = max(p.min_chunk, (int)fminf(c, 1e9f) + 1);
+    C = chunk_for(c, p.min_chunk);
     if (p.B <= 64 && p.Tk < 1 << 23) {  // (where the quotients below are exact enough)
       // The smallest of 64 lengths, one a lane, that gives no more units than
       // fit: from the work's share of all of them up to C, which does.
       const float least = work / (float)p.total_units;
-      const int mine = lane == 63 ? C : max(p.min_chunk, (int)fminf(least + (c - least) * lane / 63.0f, 1e9f) + 1);
+      const int mine = lane == 63 ? C : chunk_for(least + (c - least) * lane / 63.0f, p.min_chunk);
       int rows = 0;
       for (int b = 0; b < p.B; ++b) {
         const int n = __builtin_amdgcn_readlane(nqb0, b), L = __builtin_amdgcn_readlane(Lk0, b);
