@@ -322,7 +322,7 @@ int sigattn_paged_plan(int64_t B, const int32_t *context_lens, const int32_t *ne
  * slot_mapping[t].  Rows with a slot outside [0, num_pages * page_size) are not
  * written.  Strides in elements; k and v share theirs, and so do the caches.
  * Slots within a call are distinct: which of two rows with one slot stays is
- * not defined.  esize: bytes of an element, 2 or 4.
+ * not defined.  esize: bytes of an element, 2 or 4.  Up to 65535 heads.
  */
 typedef struct sigattn_paged_rows {
   int32_t esize, reserved;

@@ -290,7 +290,12 @@ void plan_and_writer() {
           EXPECT(g_kernels[0].grid.x >= 1 && g_kernels[0].grid.x <= 1 << 20 && g_kernels[0].grid.y == 2);
           g_kernels.clear();
         }
-  r.rows = 0;
+  // More heads than attention takes: refused, their products pass 63 bits.
+  for (int64_t heads : {int64_t(65536), int64_t(INT_MAX), int64_t(INT_MAX) + 1}) {
+    r.kv_heads = heads;
+    EXPECT(sigattn_paged_write(&r, nullptr) == SIGATTN_ERR_SHAPE && g_kernels.empty());
+  }
+  r.rows = 0, r.kv_heads = 8;
   EXPECT(sigattn_paged_write(&r, nullptr) == SIGATTN_OK && g_kernels.empty());
   EXPECT(sigattn_paged_write(nullptr, nullptr) == SIGATTN_ERR_NULL_ARG);
   EXPECT(sigattn_paged_check(nullptr) == SIGATTN_ERR_NULL_ARG);

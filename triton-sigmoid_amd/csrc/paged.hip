@@ -287,7 +287,8 @@ extern "C" int sigattn_paged_write(const sigattn_paged_rows *r, void *stream) {
   if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
   if (r->esize != 2 && r->esize != 4) return SIGATTN_ERR_DTYPE;
   if (r->D != 16 && r->D != 32 && r->D != 64 && r->D != 128) return SIGATTN_ERR_HEAD_DIM;
-  if (r->rows < 0 || r->kv_heads < 0 || r->num_pages < 0 || r->rows > INT32_MAX / 2 || r->kv_heads > INT32_MAX ||
+  // (rows * kv_heads * pieces of a row fit 63 bits.)
+  if (r->rows < 0 || r->kv_heads < 0 || r->num_pages < 0 || r->rows > INT32_MAX / 2 || r->kv_heads > 65535 ||
       !page_size_ok(r->page_size) || r->num_pages > INT32_MAX / r->page_size)
     return SIGATTN_ERR_SHAPE;
   const int64_t strides[5] = {r->src_stride_t, r->src_stride_h, r->cache_stride_p, r->cache_stride_t,
