@@ -39,3 +39,8 @@ needs_hipcc = pytest.mark.skipif(shutil.which("hipcc") is None and not Path("/op
 @needs_hipcc
 def test_paged_capi_under_address_and_ub_sanitizers(tmp_path):
     _run(tmp_path, CSRC / "paged_capi.cpp", CSRC / "paged.hip", ROOT / "tests" / "asan" / "paged_driver.cpp")
+
+
+@needs_hipcc
+def test_grouped_dispatch_under_address_and_ub_sanitizers(tmp_path):
+    _run(tmp_path, CSRC / "capi.cpp", ROOT / "tests" / "asan" / "grouped_driver.cpp")
