@@ -122,7 +122,7 @@ int64_t units_of(const PagedParams &p, int block, const std::vector<int> &tokens
     const int64_t cols = (int64_t)tokens[b] * p.G;
     return (int)(cols > p.cols_lo && cols <= p.cols_hi ? (cols + block - 1) / block : 0);
   };
-  if (block == 32 && p.split_units == 0) return (int64_t)B * p.Hkv;
+  if (block == sigattn::kDecodeCols && p.split_units == 0) return (int64_t)B * p.Hkv;
   int C = sigattn::kNoCut;
   if (p.split_units > 0) {
     float work = 0.0f;
@@ -143,7 +143,7 @@ int64_t units_of(const PagedParams &p, int block, const std::vector<int> &tokens
   }
   int64_t units = 0;
   for (int b = 0; b < B; ++b) {
-    const int64_t L = keys[b], round = block == 32 ? 32 : 64;
+    const int64_t L = keys[b], round = block == sigattn::kDecodeCols ? 32 : 64;
     const int64_t most = std::min<int64_t>(std::max<int64_t>((L + C - 1) / C, 1), sigattn::kMostChunks);
     const int64_t len = std::max<int64_t>(((L + most - 1) / most + round - 1) / round * round, round);
     units += blocks(b) * std::max<int64_t>((L + len - 1) / len, 1) * p.Hkv;
@@ -222,7 +222,7 @@ void sweep() {
     if (c.nf > 0 && c.nd > 0) EXPECT(c.f.cols_lo == c.d.cols_hi && c.d.cols_lo == 0 && c.f.cols_hi == INT_MAX);
     else if (c.nf > 0) EXPECT(c.f.cols_lo == 0 && c.f.cols_hi == INT_MAX);
     else EXPECT(c.d.cols_lo == 0 && (int64_t)c.d.Tq * c.d.G <= c.d.cols_hi);
-    if (c.nd > 0) EXPECT(c.d.cols_hi == 32);
+    if (c.nd > 0) EXPECT(c.d.cols_hi == sigattn::kDecodeCols);
     mixed += c.nf > 0 && c.nd > 0;
     const char *parts = kWs;
     if (n > 0) {
@@ -240,7 +240,7 @@ void sweep() {
       EXPECT(g_calls[0].f.split_units == 0 && g_calls[0].d.split_units == 0);
     }
     if (c.nf > 0) part(c.f, c.nf, block, c.D, parts, end, rng, p.rows_q);
-    if (c.nd > 0) part(c.d, c.nd, 32, c.D, parts, end, rng, p.rows_q);
+    if (c.nd > 0) part(c.d, c.nd, sigattn::kDecodeCols, c.D, parts, end, rng, p.rows_q);
   }
   EXPECT(valid > 10000 && cut > 2000 && mixed > 1000);
 }

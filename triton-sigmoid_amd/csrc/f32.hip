@@ -1055,13 +1055,14 @@ __global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const PagedParams
 template <int D, bool CAUSAL, bool SCOREMOD>
 __global__ __launch_bounds__(64 * FW, 1) void paged_f32_decode_kernel(const PagedParams p) {
   constexpr int NDB = D / 32, NW = FW;
+  static_assert(kDecodeCols == 32, "a column a lane");
   __shared__ __attribute__((aligned(16))) float sK[NW][FB * D], sV[NW][FB * D];
   const int wg = gap_prologue<4>(p, sK);
   if (wg < 0) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
-  const PagedUnit un = paged_unit(p, wg * NW + w, 32);
+  const PagedUnit un = paged_unit(p, wg * NW + w, kDecodeCols);
   if (un.nck == 0) return;
   const bool half = p.half_head(D);
   const int cols = un.Lq * p.G, keys = un.k1 - un.k0, ntiles = (keys + FB - 1) / FB;
@@ -1134,7 +1135,7 @@ __global__ __launch_bounds__(64 * FW, 1) void paged_f32_decode_kernel(const Page
   }
   if (l32 >= cols) return;
   if (un.nck == 1) store_row<D>((float *)p.out + ((row0 + tok) * p.H + head) * p.dmem, acc, 1.0f, true, hi, half);
-  else store_row<D>(p.ws + ((int64_t)(wg * NW + w) * 32 + l32) * D, acc, 1.0f, true, hi, half);
+  else store_row<D>(p.ws + ((int64_t)(wg * NW + w) * kDecodeCols + l32) * D, acc, 1.0f, true, hi, half);
 }
 
 template <int D> void paged_decode_t(const PagedParams &p, int units, bool causal, hipStream_t st) {

@@ -55,6 +55,11 @@ __host__ __device__ inline int chunk_for(float keys, int least) {
   return n > least ? n : least;
 }
 
+// Columns of a decoding unit: sequences of up to this many (new tokens times the
+// query heads of a K / V head) are the decoding kernels', longer ones the blocks'.
+// The matrix instructions' 32 columns; no block of columns is as small.
+constexpr int kDecodeCols = 32;
+
 struct PagedUnit {
   int b = 0, hk = 0, qb = 0;  // sequence, K / V head, column block
   int Lq = 0, Lk = 0;         // its tokens and keys
@@ -93,7 +98,7 @@ __device__ __forceinline__ float wave_sum(float x) {
 // of up to 64 sequences take a shorter C where that many units allow it.
 __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int block) {
   const int lane = __lane_id();
-  if (block == 32 && p.split_units == 0) {
+  if (block == kDecodeCols && p.split_units == 0) {
     // Decoding, nothing cut: a unit is a sequence's K / V head.
     PagedUnit un;
     un.b = u / p.Hkv, un.hk = u - un.b * p.Hkv;
@@ -148,7 +153,7 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedParams &p, int u, int
     // Equal chunks of a multiple of `round` keys, as few as that takes.  Quotients
     // in floats, corrected, where lengths are exact in them (0.5 to 1 us a call
     // faster than by integer division).
-    const int round = block == 32 ? 32 : 64;
+    const int round = block == kDecodeCols ? 32 : 64;
     int len, nck;
     if (p.Tk < 1 << 23) {
       len = round * max((int)((float)Lk * __builtin_amdgcn_rcpf((float)(most * round))), 1);
@@ -327,8 +332,8 @@ template <int ROWS, int D, int NWAVES, bool NT = false, int ESIZE = 2> struct Pa
 void launch_paged_generic(const PagedParams &p, int dtype, int D, bool causal, hipStream_t st);
 // MFMA kernels, dtype in {kF16, kBF16}, D in {32, 64, 128} (16 as 32 with
 // dmem = 16), 16-byte aligned rows: blocks of paged_block(D) columns; a wave
-// per chunk for sequences of up to 32 columns; and the sums of cut sequences.  ngap leading workgroups (pf's) zero the rows
-// outside every sequence.
+// per chunk for sequences of up to kDecodeCols columns; and the sums of cut
+// sequences.  ngap leading workgroups (pf's) zero the rows outside every sequence.
 int paged_block(int D);
 void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
 void launch_paged_decode(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
@@ -336,7 +341,7 @@ void launch_paged_decode(const PagedParams &p, int units, int dtype, int D, bool
 void launch_paged_mixed(const PagedParams &pf, int nf, const PagedParams &pd, int nd, int dtype, int D, bool causal,
                         hipStream_t st);
 // fp32, D in {32, 64, 128} (16 as above): blocks of kPagedBlockF32 columns, and a
-// wave per chunk where every sequence has up to 32.
+// wave per chunk where every sequence has up to kDecodeCols.
 constexpr int kPagedBlockF32 = 128;
 void launch_paged_decode_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st);
 void launch_paged_f32(const PagedParams &p, int units, int D, bool causal, hipStream_t st);

@@ -9,6 +9,7 @@
 #include "launch.h"
 #include "paged.h"
 
+using sigattn::kDecodeCols;
 using sigattn::PagedParams;
 
 namespace {
@@ -70,8 +71,7 @@ struct Part {
 // 101, B=64 8000..9000 H=8 338 / 343 (6.57 TB/s); chunks of 64 / 128 / 192 keys at
 // least, B=1 2000 keys 13.9 / 16.1 / 17.3, B=16 200..300 18.2 / 20.2 / 21.4, B=3
 // up to 8000 15.2 / 16.6 / 18.7, longer ones alike.
-constexpr int kDecodeCols = 32;
-constexpr int64_t kDecodeWaves = 4, kDecodeChunk = 64;
+constexpr int64_t kDecodeWavesPerCu = 4, kDecodeChunk = 64;
 // The forward kernel's chunks, where its blocks do not fill the GPU: a round of
 // its workgroups, of 1024 keys at least.  Whole call, us, one / two rounds: bf16
 // H=32 Hkv=8 D=128, 2 x 1024 tokens on up to 12000 keys 324 / 343, 256 on 12000
@@ -128,10 +128,10 @@ Plan make_plan(const sigattn_paged_problem *p, const PagedParams &k, int D) {
   // (fp32: no launch for both, so one long sequence takes all to the blocks.)
   const bool f32 = p->dtype == SIGATTN_F32;
   const bool decode = cols <= kDecodeCols || (k.B > 1 && !f32), fwd = cols > kDecodeCols;
-  pl.fwd.block = f32 ? sigattn::kPagedBlockF32 : sigattn::paged_block(D), pl.decode.block = 32;
+  pl.fwd.block = f32 ? sigattn::kPagedBlockF32 : sigattn::paged_block(D), pl.decode.block = kDecodeCols;
   if (decode) {
     const int64_t pairs = (int64_t)k.B * k.Hkv;
-    cut_part(pl.decode, pairs, kDecodeWaves * cus, kDecodeChunk, k, D, true, f32);
+    cut_part(pl.decode, pairs, kDecodeWavesPerCu * cus, kDecodeChunk, k, D, true, f32);
   }
   if (fwd) {
     if (decode) pl.cols_lo = kDecodeCols;

@@ -24,7 +24,6 @@
 
 namespace sigattn {
 
-constexpr int kDecodeCols = 32;
 // Waves per workgroup.  1 / 2 / 4, us (as the caller's figures): B=16 contexts
 // 1024..8191 61 / 48 / 49, B=64 8000..9000 438 / 333 / 338, D=64 35 / 34 / 29.
 constexpr int kDecodeWaves = 4;
@@ -39,6 +38,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams &p, const in
                                                   DecodeTiles<D, NW> &sV, DecodeTerms<NW, SCOREMOD> &sM) {
   constexpr int KB = 32;  // keys per block
   constexpr int NKS = D / 16, NDB = D / 32;
+  static_assert(kDecodeCols == 32, "a column a lane");
   using Dma = PagedDma<KB, D, 1, true>;
   constexpr int NI = Dma::NI;                  // copy instructions per block of V
   constexpr int NK = NI + (SCOREMOD ? 1 : 0);  // ... of K, with its keys' score_mod

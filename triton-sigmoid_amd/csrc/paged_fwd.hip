@@ -161,6 +161,7 @@ template <class F> void by_type(int dtype, int D, F &&f) {
 
 }  // namespace
 
+static_assert(32 * waves_of(32) > kDecodeCols && kPagedBlockF32 > kDecodeCols, "blocks and decoding units differ");
 int paged_block(int D) { return 32 * waves_of(D); }
 
 void launch_paged_fwd(const PagedParams &p, int units, int dtype, int D, bool causal, hipStream_t st) {
@@ -185,7 +186,7 @@ void launch_paged_reduce(const PagedParams &fwd, const PagedParams &decode, int 
   a.cut[0] = fwd.split_units > 0 ? fwd.cut : nullptr;
   a.cut[1] = decode.split_units > 0 ? decode.cut : nullptr;
   a.units[0] = fwd.max_units, a.units[1] = decode.max_units;
-  a.block[0] = dtype == kF32 ? kPagedBlockF32 : paged_block(D), a.block[1] = 32, a.cols = decode.cols_hi;
+  a.block[0] = dtype == kF32 ? kPagedBlockF32 : paged_block(D), a.block[1] = kDecodeCols, a.cols = decode.cols_hi;
   by_type(dtype, D, [&](auto *t, auto d) {
     reduce_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(a, st);
   });
