@@ -458,3 +458,29 @@ def test_backward_past_the_workspace_limit(monkeypatch, binding):
     full, size = lib.sigattn_bwd_workspace_bytes(ctypes.byref(pr)), _capi.bwd_workspace_bytes(lib, pr, q.device)
     assert 0 < size <= 180 << 20 < full
     check(q, k, v, do, cu, cu, True)
+
+
+def test_dense_and_padded_tensors_as_packed_ones():
+    """[B, T, H, D] tensors with grouped heads through views and the valid rows."""
+    B, T, H, Hkv, D = 3, 70, 4, 2, 64
+    q, k, v, do = make(B * T, B * T, H, Hkv, D, torch.bfloat16, 34)
+    cu = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device="cuda")
+    leaves = [t.view(B, T, -1, D).requires_grad_(True) for t in (q.clone(), k.clone(), v.clone())]
+    a, b, c = leaves
+    out = ts.sigmoid_attention_varlen(a.flatten(0, 1), b.flatten(0, 1), c.flatten(0, 1), cu, cu, T, T,
+                                      is_causal=True).view_as(a)
+    got = dict(zip(("o", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do.view_as(out)))))
+    want = packed(q, k, v, do, cu.tolist(), cu.tolist(), True)
+    for x in got:
+        assert_within(got[x].flatten(0, 1), want[x], x)
+    lens = torch.tensor([70, 0, 33], device="cuda")
+    valid = torch.arange(T, device="cuda") < lens[:, None]
+    cu = torch.nn.functional.pad(lens.cumsum(0, dtype=torch.int32), (1, 0))
+    out = torch.zeros_like(a).masked_scatter(valid[..., None, None], ts.sigmoid_attention_varlen(
+        a[valid], b[valid], c[valid], cu, cu, T, T, is_causal=True))
+    got = dict(zip(("o", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do.view_as(out)))))
+    rows = valid.flatten()
+    want = packed(q[rows], k[rows], v[rows], do[rows], cu.tolist(), cu.tolist(), True)
+    for x in got:
+        assert_within(got[x].flatten(0, 1)[rows], want[x], x)
+        assert not got[x].flatten(0, 1)[~rows].any()
