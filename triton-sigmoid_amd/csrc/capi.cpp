@@ -119,7 +119,9 @@ struct SplitPlan {
 // D = 16 and 32 the main forward and the recompute backward serve every shape.
 bool wide_head(const sigattn_problem *p) { return p->D == 64 || p->D == 128; }
 
-// ... and with grouped heads at D = 128 alone (below it the recompute kernels are faster).
+// ... and with grouped heads at D = 128 alone: the Python layers take it nowhere
+// else (at D = 64 the recompute kernels measured faster with a K / V head per query
+// head), and the dK/dV kernel of groups that stores dS is not built below.
 bool two_pass_head(const sigattn_problem *p) { return wide_head(p) && (p->D == 128 || head_group(p) == 1); }
 
 // Head dim of the MFMA kernel instance: head_dim 16 runs in the D = 32

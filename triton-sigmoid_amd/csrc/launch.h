@@ -97,8 +97,9 @@ hipError_t splitkv_scratch(float **ptr);
 // one launch (an axis with rows = 0 takes no workgroups); esize = 2 or 4.
 void launch_zero_gaps(const GapAxis &a, const GapAxis &b, int esize, hipStream_t st);
 
-// fp32 kernels on the matrix cores (v_mfma_f32_32x32x2_f32): D in {32, 64,
-// 128} (head_dim 16 as D = 32 with KParams::dmem = 16), 16-byte aligned rows.
+// fp32 kernels on the matrix cores (three bf16 parts an operand, see f32.hip): D
+// in {32, 64, 128} (head_dim 16 as D = 32 with KParams::dmem = 16), 16-byte
+// aligned rows.
 void launch_fwd_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);
 void launch_bwd_dq_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);
 void launch_bwd_dkdv_f32(const KParams &p, int D, bool causal, bool scoremod, hipStream_t st);

@@ -1,5 +1,5 @@
 // Paged key/value cache: its bookkeeping, its writer, and the portable
-// attention kernel (fp32, and tensors off 16-byte boundaries).
+// attention kernel (any type; tensors off 16-byte boundaries).
 //
 // The entry points of include/sigattn.h for the paged cache are here and in
 // paged_capi.cpp; none allocates, synchronises the host or throws.

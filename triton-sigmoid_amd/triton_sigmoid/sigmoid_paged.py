@@ -405,8 +405,8 @@ def sigmoid_attention_paged(
         cu_seqlens_q: [B + 1] non-decreasing offsets, cu[0] = 0.
         max_seqlen_q: most new tokens of a sequence (a longer one is cut to
             its first max_seqlen_q rows, whose places among the keys then
-            end seq_lens_k too); None takes N.  It picks the kernels, so
-            give it for decoding.
+            end seq_lens_k too); None takes N.  It picks the kernels and sizes
+            the workspace, so give it for decoding.
         is_causal: query i of n new tokens sees keys up to position
             seq_lens_k - n + i (bottom-right: the last query sees every key); a
             row whose position is negative sees none and is zeros.
@@ -417,8 +417,8 @@ def sigmoid_attention_paged(
 
     Returns:
         [N, H, D] output, contiguous.  Rows outside every sequence are zeros.
-        Slots of the cache past a sequence's length are never read; keys and
-        values of a sequence itself have to be finite.  Deterministic.
+        Slots of the cache past a sequence's length are never read; the query,
+        and keys and values of a sequence itself, have to be finite.  Deterministic.
         Forward only: tensors that ask for a gradient (under grad mode) or
         carry a forward-mode tangent are refused.
     """
