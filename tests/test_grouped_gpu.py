@@ -484,3 +484,44 @@ def test_dense_and_padded_tensors_as_packed_ones():
     for x in got:
         assert_within(got[x].flatten(0, 1)[rows], want[x], x)
         assert not got[x].flatten(0, 1)[~rows].any()
+
+
+def test_large_ragged_grids():
+    """Not causal, D = 64, eight row blocks a compute unit: dQ beside dK/dV on a
+    second stream; with few K / V heads their groups in parts there."""
+    for heads, lens in (((16, 4), [512 - 7 * i for i in range(34)]), ((64, 1), [400, 1, 0, 257, 512, 130, 511, 300, 64])):
+        cu = offsets(lens)
+        q, k, v, do = make(cu[-1], cu[-1], *heads, 64, torch.float16, 35)
+        units = torch.cuda.get_device_properties(0).multi_processor_count
+        assert len(lens) * heads[0] * (512 // 128) >= 8 * units
+        got = check(q, k, v, do, cu, cu, False)
+        same = run(q, k, v, do, cu, cu, is_causal=False)
+        for x in got:
+            assert torch.equal(got[x], same[x])
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_fp32_of_many_blocks(D, causal):
+    """Grids from a workgroup per compute unit on, where fewer waves share rows;
+    lengths that end inside a block, and short ones between them."""
+    for heads, lens in (((32, 8), [700, 5, 513, 640, 128, 0, 699, 1]), ((12, 6), [130] * 70)):
+        cu = offsets(lens)
+        q, k, v, do = make(cu[-1], cu[-1], *heads, D, torch.float32, 36)
+        check(q, k, v, do, cu, cu, causal)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_off_16_bytes_in_other_types(dtype):
+    cu = offsets([33, 0, 70, 200])
+    q, k, v, do = make(cu[-1], cu[-1], 6, 2, 64, DT[dtype], 37)
+    mod = torch.randn(cu[-1], generator=torch.Generator().manual_seed(38)).cuda()
+    mod[7] = -torch.inf
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+
+    for causal in (False, True):
+        check(off(q), off(k), off(v), off(do), cu, cu, causal, mod)

@@ -802,3 +802,25 @@ def test_rows_off_16_bytes(dtype, D, causal):
         assert not got[sum(new):].any()
     got = ts.sigmoid_attention_paged(q, off(kc), off(vc), table, ints([0, 53, 0, -5]), cu, 20, is_causal=causal)
     assert got[1:21].any() and not got[:1].any() and not got[21:].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [16, 32])
+def test_terms_per_key_of_small_heads(D, dtype):
+    for shape in ("decode", "few", "chunk", "mixed", "long"):
+        ctx, new = SHAPES[shape]
+        check(ctx, new, 16, 8, 2, D, DT[dtype], mod=True)
+        check(ctx, new, 32, 6, 3, D, DT[dtype], causal=False, mod=True, sigmoid_bias=-2.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_cuts_among_more_lengths_than_are_kept(dtype):
+    """Batches of more than 256 sequences (whose lengths the waves hold) that are
+    cut: decoding, chunks, and both."""
+    r = random.Random(21)
+    ctx = [r.choice((0, 1, 17, r.randint(0, 300), r.randint(0, 900))) for _ in range(300)]
+    ctx[290], ctx[3] = 2600, 1500
+    check(ctx, [1] * 300, 16, 4, 2, 32, DT[dtype])
+    new = [r.choice((0, 1, 1, 1, 2)) for _ in ctx]
+    new[290], new[270] = 40, 20
+    check(ctx, new, 32, 4, 1, 64, DT[dtype])
