@@ -321,8 +321,8 @@ int sigattn_paged_plan(int64_t B, const int32_t *context_lens, const int32_t *ne
  * Writes packed K and V rows [rows, kv_heads, D] into the caches: row t goes to
  * slot_mapping[t].  Rows with a slot outside [0, num_pages * page_size) are not
  * written.  Strides in elements; k and v share theirs, and so do the caches.
- * Slots within a call are distinct: which of two rows with one slot stays is
- * not defined.  esize: bytes of an element, 2 or 4.  Up to 65535 heads.
+ * Slots within a call are distinct: of two rows with one slot either may stay, or
+ * pieces of both.  esize: bytes of an element, 2 or 4.  Up to 65535 heads.
  */
 typedef struct sigattn_paged_rows {
   int32_t esize, reserved;

@@ -269,8 +269,8 @@ def paged_cache_write(
             transposed view); changed in place.
         slot_mapping: [N] slot page * page_size + row of each token, as
             paged_plan gives it; rows with a slot outside the cache (-1) are not
-            written.  The slots of one call have to be distinct: which of two
-            rows with one slot stays is not defined.
+            written.  The slots of one call have to be distinct: of two rows
+            with one slot either may stay, or pieces of both.
     """
     quick = _quick()
     if quick is not None and quick.quick_write(key, value, key_cache, value_cache, slot_mapping):
