@@ -525,3 +525,24 @@ def test_rows_off_16_bytes_in_other_types(dtype):
 
     for causal in (False, True):
         check(off(q), off(k), off(v), off(do), cu, cu, causal, mod)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_training_steps_on_two_streams(D):
+    """Two grouped steps at once, each on a stream of its own and with the parts of
+    its groups in a workspace of its own: as one after the other."""
+    cus, data, want = [offsets([300, 70, 512]), offsets([411, 0, 200])], [], []
+    for i, cu in enumerate(cus):
+        data.append(make(cu[-1], cu[-1], 16, 2, D, torch.bfloat16, 40 + i))
+        want.append(run(*data[i], cu, cu, max_seqlen_q=512, max_seqlen_k=512, is_causal=True))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, d, cu in zip(streams, data, cus):
+            with torch.cuda.stream(s):
+                got.append(run(*d, cu, cu, max_seqlen_q=512, max_seqlen_k=512, is_causal=True))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for x in a:
+                assert torch.equal(a[x], b[x])

@@ -824,3 +824,34 @@ def test_cuts_among_more_lengths_than_are_kept(dtype):
     new = [r.choice((0, 1, 1, 1, 2)) for _ in ctx]
     new[290], new[270] = 40, 20
     check(ctx, new, 32, 4, 1, 64, DT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_graphs_of_one_pool(dtype):
+    """Two captured calls whose workspaces lie in one pool, replayed in turn on
+    changing lengths: each equals the eager call."""
+    sets = [make([3000, 50, 900], [1, 1, 1], 16, 8, 2, 64, DT[dtype], 1),
+            make([1500, 2500], [40, 1], 16, 8, 2, 64, DT[dtype], 2)]
+    longest, calls = (1, 40), []
+    call = lambda i: ts.sigmoid_attention_paged(*sets[i][:6], longest[i], is_causal=True)  # noqa: E731
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call(0), call(1)
+    side.synchronize()
+    pool = None
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = call(i)
+        pool = graph.pool()
+        calls.append((graph, out))
+    for cut in (0, 700, 1234):
+        for i in (0, 1, 1, 0):
+            lens = sets[i][4]
+            whole = lens.clone()
+            lens.sub_(cut).clamp_(min=longest[i])
+            calls[i][0].replay()
+            torch.cuda.synchronize()
+            have = calls[i][1].clone()
+            assert torch.equal(have, call(i))
+            lens.copy_(whole)
