@@ -55,8 +55,11 @@ enum sigattn_status {
   SIGATTN_ERR_WORKSPACE = -10,    /* workspace too small for the call, or misaligned */
   SIGATTN_ERR_SCRATCH = -11,      /* sigattn_fwd_noalloc: scratch need above
                                      SIGATTN_NOALLOC_SCRATCH_BYTES */
-  SIGATTN_ERR_KV_HEADS = -12      /* kv_heads does not divide H, or is set to
+  SIGATTN_ERR_KV_HEADS = -12,     /* kv_heads does not divide H, or is set to
                                      another number in a layout that is not packed */
+  SIGATTN_ERR_REL_BIAS = -13,     /* sigattn_rel_bias: max_distance or num_buckets out of
+                                     range, a score_mod beside it, or sequences not packed */
+  SIGATTN_ERR_ROTARY = -14        /* sigattn_rotary: rot_dim odd or beyond D, or no positions */
 };
 
 /*
@@ -375,6 +378,79 @@ int sigattn_paged_check(const sigattn_paged_problem *p);
 size_t sigattn_paged_fwd_workspace_bytes(const sigattn_paged_problem *p);
 int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace, size_t workspace_bytes,
                       void *stream);
+
+/*
+ * Learned bias by relative position (no counterpart in the reference): the score
+ * of query i and key j of a sequence gets table[buckets[max_distance + d], h], d = j - i
+ * clamped to [-max_distance, max_distance] and h the query head, beside scale
+ * and bias.  Buckets outside [0, num_buckets) add nothing and get no gradient.
+ * Packed problems (both axes) without score_mod.
+ */
+#define SIGATTN_REL_MAX_DISTANCE 2048
+#define SIGATTN_REL_MAX_BUCKETS 65536
+typedef struct sigattn_rel_bias {
+  int32_t dtype;          /* enum sigattn_dtype of the table and its gradient */
+  int32_t num_buckets;
+  int64_t max_distance;
+  const void *table;      /* [num_buckets, H], contiguous */
+  const int32_t *buckets; /* [2 max_distance + 1] */
+} sigattn_rel_bias;
+
+int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r);
+/*
+ * Forward and backward with that bias.  Both need their workspace (16-byte
+ * aligned, used until the call's kernels finish; SIGATTN_ERR_WORKSPACE without it).
+ * `dtable` is the table's gradient, [num_buckets, H] of its type, written whole:
+ * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed).
+ * Deterministic.
+ */
+size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
+int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
+                    size_t workspace_bytes, void *stream);
+size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
+int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
+                    void *dtable, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * sigattn_paged_fwd with that bias; query i of n new tokens sits at position
+ * L - n + i.  The workspace is needed.
+ */
+int sigattn_paged_rel_check(const sigattn_paged_problem *p, const sigattn_rel_bias *r);
+size_t sigattn_paged_rel_fwd_workspace_bytes(const sigattn_paged_problem *p, const sigattn_rel_bias *r);
+int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/*
+ * Rotary embedding (no counterpart in the reference): the first rot_dim columns
+ * of a head's row turn in pairs by the angles of the row's position,
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * pair i being columns i and i + rot_dim / 2, or (interleaved) 2i and 2i + 1, its
+ * angle's cosine and sine angles[position][i] and angles[position][i + rot_dim / 2].
+ * Positions are clamped to the table's.  inverse: by the negative angles (the backward).
+ * The products are fp32, rounded once; the other columns are copied.
+ *
+ * sigattn_rotary_apply turns q into q_out and k into k_out (contiguous [rows,
+ * heads, D]); kv_heads may be 0.  sigattn_paged_write_rotary turns q into q_out, writes
+ * the turned k and v itself to their slots as sigattn_paged_write does.  Inputs and
+ * outputs do not overlap.
+ */
+typedef struct sigattn_rotary {
+  int32_t dtype;
+  int32_t interleaved, inverse, reserved;
+  int64_t rows, q_heads, kv_heads, D, rot_dim, num_positions;
+  int64_t q_stride_t, q_stride_h;                        /* q */
+  int64_t k_stride_t, k_stride_h;                        /* k and v */
+  int64_t cache_stride_p, cache_stride_t, cache_stride_h; /* both caches: page, token, head */
+  int64_t num_pages, page_size;
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  void *k_cache, *v_cache;
+  const int32_t *positions;    /* [rows] */
+  const float *angles;         /* [num_positions, rot_dim], contiguous */
+  const int32_t *slot_mapping; /* [rows] */
+} sigattn_rotary;
+int sigattn_rotary_apply(const sigattn_rotary *r, void *stream);
+int sigattn_paged_write_rotary(const sigattn_rotary *r, void *stream);
 
 #ifdef __cplusplus
 }

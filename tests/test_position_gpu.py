@@ -1,0 +1,461 @@
+"""The learned bias by relative position, in packed sequences (forward, backward
+and the table's gradient) and over a paged cache, against its definition in 64 bits."""
+
+import math
+import random
+
+import pytest
+import torch
+
+import triton_sigmoid as ts
+from reference64 import assert_within, one_head
+from reference64_rel import line_of, packed_rel
+
+pytestmark = pytest.mark.gpu
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+I32 = torch.int32
+
+
+def ints(v):
+    return torch.tensor(v, dtype=I32, device="cuda")
+
+
+def offsets(lens, first=0):
+    at = [first]
+    for n in lens:
+        at.append(at[-1] + n)
+    return at
+
+
+def randn(g, *shape, dtype, f=1.0):
+    return (f * torch.randn(shape, generator=g)).to(dtype).cuda()
+
+
+def make(lens_q, lens_k, H, Hkv, D, dtype, num, R, seed=0, table_dtype=None, first=0, rest=0):
+    g = torch.Generator().manual_seed(seed)
+    nq, nk = first + sum(lens_q) + rest, first + sum(lens_k) + rest
+    q, do = (randn(g, nq, H, D, dtype=dtype) for _ in range(2))
+    k, v = (randn(g, nk, Hkv, D, dtype=dtype) for _ in range(2))
+    table = randn(g, num, H, dtype=table_dtype or dtype, f=2.0)
+    buckets = torch.randint(0, num, (2 * R + 1,), generator=g).to(I32).cuda()
+    return q, k, v, do, table, buckets, offsets(lens_q, first), offsets(lens_k, first)
+
+
+def run(q, k, v, do, table, buckets, cu_q, cu_k, causal, bias=None, mq=None, mk=None):
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v, table)]
+    mq = max(b - a for a, b in zip(cu_q, cu_q[1:])) if mq is None else mq
+    mk = max(b - a for a, b in zip(cu_k, cu_k[1:])) if mk is None else mk
+    o = ts.sigmoid_attention_varlen(*leaves[:3], ints(cu_q), ints(cu_k), mq, mk, is_causal=causal, sigmoid_bias=bias,
+                                    bias_table=leaves[3], bias_buckets=buckets)
+    return dict(zip(("o", "dq", "dk", "dv", "dtable"), (o, *torch.autograd.grad(o, leaves, do))))
+
+
+def check(args, causal, bias=None):
+    got = run(*args, causal, bias)
+    want = packed_rel(*args, causal, bias)
+    for x in want:
+        assert_within(got[x], want[x], x)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_types_and_head_dims(dtype, D, causal):
+    lens = [131, 1, 70, 0, 33]
+    check(make(lens, lens, 4, 2, D, DT[dtype], 8, 20, seed=D), causal)
+
+
+@pytest.mark.parametrize("R", [0, 1, 7, 31, 32, 33, 64, 128, 300, 2048])
+@pytest.mark.parametrize("causal", [False, True])
+def test_reaches(R, causal):
+    lens = [290, 65]
+    check(make(lens, lens, 2, 2, 64, torch.bfloat16, 11, R, seed=R), causal)
+
+
+@pytest.mark.parametrize("num", [1, 2, 255, 256, 257, 700])
+def test_numbers_of_buckets(num):
+    check(make([150, 40], [150, 40], 2, 1, 32, torch.float16, num, 200, seed=num), False)
+
+
+@pytest.mark.parametrize("H, Hkv", [(1, 1), (3, 1), (8, 8), (12, 4), (16, 1), (6, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_heads(H, Hkv, D):
+    lens = [100, 200, 37]
+    check(make(lens, lens, H, Hkv, D, torch.bfloat16, 16, 50, seed=H), True)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 513])
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 64), ("bf16", 32)])
+def test_lengths(n, dtype, D):
+    for causal in (False, True):
+        check(make([n], [n], 2, 2, D, DT[dtype], 12, 40, seed=n), causal)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 32), ("bf16", 16)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_keys_of_other_lengths(dtype, D, causal):
+    """Positions count from both starts; sequences without queries or without keys."""
+    check(make([5, 150, 0, 40, 70], [200, 30, 17, 0, 71], 4, 2, D, DT[dtype], 12, 40, seed=D), causal)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("bf16", 128), ("f32", 64)])
+def test_long_sequences(dtype, D):
+    lens = [1500, 777]
+    check(make(lens, lens, 2, 1, D, DT[dtype], 32, 128, seed=3), True)
+    check(make(lens, lens, 2, 2, D, DT[dtype], 32, 128, seed=4), False)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 64), ("f16", 32)])
+def test_many_sequences(dtype, D):
+    """More of them than a wave has lanes, many empty."""
+    r = random.Random(5)
+    lens = [r.choice((0, 1, 3, r.randint(1, 90))) for _ in range(150)]
+    for causal in (False, True):
+        check(make(lens, lens, 2, 1, D, DT[dtype], 10, 25, seed=7), causal)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 64)])
+def test_rows_outside_every_sequence_are_zeros(dtype, D):
+    q, k, v, do, table, buckets, cu, _ = make([60, 100], [60, 100], 2, 2, D, DT[dtype], 8, 16, first=13, rest=70)
+    got = run(q, k, v, do, table, buckets, cu, cu, True, mq=80, mk=80)
+    cut = [13, 73, 153]  # the second sequence to 80 rows; its default bias is the whole one's
+    want = packed_rel(q[:153], k[:153], v[:153], do[:153], table, buckets, cut, cut, True, [-math.log(60), -math.log(100)])
+    for x in ("o", "dq", "dk", "dv"):
+        assert_within(got[x][:153], want[x], x)
+        assert not got[x][153:].any() and not got[x][:13].any(), x
+    assert_within(got["dtable"], want["dtable"], "dtable")
+
+
+@pytest.mark.parametrize("table_dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_the_table_has_a_type_of_its_own(dtype, table_dtype):
+    args = make([90, 30], [90, 30], 3, 3, 64, DT[dtype], 8, 30, table_dtype=DT[table_dtype])
+    assert check(args, True)["dtable"].dtype == DT[table_dtype]
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 64), ("f32", 16)])
+def test_values_at_the_types_ends(dtype, D):
+    """Buckets of -inf and of the type's lowest value leave nothing, huge ones all."""
+    q, k, v, do, table, buckets, cu, _ = make([140, 3], [140, 3], 2, 2, D, DT[dtype], 8, 30, seed=9)
+    table[0], table[1], table[2] = -math.inf, torch.finfo(table.dtype).min, torch.finfo(table.dtype).max
+    check((q, k, v, do, table, buckets, cu, cu), False)
+    table[:] = -math.inf  # rows that see nothing
+    got = check((q, k, v, do, table, buckets, cu, cu), True)
+    assert all(not got[x].any() for x in got)
+
+
+def test_buckets_outside_the_table_add_nothing():
+    q, k, v, do, table, buckets, cu, _ = make([100, 31], [100, 31], 2, 2, 64, torch.float32, 8, 20)
+    buckets[::3], buckets[1], buckets[5] = 8, -1, 1 << 30
+    check((q, k, v, do, table, buckets, cu, cu), False)
+    wide = buckets.long()
+    wide[0] = 1 << 40
+    got = run(q, k, v, do, table, wide, cu, cu, False)
+    assert torch.equal(got["o"], run(q, k, v, do, table, buckets, cu, cu, False)["o"])
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f32", 64), ("f16", 128)])
+def test_strides_and_alignment(dtype, D):
+    """Views with other strides, and rows off 16-byte boundaries."""
+    q, k, v, do, table, buckets, cu, _ = make([75, 20], [75, 20], 2, 2, D, DT[dtype], 8, 20)
+    want = packed_rel(q, k, v, do, table, buckets, cu, cu, True)
+
+    def odd(t):
+        s = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        return s.copy_(t)
+
+    for f in (odd, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)):
+        views = [f(t).requires_grad_() for t in (q, k, v)] + [table.t().contiguous().t().requires_grad_()]
+        o = ts.sigmoid_attention_varlen(*views[:3], ints(cu), ints(cu), 75, 75, is_causal=True, bias_table=views[3],
+                                        bias_buckets=buckets)
+        got = (o, *torch.autograd.grad(o, views, f(do)))
+        for x, t in zip(("o", "dq", "dk", "dv", "dtable"), got):
+            assert_within(t, want[x], x)
+
+
+def test_zero_values_change_nothing():
+    """A table of zeros: within the bounds, as the attention without one is."""
+    q, k, v, do, table, buckets, cu, _ = make([200, 90], [200, 90], 4, 4, 64, torch.bfloat16, 8, 20)
+    plain = ts.sigmoid_attention_varlen(q, k, v, ints(cu), ints(cu), 200, 200, is_causal=True)
+    none = torch.zeros_like(table)
+    check((q, k, v, do, none, buckets, cu, cu), True)
+    assert_within(plain, packed_rel(q, k, v, do, none, buckets, cu, cu, True)["o"])
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 32), ("bf16", 32)])
+def test_deterministic(dtype, D):
+    args = make([700, 333, 90], [700, 333, 90], 4, 2, D, DT[dtype], 32, 128)
+    first = run(*args, True)
+    for _ in range(3):
+        again = run(*args, True)
+        assert all(torch.equal(first[x], again[x]) for x in first)
+
+
+def test_gradient_against_differences():
+    """fp32 against central differences of the op in the table's own direction: off by
+    step^2 / 6 times the third derivative (|sigmoid'''| <= 1/8, of every score that the
+    bucket reaches), and by the two values' rounding over the step."""
+    args = q, k, v, do, table, buckets, cu, _ = make([40, 25], [40, 25], 2, 2, 32, torch.float32, 6, 12, seed=2)
+    got = run(*args, False)["dtable"]
+    want = packed_rel(*args, False)
+    step, dO = 2.0 ** -6, do.double()
+    for u, h in ((0, 0), (3, 1), (5, 0)):
+        values = []
+        for sign in (1.0, -1.0):
+            moved = table.clone()
+            moved[u, h] += sign * step
+            o = run(q, k, v, do, moved, buckets, cu, cu, False)["o"].double()
+            values.append((o * dO).sum())
+        slope = (values[0] - values[1]) / (2 * step)
+        third = sum((do[a:b, h].double() @ v[a:b, h].double().t()).abs().sum() for a, b in zip(cu, cu[1:])) / 8
+        noise = (want["o"][1] * dO.abs()).sum() / step
+        assert (slope - got[u, h].double()).abs() <= step ** 2 / 6 * third + noise + want["dtable"][1][u, h]
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_a_table_without_gradient(frozen):
+    q, k, v, do, table, buckets, cu, _ = make([200], [200], 2, 2, 64, torch.bfloat16, 8, 20)
+    full = run(q, k, v, do, table, buckets, cu, cu, True)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)] if frozen else [q, k, v]
+    t = table.clone().requires_grad_(not frozen)
+    o = ts.sigmoid_attention_varlen(*leaves, ints(cu), ints(cu), 200, 200, is_causal=True, bias_table=t,
+                                    bias_buckets=buckets)
+    got = torch.autograd.grad(o, leaves if frozen else [t], do)
+    for x, y in zip(("dq", "dk", "dv") if frozen else ("dtable",), got):
+        assert torch.equal(full[x], y)
+
+
+def test_captured_step_replays():
+    q, k, v, do, table, buckets, cu, _ = make([300, 170, 64], [300, 170, 64], 4, 2, 64, torch.bfloat16, 32, 100)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    at = ints(cu)
+
+    def step():
+        o = ts.sigmoid_attention_varlen(*leaves[:3], at, at, 300, 300, is_causal=True, bias_table=leaves[3],
+                                        bias_buckets=buckets)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_(torch.roll(t, 1, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        del want
+
+
+def test_streams_and_two_calls_at_once():
+    a = make([400, 100], [400, 100], 4, 4, 64, torch.bfloat16, 16, 60, seed=1)
+    b = make([350, 222], [350, 222], 4, 4, 64, torch.bfloat16, 16, 60, seed=2)
+    want = run(*a, True), run(*b, True)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [None, None]
+    for _ in range(3):
+        for i, (s, x) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[i] = run(*x, True)
+        torch.cuda.synchronize()
+        for w, y in zip(want, got):
+            assert all(torch.equal(w[x], y[x]) for x in w)
+
+
+def test_compiled_and_eager_alike():
+    q, k, v, do, table, buckets, cu, _ = make([90, 40], [90, 40], 2, 2, 64, torch.bfloat16, 8, 20)
+    at = ints(cu)
+
+    def f(q, k, v, t):
+        return ts.sigmoid_attention_varlen(q, k, v, at, at, 90, 90, is_causal=True, bias_table=t, bias_buckets=buckets)
+
+    want = run(q, k, v, do, table, buckets, cu, cu, True)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+    o = torch.compile(f, fullgraph=True, backend="aot_eager")(*leaves)
+    got = (o, *torch.autograd.grad(o, leaves, do))
+    assert all(torch.equal(want[x], y) for x, y in zip(("o", "dq", "dk", "dv", "dtable"), got))
+
+
+def test_empty_calls():
+    z = lambda n, h: torch.zeros(n, h, 64, device="cuda", requires_grad=True)  # noqa: E731
+    table = torch.ones(4, 2, device="cuda", requires_grad=True)
+    buckets = ints([0, 1, 2])
+    for nq, nk, cu_q, cu_k in ((0, 0, [0, 0], [0, 0]), (3, 0, [0, 3], [0, 0]), (0, 3, [0, 0], [0, 3]), (3, 3, [0], [0])):
+        q, k, v = z(nq, 2), z(nk, 2), z(nk, 2)
+        o = ts.sigmoid_attention_varlen(q, k, v, ints(cu_q), ints(cu_k), nq, nk, bias_table=table, bias_buckets=buckets)
+        assert o.shape == q.shape and not o.any()
+        for t, g in zip((q, k, v, table), torch.autograd.grad(o, (q, k, v, table), torch.ones_like(o))):
+            assert g.shape == t.shape and not g.any()
+
+
+# --- over a paged cache ---------------------------------------------------------------
+
+def check_paged(ctx, new, H, Hkv, D, dtype, ps=16, num=16, R=40, causal=True, bias=None, mq="longest", seed=0,
+                drop_page=False, layout="nhd", extra=0):
+    g, r = torch.Generator().manual_seed(seed), random.Random(seed)
+    lens = [c + n for c, n in zip(ctx, new)]
+    pages = [-(-x // ps) for x in lens]
+    pool = r.sample(range(sum(pages) + 3), sum(pages) + 3)
+    width = max(1, max(pages)) + 1
+    table = torch.full((len(ctx), width), -1, dtype=I32)
+    for b, n in enumerate(pages):
+        for j in range(n):
+            table[b, j] = pool.pop()
+    shape = (sum(pages) + 3, ps, Hkv, D)
+    if layout == "nhd":
+        kc, vc = (randn(g, *shape, dtype=dtype) for _ in range(2))
+    else:  # heads before tokens
+        kc, vc = (randn(g, shape[0], Hkv, ps, D, dtype=dtype).transpose(1, 2) for _ in range(2))
+    q = randn(g, sum(new) + extra, H, D, dtype=dtype)
+    values, buckets = randn(g, num, H, dtype=dtype, f=2.0), torch.randint(0, num, (2 * R + 1,), generator=g).to(I32).cuda()
+    gone = {}
+    if drop_page:
+        for b, n in enumerate(pages):
+            if n > 1:
+                gone[b] = n // 2
+                table[b, n // 2] = -1
+    # What no sequence holds is never read.
+    held = torch.zeros(shape[:2], dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        for j in range(pages[b]):
+            if table[b, j] >= 0:
+                held[table[b, j], : min(ps, n - j * ps)] = True
+    for c in (kc, vc):
+        c[~held] = math.nan
+    table = table.cuda()
+    mq = max(new) if mq == "longest" else mq
+    got = ts.sigmoid_attention_paged(q, kc, vc, table, ints(lens), ints(offsets(new)), mq, is_causal=causal,
+                                     sigmoid_bias=bias, bias_table=values, bias_buckets=buckets)
+    want = torch.zeros(2, *q.shape, dtype=torch.float64, device="cuda")
+    for b, (n, L, first) in enumerate(zip(new, lens, offsets(new))):
+        if n == 0 or L == 0:
+            continue
+        pos = torch.arange(L, device="cuda")
+        there = torch.ones(L, dtype=torch.bool, device="cuda")
+        if b in gone:
+            there = pos // ps != gone[b]
+        pos = pos[there]
+        rows = table[b].long()[pos // ps], pos % ps
+        d = pos[None] - (torch.arange(n, device="cuda")[:, None] + L - n)
+        for h in range(H):
+            add = line_of(values, buckets, h, d)[0] + (-math.log(L) if bias is None else bias)
+            if causal:
+                add = torch.where(d > 0, -math.inf, add)
+            at = slice(first, first + n)
+            val, err = one_head(q[at, h], kc[rows][:, h // (H // Hkv)], vc[rows][:, h // (H // Hkv)], None, add, dtype)["o"]
+            want[0][at, h], want[1][at, h] = val, err
+    assert_within(got, tuple(want), "o")
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_paged_types_and_head_dims(dtype, D, causal):
+    check_paged([100, 0, 33, 7], [1, 1, 1, 1], 8, 2, D, DT[dtype], causal=causal, seed=D)  # decoding
+    check_paged([50, 0, 100], [70, 131, 40], 4, 2, D, DT[dtype], causal=causal, seed=D)  # chunks
+    check_paged([100, 0, 33], [1, 60, 2], 8, 2, D, DT[dtype], causal=causal, seed=D)  # both
+
+
+@pytest.mark.parametrize("H, Hkv", [(1, 1), (8, 1), (6, 2), (32, 8), (16, 16), (40, 1)])
+def test_paged_heads(H, Hkv):
+    check_paged([200, 31], [1, 1], H, Hkv, 64, torch.bfloat16, seed=H)
+    check_paged([200, 31], [5, 60], H, Hkv, 64, torch.bfloat16, seed=H)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 128), ("f16", 64), ("f32", 64), ("bf16", 32)])
+@pytest.mark.parametrize("R", [0, 1, 31, 64, 500, 2048])
+def test_paged_reaches(dtype, D, R):
+    check_paged([700, 64, 1], [1, 1, 1], 8, 2, D, DT[dtype], R=R, num=9, seed=R)
+    check_paged([700, 64, 1], [200, 33, 1], 8, 2, D, DT[dtype], R=R, num=9, causal=R % 2 == 0, seed=R)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 128), ("f16", 64), ("f32", 128), ("f32", 32)])
+def test_paged_long_contexts_are_cut(dtype, D):
+    check_paged([9000], [1], 8, 2, D, DT[dtype], ps=64, R=128, seed=1)
+    check_paged([5000, 300], [1, 1], 4, 4, D, DT[dtype], ps=32, R=700, seed=2)
+    check_paged([4000], [150], 4, 2, D, DT[dtype], ps=16, R=128, seed=3)
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 128), ("f16", 64), ("f32", 64)])
+def test_paged_page_sizes_pages_that_are_gone_and_padding(dtype, D):
+    for ps in (16, 128, 1024):
+        check_paged([300, 40], [1, 3], 8, 2, D, DT[dtype], ps=ps, drop_page=True, seed=ps)
+    got = check_paged([300, 40, 5], [1, 90, 0], 8, 2, D, DT[dtype], extra=9, mq=None)
+    assert not got[-9:].any()
+    check_paged([60, 500], [4, 1], 8, 2, D, DT[dtype], layout="hnd", seed=4)
+    check_paged([60, 500], [4, 1], 8, 2, D, DT[dtype], bias=-3.0, causal=False, seed=5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_paged_rows_off_boundaries(dtype):
+    g = torch.Generator().manual_seed(3)
+    kc, vc = (randn(g, 4, 16, 2, 65, dtype=DT[dtype])[..., :64] for _ in range(2))
+    q, values = randn(g, 2, 4, 64, dtype=DT[dtype]), randn(g, 6, 4, dtype=DT[dtype])
+    buckets = torch.randint(0, 6, (21,), generator=g).to(I32).cuda()
+    table, args = ints([[2, 0], [3, 1]]), (ints([20, 31]), ints([0, 1, 2]), 1)
+    got = ts.sigmoid_attention_paged(q, kc, vc, table, *args, is_causal=True, bias_table=values, bias_buckets=buckets)
+    want = ts.sigmoid_attention_paged(q, kc.contiguous(), vc.contiguous(), table, *args, is_causal=True,
+                                      bias_table=values, bias_buckets=buckets)
+    # Both within the bounds of the definition: apart by two of them at most.
+    assert (got.float() - want.float()).abs().max() <= 4 * torch.finfo(DT[dtype]).eps * want.float().abs().max() + 1e-5
+
+
+def test_paged_captured_step_replays():
+    g = torch.Generator().manual_seed(0)
+    kc, vc = (randn(g, 40, 16, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    q, values = randn(g, 4, 8, 64, dtype=torch.bfloat16), randn(g, 16, 8, dtype=torch.bfloat16)
+    buckets = torch.randint(0, 16, (201,), generator=g).to(I32).cuda()
+    table, lens, cu = torch.arange(40, dtype=I32, device="cuda").view(4, 10), ints([100, 3, 64, 160]), ints([0, 1, 2, 3, 4])
+    step = lambda: ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 1, is_causal=True, bias_table=values,  # noqa: E731
+                                              bias_buckets=buckets)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for new in ([100, 3, 64, 160], [1, 160, 17, 33], [159, 158, 2, 90]):
+        lens.copy_(ints(new))
+        values.copy_(torch.roll(values, 1, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, step())
+
+
+def test_what_was_trained_is_served():
+    """A sequence in one training-shaped call, and token by token over a paged cache."""
+    g = torch.Generator().manual_seed(8)
+    n, H, Hkv, D, dtype = 75, 4, 2, 64, torch.float32
+    q, k, v = randn(g, n, H, D, dtype=dtype), randn(g, n, Hkv, D, dtype=dtype), randn(g, n, Hkv, D, dtype=dtype)
+    values, buckets = randn(g, 16, H, dtype=dtype), ts.relative_position_buckets(16, 40, False, device="cuda")
+    cu = ints([0, n])
+    whole = ts.sigmoid_attention_varlen(q, k, v, cu, cu, n, n, is_causal=True, sigmoid_bias=-2.0, bias_table=values,
+                                        bias_buckets=buckets)
+    want = packed_rel(q, k, v, None, values, buckets, [0, n], [0, n], True, bias=-2.0)["o"]
+    assert_within(whole, want)
+    kc, vc = (torch.zeros(8, 16, Hkv, D, dtype=dtype, device="cuda") for _ in range(2))
+    table, free = torch.full((1, 8), -1, dtype=I32, device="cuda"), torch.arange(8, dtype=I32, device="cuda").flip(0)
+    at, rows = 0, []
+    for step in (30, 1, 1, 17, 1, 25):
+        plan = ts.paged_plan(ints([at]), ints([step]), table, free, 16, step)
+        free = free[int(plan.pages_needed):].contiguous()
+        new = slice(at, at + step)
+        ts.paged_cache_write(k[new], v[new], kc, vc, plan.slot_mapping)
+        rows.append(ts.sigmoid_attention_paged(q[new], kc, vc, plan.block_table, plan.seq_lens, plan.cu_seqlens, step,
+                                               is_causal=True, sigmoid_bias=-2.0, bias_table=values,
+                                               bias_buckets=buckets))
+        at += step
+    assert_within(torch.cat(rows), want)

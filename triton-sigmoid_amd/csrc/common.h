@@ -82,7 +82,7 @@ struct GapAxis {
 // Padded outputs write zeros to the invalid rows of each batch; packed
 // outputs write exactly the rows of each sequence and nothing else.
 struct KParams {
-  static constexpr bool kPaged = false;
+  static constexpr bool kPaged = false, kRel = false;
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;
   const float *bias;       // [B]

@@ -8,6 +8,7 @@
 // (key <= query, top-left) and seq_lens bounds, padded rows are written as 0.
 #include "common.h"
 #include "launch.h"
+#include "rel.h"
 
 namespace sigattn {
 
@@ -26,11 +27,11 @@ __device__ __forceinline__ float sigmoid_of(float s, float scale, float c) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
-constexpr int GB = 64;  // rows per block (one per thread)
+constexpr int GB = kGenericRows;  // rows per block (one per thread)
 constexpr int GT = 32;  // tile length along the walked sequence
 
-template <typename T, int D, bool CAUSAL>
-__global__ __launch_bounds__(GB) void fwd_generic_kernel(const KParams p) {
+template <typename T, int D, bool CAUSAL, class P>
+__global__ __launch_bounds__(GB) void fwd_generic_kernel(const P p) {
   __shared__ float sK[GT][D + 1];
   __shared__ float sV[GT][D + 1];
   __shared__ float sC[GT];
@@ -71,7 +72,9 @@ __global__ __launch_bounds__(GB) void fwd_generic_kernel(const KParams p) {
       float s = 0.0f;
 #pragma unroll
       for (int d = 0; d < D; ++d) s = __builtin_fmaf(qv[d], sK[j][d], s);
-      float pr = sigmoid_of(s, scale, bias + sC[j]);
+      float c = bias + sC[j];
+      if constexpr (P::kRel) c = bias + rel_at(p, h, key - q);
+      float pr = sigmoid_of(s, scale, c);
       if (CAUSAL && key > q) pr = 0.0f;
       pr = round_to<T>(pr);
 #pragma unroll
@@ -85,8 +88,8 @@ __global__ __launch_bounds__(GB) void fwd_generic_kernel(const KParams p) {
   }
 }
 
-template <typename T, int D, bool CAUSAL>
-__global__ __launch_bounds__(GB) void dq_generic_kernel(const KParams p) {
+template <typename T, int D, bool CAUSAL, class P>
+__global__ __launch_bounds__(GB) void dq_generic_kernel(const P p) {
   __shared__ float sK[GT][D + 1];
   __shared__ float sV[GT][D + 1];
   __shared__ float sC[GT];
@@ -98,6 +101,12 @@ __global__ __launch_bounds__(GB) void dq_generic_kernel(const KParams p) {
   const int64_t qbase = p.q_base(b, h);
   const int64_t kbase = p.k_base(b, h);
   const float scale = *p.scale, bias = p.bias[b];
+  extern __shared__ float line[];  // P::kRel: sums of dS by relative position
+  [[maybe_unused]] float far[2] = {0.0f, 0.0f};
+  if constexpr (P::kRel) {
+    for (int i = threadIdx.x; i < p.places(); i += GB) line[i] = 0.0f;
+    __syncthreads();
+  }
 
   float qv[D], dov[D], acc[D];
   const bool qok = q < Lq;
@@ -131,10 +140,22 @@ __global__ __launch_bounds__(GB) void dq_generic_kernel(const KParams p) {
         s = __builtin_fmaf(qv[d], sK[j][d], s);
         dp = __builtin_fmaf(dov[d], sV[j][d], dp);
       }
-      const float pr = sigmoid_of(s, scale, bias + sC[j]);
+      float c = bias + sC[j];
+      if constexpr (P::kRel) c = bias + rel_at(p, h, key - q);
+      const float pr = sigmoid_of(s, scale, c);
       const float t = pr * dp;
       float ds = __builtin_fmaf(-pr, t, t);
       if (CAUSAL && key > q) ds = 0.0f;
+      if constexpr (P::kRel) {
+        // Of the relative positions within reach no two lanes have one alike; the
+        // sums of those at its ends and beyond stay with the lane.
+        const int d = key - q;
+        const float x = qok ? ds : 0.0f;
+        if (d <= -p.reach) far[0] += x;
+        else if (d >= p.reach) far[1] += x;
+        else line[p.reach + d] += x;
+        __syncthreads();
+      }
       ds = round_to<T>(ds);
 #pragma unroll
       for (int d = 0; d < D; ++d) acc[d] = __builtin_fmaf(ds, sK[j][d], acc[d]);
@@ -146,10 +167,25 @@ __global__ __launch_bounds__(GB) void dq_generic_kernel(const KParams p) {
     for (int d = 0; d < D; ++d)
       st<T>(p.dq, qbase + (int64_t)q * p.sq_t + d, qok ? acc[d] * scale : 0.0f);
   }
+  if constexpr (P::kRel) {
+    if (p.part == nullptr || qb * GB >= Lq) return;  // (no such block: not read either)
+    __shared__ float ends[2][GB];
+    ends[0][threadIdx.x] = far[0], ends[1][threadIdx.x] = far[1];
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e == 0 || (e == 1 && p.reach > 0)) {
+      float sum = 0.0f;
+      for (int i = 0; i < GB; ++i) sum += ends[e][i] + (p.reach == 0 ? ends[1][i] : 0.0f);
+      line[2 * p.reach * e] = sum;
+    }
+    __syncthreads();
+    float *row = p.part_row(b, qb, h);
+    for (int i = threadIdx.x; i < p.places(); i += GB) row[i] = line[i];
+  }
 }
 
-template <typename T, int D, bool CAUSAL>
-__global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
+template <typename T, int D, bool CAUSAL, class P>
+__global__ __launch_bounds__(GB) void dkdv_generic_kernel(const P p) {
   __shared__ float sQ[GT][D + 1];
   __shared__ float sO[GT][D + 1];
   const int BH = p.B * p.H;
@@ -173,7 +209,8 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
   const int mstart = CAUSAL ? (kb * GB) / GT * GT : 0;
   const int mend = (kb * GB >= Lk) ? 0 : Lq;
   for (int g = 0; g < p.q_heads(); ++g) {  // the query heads of this K / V head
-    const int64_t qbase = p.q_base(b, p.first_q_head(h) + g);
+    const int hq = p.first_q_head(h) + g;
+    const int64_t qbase = p.q_base(b, hq);
     for (int m0 = mstart; m0 < mend; m0 += GT) {
       for (int e = threadIdx.x; e < GT * D; e += GB) {
         const int r = e / D, d = e % D, q = m0 + r;
@@ -191,7 +228,7 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
           s = __builtin_fmaf(sQ[j][d], kv[d], s);
           dp = __builtin_fmaf(sO[j][d], vv[d], dp);
         }
-        float pr = sigmoid_of(s, scale, c);
+        float pr = sigmoid_of(s, scale, P::kRel ? bias + rel_at(p, hq, key - q) : c);
         const float t = pr * dp;
         float ds = __builtin_fmaf(-pr, t, t);
         if (CAUSAL && key > q) { pr = 0.0f; ds = 0.0f; }
@@ -217,17 +254,22 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
 
 // ---- launchers ---------------------------------------------------------------
 
-#define SIGATTN_GENERIC_LAUNCHER(NAME, KERNEL, ROWS)                                   \
+template <class P, class F> static void generic_grid(const P &kp, int rows, F &&launch) {
+  P p = kp;
+  p.nblk = (rows + GB - 1) / GB;
+  launch(p, dim3((unsigned)(p.nblk * p.B * p.H)));
+}
+
+#define SIGATTN_GENERIC_LAUNCHER(NAME, KERNEL, ROWS, P, LDS)                           \
   template <typename T, int D>                                                         \
-  static void NAME##_t(const KParams &kp, bool causal, hipStream_t s) {                \
-    KParams p = kp;                                                                    \
-    p.nblk = ((ROWS) + GB - 1) / GB;                                                   \
-    const dim3 grid((unsigned)(p.nblk * p.B * p.H));                                   \
-    if (causal) KERNEL<T, D, true><<<grid, dim3(GB), 0, s>>>(p);                       \
-    else KERNEL<T, D, false><<<grid, dim3(GB), 0, s>>>(p);                             \
+  static void NAME##_t(const P &kp, bool causal, hipStream_t s) {                      \
+    generic_grid(kp, kp.ROWS, [&](const P &p, dim3 grid) {                             \
+      if (causal) KERNEL<T, D, true, P><<<grid, dim3(GB), LDS, s>>>(p);                \
+      else KERNEL<T, D, false, P><<<grid, dim3(GB), LDS, s>>>(p);                      \
+    });                                                                                \
   }                                                                                    \
   template <typename T>                                                                \
-  static void NAME##_d(const KParams &p, int D, bool causal, hipStream_t s) {          \
+  static void NAME##_d(const P &p, int D, bool causal, hipStream_t s) {                \
     switch (D) {                                                                       \
       case 16: NAME##_t<T, 16>(p, causal, s); break;                                   \
       case 32: NAME##_t<T, 32>(p, causal, s); break;                                   \
@@ -235,15 +277,18 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const KParams p) {
       default: NAME##_t<T, 128>(p, causal, s); break;                                  \
     }                                                                                  \
   }                                                                                    \
-  void NAME(const KParams &p, int dtype, int D, bool causal, hipStream_t s) {          \
+  void NAME(const P &p, int dtype, int D, bool causal, hipStream_t s) {                \
     if (dtype == kF32) NAME##_d<float>(p, D, causal, s);                               \
     else if (dtype == kBF16) NAME##_d<__bf16>(p, D, causal, s);                        \
     else NAME##_d<_Float16>(p, D, causal, s);                                          \
   }
 
-SIGATTN_GENERIC_LAUNCHER(launch_fwd_generic, fwd_generic_kernel, p.Tq)
-SIGATTN_GENERIC_LAUNCHER(launch_bwd_dq_generic, dq_generic_kernel, p.Tq)
-SIGATTN_GENERIC_LAUNCHER(launch_bwd_dkdv_generic, dkdv_generic_kernel, p.Tk)
+SIGATTN_GENERIC_LAUNCHER(launch_fwd_generic, fwd_generic_kernel, Tq, KParams, 0)
+SIGATTN_GENERIC_LAUNCHER(launch_bwd_dq_generic, dq_generic_kernel, Tq, KParams, 0)
+SIGATTN_GENERIC_LAUNCHER(launch_bwd_dkdv_generic, dkdv_generic_kernel, Tk, KParams, 0)
+SIGATTN_GENERIC_LAUNCHER(launch_rel_fwd_generic, fwd_generic_kernel, Tq, RelParams, 0)
+SIGATTN_GENERIC_LAUNCHER(launch_rel_dq_generic, dq_generic_kernel, Tq, RelParams, p.places() * sizeof(float))
+SIGATTN_GENERIC_LAUNCHER(launch_rel_dkdv_generic, dkdv_generic_kernel, Tk, RelParams, 0)
 
 #undef SIGATTN_GENERIC_LAUNCHER
 

@@ -8,6 +8,7 @@
 #include "../../include/sigattn.h"
 #include "launch.h"
 #include "paged.h"
+#include "rel.h"
 
 namespace sigattn {
 namespace {
@@ -163,8 +164,8 @@ template <typename T> __device__ __forceinline__ void st_elem(void *base, int64_
 // thread walks a row of its own): 4 sequences of 2000 keys H=32 Hkv=8 D=128, 1 /
 // 16 tokens each, bf16 342 / 631 us, fp32 327 / 547, where aligned rows (the matrix
 // kernels) take 16 / 30 and 24 / 53.
-template <typename T, int D, bool CAUSAL>
-__global__ __launch_bounds__(256) void paged_generic_kernel(const PagedParams p) {
+template <typename T, int D, bool CAUSAL, class P>
+__global__ __launch_bounds__(256) void paged_generic_kernel(const P p) {
   constexpr int PARTS = 256 / D;
   __shared__ float sq[D], sp[256], red[256];
   __shared__ int64_t srow[256];  // element offset of each key's row; -1: no key there
@@ -200,7 +201,8 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(const PagedParams p)
         float s = 0.0f;
 #pragma unroll 8
         for (int d = 0; d < D; ++d) s = __builtin_fmaf(sq[d], ld_elem<T>(p.k, row + d), s);
-        const float c = bias + (p.score_mod ? p.score_mod[b * p.mod_stride + key] : 0.0f);
+        float c = bias + (p.score_mod ? p.score_mod[b * p.mod_stride + key] : 0.0f);
+        if constexpr (P::kRel) c = bias + rel_at(p, h, key - (Lk - Lq + (int)(r - first)));
         pr = round_to<T>(sigmoid_from_neg_log2(-__builtin_fmaf(s, p.fscale, c) * kLog2e));
       }
     }
@@ -222,18 +224,23 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(const PagedParams p)
   }
 }
 
-template <typename T, int D> void generic_t(const PagedParams &p, bool causal, hipStream_t st) {
+template <typename T, int D, class P> void generic_t(const P &p, bool causal, hipStream_t st) {
   const dim3 grid((unsigned)p.rows_q, (unsigned)p.H);
-  if (causal) paged_generic_kernel<T, D, true><<<grid, 256, 0, st>>>(p);
-  else paged_generic_kernel<T, D, false><<<grid, 256, 0, st>>>(p);
+  if (causal) paged_generic_kernel<T, D, true, P><<<grid, 256, 0, st>>>(p);
+  else paged_generic_kernel<T, D, false, P><<<grid, 256, 0, st>>>(p);
 }
-template <typename T> void generic_d(const PagedParams &p, int D, bool causal, hipStream_t st) {
+template <typename T, class P> void generic_d(const P &p, int D, bool causal, hipStream_t st) {
   switch (D) {
     case 16: return generic_t<T, 16>(p, causal, st);
     case 32: return generic_t<T, 32>(p, causal, st);
     case 64: return generic_t<T, 64>(p, causal, st);
     default: return generic_t<T, 128>(p, causal, st);
   }
+}
+template <class P> void generic(const P &p, int dtype, int D, bool causal, hipStream_t st) {
+  if (dtype == kF32) generic_d<float>(p, D, causal, st);
+  else if (dtype == kBF16) generic_d<__bf16>(p, D, causal, st);
+  else generic_d<_Float16>(p, D, causal, st);
 }
 
 int log2_of(int64_t x) { return 63 - __builtin_clzll((unsigned long long)x); }
@@ -245,9 +252,10 @@ bool page_size_ok(int64_t ps) { return ps >= 16 && ps <= (1 << 20) && (ps & (ps 
 }  // namespace
 
 void launch_paged_generic(const PagedParams &p, int dtype, int D, bool causal, hipStream_t st) {
-  if (dtype == kF32) generic_d<float>(p, D, causal, st);
-  else if (dtype == kBF16) generic_d<__bf16>(p, D, causal, st);
-  else generic_d<_Float16>(p, D, causal, st);
+  generic(p, dtype, D, causal, st);
+}
+void launch_paged_rel_generic(const PagedRelParams &p, int dtype, int D, bool causal, hipStream_t st) {
+  generic(p, dtype, D, causal, st);
 }
 
 }  // namespace sigattn

@@ -8,6 +8,7 @@
 #include "../../include/sigattn.h"
 #include "launch.h"
 #include "paged.h"
+#include "rel.h"
 
 using sigattn::kDecodeCols;
 using sigattn::PagedParams;
@@ -158,6 +159,12 @@ PagedParams of_part(const PagedParams &k, const Part &part, int lo, int hi, int2
   return s;
 }
 
+// The learned bias's table as far as the cache's sequences reach.
+sigattn::RelTable rel_table_of(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  return sigattn::rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q,
+                            p->max_pages * p->page_size);
+}
+
 int launch_status() { return hipGetLastError() == hipSuccess ? SIGATTN_OK : SIGATTN_ERR_LAUNCH; }
 
 }  // namespace
@@ -245,6 +252,40 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
   else if (dt == SIGATTN_F32) sigattn::launch_paged_f32(first, (int)pl.fwd.units, D, causal, st);
   else sigattn::launch_paged_fwd(first, (int)pl.fwd.units, dt, D, causal, st);
   if (kf.split_units > 0 || kd.split_units > 0) sigattn::launch_paged_reduce(kf, kd, dt, D, st);
+  return launch_status();
+}
+
+int sigattn_paged_rel_check(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  const int rc = sigattn_paged_check(p);
+  if (rc != SIGATTN_OK) return rc;
+  if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
+  if (r->dtype != SIGATTN_F16 && r->dtype != SIGATTN_BF16 && r->dtype != SIGATTN_F32) return SIGATTN_ERR_DTYPE;
+  if (!sigattn::rel_table_ok(r) || p->score_mod != nullptr) return SIGATTN_ERR_REL_BIAS;
+  if (p->H > 0 && (r->table == nullptr || r->buckets == nullptr)) return SIGATTN_ERR_NULL_ARG;
+  return SIGATTN_OK;
+}
+
+size_t sigattn_paged_rel_fwd_workspace_bytes(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  if (sigattn_paged_rel_check(p, r) != SIGATTN_OK || p->rows_q == 0 || p->H == 0 || p->B == 0) return 0;
+  return (size_t)sigattn::rel_line_bytes(rel_table_of(p, r));
+}
+
+int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
+                          size_t workspace_bytes, void *stream) {
+  const int rc = sigattn_paged_rel_check(p, r);
+  if (rc != SIGATTN_OK) return rc;
+  if (p->rows_q == 0 || p->H == 0 || p->B == 0) return sigattn_paged_fwd(p, out, nullptr, 0, stream);
+  if (out == nullptr) return SIGATTN_ERR_NULL_ARG;
+  const sigattn::RelTable t = rel_table_of(p, r);
+  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < sigattn::rel_line_bytes(t))
+    return SIGATTN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  sigattn::PagedRelParams k{};
+  (PagedParams &)k = make_params(p, out);
+  k.line = (const float *)workspace, k.reach = t.reach;
+  (void)hipGetLastError();
+  sigattn::launch_rel_line(t, (float *)workspace, st);
+  sigattn::launch_paged_rel_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
   return launch_status();
 }
 

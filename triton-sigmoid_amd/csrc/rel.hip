@@ -1,0 +1,116 @@
+// The learned bias by relative position outside the attention kernels: a line of
+// values per head from the table, and the table's gradient from their sums.
+#include "launch.h"
+#include "rel.h"
+
+namespace sigattn {
+namespace {
+
+__device__ __forceinline__ int bucket_of(const RelTable &t, int place) {
+  return t.bucket[t.max_distance + place - t.reach];
+}
+// (Buckets outside the table add nothing and get nothing.)
+__device__ __forceinline__ bool inside(const RelTable &t, int u) { return u >= 0 && u < t.buckets; }
+
+// One thread per place.  A few KB: bound by its launch.
+template <typename T> __global__ __launch_bounds__(256) void rel_line_kernel(const RelTable t, float *line) {
+  const int place = blockIdx.x * 256 + threadIdx.x, places = 2 * t.reach + 1, h = blockIdx.y;
+  if (place >= places) return;
+  const int u = bucket_of(t, place);
+  float x = 0.0f;
+  if (inside(t, u)) {
+    const int64_t at = (int64_t)u * t.H + h;
+    if constexpr (sizeof(T) == 4) x = ((const float *)t.table)[at];
+    else x = Elem<T>::to_f32(((const uint16_t *)t.table)[at]);
+  }
+  line[(int64_t)h * places + place] = x;
+}
+
+// sums[h][place] of all query blocks: 64 places a workgroup, 16 shares of the
+// slots (in turn), added in their order.  Which slots hold a block is found for
+// 1024 of them at a time, a thread each.
+constexpr int kShares = 16;
+__global__ __launch_bounds__(64 * kShares) void rel_sums_kernel(const RelParams p, float *sums) {
+  __shared__ float got[kShares][64];
+  __shared__ bool held[64 * kShares];
+  const int h = blockIdx.y, lane = threadIdx.x & 63, share = threadIdx.x >> 6, places = p.places();
+  const int place = blockIdx.x * 64 + lane;
+  const int64_t slots = p.part != nullptr ? p.part_slots() : 0;
+  float x = 0.0f;
+  for (int64_t s0 = 0; s0 < slots; s0 += 64 * kShares) {
+    const int64_t mine = s0 + threadIdx.x;
+    int lo = 0, hi = p.B - 1;  // the last batch that begins at or before the slot
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (p.first_slot(mid) <= mine) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t blk = mine - p.first_slot(lo);
+    __syncthreads();
+    held[threadIdx.x] = blk >= 0 && blk * p.part_rows < p.len_q(lo);
+    __syncthreads();
+    const int n = (int)(slots - s0 < 64 * kShares ? slots - s0 : 64 * kShares);
+    if (place < places)
+#pragma unroll 4
+      for (int i = share; i < n; i += kShares)
+        if (held[i]) x += p.part[((s0 + i) * p.H + h) * places + place];
+  }
+  got[share][lane] = x;
+  __syncthreads();
+  if (share != 0 || place >= places) return;
+#pragma unroll
+  for (int s = 1; s < kShares; ++s) x += got[s][lane];
+  sums[(int64_t)h * places + place] = x;
+}
+
+// grad[u][h] = the sum over the places of bucket u, in their order.  A workgroup per
+// head; `shares` threads a bucket, each a run of places, added in order.
+template <typename T> __global__ __launch_bounds__(256) void rel_grad_kernel(const RelTable t, const float *sums, T *grad) {
+  __shared__ float got[256];
+  const int h = blockIdx.x, places = 2 * t.reach + 1, per = min(t.buckets, 256), shares = 256 / per;
+  const int share = threadIdx.x / per, run = (places + shares - 1) / shares;
+  const float *row = sums + (int64_t)h * places;
+  for (int u0 = 0; u0 < t.buckets; u0 += per) {
+    const int u = u0 + (int)threadIdx.x - share * per;
+    float x = 0.0f;
+    if (share < shares && u < t.buckets)
+      for (int i = share * run; i < min(places, (share + 1) * run); ++i)
+        if (bucket_of(t, i) == u) x += row[i];
+    got[threadIdx.x] = x;
+    __syncthreads();
+    if (share == 0 && u < t.buckets) {
+      for (int s = 1; s < shares; ++s) x += got[s * per + threadIdx.x];
+      if constexpr (sizeof(T) == 4) grad[(int64_t)u * t.H + h] = x;
+      else ((uint16_t *)grad)[(int64_t)u * t.H + h] = Elem<T>::from_f32(x);
+    }
+    __syncthreads();
+  }
+}
+
+template <class F> void by_type(int dtype, F &&f) {
+  if (dtype == kF32) f((float *)nullptr);
+  else if (dtype == kBF16) f((__bf16 *)nullptr);
+  else f((_Float16 *)nullptr);
+}
+
+}  // namespace
+
+void launch_rel_line(const RelTable &t, float *line, hipStream_t st) {
+  if (t.H == 0) return;
+  const dim3 grid((unsigned)((2 * t.reach + 1 + 255) / 256), (unsigned)t.H);
+  by_type(t.dtype, [&](auto *x) {
+    rel_line_kernel<std::remove_pointer_t<decltype(x)>><<<grid, dim3(256), 0, st>>>(t, line);
+  });
+}
+
+void launch_rel_grad(const RelTable &t, const RelParams &p, float *sums, void *grad, hipStream_t st) {
+  if (t.H == 0 || t.buckets == 0) return;
+  const dim3 grid((unsigned)((p.places() + 63) / 64), (unsigned)t.H);
+  rel_sums_kernel<<<grid, dim3(64 * kShares), 0, st>>>(p, sums);
+  by_type(t.dtype, [&](auto *x) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    rel_grad_kernel<T><<<dim3((unsigned)t.H), dim3(256), 0, st>>>(t, sums, (T *)grad);
+  });
+}
+
+}  // namespace sigattn

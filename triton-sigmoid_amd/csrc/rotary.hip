@@ -1,0 +1,140 @@
+// Rotary embedding: pairs of a head's columns turned by the angles of the row's
+// position, for queries and keys (and their gradients, by the negative angles), or
+// with the keys and values going straight to their slots of a paged cache.
+#include <hip/hip_runtime.h>
+
+#include "../../include/sigattn.h"
+#include "launch.h"
+
+namespace sigattn {
+namespace {
+
+struct RotaryArgs {
+  const char *src[3];  // q, k, v (v: only copied; nullptr without a cache)
+  char *out[3];        // q_out; k_out, or the caches
+  const int32_t *positions, *slots;
+  const float *angles;
+  int64_t src_t[3], src_h[3], dst_p, dst_t, dst_h, out_t[2];  // bytes
+  int64_t rows, num_slots;
+  int heads[3], D, rot, num_positions, lp;
+  float sign;
+};
+
+template <typename T> __device__ __forceinline__ float rot_ld(const char *row, int i) {
+  if constexpr (sizeof(T) == 4) return ((const float *)row)[i];
+  else return Elem<T>::to_f32(((const uint16_t *)row)[i]);
+}
+template <typename T> __device__ __forceinline__ void rot_st(char *row, int i, float x) {
+  if constexpr (sizeof(T) == 4) ((float *)row)[i] = x;
+  else ((uint16_t *)row)[i] = Elem<T>::from_f32(x);
+}
+
+// A workgroup per row, a thread per pair (or two copied columns).
+template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+  const int64_t t = blockIdx.x;
+  const int half = a.rot / 2, dh = a.D / 2;
+  const int pos = min(max(a.positions[t], 0), a.num_positions - 1);
+  const float *row = a.angles + (int64_t)pos * a.rot;
+  const int32_t slot = a.slots != nullptr ? a.slots[t] : 0;
+  const bool there = a.slots == nullptr || (slot >= 0 && slot < a.num_slots);
+  const int all = (a.heads[0] + a.heads[1] + a.heads[2]) * dh;
+  for (int i = threadIdx.x; i < all; i += 256) {
+    int h = i / dh;
+    const int c = i - h * dh;
+    const int which = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
+    h -= which > 0 ? a.heads[0] : 0;
+    h -= which > 1 ? a.heads[1] : 0;
+    const char *src = a.src[which] + t * a.src_t[which] + h * a.src_h[which];
+    char *dst;
+    if (which == 0 || a.slots == nullptr) {
+      dst = a.out[which] + t * a.out_t[which] + (int64_t)h * a.D * sizeof(T);
+    } else {
+      if (!there) continue;
+      dst = a.out[which] + (int64_t)(slot >> a.lp) * a.dst_p + (slot & ((1 << a.lp) - 1)) * a.dst_t + h * a.dst_h;
+    }
+    const bool turn = which < 2 && c < half;
+    const int x = turn ? (PAIRS ? 2 * c : c) : (which < 2 ? a.rot + 2 * (c - half) : 2 * c);
+    const int y = turn && !PAIRS ? c + half : x + 1;
+    float u = rot_ld<T>(src, x), w = rot_ld<T>(src, y);
+    if (turn) {
+      const float cs = row[c], sn = row[c + half] * a.sign, v = u;
+      u = v * cs - w * sn, w = w * cs + v * sn;
+    }
+    rot_st<T>(dst, x, u), rot_st<T>(dst, y, w);
+  }
+}
+
+template <typename T> void rotary_t(const RotaryArgs &a, bool pairs, hipStream_t st) {
+  if (pairs) rotary_kernel<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
+  else rotary_kernel<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
+}
+
+int rotary_run(const sigattn_rotary *r, bool cache, hipStream_t st) {
+  RotaryArgs a{};
+  const int64_t es = r->dtype == SIGATTN_F32 ? 4 : 2;
+  a.src[0] = (const char *)r->q, a.src[1] = (const char *)r->k, a.src[2] = cache ? (const char *)r->v : nullptr;
+  a.out[0] = (char *)r->q_out, a.out[1] = (char *)(cache ? r->k_cache : r->k_out);
+  a.out[2] = cache ? (char *)r->v_cache : nullptr;
+  a.positions = r->positions, a.slots = cache ? r->slot_mapping : nullptr, a.angles = r->angles;
+  a.src_t[0] = r->q_stride_t * es, a.src_h[0] = r->q_stride_h * es;
+  for (int i = 1; i < 3; ++i) a.src_t[i] = r->k_stride_t * es, a.src_h[i] = r->k_stride_h * es;
+  a.dst_p = r->cache_stride_p * es, a.dst_t = r->cache_stride_t * es, a.dst_h = r->cache_stride_h * es;
+  a.out_t[0] = r->q_heads * r->D * es, a.out_t[1] = r->kv_heads * r->D * es;
+  a.rows = r->rows, a.num_slots = r->num_pages * r->page_size;
+  a.heads[0] = (int)r->q_heads, a.heads[1] = (int)r->kv_heads, a.heads[2] = cache ? (int)r->kv_heads : 0;
+  a.D = (int)r->D, a.rot = (int)r->rot_dim, a.num_positions = (int)r->num_positions;
+  a.lp = cache ? 63 - __builtin_clzll((unsigned long long)r->page_size) : 0;
+  a.sign = r->inverse != 0 ? -1.0f : 1.0f;
+  (void)hipGetLastError();
+  const bool pairs = r->interleaved != 0;
+  if (r->dtype == SIGATTN_F32) rotary_t<float>(a, pairs, st);
+  else if (r->dtype == SIGATTN_BF16) rotary_t<__bf16>(a, pairs, st);
+  else rotary_t<_Float16>(a, pairs, st);
+  return hipGetLastError() == hipSuccess ? SIGATTN_OK : SIGATTN_ERR_LAUNCH;
+}
+
+int rotary_check(const sigattn_rotary *r) {
+  if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
+  if (r->dtype != SIGATTN_F16 && r->dtype != SIGATTN_BF16 && r->dtype != SIGATTN_F32) return SIGATTN_ERR_DTYPE;
+  if (r->D != 16 && r->D != 32 && r->D != 64 && r->D != 128) return SIGATTN_ERR_HEAD_DIM;
+  // (A row's heads times columns fit 31 bits.)
+  if (r->rows < 0 || r->rows > INT32_MAX / 2 || r->q_heads < 0 || r->kv_heads < 0 || r->q_heads > 65535 ||
+      r->kv_heads > 65535 || r->num_positions > INT32_MAX)
+    return SIGATTN_ERR_SHAPE;
+  if (r->rot_dim < 2 || r->rot_dim > r->D || r->rot_dim % 2 != 0 || r->num_positions < 1) return SIGATTN_ERR_ROTARY;
+  const int64_t strides[4] = {r->q_stride_t, r->q_stride_h, r->k_stride_t, r->k_stride_h};
+  for (int64_t s : strides)
+    if (s < 0) return SIGATTN_ERR_STRIDE;
+  return SIGATTN_OK;
+}
+
+}  // namespace
+}  // namespace sigattn
+
+extern "C" int sigattn_rotary_apply(const sigattn_rotary *r, void *stream) {
+  const int rc = sigattn::rotary_check(r);
+  if (rc != SIGATTN_OK) return rc;
+  if (r->rows == 0 || r->q_heads + r->kv_heads == 0) return SIGATTN_OK;
+  if (r->positions == nullptr || r->angles == nullptr || (r->q_heads > 0 && (r->q == nullptr || r->q_out == nullptr)) ||
+      (r->kv_heads > 0 && (r->k == nullptr || r->k_out == nullptr)))
+    return SIGATTN_ERR_NULL_ARG;
+  return sigattn::rotary_run(r, false, (hipStream_t)stream);
+}
+
+extern "C" int sigattn_paged_write_rotary(const sigattn_rotary *r, void *stream) {
+  const int rc = sigattn::rotary_check(r);
+  if (rc != SIGATTN_OK) return rc;
+  if (r->num_pages < 0 || r->page_size < 16 || r->page_size > (1 << 20) || (r->page_size & (r->page_size - 1)) != 0 ||
+      r->num_pages > INT32_MAX / r->page_size)
+    return SIGATTN_ERR_SHAPE;
+  const int64_t strides[3] = {r->cache_stride_p, r->cache_stride_t, r->cache_stride_h};
+  for (int64_t s : strides)
+    if (s < 0) return SIGATTN_ERR_STRIDE;
+  if (r->rows == 0 || r->q_heads + r->kv_heads == 0) return SIGATTN_OK;
+  if (r->positions == nullptr || r->angles == nullptr || r->slot_mapping == nullptr ||
+      (r->q_heads > 0 && (r->q == nullptr || r->q_out == nullptr)) ||
+      (r->kv_heads > 0 && (r->k == nullptr || r->v == nullptr ||
+                           (r->num_pages > 0 && (r->k_cache == nullptr || r->v_cache == nullptr)))))
+    return SIGATTN_ERR_NULL_ARG;
+  return sigattn::rotary_run(r, true, (hipStream_t)stream);
+}

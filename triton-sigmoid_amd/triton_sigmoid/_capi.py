@@ -123,6 +123,58 @@ class SigattnPagedProblem(ctypes.Structure):
     ]
 
 
+class SigattnRelBias(ctypes.Structure):
+    """Mirror of `struct sigattn_rel_bias` (include/sigattn.h)."""
+
+    _fields_ = [
+        ("dtype", _c_i32),
+        ("num_buckets", _c_i32),
+        ("max_distance", _c_i64),
+        ("table", _c_vp),
+        ("buckets", _c_vp),
+    ]
+
+
+class SigattnRotary(ctypes.Structure):
+    """Mirror of `struct sigattn_rotary` (include/sigattn.h)."""
+
+    _fields_ = [
+        ("dtype", _c_i32),
+        ("interleaved", _c_i32),
+        ("inverse", _c_i32),
+        ("reserved", _c_i32),
+        ("rows", _c_i64),
+        ("q_heads", _c_i64),
+        ("kv_heads", _c_i64),
+        ("D", _c_i64),
+        ("rot_dim", _c_i64),
+        ("num_positions", _c_i64),
+        ("q_stride_t", _c_i64),
+        ("q_stride_h", _c_i64),
+        ("k_stride_t", _c_i64),
+        ("k_stride_h", _c_i64),
+        ("cache_stride_p", _c_i64),
+        ("cache_stride_t", _c_i64),
+        ("cache_stride_h", _c_i64),
+        ("num_pages", _c_i64),
+        ("page_size", _c_i64),
+        ("q", _c_vp),
+        ("k", _c_vp),
+        ("v", _c_vp),
+        ("q_out", _c_vp),
+        ("k_out", _c_vp),
+        ("k_cache", _c_vp),
+        ("v_cache", _c_vp),
+        ("positions", _c_vp),
+        ("angles", _c_vp),
+        ("slot_mapping", _c_vp),
+    ]
+
+
+# Farthest relative position and most buckets of the learned bias
+# (SIGATTN_REL_MAX_DISTANCE, SIGATTN_REL_MAX_BUCKETS).
+REL_MAX_DISTANCE, REL_MAX_BUCKETS = 2048, 65536
+
 # Largest batch of sigattn_paged_plan (SIGATTN_PLAN_MAX_BATCH).
 PLAN_MAX_BATCH = 8192
 
@@ -156,6 +208,22 @@ SIGNATURES = {
     "sigattn_paged_check": ([ctypes.POINTER(SigattnPagedProblem)], _c_i32),
     "sigattn_paged_fwd_workspace_bytes": ([ctypes.POINTER(SigattnPagedProblem)], ctypes.c_size_t),
     "sigattn_paged_fwd": ([ctypes.POINTER(SigattnPagedProblem), _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
+    "sigattn_rel_check": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)], _c_i32),
+    "sigattn_rel_fwd_workspace_bytes": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)],
+                                        ctypes.c_size_t),
+    "sigattn_rel_fwd": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias), _c_vp, _c_vp, ctypes.c_size_t,
+                         _c_vp], _c_i32),
+    "sigattn_rel_bwd_workspace_bytes": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)],
+                                        ctypes.c_size_t),
+    "sigattn_rel_bwd": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias), _c_vp, _c_vp, _c_vp, _c_vp,
+                         _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
+    "sigattn_paged_rel_check": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias)], _c_i32),
+    "sigattn_paged_rel_fwd_workspace_bytes": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias)],
+                                              ctypes.c_size_t),
+    "sigattn_paged_rel_fwd": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias), _c_vp, _c_vp,
+                               ctypes.c_size_t, _c_vp], _c_i32),
+    "sigattn_rotary_apply": ([ctypes.POINTER(SigattnRotary), _c_vp], _c_i32),
+    "sigattn_paged_write_rotary": ([ctypes.POINTER(SigattnRotary), _c_vp], _c_i32),
 }
 
 _lib = None
@@ -605,6 +673,96 @@ def backward_packed(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_s
                   packed=_packed_dims(Q, K, cu_q, cu_k, max_seqlen_q, max_seqlen_k))
     _launch_bwd(lib, pr, dO, dQ, dK, dV)
     return dQ, dK, dV
+
+
+def check_rel(table: Optional[torch.Tensor], buckets: Optional[torch.Tensor], H: int,
+              score_mod: Optional[torch.Tensor]):
+    """(table, buckets) of the learned bias by relative position, or None where it
+    is not given; ValueError or RuntimeError for what the kernels do not take."""
+    if table is None and buckets is None:
+        return None
+    if table is None or buckets is None:
+        raise ValueError("bias_table and bias_buckets go together")
+    if score_mod is not None:
+        raise ValueError("bias_table and score_mod exclude each other")
+    if table.dim() != 2 or table.shape[1] != H or not 1 <= table.shape[0] <= REL_MAX_BUCKETS:
+        raise ValueError(f"bias_table must have shape (num_buckets, {H}), 1 to {REL_MAX_BUCKETS} buckets, got "
+                         f"{tuple(table.shape)}")
+    if buckets.dim() != 1 or buckets.numel() % 2 == 0 or buckets.numel() > 2 * REL_MAX_DISTANCE + 1:
+        raise ValueError(f"bias_buckets must have shape (2 R + 1,) with R up to {REL_MAX_DISTANCE}, got "
+                         f"{tuple(buckets.shape)}")
+    if buckets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"bias_buckets must be int32 or int64, got {buckets.dtype}")
+    if table.dtype not in _DTYPE_CODE:
+        raise RuntimeError(f"unsupported bias_table dtype {table.dtype}; expected float16, bfloat16 or float32")
+    return table, buckets
+
+
+def rel_bias(table: torch.Tensor, buckets: torch.Tensor, dev: torch.device):
+    """(struct sigattn_rel_bias, and the tensors that it points at)."""
+    for name, t in (("bias_table", table), ("bias_buckets", buckets)):
+        if t.device != dev:
+            raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+    table = table.contiguous()
+    if buckets.dtype == torch.int64:
+        buckets = buckets.clamp(-1, REL_MAX_BUCKETS)
+    buckets = _as(buckets, torch.int32, dev)
+    r = SigattnRelBias()
+    r.dtype, r.num_buckets, r.max_distance = _DTYPE_CODE[table.dtype], table.shape[0], buckets.numel() // 2
+    r.table, r.buckets = table.data_ptr(), buckets.data_ptr()
+    return r, table, buckets
+
+
+def forward_rel(Q, K, V, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, bias, table, buckets, sm_scale,
+                causal) -> torch.Tensor:
+    """forward_packed with the learned bias by relative position (sigattn_rel_fwd)."""
+    lib = load_library()
+    Q, K, V, bias, _, sm_scale, _, _ = _prepare(Q, K, V, bias, None, sm_scale, None, None)
+    cu_q, cu_k = _prepare_packed(cu_seqlens_q, cu_seqlens_k, Q.device)
+    r, *kept = rel_bias(table, buckets, Q.device)
+    if cu_q.numel() == 1:
+        return torch.zeros_like(Q)
+    out = torch.empty_like(Q)
+    if out.numel() == 0:
+        return out
+    pr = _problem(Q, K, V, bias, None, sm_scale, None, None, causal,
+                  packed=_packed_dims(Q, K, cu_q, cu_k, max_seqlen_q, max_seqlen_k))
+
+    def run(stream):
+        nbytes = int(lib.sigattn_rel_fwd_workspace_bytes(ctypes.byref(pr), ctypes.byref(r)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        _raise(lib.sigattn_rel_fwd(ctypes.byref(pr), ctypes.byref(r), out.data_ptr(), ws.data_ptr(), nbytes, stream),
+               "sigattn_rel_fwd")
+
+    _on_device(Q.device, run)
+    return out
+
+
+def backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, bias, table, buckets, sm_scale,
+                 causal, want_table=True):
+    """(dQ, dK, dV, the table's gradient or None) via sigattn_rel_bwd."""
+    lib = load_library()
+    Q, K, V, bias, _, sm_scale, _, _ = _prepare(Q, K, V, bias, None, sm_scale, None, None)
+    cu_q, cu_k = _prepare_packed(cu_seqlens_q, cu_seqlens_k, Q.device)
+    r, table, _kept = rel_bias(table, buckets, Q.device)
+    dO = _as(dO, Q.dtype, Q.device)
+    if dO.shape != Q.shape:
+        raise RuntimeError(f"dO shape {tuple(dO.shape)} != Q shape {tuple(Q.shape)}")
+    if cu_q.numel() == 1 or (Q.numel() == 0 and K.numel() == 0):
+        return torch.zeros_like(Q), torch.zeros_like(K), torch.zeros_like(V), torch.zeros_like(table)
+    dQ, dK, dV = torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)
+    dtable = torch.empty_like(table) if want_table else None
+    pr = _problem(Q, K, V, bias, None, sm_scale, None, None, causal,
+                  packed=_packed_dims(Q, K, cu_q, cu_k, max_seqlen_q, max_seqlen_k))
+
+    def run(stream):
+        nbytes = int(lib.sigattn_rel_bwd_workspace_bytes(ctypes.byref(pr), ctypes.byref(r)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        _raise(lib.sigattn_rel_bwd(ctypes.byref(pr), ctypes.byref(r), _ptr(dO), _ptr(dQ), _ptr(dK), _ptr(dV),
+                                   _ptr(dtable), ws.data_ptr(), nbytes, stream), "sigattn_rel_bwd")
+
+    _on_device(Q.device, run)
+    return dQ, dK, dV, dtable
 
 
 def default_bias(device: torch.device, seq_lens: Optional[torch.Tensor] = None,

@@ -17,8 +17,8 @@ with query / key / value the packed rows of the step's new tokens, one for
 each decoding request and many for a prompt.  Nothing synchronises the host, so
 a step can be captured into a graph and replayed on other lengths.
 
-Ops: `myops::paged_plan`, `myops::paged_cache_write` and
-`myops::sigmoid_attn_paged_fwd` (torch.compile traces them without graph
+Ops: `myops::paged_plan`, `myops::paged_cache_write`,
+`myops::sigmoid_attn_paged_fwd` and `myops::sigmoid_attn_paged_rel_fwd` (torch.compile traces them without graph
 breaks).  Forward only.
 """
 
@@ -252,6 +252,24 @@ def _check_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
     _check_page_size(key_cache.shape[1])
 
 
+def _check_write(key, value, key_cache, value_cache, slot_mapping) -> None:
+    _check_caches(key_cache, value_cache)
+    if any(n > 1 and s == 0 for n, s in zip(key_cache.shape[:3], key_cache.stride())):
+        raise ValueError(f"the caches must not repeat rows (they are changed in place), got strides "
+                         f"{key_cache.stride()}")
+    if key.dim() != 3 or value.dim() != 3:
+        raise ValueError("Expected key and value to be 3D tensors (total_tokens, H_kv, D)")
+    if key.shape != value.shape:
+        raise ValueError(f"key and value must have the same shape, got {tuple(key.shape)} and {tuple(value.shape)}")
+    if key.shape[1:] != key_cache.shape[2:]:
+        raise ValueError(f"key rows {tuple(key.shape[1:])} do not fit cache rows {tuple(key_cache.shape[2:])}")
+    if slot_mapping.shape != (key.shape[0],):
+        raise ValueError(f"slot_mapping must have shape ({key.shape[0]},), got {tuple(slot_mapping.shape)}")
+    if key.dtype != key_cache.dtype or value.dtype != key_cache.dtype:
+        raise RuntimeError(f"key, value and the caches must share a dtype, got {key.dtype}, {value.dtype}, "
+                           f"{key_cache.dtype}")
+
+
 def paged_cache_write(
     key: torch.Tensor,
     value: torch.Tensor,
@@ -275,21 +293,7 @@ def paged_cache_write(
     quick = _quick()
     if quick is not None and quick.quick_write(key, value, key_cache, value_cache, slot_mapping):
         return
-    _check_caches(key_cache, value_cache)
-    if any(n > 1 and s == 0 for n, s in zip(key_cache.shape[:3], key_cache.stride())):
-        raise ValueError(f"the caches must not repeat rows (they are changed in place), got strides "
-                         f"{key_cache.stride()}")
-    if key.dim() != 3 or value.dim() != 3:
-        raise ValueError("Expected key and value to be 3D tensors (total_tokens, H_kv, D)")
-    if key.shape != value.shape:
-        raise ValueError(f"key and value must have the same shape, got {tuple(key.shape)} and {tuple(value.shape)}")
-    if key.shape[1:] != key_cache.shape[2:]:
-        raise ValueError(f"key rows {tuple(key.shape[1:])} do not fit cache rows {tuple(key_cache.shape[2:])}")
-    if slot_mapping.shape != (key.shape[0],):
-        raise ValueError(f"slot_mapping must have shape ({key.shape[0]},), got {tuple(slot_mapping.shape)}")
-    if key.dtype != key_cache.dtype or value.dtype != key_cache.dtype:
-        raise RuntimeError(f"key, value and the caches must share a dtype, got {key.dtype}, {value.dtype}, "
-                           f"{key_cache.dtype}")
+    _check_write(key, value, key_cache, value_cache, slot_mapping)
     _no_grad("paged_cache_write", key, value, key_cache, value_cache)
     if torch.compiler.is_compiling():
         paged_cache_write_op(key, value, key_cache, value_cache, slot_mapping)
@@ -301,9 +305,9 @@ def paged_cache_write(
 # --- attention ----------------------------------------------------------------------
 
 def _attend(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, score_mod, scale,
-            bias, is_causal):
-    """bias None: -log(key length)."""
-    _no_tangent("sigmoid_attention_paged", query, key_cache, value_cache, score_mod)
+            bias, is_causal, rel=None):
+    """bias None: -log(key length).  rel: (bias_table, bias_buckets)."""
+    _no_tangent("sigmoid_attention_paged", query, key_cache, value_cache, score_mod, *(rel or ())[:1])
     lib = _capi.load_library()
     _capi._check_device(query)
     dev = query.device
@@ -338,6 +342,13 @@ def _attend(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q
         p.bias, p.own_bias = bias, 1
 
     def run(stream):
+        if rel is not None:
+            r, *kept = _capi.rel_bias(*rel, dev)
+            nbytes = int(lib.sigattn_paged_rel_fwd_workspace_bytes(ctypes.byref(p), ctypes.byref(r)))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _capi._raise(lib.sigattn_paged_rel_fwd(ctypes.byref(p), ctypes.byref(r), out.data_ptr(), ws.data_ptr(),
+                                                   nbytes, stream), "sigattn_paged_rel_fwd")
+            return
         nbytes = int(lib.sigattn_paged_fwd_workspace_bytes(ctypes.byref(p)))
         ws, nbytes = _capi._bwd_workspace(nbytes, dev)  # without it: unsplit
         _capi._raise(lib.sigattn_paged_fwd(ctypes.byref(p), out.data_ptr(), _capi._ptr(ws), nbytes, stream),
@@ -371,6 +382,32 @@ def _(Q, K_cache, V_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, 
     return Q.new_empty(Q.shape)
 
 
+@torch.library.custom_op("myops::sigmoid_attn_paged_rel_fwd", mutates_args=())
+def sigmoid_attn_paged_rel_fwd_op(
+    Q: torch.Tensor,
+    K_cache: torch.Tensor,
+    V_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens_k: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_q: int,
+    bias_table: torch.Tensor,
+    bias_buckets: torch.Tensor,
+    sm_scale: float,
+    bias: Optional[float],
+    is_causal: bool,
+) -> torch.Tensor:
+    """Forward over a paged cache with the learned bias by relative position."""
+    return _attend(Q, K_cache, V_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, None, sm_scale, bias,
+                   is_causal, (bias_table, bias_buckets))
+
+
+@sigmoid_attn_paged_rel_fwd_op.register_fake
+def _(Q, K_cache, V_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, bias_table, bias_buckets, sm_scale, bias,
+      is_causal):
+    return Q.new_empty(Q.shape)
+
+
 def sigmoid_attention_paged(
     query: torch.Tensor,
     key_cache: torch.Tensor,
@@ -383,11 +420,14 @@ def sigmoid_attention_paged(
     scale: Optional[float] = None,
     sigmoid_bias: Optional[float] = None,
     score_mod: Optional[torch.Tensor] = None,
+    bias_table: Optional[torch.Tensor] = None,
+    bias_buckets: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Sigmoid attention of new tokens over a paged cache that holds them already.
 
     output = sigmoid(Q·Kᵀ·scale + sigmoid_bias + score_mod[k_idx]) · V over the
-    keys of each sequence.
+    keys of each sequence; with bias_table, that of the relative position
+    (k_idx - seq_lens_k + n - i) is added.
 
     Args:
         query: [N, H, D] packed new tokens: sequence b's are rows
@@ -414,6 +454,9 @@ def sigmoid_attention_paged(
         sigmoid_bias: default -log(seq_lens_k[b]) per sequence.
         score_mod: optional [B, max_pages * page_size] per-key term by position
             (no NaN below seq_lens_k).
+        bias_table, bias_buckets: the learned bias by relative position, as
+            sigmoid_attention_varlen takes it (not with score_mod); query i of n
+            sits at position seq_lens_k - n + i.
 
     Returns:
         [N, H, D] output, contiguous.  Rows outside every sequence are zeros.
@@ -422,7 +465,7 @@ def sigmoid_attention_paged(
         Forward only: tensors that ask for a gradient (under grad mode) or
         carry a forward-mode tangent are refused.
     """
-    quick = _quick()
+    quick = _quick() if bias_table is None and bias_buckets is None else None
     if quick is not None:
         out = quick.quick_paged(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q,
                                 is_causal, scale, sigmoid_bias, score_mod)
@@ -453,11 +496,15 @@ def sigmoid_attention_paged(
         raise ValueError(f"max_seqlen_q must be non-negative, got {max_seqlen_q}")
     if query.dtype != key_cache.dtype:
         raise RuntimeError(f"query and the caches must share a dtype, got {query.dtype}, {key_cache.dtype}")
-    _no_grad("sigmoid_attention_paged", query, key_cache, value_cache, score_mod)
+    rel = _capi.check_rel(bias_table, bias_buckets, H, score_mod)
+    _no_grad("sigmoid_attention_paged", query, key_cache, value_cache, score_mod, bias_table)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     bias = None if sigmoid_bias is None else float(sigmoid_bias)
+    if rel is not None and torch.compiler.is_compiling():
+        return sigmoid_attn_paged_rel_fwd_op(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q,
+                                             int(max_seqlen_q), *rel, scale, bias, is_causal)
     if torch.compiler.is_compiling():
         return sigmoid_attn_paged_fwd_op(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q,
                                          int(max_seqlen_q), score_mod, scale, bias, is_causal)
     return _attend(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q, score_mod, scale,
-                   bias, is_causal)
+                   bias, is_causal, rel)

@@ -13,7 +13,8 @@ is read, computed or written.
 
 Ops: `myops::sigmoid_attn_varlen_fwd` / `myops::sigmoid_attn_varlen_bwd`
 (the padded ops' schemas with cu_seqlens in place of seq_lens and the two
-max_seqlen integers), with register_fake and register_autograd so
+max_seqlen integers), and `myops::sigmoid_attn_varlen_rel_fwd` / `_rel_bwd` with the
+learned bias by relative position, with register_fake and register_autograd so
 torch.compile traces them without graph breaks.
 """
 
@@ -133,6 +134,98 @@ class _VarlenEager(torch.autograd.Function):
         return dQ, dK, dV, None, None, None, None, None, None, None, None
 
 
+# With the learned bias by relative position (bias_table, bias_buckets).
+
+@torch.library.custom_op("myops::sigmoid_attn_varlen_rel_fwd", mutates_args=())
+def sigmoid_attn_varlen_rel_fwd_op(
+    Q: torch.Tensor,
+    K: torch.Tensor,
+    V: torch.Tensor,
+    bias_table: torch.Tensor,
+    bias_buckets: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_k: int,
+    max_seqlen_q: int,
+    bias: torch.Tensor,
+    sm_scale: torch.Tensor,
+    is_causal: bool,
+) -> torch.Tensor:
+    """Packed forward with the learned bias."""
+    return _capi.forward_rel(Q, K, V, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, bias, bias_table,
+                             bias_buckets, sm_scale, is_causal)
+
+
+@sigmoid_attn_varlen_rel_fwd_op.register_fake
+def _(Q, K, V, bias_table, bias_buckets, cu_seqlens_k, cu_seqlens_q, max_seqlen_k, max_seqlen_q, bias, sm_scale,
+      is_causal):
+    return torch.empty_like(Q)
+
+
+@torch.library.custom_op("myops::sigmoid_attn_varlen_rel_bwd", mutates_args=())
+def sigmoid_attn_varlen_rel_bwd_op(
+    Q: torch.Tensor,
+    K: torch.Tensor,
+    V: torch.Tensor,
+    dO: torch.Tensor,
+    bias_table: torch.Tensor,
+    bias_buckets: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_k: int,
+    max_seqlen_q: int,
+    bias: torch.Tensor,
+    sm_scale: torch.Tensor,
+    is_causal: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Packed backward with the learned bias: (dQ, dK, dV, the table's gradient)."""
+    return _capi.backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, bias, bias_table,
+                              bias_buckets, sm_scale, is_causal)
+
+
+@sigmoid_attn_varlen_rel_bwd_op.register_fake
+def _(Q, K, V, dO, bias_table, bias_buckets, cu_seqlens_k, cu_seqlens_q, max_seqlen_k, max_seqlen_q, bias, sm_scale,
+      is_causal):
+    return torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V), bias_table.new_empty(bias_table.shape)
+
+
+def _varlen_rel_setup_context(ctx, inputs, output):
+    (Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, ctx.max_seqlen_k, ctx.max_seqlen_q, bias, sm_scale,
+     ctx.is_causal) = inputs
+    ctx.save_for_backward(Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, bias, sm_scale)
+
+
+def _varlen_rel_backward(ctx, dO):
+    """Returns (dQ, dK, dV, the table's gradient, None x 8)."""
+    Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, bias, sm_scale = ctx.saved_tensors
+    grads = sigmoid_attn_varlen_rel_bwd_op(Q, K, V, dO, table, buckets, cu_seqlens_k, cu_seqlens_q, ctx.max_seqlen_k,
+                                           ctx.max_seqlen_q, bias, sm_scale, ctx.is_causal)
+    return (*grads, *(None,) * 8)
+
+
+sigmoid_attn_varlen_rel_fwd_op.register_autograd(_varlen_rel_backward, setup_context=_varlen_rel_setup_context)
+
+
+class _VarlenRelEager(torch.autograd.Function):
+    """Eager path of sigmoid_attention_varlen with the learned bias."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, max_seqlen_k, max_seqlen_q, bias, sm_scale,
+                is_causal):
+        _varlen_rel_setup_context(ctx, (Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, max_seqlen_k,
+                                        max_seqlen_q, bias, sm_scale, is_causal), None)
+        return _capi.forward_rel(Q, K, V, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, bias, table, buckets,
+                                 sm_scale, is_causal)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dO):
+        Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, bias, sm_scale = ctx.saved_tensors
+        grads = _capi.backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k, bias,
+                                   table, buckets, sm_scale, ctx.is_causal, ctx.needs_input_grad[3])
+        return (*grads, *(None,) * 8)
+
+
 def _check_cu(name: str, cu: torch.Tensor) -> torch.Tensor:
     if cu.dim() != 1 or cu.numel() < 1:
         raise ValueError(f"{name} must have shape (B + 1,), got {cu.shape}")
@@ -153,11 +246,15 @@ def sigmoid_attention_varlen(
     scale: Optional[float] = None,
     sigmoid_bias: Optional[float] = None,
     score_mod: Optional[torch.Tensor] = None,
+    bias_table: Optional[torch.Tensor] = None,
+    bias_buckets: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Sigmoid attention over packed variable-length sequences, with autograd.
 
     output = sigmoid(Q·Kᵀ·scale + sigmoid_bias + score_mod[k_idx]) · V within
-    each sequence.
+    each sequence; with bias_table,
+    bias_table[bias_buckets[R + clamp(k_idx - q_idx, -R, R)], h] is added to the
+    scores of query head h.
 
     Args:
         query: [total_q, H, D]; key, value: [total_k, H_kv, D] with H a
@@ -176,6 +273,13 @@ def sigmoid_attention_varlen(
         sigmoid_bias: default -log(key length of each sequence).
         score_mod: optional [total_k] per-key bias (packed like the keys);
             receives no gradient.
+        bias_table: optional [num_buckets, H] learned bias by relative position
+            (float16, bfloat16 or float32, whatever the query's dtype), with
+            a gradient of its dtype, summed in fp32.  Not with score_mod.
+        bias_buckets: [2 R + 1] int32 or int64 bucket of each relative position
+            -R .. R of key to query (R up to 2048), as
+            relative_position_buckets gives them; buckets outside the table add
+            nothing.  Positions count from the start of each sequence.
 
     Returns:
         [total_q, H, D] output, equal row for row to what
@@ -188,7 +292,8 @@ def sigmoid_attention_varlen(
     the output and in dQ / dK / dV (they take no part in the attention), so
     no gradient row is left uninitialised.
     """
-    if not torch.compiler.is_compiling() and _capi.quick_module is not None:
+    plain = bias_table is None and bias_buckets is None
+    if plain and not torch.compiler.is_compiling() and _capi.quick_module is not None:
         out = _capi.quick_module.quick_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                                               is_causal, scale, sigmoid_bias, score_mod)
         if out is not None:
@@ -214,6 +319,7 @@ def sigmoid_attention_varlen(
         if score_mod.shape != (N_k,):
             raise ValueError(f"score_mod must have shape ({N_k},), got {score_mod.shape}")
         score_mod = score_mod.contiguous()
+    rel = _capi.check_rel(bias_table, bias_buckets, H, score_mod)
 
     if max_seqlen_q is None:
         max_seqlen_q = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item()) if B > 0 else 0
@@ -236,6 +342,10 @@ def sigmoid_attention_varlen(
         scale = 1.0 / math.sqrt(D)
     scale_tensor = _capi.device_constant((), float(scale), torch.float32, query.device)
     cu_seqlens_k, cu_seqlens_q = cu_seqlens_k.to(query.device), cu_seqlens_q.to(query.device)
+    if rel is not None:
+        fn = sigmoid_attn_varlen_rel_fwd_op if torch.compiler.is_compiling() else _VarlenRelEager.apply
+        return fn(query, key, value, *rel, cu_seqlens_k, cu_seqlens_q, int(max_seqlen_k), int(max_seqlen_q), bias,
+                  scale_tensor, is_causal)
     if torch.compiler.is_compiling():
         return sigmoid_attn_varlen_fwd_op(query, key, value, cu_seqlens_k, cu_seqlens_q, int(max_seqlen_k),
                                           int(max_seqlen_q), bias, score_mod, scale_tensor, is_causal)
