@@ -1,0 +1,152 @@
+// C ABI of the learned bias by relative position (include/sigattn.h): validation on
+// the host, before any HIP call, and the choice of kernels.
+#include "paged_problem.h"
+#include "rel.h"
+
+using namespace sigattn;
+
+namespace {
+
+RelParams rel_params(const sigattn_problem *p, const RelTable &t, void *line) {
+  RelParams k{};
+  (KParams &)k = make_params(p);
+  k.line = (const float *)line;
+  k.reach = t.reach;
+  return k;
+}
+
+int64_t rel_part_bytes(const sigattn_problem *p, const RelTable &t) {
+  return (p->rows_q / kGenericRows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float);
+}
+
+RelParams rel_kv_items(const RelParams &k) {
+  RelParams s = k;
+  (KParams &)s = kv_items(k);
+  return s;
+}
+
+// The learned bias's table as far as the cache's sequences reach.
+RelTable rel_table_of(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  return rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q,
+                            p->max_pages * p->page_size);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r) {
+  const int rc = sigattn_check(p);
+  if (rc != SIGATTN_OK) return rc;
+  if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
+  if (r->dtype != SIGATTN_F16 && r->dtype != SIGATTN_BF16 && r->dtype != SIGATTN_F32) return SIGATTN_ERR_DTYPE;
+  if (!rel_table_ok(r) || p->score_mod != nullptr || p->cu_seqlens_q == nullptr || p->cu_seqlens_k == nullptr)
+    return SIGATTN_ERR_REL_BIAS;
+  if (p->H > 65535) return SIGATTN_ERR_SHAPE;  // the launches' second dimension
+  if (p->H > 0 && (r->table == nullptr || r->buckets == nullptr)) return SIGATTN_ERR_NULL_ARG;
+  return SIGATTN_OK;
+}
+
+size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
+  return sigattn_rel_check(p, r) == SIGATTN_OK ? (size_t)rel_line_bytes(rel_table(r, p->H, p->Tq, p->Tk)) : 0;
+}
+
+int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
+                    size_t workspace_bytes, void *stream) {
+  const int rc = sigattn_rel_check(p, r);
+  if (rc != SIGATTN_OK) return rc;
+  if (p->H == 0 || p->rows_q == 0) return SIGATTN_OK;
+  if (out == nullptr) return SIGATTN_ERR_NULL_ARG;
+  const hipStream_t st = (hipStream_t)stream;
+  if (p->B == 0 || p->Tq == 0) {
+    (void)hipGetLastError();
+    zero_packed_gaps(p, out, nullptr, nullptr, st);
+    return launch_status();
+  }
+  const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
+  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < rel_line_bytes(t))
+    return SIGATTN_ERR_WORKSPACE;
+  RelParams k = rel_params(p, t, workspace);
+  k.out = out;
+  (void)hipGetLastError();
+  launch_rel_line(t, (float *)workspace, st);
+  zero_packed_gaps(p, out, nullptr, nullptr, st);
+  launch_rel_fwd_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
+  return launch_status();
+}
+
+size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
+  if (sigattn_rel_check(p, r) != SIGATTN_OK) return 0;
+  const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
+  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t));
+}
+
+int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
+                    void *dtable, void *workspace, size_t workspace_bytes, void *stream) {
+  const int rc = sigattn_rel_check(p, r);
+  if (rc != SIGATTN_OK) return rc;
+  if (p->H == 0) return SIGATTN_OK;
+  const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
+  if ((p->rows_q > 0 && (dq == nullptr || dout == nullptr)) ||
+      (p->rows_k > 0 && (dk == nullptr || dv == nullptr)))
+    return SIGATTN_ERR_NULL_ARG;
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < sigattn_rel_bwd_workspace_bytes(p, r))
+    return SIGATTN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  RelParams k = rel_params(p, t, workspace);
+  float *sums = (float *)((char *)workspace + rel_line_bytes(t));
+  k.dout = dout;
+  k.dq = dq;
+  k.dk = dk;
+  k.dv = dv;
+  (void)hipGetLastError();
+  zero_packed_gaps(p, dq, dk, dv, st);
+  if (p->B == 0 || p->Tq == 0) {  // no query row is in a sequence
+    if (p->B > 0 && p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, (int)p->D, false, st);
+    if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
+    return launch_status();
+  }
+  launch_rel_line(t, (float *)workspace, st);
+  if (dtable != nullptr) k.part = (float *)((char *)workspace + 2 * rel_line_bytes(t));
+  k.part_rows = kGenericRows;
+  launch_rel_dq_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
+  if (p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, (int)p->D, p->causal != 0, st);
+  if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
+  return launch_status();
+}
+
+int sigattn_paged_rel_check(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  const int rc = sigattn_paged_check(p);
+  if (rc != SIGATTN_OK) return rc;
+  if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
+  if (r->dtype != SIGATTN_F16 && r->dtype != SIGATTN_BF16 && r->dtype != SIGATTN_F32) return SIGATTN_ERR_DTYPE;
+  if (!rel_table_ok(r) || p->score_mod != nullptr) return SIGATTN_ERR_REL_BIAS;
+  if (p->H > 0 && (r->table == nullptr || r->buckets == nullptr)) return SIGATTN_ERR_NULL_ARG;
+  return SIGATTN_OK;
+}
+
+size_t sigattn_paged_rel_fwd_workspace_bytes(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
+  if (sigattn_paged_rel_check(p, r) != SIGATTN_OK || p->rows_q == 0 || p->H == 0 || p->B == 0) return 0;
+  return (size_t)rel_line_bytes(rel_table_of(p, r));
+}
+
+int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
+                          size_t workspace_bytes, void *stream) {
+  const int rc = sigattn_paged_rel_check(p, r);
+  if (rc != SIGATTN_OK) return rc;
+  if (p->rows_q == 0 || p->H == 0 || p->B == 0) return sigattn_paged_fwd(p, out, nullptr, 0, stream);
+  if (out == nullptr) return SIGATTN_ERR_NULL_ARG;
+  const RelTable t = rel_table_of(p, r);
+  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < rel_line_bytes(t))
+    return SIGATTN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  PagedRelParams k{};
+  (PagedParams &)k = make_params(p, out);
+  k.line = (const float *)workspace, k.reach = t.reach;
+  (void)hipGetLastError();
+  launch_rel_line(t, (float *)workspace, st);
+  launch_paged_rel_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
+  return launch_status();
+}
+
+}  // extern "C"
