@@ -73,6 +73,12 @@ def test_reaches(R, causal):
     check(make(lens, lens, 2, 2, 64, torch.bfloat16, 11, R, seed=R), causal)
 
 
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 64), ("bf16", 32)])
+@pytest.mark.parametrize("R", [1000, 2048])
+def test_far_reaches(R, dtype, D):
+    check(make([2150, 70], [2150, 70], 1, 1, D, DT[dtype], 40, R, seed=R), False)
+
+
 @pytest.mark.parametrize("num", [1, 2, 255, 256, 257, 700])
 def test_numbers_of_buckets(num):
     check(make([150, 40], [150, 40], 2, 1, 32, torch.float16, num, 200, seed=num), False)

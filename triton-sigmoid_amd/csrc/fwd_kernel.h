@@ -32,6 +32,7 @@
 
 #include "common.h"
 #include "paged.h"
+#include "rel.h"
 
 namespace sigattn {
 
@@ -79,13 +80,26 @@ template <int D, int WK = 1, int NCB = 1> constexpr int fwd_occupancy() {
 // The kernel's LDS, in arrays of their own: as members of one struct their
 // addresses took so many more registers that the D = 128 kernel spilled 100.
 template <int D, int WK> using FwdTiles = uint16_t[fwd_stages<D, WK>()][64 * D];
-template <int D, int WK, bool SCOREMOD> using FwdTerms = float[SCOREMOD ? fwd_stages<D, WK>() * 64 : 4];
+// What a tile's scores have added, times -log2(e): score_mod per key, or (WIN: a
+// window of that many places) the learned bias by relative position.
+template <int D, int WK, bool SCOREMOD, int WIN = 0>
+using FwdTerms = float[WIN > 0 ? fwd_stages<D, WK>() * WIN : (SCOREMOD ? fwd_stages<D, WK>() * 64 : 4)];
+// Places of a 64-key tile's window against the BM queries of a workgroup.
+template <class P, int NWV, int NCB, int WK> constexpr int fwd_window() {
+  return P::kRel && !P::kPaged ? 32 * NCB * NWV / WK + 64 : 0;
+}
 
 // Work item `wg` of the kernel's.
 template <typename T, int D, int NWV, int NCB, int WK, bool CAUSAL, bool SCOREMOD, class P>
 __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles<D, WK> &sK, FwdTiles<D, WK> &sV,
-                                              FwdTerms<D, WK, SCOREMOD> &sC) {
+                                              FwdTerms<D, WK, SCOREMOD, fwd_window<P, NWV, NCB, WK>()> &sC) {
   constexpr bool PAGED = P::kPaged;
+  // Learned bias by relative position: the values of a tile and the workgroup's
+  // queries are a window of WIN places of the head's line, staged beside the
+  // tile; a lane's keys are neighbours in it, its query their distance from its end.
+  constexpr int WIN = fwd_window<P, NWV, NCB, WK>();
+  constexpr bool REL = WIN > 0;
+  static_assert(!(REL && SCOREMOD) && (!REL || (NCB == 1 && WIN <= 64 * NWV)), "terms");
   static_assert(!PAGED || WK == 1, "pairs of waves: contiguous keys only");
   // NWV waves per workgroup (8: two per SIMD), NCB 32-query column blocks each.
   // WK = 2: the waves form pairs that hold the same queries; wave `wt` of a
@@ -105,7 +119,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
   // another 1-2.5 % (16 vs 8) at the headline shapes.  D = 64: 4 (three waves
   // per SIMD, 168 registers each); D = 32: 4, a whole region (2 with
   // score_mod, which spills at four waves per SIMD otherwise).
-  constexpr int LA = D == 128 ? (SCOREMOD ? 8 : 16) : (D == 32 && SCOREMOD ? 2 : 4);
+  constexpr int LA = D == 128 ? (SCOREMOD || REL ? 8 : 16) : (D == 32 && (SCOREMOD || REL) ? 2 : 4);
   constexpr int NWD = 8 * NCB;          // packed P words per block
   constexpr int BAR = NSTEP - LA;       // step of the tile barrier (in odd regions; WK = 2: in all)
   static_assert(NSTEP % LA == 0, "region shape");
@@ -271,13 +285,24 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     }
 
     float creg = 0.0f;
+    [[maybe_unused]] const int win0 = WIN - 64 - slot * QW - l32 + 4 * hi;  // this lane's place of the tile's key 0
     auto load_c = [&](int n0) SIGATTN_INLINE {
+      if constexpr (REL) {
+        if (tid < WIN) creg = -(bias + rel_at(p, h, n0 + tid - q0 - BM)) * kLog2e;
+      }
       if (SCOREMOD && tid < BN) {
         const int key = n0 + tid;
         int64_t at;
         if constexpr (PAGED) at = b * p.mod_stride;
         else at = p.mod_base(b);
         creg = key < Lk ? -(bias + p.score_mod[at + key0 + key]) * kLog2e : 0.0f;
+      }
+    };
+    // (After the copies' wait: the write of what load_c fetched for tile t.)
+    auto store_c = [&](int t) SIGATTN_INLINE {
+      if (SCOREMOD && tid < BN) sC[(t % NST) * BN + tid] = creg;
+      if constexpr (REL) {
+        if (tid < WIN) sC[(t % NST) * WIN + tid] = creg;
       }
     };
     auto issue = [&](int st, int t) SIGATTN_INLINE {
@@ -367,7 +392,12 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       const uint32_t(&pp)[NCB][8] = pbuf[SL];
       float c[16];   // exp2 offsets of block r-1 (per key row)
       float cn[2];   // ... of block r's first word
-      if constexpr (SCOREMOD) {
+      if constexpr (REL) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] = sC[STVn * WIN + KLn + cl + 8 * (i / 4) + i % 4 + win0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) cn[i] = sC[STC * WIN + KL + cl + i + win0];
+      } else if constexpr (SCOREMOD) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 cv = *(const float4 *)&sC[STVn * BN + KLn + cl + 8 * g + 4 * hi];
@@ -386,11 +416,11 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
           const int u = (r + 1) / RPT;
           if (u < ntiles) {
             wait_dma();
-            if (SCOREMOD && tid < BN) sC[(u % NST) * BN + tid] = creg;
+            store_c(u);
             // With three stages (four when a region is a tile) the copy below
             // refills the stage this region's Vᵀ operands came from: every
             // wave's reads of it complete first.
-            if constexpr (NST == 3 || WK == 2) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if constexpr (NST == 3 || WK == 2 || REL) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -469,7 +499,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     if (ntiles > 0) {
       issue(0, 0);
       wait_dma();
-      if (SCOREMOD && tid < BN) sC[tid] = creg;
+      store_c(0);
     }
     __syncthreads();
     if (ntiles > 1) issue(1, 1);
@@ -501,8 +531,8 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       const int u = (r + 1) * WK / 2;
       if (u < ntiles) {
         wait_dma();
-        if (SCOREMOD && tid < BN) sC[(u % NST) * BN + tid] = creg;
-        if constexpr (NST == 3 || WK == 2) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        store_c(u);
+        if constexpr (NST == 3 || WK == 2 || REL) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -557,7 +587,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
 template <typename T, int D, int NWV, int NCB, int WK, bool CAUSAL, bool SCOREMOD, class P>
 __global__ __launch_bounds__(64 * NWV, (fwd_occupancy<D, WK, NCB>())) void fwd_mfma_kernel(const P p) {
   __shared__ __attribute__((aligned(16))) FwdTiles<D, WK> sK, sV;
-  __shared__ __attribute__((aligned(16))) FwdTerms<D, WK, SCOREMOD> sC;
+  __shared__ __attribute__((aligned(16))) FwdTerms<D, WK, SCOREMOD, fwd_window<P, NWV, NCB, WK>()> sC;
   const int wg = gap_prologue<2>(p, sK);  // packed layouts: leading gap-zeroing workgroups
   if (wg < 0) return;
   fwd_mfma_body<T, D, NWV, NCB, WK, CAUSAL, SCOREMOD, P>(p, wg, sK, sV, sC);

@@ -75,6 +75,15 @@ void launch_rel_line(const RelTable &t, float *line, hipStream_t st);
 // p.part (nullptr: zeros); sums: [H, 2 reach + 1] floats of scratch.
 void launch_rel_grad(const RelTable &t, const RelParams &p, float *sums, void *grad, hipStream_t st);
 
+// MFMA forward, as launch_fwd_mfma.
+void launch_rel_fwd_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+
+// MFMA backward, as launch_bwd_dq_mfma and launch_bwd_dkdv_mfma; the dQ kernel fills
+// RelParams::part in blocks of rel_dq_rows rows.
+int rel_dq_rows(const RelParams &p, int D, bool causal);
+void launch_rel_dq_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+void launch_rel_dkdv_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+
 // Portable kernels (launch.h); the dQ one fills RelParams::part, in blocks of
 // kGenericRows rows.
 constexpr int kGenericRows = 64;

@@ -16,7 +16,8 @@ RelParams rel_params(const sigattn_problem *p, const RelTable &t, void *line) {
 }
 
 int64_t rel_part_bytes(const sigattn_problem *p, const RelTable &t) {
-  return (p->rows_q / kGenericRows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float);
+  // (Blocks of 64 rows, the shortest; a multiple of 256 bytes.)
+  return ((p->rows_q / kGenericRows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
 RelParams rel_kv_items(const RelParams &k) {
@@ -70,6 +71,14 @@ int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *o
   k.out = out;
   (void)hipGetLastError();
   launch_rel_line(t, (float *)workspace, st);
+  const void *ptrs[4] = {p->q, p->k, p->v, out};
+  if (use_mfma(p, ptrs, 4)) {
+    GapAxis gq, gk;
+    gap_axes(p, out, nullptr, nullptr, gq, gk);
+    use_gaps(k, gq, gk);
+    launch_rel_fwd_mfma(k, p->dtype, mfma_head_dim(p), p->causal != 0, st);
+    return launch_status();
+  }
   zero_packed_gaps(p, out, nullptr, nullptr, st);
   launch_rel_fwd_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
   return launch_status();
@@ -78,7 +87,9 @@ int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *o
 size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
   if (sigattn_rel_check(p, r) != SIGATTN_OK) return 0;
   const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
-  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t));
+  // (Pointers are not known yet: aligned rows, as everywhere.)
+  const void *none[1] = {nullptr};
+  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0)).bytes);
 }
 
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
@@ -99,18 +110,35 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
   k.dq = dq;
   k.dk = dk;
   k.dv = dv;
+  const void *ptrs[7] = {p->q, p->k, p->v, dout, dq, dk, dv};
+  const bool mfma = use_mfma(p, ptrs, 7) && p->Tq > 0 && p->Tk > 0, causal = p->causal != 0;
+  const int D = mfma ? mfma_head_dim(p) : (int)p->D;
   (void)hipGetLastError();
-  zero_packed_gaps(p, dq, dk, dv, st);
+  if (!mfma) zero_packed_gaps(p, dq, dk, dv, st);
   if (p->B == 0 || p->Tq == 0) {  // no query row is in a sequence
-    if (p->B > 0 && p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, (int)p->D, false, st);
+    if (p->B > 0 && p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, D, causal, st);
     if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
     return launch_status();
   }
   launch_rel_line(t, (float *)workspace, st);
-  if (dtable != nullptr) k.part = (float *)((char *)workspace + 2 * rel_line_bytes(t));
-  k.part_rows = kGenericRows;
-  launch_rel_dq_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
-  if (p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, (int)p->D, p->causal != 0, st);
+  char *parts = (char *)workspace + 2 * rel_line_bytes(t);
+  if (dtable != nullptr) k.part = (float *)parts;
+  if (mfma) {
+    const HeadSplit hs = head_split(p, mfma);
+    k.qsplit = hs.n;
+    k.kv_part = (float *)(parts + rel_part_bytes(p, t));
+    k.part_rows = rel_dq_rows(k, D, causal);
+    RelParams kq = k;
+    GapAxis gq, gk;
+    gap_axes(p, dq, dk, dv, gq, gk);
+    use_gaps(kq, gq, gk);
+    launch_rel_dq_mfma(kq, p->dtype, D, causal, st);
+    launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, st);
+  } else {
+    k.part_rows = kGenericRows;
+    launch_rel_dq_generic(k, p->dtype, D, causal, st);
+    if (p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, D, causal, st);
+  }
   if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
   return launch_status();
 }

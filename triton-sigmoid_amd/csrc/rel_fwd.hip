@@ -1,0 +1,41 @@
+// The forward kernel (fwd_kernel.h) with the learned bias by relative position.
+#include "fwd_kernel.h"
+#include "launch.h"
+#include "rel.h"
+
+namespace sigattn {
+namespace {
+
+template <typename T, int D, int NWV, int WK>
+void fwd_w(const RelParams &kp, bool causal, hipStream_t st) {
+  constexpr int BM = NWV * 32 / WK;
+  RelParams p = kp;
+  p.nblk = (p.Tq + BM - 1) / BM;
+  p.rsplit = 1;
+  const dim3 grid((unsigned)(p.nblk * p.B * p.H + p.ngap[0] + p.ngap[1])), block(64 * NWV);
+  if (causal) fwd_mfma_kernel<T, D, NWV, 1, WK, true, false, RelParams><<<grid, block, 0, st>>>(p);
+  else fwd_mfma_kernel<T, D, NWV, 1, WK, false, false, RelParams><<<grid, block, 0, st>>>(p);
+}
+
+// Waves and pairs of them as without the bias.
+template <typename T, int D> void fwd_t(const RelParams &p, bool causal, hipStream_t st) {
+  if constexpr (D <= 64) {
+    if (fwd_wave_pairs(p)) return fwd_w<T, D, 4, 2>(p, causal, st);
+  }
+  fwd_w<T, D, D <= 64 ? 4 : 8, 1>(p, causal, st);
+}
+
+template <typename T> void fwd_d(const RelParams &p, int D, bool causal, hipStream_t st) {
+  if (D == 128) fwd_t<T, 128>(p, causal, st);
+  else if (D == 64) fwd_t<T, 64>(p, causal, st);
+  else fwd_t<T, 32>(p, causal, st);
+}
+
+}  // namespace
+
+void launch_rel_fwd_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st) {
+  if (dtype == kBF16) fwd_d<__bf16>(p, D, causal, st);
+  else fwd_d<_Float16>(p, D, causal, st);
+}
+
+}  // namespace sigattn
