@@ -99,6 +99,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
   // tile; a lane's keys are neighbours in it, its query their distance from its end.
   constexpr int WIN = fwd_window<P, NWV, NCB, WK>();
   constexpr bool REL = WIN > 0;
+  constexpr bool LANE_REL = P::kRel && P::kPaged;  // each lane reads its column's (RelColumn)
   static_assert(!(REL && SCOREMOD) && (!REL || (NCB == 1 && WIN <= 64 * NWV)), "terms");
   static_assert(!PAGED || WK == 1, "pairs of waves: contiguous keys only");
   // NWV waves per workgroup (8: two per SIMD), NCB 32-query column blocks each.
@@ -119,7 +120,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
   // another 1-2.5 % (16 vs 8) at the headline shapes.  D = 64: 4 (three waves
   // per SIMD, 168 registers each); D = 32: 4, a whole region (2 with
   // score_mod, which spills at four waves per SIMD otherwise).
-  constexpr int LA = D == 128 ? (SCOREMOD || REL ? 8 : 16) : (D == 32 && (SCOREMOD || REL) ? 2 : 4);
+  constexpr int LA = D == 128 ? (SCOREMOD || P::kRel ? 8 : 16) : (D == 32 && (SCOREMOD || P::kRel) ? 2 : 4);
   constexpr int NWD = 8 * NCB;          // packed P words per block
   constexpr int BAR = NSTEP - LA;       // step of the tile barrier (in odd regions; WK = 2: in all)
   static_assert(NSTEP % LA == 0, "region shape");
@@ -284,6 +285,11 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       all_see = seen(min(qw, Lq - 1));
     }
 
+    [[maybe_unused]] RelColumn rc;
+    if constexpr (LANE_REL) {
+      const int col = min(myq0, Lq - 1), tok = col / p.G;
+      if (q0 < Lq) rc.init(p, h * p.G + col - tok * p.G, un.Lk - un.Lq + tok - key0, bias);
+    }
     float creg = 0.0f;
     [[maybe_unused]] const int win0 = WIN - 64 - slot * QW - l32 + 4 * hi;  // this lane's place of the tile's key 0
     auto load_c = [&](int n0) SIGATTN_INLINE {
@@ -392,7 +398,10 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       const uint32_t(&pp)[NCB][8] = pbuf[SL];
       float c[16];   // exp2 offsets of block r-1 (per key row)
       float cn[2];   // ... of block r's first word
-      if constexpr (REL) {
+      if constexpr (LANE_REL) {
+        rc.block(32 * block_of(r - 1), hi, c);
+        rc.block(32 * block_of(r), hi, cn);
+      } else if constexpr (REL) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) c[i] = sC[STVn * WIN + KLn + cl + 8 * (i / 4) + i % 4 + win0];
 #pragma unroll

@@ -63,37 +63,21 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
     pl.fwd.split_units = pl.decode.split_units = 0;
   }
   (void)hipGetLastError();
-  sigattn::GapAxis gap;
-  gap.cu = p->cu_seqlens_q, gap.B = k.B, gap.T = k.Tq, gap.H = k.H, gap.D = (int)p->D;
-  gap.rows = p->rows_q, gap.st = p->H * p->D, gap.sh = p->D, gap.out[0] = out;
   if (p->B == 0) {  // no sequence: every row is outside
-    sigattn::launch_zero_gaps(gap, sigattn::GapAxis{}, dt == SIGATTN_F32 ? 4 : 2, st);
+    launch_zero_gaps(paged_gap(p, k, out), GapAxis{}, dt == SIGATTN_F32 ? 4 : 2, st);
     return launch_status();
   }
   if (!mfma) {
-    sigattn::launch_paged_generic(k, dt, (int)p->D, causal, st);
+    launch_paged_generic(k, dt, (int)p->D, causal, st);
     return launch_status();
   }
-  // The workspace: both parts' cuts, then their partials.
-  const auto at = [&](size_t bytes) -> void * { return workspace != nullptr ? (char *)workspace + bytes : nullptr; };
-  k.gap[0] = gap;
-  // The kernel also zeroes the rows outside every sequence (workgroups in
-  // a multiple of 8, so that its items keep their XCDs).
-  const int gaps = (int)(cdiv(cdiv(p->rows_q, 64), 8) * 8);
-  const PagedParams kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, (int2 *)at(0), (float *)at(pl.cut_bytes));
-  const PagedParams kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0,
-                                 (int2 *)at((size_t)p->B * sizeof(int2)),
-                                 (float *)at(pl.cut_bytes + pl.fwd.partial_bytes));
-  PagedParams first = pl.fwd.units > 0 ? kf : kd;
-  first.ngap[0] = gaps;
-  if (pl.fwd.units > 0 && pl.decode.units > 0)
-    sigattn::launch_paged_mixed(first, (int)pl.fwd.units, kd, (int)pl.decode.units, dt, D, causal, st);
-  else if (pl.decode.units > 0 && dt == SIGATTN_F32)
-    sigattn::launch_paged_decode_f32(first, (int)pl.decode.units, D, causal, st);
-  else if (pl.decode.units > 0) sigattn::launch_paged_decode(first, (int)pl.decode.units, dt, D, causal, st);
-  else if (dt == SIGATTN_F32) sigattn::launch_paged_f32(first, (int)pl.fwd.units, D, causal, st);
-  else sigattn::launch_paged_fwd(first, (int)pl.fwd.units, dt, D, causal, st);
-  if (kf.split_units > 0 || kd.split_units > 0) sigattn::launch_paged_reduce(kf, kd, dt, D, st);
+  run_plan(p, k, pl, (char *)workspace, out, st, [&](const PagedParams &first, int nf, const PagedParams &kd, int nd) {
+    if (nf > 0 && nd > 0) launch_paged_mixed(first, nf, kd, nd, dt, D, causal, st);
+    else if (nd > 0 && dt == SIGATTN_F32) launch_paged_decode_f32(first, nd, D, causal, st);
+    else if (nd > 0) launch_paged_decode(first, nd, dt, D, causal, st);
+    else if (dt == SIGATTN_F32) launch_paged_f32(first, nf, D, causal, st);
+    else launch_paged_fwd(first, nf, dt, D, causal, st);
+  });
   return launch_status();
 }
 

@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "paged.h"
+#include "rel.h"
 
 namespace sigattn {
 
@@ -33,8 +34,8 @@ template <int D, int NW> using DecodeTiles = uint16_t[NW][2][32 * D];
 template <int NW, bool SCOREMOD> using DecodeTerms = float[SCOREMOD ? NW : 1][2][64];
 
 // The units of workgroup `wg`, on its first NW waves.
-template <typename T, int D, int NW, bool CAUSAL, bool SCOREMOD>
-__device__ __forceinline__ void paged_decode_body(const PagedParams &p, const int wg, DecodeTiles<D, NW> &sK,
+template <typename T, int D, int NW, bool CAUSAL, bool SCOREMOD, class P>
+__device__ __forceinline__ void paged_decode_body(const P &p, const int wg, DecodeTiles<D, NW> &sK,
                                                   DecodeTiles<D, NW> &sV, DecodeTerms<NW, SCOREMOD> &sM) {
   constexpr int KB = 32;  // keys per block
   constexpr int NKS = D / 16, NDB = D / 32;
@@ -69,6 +70,12 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams &p, const in
   }
   // Keys of the chunk that this lane's token sees, and that every token sees.
   const int lim = un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0, all_see = un.Lk - un.Lq + 1 - un.k0;
+
+  [[maybe_unused]] RelColumn rc;
+  if constexpr (P::kRel) {
+    const int col = min(l32, cols - 1), t = col / p.G;
+    rc.init(p, un.hk * p.G + col - t * p.G, un.Lk - un.Lq + t - un.k0, bias);
+  }
 
   f32x16 acc[1][NDB];
 #pragma unroll
@@ -113,8 +120,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams &p, const in
     const uint16_t *tK = sK[w][i & 1], *tV = sV[w][i & 1];
     f32x16 sc = zero16();
     float c[16];
+    if constexpr (P::kRel) rc.block(KB * i, hi, c);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < (P::kRel ? 0 : 4); ++g) {
       f32x4 m = {nbl, nbl, nbl, nbl};
       if (SCOREMOD) {
         const f32x4 x = *(const f32x4 *)&sM[w][i & 1][8 * g + 4 * hi];

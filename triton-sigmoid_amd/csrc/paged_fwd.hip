@@ -9,67 +9,11 @@
 // Bound by its products and sigmoids as the forward is: 2 x 1024 tokens on 5000 ..
 // 12000 keys bf16 H=32 Hkv=8 D=128 319 us, 1.02 PFLOP/s (matrix cores busy 48 % of
 // the time; HBM 0.36 TB/s, a group's heads and its blocks share what L2 holds).
-#include "fwd_kernel.h"
 #include "launch.h"
-#include "paged_decode.h"
+#include "paged_launch.h"
 
 namespace sigattn {
 namespace {
-
-// D = 128: eight waves, one workgroup per CU; below, four, three and four per
-// CU (fwd_kernel.h).
-constexpr int waves_of(int D) { return D == 128 ? 8 : 4; }
-
-template <typename T, int D> void fwd_t(const PagedParams &p, int units, bool causal, hipStream_t st) {
-  constexpr int NWV = waves_of(D);
-  const dim3 grid((unsigned)(units + p.ngap[0])), block(64 * NWV);
-  if (causal) {
-    if (p.score_mod) fwd_mfma_kernel<T, D, NWV, 1, 1, true, true, PagedParams><<<grid, block, 0, st>>>(p);
-    else fwd_mfma_kernel<T, D, NWV, 1, 1, true, false, PagedParams><<<grid, block, 0, st>>>(p);
-  } else {
-    if (p.score_mod) fwd_mfma_kernel<T, D, NWV, 1, 1, false, true, PagedParams><<<grid, block, 0, st>>>(p);
-    else fwd_mfma_kernel<T, D, NWV, 1, 1, false, false, PagedParams><<<grid, block, 0, st>>>(p);
-  }
-}
-
-// Batches with sequences of both kernels: the first nf workgroups (after the gap
-// ones) run blocks of columns, the others decode, so that the longer part's
-// last workgroups run beside the shorter part's, and a launch less.  The parts
-// share their LDS; at D = 64 decoding takes three waves, which fit what three
-// workgroups of a CU leave each, and everywhere as many as the LDS holds.
-// fp16 H=12 Hkv=4 D=64, 20 requests of a token and 4 of 100 .. 700 on up to 4096
-// keys: 38 us (the whole call 41; when it was two launches, one after the other,
-// 11 more).
-template <int D> constexpr int mixed_waves() { return D == 64 ? 3 : 4; }
-template <typename T, int D, bool CAUSAL, bool SCOREMOD>
-__global__ __launch_bounds__(64 * waves_of(D), (fwd_occupancy<D, 1, 1>())) void paged_mixed_kernel(
-    const PagedParams pf, const PagedParams pd, const int nf) {
-  constexpr int NW = mixed_waves<D>();
-  __shared__ __attribute__((aligned(16))) FwdTiles<D, 1> sK, sV;
-  __shared__ __attribute__((aligned(16))) FwdTerms<D, 1, SCOREMOD> sC;
-  __shared__ __attribute__((aligned(16))) DecodeTerms<NW, SCOREMOD> sM;
-  static_assert(sizeof(sK) == sizeof(DecodeTiles<D, NW>), "the parts share their tiles");
-  const int wg = gap_prologue<2>(pf, sK);
-  if (wg < 0) return;
-  if (wg < nf)
-    fwd_mfma_body<T, D, waves_of(D), 1, 1, CAUSAL, SCOREMOD, PagedParams>(pf, wg, sK, sV, sC);
-  else
-    paged_decode_body<T, D, NW, CAUSAL, SCOREMOD>(pd, wg - nf, reinterpret_cast<DecodeTiles<D, NW> &>(sK),
-                                                  reinterpret_cast<DecodeTiles<D, NW> &>(sV), sM);
-}
-
-template <typename T, int D>
-void mixed_t(const PagedParams &pf, int nf, const PagedParams &pd, int nd, bool causal, hipStream_t st) {
-  constexpr int NW = mixed_waves<D>();
-  const dim3 grid((unsigned)(nf + (nd + NW - 1) / NW + pf.ngap[0])), block(64 * waves_of(D));
-  if (causal) {
-    if (pf.score_mod) paged_mixed_kernel<T, D, true, true><<<grid, block, 0, st>>>(pf, pd, nf);
-    else paged_mixed_kernel<T, D, true, false><<<grid, block, 0, st>>>(pf, pd, nf);
-  } else {
-    if (pf.score_mod) paged_mixed_kernel<T, D, false, true><<<grid, block, 0, st>>>(pf, pd, nf);
-    else paged_mixed_kernel<T, D, false, false><<<grid, block, 0, st>>>(pf, pd, nf);
-  }
-}
 
 // Output rows (token, query head) of cut sequences: the sum of the chunks'
 // partials in chunk order.  CG threads add CG * 4 columns of one row.  Many rows
@@ -146,17 +90,6 @@ template <typename T, int D> void reduce_t(const ReduceArgs &a, hipStream_t st) 
   const int64_t parts = rows * (D / 32);
   if (parts <= 8 * (int64_t)a.p.ncu) paged_reduce_kernel<T, D, false><<<dim3((unsigned)parts), dim3(256), 0, st>>>(a);
   else paged_reduce_kernel<T, D, true><<<dim3((unsigned)((rows + NG - 1) / NG)), dim3(256), 0, st>>>(a);
-}
-
-template <class F> void by_type(int dtype, int D, F &&f) {
-  const auto d = [&](auto *t) {
-    if (D == 128) f(t, std::integral_constant<int, 128>{});
-    else if (D == 64) f(t, std::integral_constant<int, 64>{});
-    else f(t, std::integral_constant<int, 32>{});
-  };
-  if (dtype == kBF16) d((__bf16 *)nullptr);
-  else if (dtype == kF16) d((_Float16 *)nullptr);
-  else d((float *)nullptr);
 }
 
 }  // namespace

@@ -138,13 +138,42 @@ inline PagedPlan make_plan(const sigattn_paged_problem *p, const PagedParams &k,
 }
 
 // k's fields for one part of a plan (part.split_units 0: nothing is cut).
-inline PagedParams of_part(const PagedParams &k, const PagedPart &part, int lo, int hi, int2 *cut, float *ws) {
-  PagedParams s = k;
+template <class P> P of_part(const P &k, const PagedPart &part, int lo, int hi, int2 *cut, float *ws) {
+  P s = k;
   s.cols_lo = lo, s.cols_hi = hi;
   s.split_units = part.split_units, s.total_units = part.total_units, s.min_chunk = part.min_chunk;
   s.max_units = (int)part.units;
   s.cut = cut, s.ws = ws;
   return s;
+}
+
+// The rows of `out` that no sequence covers.
+inline GapAxis paged_gap(const sigattn_paged_problem *p, const PagedParams &k, void *out) {
+  GapAxis gap;
+  gap.cu = p->cu_seqlens_q, gap.B = k.B, gap.T = k.Tq, gap.H = k.H, gap.D = (int)p->D;
+  gap.rows = p->rows_q, gap.st = p->H * p->D, gap.sh = p->D, gap.out[0] = out;
+  return gap;
+}
+
+// Runs a plan's parts, launch(first part's parameters, blocks, decoding part's
+// parameters, decoding units), and the sums of what they cut.  The workspace
+// (nullptr: the plan cuts nothing): both parts' cuts, then their partials.  P:
+// PagedParams, or with the learned bias.
+template <class P, class Launch>
+void run_plan(const sigattn_paged_problem *p, P k, const PagedPlan &pl, char *workspace, void *out, hipStream_t st,
+              Launch &&launch) {
+  const auto at = [&](size_t bytes) -> void * { return workspace != nullptr ? workspace + bytes : nullptr; };
+  k.gap[0] = paged_gap(p, k, out);
+  const P kf = of_part(k, pl.fwd, pl.cols_lo, INT_MAX, (int2 *)at(0), (float *)at(pl.cut_bytes));
+  const P kd = of_part(k, pl.decode, 0, pl.decode.units > 0 ? kDecodeCols : 0, (int2 *)at((size_t)p->B * sizeof(int2)),
+                       (float *)at(pl.cut_bytes + pl.fwd.partial_bytes));
+  // The kernel also zeroes the rows outside every sequence (workgroups in
+  // a multiple of 8, so that its items keep their XCDs).
+  P first = pl.fwd.units > 0 ? kf : kd;
+  first.ngap[0] = (int)(cdiv(cdiv(p->rows_q, 64), 8) * 8);
+  launch(first, (int)pl.fwd.units, kd, (int)pl.decode.units);
+  if (kf.split_units > 0 || kd.split_units > 0)
+    launch_paged_reduce(kf, kd, p->dtype, p->D == 16 ? 32 : (int)p->D, st);
 }
 
 }  // namespace sigattn

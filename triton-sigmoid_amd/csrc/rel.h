@@ -30,16 +30,61 @@ struct RelParams : KParams {
   }
 };
 
-// Over a paged cache: query i of n at position L - n + i (forward only).
+// Over a paged cache: query i of n at position L - n + i (forward only).  A lane of
+// the matrix kernels has a column, so a head and a position of its own: it reads the
+// values of a 32-key block itself, from a line with kRelPad places more on either
+// side, so that the block's first place is all that is clamped.  Blocks that lie
+// beyond the line's end for every lane, nearly all of a long context, cost nothing:
+// their value is the lane's constant.
+constexpr int kRelPad = 64;
 struct PagedRelParams : PagedParams {
   static constexpr bool kRel = true;
-  const float *line;
+  const float *line;  // [H, 2 reach + 1 + 2 kRelPad], places from the padding's first
   int reach;
+
+  __device__ __forceinline__ const float *row(int h) const {
+    return line + (int64_t)h * (2 * reach + 1 + 2 * kRelPad) + kRelPad + reach;
+  }
+};
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// What a lane's scores have added beyond scale, times -log2(e), block by block.
+struct RelColumn {
+  const float *row;  // relative position 0
+  float nbl, ends[2];
+  int reach, pos;    // the query's position, from the chunk's first key
+  __device__ __forceinline__ void init(const PagedRelParams &p, int h, int position, float bias) {
+    row = p.row(h), reach = p.reach, pos = position;
+    nbl = -bias * kLog2e;
+    ends[0] = __builtin_fmaf(row[-reach], -kLog2e, nbl), ends[1] = __builtin_fmaf(row[reach], -kLog2e, nbl);
+  }
+  // The 32-key block from key `first` on, 16 keys of this half of the wave; `n` of
+  // them (2 or 16) are wanted.
+  template <int N> __device__ __forceinline__ void block(int first, int hi, float (&c)[N]) const {
+    const int d = first - pos;  // of the block's first key
+    const bool before = d + 31 <= -reach, after = d >= reach;
+    if (__all(before || after)) {
+      const float x = before ? ends[0] : ends[1];
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[i] = x;
+      return;
+    }
+    const float *at = row + min(max(d, -reach - 32), reach) + 4 * hi;
+#pragma unroll
+    for (int g = 0; g < (N + 3) / 4; ++g) {
+      const f32x4 v = *(const f32x4_any *)(at + 8 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * g + j < N) c[4 * g + j] = __builtin_fmaf(v[j], -kLog2e, nbl);
+    }
+  }
 };
 
 // Value of query head h at relative position d.
 template <class P> __device__ __forceinline__ float rel_at(const P &p, int h, int d) {
-  if constexpr (P::kRel) return p.line[(int64_t)h * (2 * p.reach + 1) + p.reach + min(max(d, -p.reach), p.reach)];
+  if constexpr (P::kRel && P::kPaged) return p.row(h)[min(max(d, -p.reach), p.reach)];
+  else if constexpr (P::kRel) return p.line[(int64_t)h * (2 * p.reach + 1) + p.reach + min(max(d, -p.reach), p.reach)];
   else return 0.0f;
 }
 
@@ -49,6 +94,9 @@ struct RelTable {
   const void *table;
   const int32_t *bucket;
   int dtype, buckets, max_distance, H, reach;
+  int pad;  // places of the lines before -reach and after reach
+
+  __host__ __device__ __forceinline__ int places() const { return 2 * (reach + pad) + 1; }
 };
 
 // The host's side: the caller's table for H heads and two lengths (reach: no two
@@ -66,10 +114,10 @@ inline RelTable rel_table(const sigattn_rel_bias *r, int64_t H, int64_t Tq, int6
   return t;
 }
 inline int64_t rel_line_bytes(const RelTable &t) {
-  return ((int64_t)t.H * (2 * t.reach + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
+  return ((int64_t)t.H * t.places() * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
-// line [H, 2 reach + 1] from the table.
+// line [H, places] from the table.
 void launch_rel_line(const RelTable &t, float *line, hipStream_t st);
 // The table's gradient (`grad`, the table's type) from the dQ kernels' sums in
 // p.part (nullptr: zeros); sums: [H, 2 reach + 1] floats of scratch.
@@ -90,6 +138,12 @@ constexpr int kGenericRows = 64;
 void launch_rel_fwd_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
 void launch_rel_dq_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
 void launch_rel_dkdv_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+// MFMA kernels over a paged cache, as launch_paged_fwd, launch_paged_decode and
+// launch_paged_mixed (paged.h).
+void launch_paged_rel_fwd(const PagedRelParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
+void launch_paged_rel_decode(const PagedRelParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
+void launch_paged_rel_mixed(const PagedRelParams &pf, int nf, const PagedRelParams &pd, int nd, int dtype, int D, bool causal,
+                            hipStream_t st);
 void launch_paged_rel_generic(const PagedRelParams &p, int dtype, int D, bool causal, hipStream_t st);
 
 }  // namespace sigattn

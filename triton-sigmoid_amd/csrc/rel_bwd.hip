@@ -11,7 +11,7 @@ template <typename T, int D, int WK, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelParams p) {
   __shared__ __attribute__((aligned(16))) DqLds<D, false, dq_window<RelParams, WK>()> lds;
   __shared__ unsigned long long gap_lds[2];
-  extern __shared__ float near[];  // the four waves' lines
+  extern __shared__ __attribute__((aligned(16))) float near[];  // the four waves' lines and pieces
   const int wg = gap_prologue<2>(p, gap_lds);
   if (wg >= 0) bwd_dq_body<T, D, WK, CAUSAL, false, RelParams>(p, wg, lds, near);
 }
@@ -27,7 +27,7 @@ template <typename T, int D, int WK> void dq_w(const RelParams &kp, bool causal,
   p.part_rows = 128 / WK;
   p.nblk = (p.Tq + p.part_rows - 1) / p.part_rows;
   const dim3 grid((unsigned)(p.nblk * p.B * p.H + p.ngap[0] + p.ngap[1]));
-  const size_t line = p.part != nullptr ? 4 * near_places(p.reach) * sizeof(float) : 0;
+  const size_t line = p.part != nullptr ? near_floats(p.reach) * sizeof(float) : 0;
   if (causal) rel_dq_kernel<T, D, WK, true><<<grid, 256, line, st>>>(p);
   else rel_dq_kernel<T, D, WK, false><<<grid, 256, line, st>>>(p);
 }

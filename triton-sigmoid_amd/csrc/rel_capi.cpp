@@ -28,9 +28,13 @@ RelParams rel_kv_items(const RelParams &k) {
 
 // The learned bias's table as far as the cache's sequences reach.
 RelTable rel_table_of(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
-  return rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q,
-                            p->max_pages * p->page_size);
+  RelTable t = rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q, p->max_pages * p->page_size);
+  t.pad = kRelPad;
+  return t;
 }
+
+// The matrix kernels with the bias: f16 / bf16.
+bool paged_mfma(const sigattn_paged_problem *p, const void *out) { return p->dtype != SIGATTN_F32 && use_mfma(p, out); }
 
 }  // namespace
 
@@ -155,7 +159,8 @@ int sigattn_paged_rel_check(const sigattn_paged_problem *p, const sigattn_rel_bi
 
 size_t sigattn_paged_rel_fwd_workspace_bytes(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
   if (sigattn_paged_rel_check(p, r) != SIGATTN_OK || p->rows_q == 0 || p->H == 0 || p->B == 0) return 0;
-  return (size_t)rel_line_bytes(rel_table_of(p, r));
+  const size_t plan = paged_mfma(p, nullptr) ? make_plan(p, make_params(p, nullptr), kernel_dim(p)).bytes : 0;
+  return (size_t)rel_line_bytes(rel_table_of(p, r)) + plan;
 }
 
 int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
@@ -165,15 +170,28 @@ int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias
   if (p->rows_q == 0 || p->H == 0 || p->B == 0) return sigattn_paged_fwd(p, out, nullptr, 0, stream);
   if (out == nullptr) return SIGATTN_ERR_NULL_ARG;
   const RelTable t = rel_table_of(p, r);
-  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < rel_line_bytes(t))
-    return SIGATTN_ERR_WORKSPACE;
-  const hipStream_t st = (hipStream_t)stream;
   PagedRelParams k{};
   (PagedParams &)k = make_params(p, out);
+  const bool mfma = paged_mfma(p, out), causal = p->causal != 0;
+  const int D = kernel_dim(p);
+  PagedPlan pl;
+  if (mfma) pl = make_plan(p, k, D);
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < (size_t)rel_line_bytes(t) + pl.bytes)
+    return SIGATTN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
   k.line = (const float *)workspace, k.reach = t.reach;
   (void)hipGetLastError();
   launch_rel_line(t, (float *)workspace, st);
-  launch_paged_rel_generic(k, p->dtype, (int)p->D, p->causal != 0, st);
+  if (!mfma) {
+    launch_paged_rel_generic(k, p->dtype, (int)p->D, causal, st);
+    return launch_status();
+  }
+  run_plan(p, k, pl, (char *)workspace + rel_line_bytes(t), out, st,
+           [&](const PagedRelParams &first, int nf, const PagedRelParams &kd, int nd) {
+             if (nf > 0 && nd > 0) launch_paged_rel_mixed(first, nf, kd, nd, p->dtype, D, causal, st);
+             else if (nd > 0) launch_paged_rel_decode(first, nd, p->dtype, D, causal, st);
+             else launch_paged_rel_fwd(first, nf, p->dtype, D, causal, st);
+           });
   return launch_status();
 }
 
