@@ -27,6 +27,7 @@
 // kernels live here.
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -64,6 +65,14 @@ struct Api {
   decltype(&sigattn_paged_write) paged_write = nullptr;
   decltype(&sigattn_paged_fwd_workspace_bytes) paged_fwd_workspace_bytes = nullptr;
   decltype(&sigattn_paged_fwd) paged_fwd = nullptr;
+  decltype(&sigattn_rel_fwd_workspace_bytes) rel_fwd_workspace_bytes = nullptr;
+  decltype(&sigattn_rel_fwd) rel_fwd = nullptr;
+  decltype(&sigattn_rel_bwd_workspace_bytes) rel_bwd_workspace_bytes = nullptr;
+  decltype(&sigattn_rel_bwd) rel_bwd = nullptr;
+  decltype(&sigattn_paged_rel_fwd_workspace_bytes) paged_rel_fwd_workspace_bytes = nullptr;
+  decltype(&sigattn_paged_rel_fwd) paged_rel_fwd = nullptr;
+  decltype(&sigattn_rotary_apply) rotary_apply = nullptr;
+  decltype(&sigattn_paged_write_rotary) paged_write_rotary = nullptr;
 };
 Api g_api;
 bool g_bound = false;
@@ -262,6 +271,123 @@ struct SigattnNode : public torch::autograd::Function<SigattnNode> {
   }
 };
 
+hipStream_t stream_of(const at::Device &dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
+
+// Gradients that have none of their own: a backward through them is an error, as
+// torch.autograd.function.once_differentiable makes it.
+void differentiable_once(tensor_list &grads) {
+  if (!at::GradMode::is_enabled()) return;
+  tensor_list outs;
+  for (const Tensor &g : grads)
+    if (g.defined()) outs.push_back(g.detach().requires_grad_());
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", outs.size());
+  const tensor_list marked = (*error)(tensor_list(outs));
+  size_t at = 0;
+  for (Tensor &g : grads)
+    if (g.defined()) g = marked[at++];
+}
+
+// The learned bias's struct over a contiguous table [num_buckets, H] and int32 buckets.
+sigattn_rel_bias make_rel(const Tensor &table, const Tensor &buckets) {
+  sigattn_rel_bias r;
+  std::memset(&r, 0, sizeof(r));
+  r.dtype = dtype_code(table);
+  r.num_buckets = (int32_t)table.size(0);
+  r.max_distance = buckets.numel() / 2;
+  r.table = table.data_ptr();
+  r.buckets = static_cast<const int32_t *>(buckets.data_ptr());
+  return r;
+}
+
+// sigmoid_attention_varlen with the learned bias, at least one sequence and one row.
+struct RelNode : public torch::autograd::Function<RelNode> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table,
+                        const Tensor &buckets, const Tensor &bias, const Tensor &scale, const Tensor &cu_q,
+                        const Tensor &cu_k, int64_t max_q, int64_t max_k, bool causal) {
+    const Layout lay{Tensor(), Tensor(), cu_q, cu_k, max_q, max_k};
+    ctx->save_for_backward({q, k, v, table, buckets, bias, scale, cu_q, cu_k});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["max_q"] = max_q;
+    ctx->saved_data["max_k"] = max_k;
+    const Tensor out = at::empty_like(q);
+    const c10::DeviceGuard guard(q.device());
+    const sigattn_problem p = make_problem(q, k, v, bias, Tensor(), scale, lay, causal);
+    const sigattn_rel_bias r = make_rel(table, buckets);
+    const int64_t nbytes = (int64_t)g_api.rel_fwd_workspace_bytes(&p, &r);
+    const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
+    check_rc(g_api.rel_fwd(&p, &r, out.data_ptr(), ws.data_ptr(), nbytes, stream_of(q.device())), "sigattn_rel_fwd");
+    return out;
+  }
+
+  static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &buckets = saved[4];
+    const Layout lay{Tensor(), Tensor(), saved[7], saved[8], ctx->saved_data["max_q"].toInt(),
+                     ctx->saved_data["max_k"].toInt()};
+    Tensor dout = grads[0];
+    if (dout.scalar_type() != q.scalar_type() || dout.device() != q.device() || !dout.is_contiguous())
+      dout = dout.to(q.device(), q.scalar_type()).contiguous();
+    TORCH_CHECK(dout.sizes() == q.sizes(), "dO shape ", dout.sizes(), " != Q shape ", q.sizes());
+    tensor_list result(12);
+    const bool want_table = ctx->needs_input_grad(3);
+    result[0] = at::empty_like(q), result[1] = at::empty_like(k), result[2] = at::empty_like(v);
+    if (want_table) result[3] = at::empty_like(table);
+    const c10::DeviceGuard guard(q.device());
+    const sigattn_problem p = make_problem(q, k, v, saved[5], Tensor(), saved[6], lay, ctx->saved_data["causal"].toBool());
+    const sigattn_rel_bias r = make_rel(table, buckets);
+    const int64_t nbytes = (int64_t)g_api.rel_bwd_workspace_bytes(&p, &r);
+    const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
+    check_rc(g_api.rel_bwd(&p, &r, dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
+                           want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes, stream_of(q.device())),
+             "sigattn_rel_bwd");
+    differentiable_once(result);
+    return result;
+  }
+};
+
+// The rotary struct over rows [N, heads, D] of any strides but the last.
+sigattn_rotary make_rotary(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &angles, bool pairs) {
+  sigattn_rotary r;
+  std::memset(&r, 0, sizeof(r));
+  r.dtype = dtype_code(q);
+  r.interleaved = pairs;
+  r.rows = q.size(0), r.q_heads = q.size(1), r.kv_heads = k.size(1), r.D = q.size(2);
+  r.rot_dim = angles.size(1), r.num_positions = angles.size(0);
+  r.q_stride_t = q.stride(0), r.q_stride_h = q.stride(1), r.k_stride_t = k.stride(0), r.k_stride_h = k.stride(1);
+  r.q = q.data_ptr(), r.k = k.data_ptr();
+  r.positions = static_cast<const int32_t *>(positions.data_ptr());
+  r.angles = static_cast<const float *>(angles.data_ptr());
+  return r;
+}
+
+Tensor unit_stride(const Tensor &t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// rotary_embedding of rows [N, heads, D]; its backward is itself, back.
+struct RotaryNode : public torch::autograd::Function<RotaryNode> {
+  static tensor_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &positions,
+                             const Tensor &angles, bool pairs, bool inverse) {
+    ctx->save_for_backward({positions, angles});
+    ctx->saved_data["pairs"] = pairs;
+    ctx->saved_data["inverse"] = inverse;
+    const c10::DeviceGuard guard(q.device());
+    const Tensor a = unit_stride(q), b = unit_stride(k);
+    const Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    sigattn_rotary r = make_rotary(a, b, positions, angles, pairs);
+    r.inverse = inverse;
+    r.q_out = qo.data_ptr(), r.k_out = ko.data_ptr();
+    check_rc(g_api.rotary_apply(&r, stream_of(q.device())), "sigattn_rotary_apply");
+    return {qo, ko};
+  }
+
+  static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const tensor_list g = RotaryNode::apply(grads[0], grads[1], saved[0], saved[1], ctx->saved_data["pairs"].toBool(),
+                                            !ctx->saved_data["inverse"].toBool());
+    return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &bias,
                  const std::optional<Tensor> &score_mod, const Tensor &scale,
                  const std::optional<Tensor> &seq_lens_q, const std::optional<Tensor> &seq_lens_k, bool causal,
@@ -413,13 +539,22 @@ py::object quick(const py::object &query, const py::object &key, const py::objec
                                      std::nullopt, std::nullopt, 0, 0));
 }
 
+// The learned bias's tensors as the kernels take them.
+bool quick_table(const py::object &table, const py::object &buckets, int64_t H, const at::Device &dev, Tensor &t,
+                 Tensor &u) {
+  return Quick::tensor(table, t) && t.dim() == 2 && t.size(1) == H && t.size(0) >= 1 &&
+         t.size(0) <= SIGATTN_REL_MAX_BUCKETS && Quick::float_type(t) && t.device() == dev &&
+         Quick::ints(buckets, u, 1, dev) && u.numel() % 2 == 1 && u.numel() <= 2 * SIGATTN_REL_MAX_DISTANCE + 1;
+}
+
 // sigmoid_attention_varlen on canonical arguments, or None.
 py::object quick_varlen(const py::object &query, const py::object &key, const py::object &value,
                         const py::object &cu_seqlens_q, const py::object &cu_seqlens_k, const py::object &max_seqlen_q,
                         const py::object &max_seqlen_k, const py::object &is_causal, const py::object &scale,
-                        const py::object &sigmoid_bias, const py::object &score_mod) {
+                        const py::object &sigmoid_bias, const py::object &score_mod, const py::object &bias_table,
+                        const py::object &bias_buckets) {
   const py::object no = py::none();
-  Tensor q, k, v, sm, cq, ck;
+  Tensor q, k, v, sm, cq, ck, table, buckets;
   int64_t mq = 0, mk = 0;
   if (!g_bound || Quick::observed() || std::getenv("SIGATTN_EAGER_BINDING") != nullptr ||
       std::getenv("SIGATTN_BWD_WORKSPACE_MB") != nullptr || !Quick::tensor(query, q) || !Quick::tensor(key, k) ||
@@ -438,6 +573,8 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
   if (!score_mod.is_none() && (!Quick::tensor(score_mod, sm) || sm.scalar_type() != at::kFloat || sm.device() != dev ||
                                sm.dim() != 1 || sm.size(0) != k.size(0)))
     return no;
+  const bool rel = !bias_table.is_none() || !bias_buckets.is_none();
+  if (rel && (sm.defined() || !quick_table(bias_table, bias_buckets, H, dev, table, buckets))) return no;
   double s = 1.0 / std::sqrt((double)D), bias_value = 0.0;
   if (!scale.is_none() && !Quick::number(scale, s)) return no;
   const bool own_bias = !sigmoid_bias.is_none();
@@ -459,6 +596,7 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
                                 static_cast<float *>(bias.data_ptr()), stream),
              "sigattn_default_bias");
   }
+  if (rel) return py::cast(RelNode::apply(q, k, v, table, buckets, bias, st, cq, ck, mq, mk, is_causal.ptr() == Py_True));
   const int64_t limit = (int64_t)(H == Hkv ? 2048 : 8192) << 20;  // _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB
   return py::cast(SigattnNode::apply(q, k, v, bias, sm.defined() ? std::optional<Tensor>(sm) : std::nullopt, st,
                                      std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
@@ -541,9 +679,10 @@ bool quick_write(const py::object &key, const py::object &value, const py::objec
 py::object quick_paged(const py::object &query, const py::object &key_cache, const py::object &value_cache,
                        const py::object &block_table, const py::object &seq_lens_k, const py::object &cu_seqlens_q,
                        const py::object &max_seqlen_q, const py::object &is_causal, const py::object &scale,
-                       const py::object &sigmoid_bias, const py::object &score_mod) {
+                       const py::object &sigmoid_bias, const py::object &score_mod, const py::object &bias_table,
+                       const py::object &bias_buckets) {
   const py::object no = py::none();
-  Tensor q, kc, vc, table, lens, cu, sm;
+  Tensor q, kc, vc, table, lens, cu, sm, learned, buckets;
   if (!Quick::usable() || !Quick::strided(query, q) || !quick_caches(key_cache, value_cache, kc, vc) ||
       !Quick::strided(block_table, table) || !PyBool_Check(is_causal.ptr()))
     return no;
@@ -564,7 +703,9 @@ py::object quick_paged(const py::object &query, const py::object &key_cache, con
   if (!scale.is_none() && !Quick::number(scale, s)) return no;
   const bool own_bias = !sigmoid_bias.is_none();
   if (own_bias && !Quick::number(sigmoid_bias, bias)) return no;
-  if (!Quick::no_grad({&q, &kc, &vc, &sm})) return no;
+  const bool rel = !bias_table.is_none() || !bias_buckets.is_none();
+  if (rel && (sm.defined() || !quick_table(bias_table, bias_buckets, q.size(1), dev, learned, buckets))) return no;
+  if (!Quick::no_grad({&q, &kc, &vc, &sm, &learned})) return no;
   sigattn_paged_problem p;
   std::memset(&p, 0, sizeof(p));
   p.abi_version = SIGATTN_ABI_VERSION;
@@ -583,10 +724,88 @@ py::object quick_paged(const py::object &query, const py::object &key_cache, con
   p.own_bias = own_bias, p.causal = is_causal.ptr() == Py_True;
   const c10::DeviceGuard guard(dev);
   const Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  if (rel) {
+    const sigattn_rel_bias r = make_rel(learned, buckets);
+    const int64_t nbytes = (int64_t)g_api.paged_rel_fwd_workspace_bytes(&p, &r);
+    const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte).requires_grad(false));
+    check_rc(g_api.paged_rel_fwd(&p, &r, out.data_ptr(), ws.data_ptr(), nbytes, stream_of(dev)), "sigattn_paged_rel_fwd");
+    return py::cast(out);
+  }
   const Tensor ws = workspace((int64_t)g_api.paged_fwd_workspace_bytes(&p), q);  // without it: unsplit
   check_rc(g_api.paged_fwd(&p, out.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
                            c10::hip::getCurrentHIPStream(dev.index()).stream()),
            "sigattn_paged_fwd");
+  return py::cast(out);
+}
+
+// A [positions, rot_dim] table of angles, and positions of `rows` rows.
+bool quick_angles(const py::object &positions, const py::object &angles, int64_t rows, int64_t D, const at::Device &dev,
+                  Tensor &p, Tensor &a) {
+  return Quick::tensor(positions, p) && p.scalar_type() == at::kInt && p.device() == dev && p.numel() == rows &&
+         Quick::tensor(angles, a) && a.dim() == 2 && a.scalar_type() == at::kFloat && a.device() == dev &&
+         a.size(0) >= 1 && a.size(1) >= 2 && a.size(1) % 2 == 0 && a.size(1) <= D;
+}
+
+bool rotary_dim(int64_t D) { return D == 16 || D == 32 || D == 64 || D == 128; }
+
+// t as rows [N, heads, D] where its batches follow one another; undefined else.
+Tensor as_rows(const Tensor &t) {
+  if (t.dim() == 3) return t;
+  const int64_t B = t.size(0), T = t.size(1);
+  if (B > 1 && t.stride(0) != T * t.stride(1)) return Tensor();
+  return t.flatten(0, 1);
+}
+
+py::object quick_rotary(const py::object &query, const py::object &key, const py::object &positions,
+                        const py::object &angles, const py::object &interleaved) {
+  const py::object no = py::none();
+  Tensor q, k, at, table;
+  if (!Quick::usable() || !Quick::strided(query, q) || !Quick::strided(key, k) || !PyBool_Check(interleaved.ptr()) ||
+      (q.dim() != 3 && q.dim() != 4) || k.dim() != q.dim() || !Quick::float_type(q) || k.scalar_type() != q.scalar_type() ||
+      !q.is_cuda() || k.device() != q.device() || !Quick::gfx950(q.device().index()) || q.size(-1) != k.size(-1) ||
+      !rotary_dim(q.size(-1)) || q._fw_grad(0).defined() || k._fw_grad(0).defined())
+    return no;
+  for (int64_t i = 0; i + 2 < q.dim(); ++i)
+    if (q.size(i) != k.size(i)) return no;
+  const int64_t rows = q.dim() == 3 ? q.size(0) : q.size(0) * q.size(1);
+  if (!quick_angles(positions, angles, rows, q.size(-1), q.device(), at, table) || at.dim() != q.dim() - 2 ||
+      at.size(0) != q.size(0))
+    return no;
+  const Tensor a = as_rows(q), b = as_rows(k);
+  if (!a.defined() || !b.defined()) return no;
+  const tensor_list got = RotaryNode::apply(a, b, at, table, interleaved.ptr() == Py_True, false);
+  if (q.dim() == 3) return py::make_tuple(got[0], got[1]);
+  return py::make_tuple(got[0].view(q.sizes()), got[1].view(k.sizes()));
+}
+
+py::object quick_write_rotary(const py::object &query, const py::object &key, const py::object &value,
+                              const py::object &key_cache, const py::object &value_cache, const py::object &slot_mapping,
+                              const py::object &positions, const py::object &angles, const py::object &interleaved) {
+  const py::object no = py::none();
+  Tensor q, k, v, kc, vc, slots, at, table;
+  if (!Quick::usable() || !quick_caches(key_cache, value_cache, kc, vc) || !Quick::strided(query, q) ||
+      !Quick::strided(key, k) || !Quick::strided(value, v) || !PyBool_Check(interleaved.ptr()))
+    return no;
+  const at::Device dev = kc.device();
+  const at::ScalarType type = kc.scalar_type();
+  if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || k.strides() != v.strides() || q.scalar_type() != type ||
+      k.scalar_type() != type || v.scalar_type() != type || q.device() != dev || k.device() != dev || v.device() != dev ||
+      q.size(0) != k.size(0) || q.size(2) != k.size(2) || k.size(1) != kc.size(2) || k.size(2) != kc.size(3) ||
+      !rotary_dim(k.size(2)) || !Quick::ints(slot_mapping, slots, 1, dev) || slots.size(0) != k.size(0) ||
+      !quick_angles(positions, angles, k.size(0), k.size(2), dev, at, table) || at.dim() != 1 ||
+      !Quick::no_grad({&q, &k, &v, &kc, &vc, &table}))
+    return no;
+  for (int i = 0; i < 3; ++i)
+    if (kc.size(i) > 1 && kc.stride(i) == 0) return no;
+  const c10::DeviceGuard guard(dev);
+  const Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  sigattn_rotary r = make_rotary(q, k, at, table, interleaved.ptr() == Py_True);
+  r.cache_stride_p = kc.stride(0), r.cache_stride_t = kc.stride(1), r.cache_stride_h = kc.stride(2);
+  r.num_pages = kc.size(0), r.page_size = kc.size(1);
+  r.v = v.data_ptr(), r.q_out = out.data_ptr(), r.k_cache = kc.data_ptr(), r.v_cache = vc.data_ptr();
+  r.slot_mapping = static_cast<const int32_t *>(slots.data_ptr());
+  check_rc(g_api.paged_write_rotary(&r, stream_of(dev)), "sigattn_paged_write_rotary");
+  changed(kc), changed(vc);
   return py::cast(out);
 }
 
@@ -611,6 +830,14 @@ void bind(const py::dict &fns, const std::vector<int64_t> &two_pass_dims, int64_
   bind_one(api.paged_write, fns, "sigattn_paged_write");
   bind_one(api.paged_fwd_workspace_bytes, fns, "sigattn_paged_fwd_workspace_bytes");
   bind_one(api.paged_fwd, fns, "sigattn_paged_fwd");
+  bind_one(api.rel_fwd_workspace_bytes, fns, "sigattn_rel_fwd_workspace_bytes");
+  bind_one(api.rel_fwd, fns, "sigattn_rel_fwd");
+  bind_one(api.rel_bwd_workspace_bytes, fns, "sigattn_rel_bwd_workspace_bytes");
+  bind_one(api.rel_bwd, fns, "sigattn_rel_bwd");
+  bind_one(api.paged_rel_fwd_workspace_bytes, fns, "sigattn_paged_rel_fwd_workspace_bytes");
+  bind_one(api.paged_rel_fwd, fns, "sigattn_paged_rel_fwd");
+  bind_one(api.rotary_apply, fns, "sigattn_rotary_apply");
+  bind_one(api.paged_write_rotary, fns, "sigattn_paged_write_rotary");
   TORCH_CHECK(dq_ds_rows > 0, "_sigattn_autograd.bind: dq_ds_rows must be positive");
   g_api = api;
   g_two_pass_dims = two_pass_dims;
@@ -633,6 +860,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("quick_plan", &quick_plan, "paged_plan's new tensors on canonical arguments, or None");
   m.def("quick_write", &quick_write, "paged_cache_write on canonical arguments: whether it took the call");
   m.def("quick_paged", &quick_paged, "sigmoid_attention_paged on canonical arguments, or None");
+  m.def("quick_rotary", &quick_rotary, "rotary_embedding on canonical arguments, or None");
+  m.def("quick_write_rotary", &quick_write_rotary, "paged_cache_write_rotary on canonical arguments, or None");
   m.def("attention", &attention,
         "Forward with autograd; arguments are the canonical tensors of _capi._prepare (and _prepare_packed "
         "for the packed layout, with the longest sequences)",

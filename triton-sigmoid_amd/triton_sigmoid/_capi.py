@@ -271,12 +271,15 @@ _AUTOGRAD_FNS = ("sigattn_strerror", "sigattn_fwd_workspace_bytes", "sigattn_fwd
                  "sigattn_fwd_decode_workspace_bytes", "sigattn_fwd_decode",
                  "sigattn_bwd_workspace_bytes", "sigattn_bwd_ws", "sigattn_bwd_split_workspace_bytes",
                  "sigattn_bwd_split", "sigattn_default_bias", "sigattn_paged_plan", "sigattn_paged_write",
-                 "sigattn_paged_fwd_workspace_bytes", "sigattn_paged_fwd")
+                 "sigattn_paged_fwd_workspace_bytes", "sigattn_paged_fwd", "sigattn_rel_fwd_workspace_bytes",
+                 "sigattn_rel_fwd", "sigattn_rel_bwd_workspace_bytes", "sigattn_rel_bwd",
+                 "sigattn_paged_rel_fwd_workspace_bytes", "sigattn_paged_rel_fwd", "sigattn_rotary_apply",
+                 "sigattn_paged_write_rotary")
 _autograd = None  # the bound module, or False after a failed import
 # The node's entries for eager calls with canonical arguments (None until the
 # node is bound): the call's result, or None where it does not take it.
 quick = None
-quick_module = None  # the module with quick_varlen, quick_plan, quick_write and quick_paged
+quick_module = None  # the module with quick_varlen, quick_plan, quick_write, quick_paged, quick_rotary, quick_write_rotary
 
 
 def autograd_node():

@@ -465,10 +465,10 @@ def sigmoid_attention_paged(
         Forward only: tensors that ask for a gradient (under grad mode) or
         carry a forward-mode tangent are refused.
     """
-    quick = _quick() if bias_table is None and bias_buckets is None else None
+    quick = _quick()
     if quick is not None:
         out = quick.quick_paged(query, key_cache, value_cache, block_table, seq_lens_k, cu_seqlens_q, max_seqlen_q,
-                                is_causal, scale, sigmoid_bias, score_mod)
+                                is_causal, scale, sigmoid_bias, score_mod, bias_table, bias_buckets)
         if out is not None:
             return out
     if query.dim() != 3:

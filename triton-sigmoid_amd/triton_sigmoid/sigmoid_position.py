@@ -218,7 +218,7 @@ def rotary_embedding(
         fp32 and rounded once).
     """
     quick = _quick()
-    if quick is not None and hasattr(quick, "quick_rotary"):
+    if quick is not None:
         got = quick.quick_rotary(query, key, positions, angles, interleaved)
         if got is not None:
             return got
@@ -302,7 +302,7 @@ def paged_cache_write_rotary(
         gradient (under grad mode) or carry a forward-mode tangent are refused.
     """
     quick = _quick()
-    if quick is not None and hasattr(quick, "quick_write_rotary"):
+    if quick is not None:
         got = quick.quick_write_rotary(query, key, value, key_cache, value_cache, slot_mapping, positions, angles,
                                        interleaved)
         if got is not None:

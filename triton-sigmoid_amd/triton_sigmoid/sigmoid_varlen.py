@@ -292,10 +292,9 @@ def sigmoid_attention_varlen(
     the output and in dQ / dK / dV (they take no part in the attention), so
     no gradient row is left uninitialised.
     """
-    plain = bias_table is None and bias_buckets is None
-    if plain and not torch.compiler.is_compiling() and _capi.quick_module is not None:
+    if not torch.compiler.is_compiling() and _capi.quick_module is not None:
         out = _capi.quick_module.quick_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
-                                              is_causal, scale, sigmoid_bias, score_mod)
+                                              is_causal, scale, sigmoid_bias, score_mod, bias_table, bias_buckets)
         if out is not None:
             return out
     if query.dim() != 3 or key.dim() != 3 or value.dim() != 3:
@@ -343,6 +342,8 @@ def sigmoid_attention_varlen(
     scale_tensor = _capi.device_constant((), float(scale), torch.float32, query.device)
     cu_seqlens_k, cu_seqlens_q = cu_seqlens_k.to(query.device), cu_seqlens_q.to(query.device)
     if rel is not None:
+        if not torch.compiler.is_compiling():
+            _capi.autograd_node()  # binds the module that takes canonical calls
         fn = sigmoid_attn_varlen_rel_fwd_op if torch.compiler.is_compiling() else _VarlenRelEager.apply
         return fn(query, key, value, *rel, cu_seqlens_k, cu_seqlens_q, int(max_seqlen_k), int(max_seqlen_q), bias,
                   scale_tensor, is_causal)
