@@ -29,7 +29,13 @@ template <typename T> __device__ __forceinline__ void rot_st(char *row, int i, f
   else ((uint16_t *)row)[i] = Elem<T>::from_f32(x);
 }
 
-// A workgroup per row, a thread per pair (or two copied columns).
+// (a, b) turned; one rounding each besides the first product's, in every kernel alike.
+__device__ __forceinline__ void turn_pair(float a, float b, float cs, float sn, float &u, float &w) {
+  u = __builtin_fmaf(-b, sn, a * cs), w = __builtin_fmaf(a, sn, b * cs);
+}
+
+// Any strides, alignment and rot_dim: a workgroup per row, a thread per pair (or two
+// copied columns).
 template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const int64_t t = blockIdx.x;
   const int half = a.rot / 2, dh = a.D / 2;
@@ -57,14 +63,114 @@ template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_
     const int y = turn && !PAIRS ? c + half : x + 1;
     float u = rot_ld<T>(src, x), w = rot_ld<T>(src, y);
     if (turn) {
-      const float cs = row[c], sn = row[c + half] * a.sign, v = u;
-      u = v * cs - w * sn, w = w * cs + v * sn;
+      const float p = u, q = w;
+      turn_pair(p, q, row[c], row[c + half] * a.sign, u, w);
     }
     rot_st<T>(dst, x, u), rot_st<T>(dst, y, w);
   }
 }
 
+// Rows on 16-byte boundaries: a thread's unit is two 16-byte pieces, E pairs
+// of columns (pieces of the two halves, or neighbours), or two pieces to copy.
+// Units of all rows and heads follow one another; the quotient by a row's units is
+// exact in fp32 (a workgroup's span and a row's units lie below 2^22).  Bound by
+// memory, at the rate of a large copy (5.1 TB/s): bf16 16384 rows H=32 Hkv=8 D=128
+// (337 MB) 60.6 us, 5.6 TB/s, fp16 16383 rows H=16 Hkv=8 D=64 into a cache 23.6 us;
+// 64 rows into a cache 3.4 us.  (Two units a thread 62.0 and 23.7, four 69.3 and
+// 25.2: more loads in flight, fewer waves.)
+template <typename T> struct RotaryPiece {
+  static constexpr int E = 16 / sizeof(T);
+  static __device__ __forceinline__ float get(const u32x4 &v, int i) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(f32x4, v)[i];
+    else return Elem<T>::to_f32((uint16_t)(i % 2 == 0 ? v[i / 2] & 0xffffu : v[i / 2] >> 16));
+  }
+  static __device__ __forceinline__ u32x4 put(const float (&x)[E]) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(u32x4, (f32x4){x[0], x[1], x[2], x[3]});
+    else return (u32x4){Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]), Elem<T>::pack(x[6], x[7])};
+  }
+};
+
+template <typename T, bool PAIRS, bool CACHE>
+__global__ __launch_bounds__(256) void rotary_wide_kernel(const RotaryArgs a, const int lu) {
+  using Piece = RotaryPiece<T>;
+  constexpr int E = Piece::E;
+  const int half = a.rot / 2;
+  const int n = (a.heads[0] + a.heads[1] + a.heads[2]) << lu;  // units of a row, 1 << lu of a head
+  const int64_t base = (int64_t)blockIdx.x * 256, row0 = base / n;
+  const int i = (int)(base - row0 * n) + (int)threadIdx.x, q = (int)(((float)i + 0.5f) * (1.0f / (float)n));
+  const int64_t t = row0 + q;
+  if (t >= a.rows) return;
+  const int r = i - q * n, u = r & ((1 << lu) - 1);
+  int h = r >> lu;
+  const int which = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
+  h -= which > 0 ? a.heads[0] : 0;
+  h -= which > 1 ? a.heads[1] : 0;
+  const bool turn = (!CACHE || which < 2) && u * E < half;
+  // Bytes of the unit's first piece within its head, and to its second.
+  const int at = turn && !PAIRS ? 16 * u : 32 * u, step = turn && !PAIRS ? half * (int)sizeof(T) : 16;
+  const char *src = (which == 0 ? a.src[0] : which == 1 ? a.src[1] : a.src[2]) +
+                    t * (which == 0 ? a.src_t[0] : a.src_t[1]) + h * (which == 0 ? a.src_h[0] : a.src_h[1]) + at;
+  char *dst;
+  if (CACHE && which > 0) {
+    const int32_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.num_slots) return;
+    dst = (which == 1 ? a.out[1] : a.out[2]) + (int64_t)(slot >> a.lp) * a.dst_p + (slot & ((1 << a.lp) - 1)) * a.dst_t +
+          h * a.dst_h + at;
+  } else {
+    dst = (which == 0 ? a.out[0] : a.out[1]) + t * (which == 0 ? a.out_t[0] : a.out_t[1]) +
+          (int64_t)h * a.D * sizeof(T) + at;
+  }
+  u32x4 x = *(const u32x4 *)src, y = *(const u32x4 *)(src + step);
+  if (turn) {
+    const float *row = a.angles + (int64_t)min(max(a.positions[t], 0), a.num_positions - 1) * a.rot + u * E;
+    float lo[E], hi[E];  // the two pieces, turned
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      // Pair e: elements 2e and 2e + 1 of the two pieces in a row, or e of each.
+      const float cs = row[e], sn = row[half + e] * a.sign;
+      if constexpr (PAIRS) {
+        float(&to)[E] = e < E / 2 ? lo : hi;
+        const u32x4 &from = e < E / 2 ? x : y;
+        const int j = 2 * e % E;
+        turn_pair(Piece::get(from, j), Piece::get(from, j + 1), cs, sn, to[j], to[j + 1]);
+      } else {
+        turn_pair(Piece::get(x, e), Piece::get(y, e), cs, sn, lo[e], hi[e]);
+      }
+    }
+    x = Piece::put(lo), y = Piece::put(hi);
+  }
+  *(u32x4 *)dst = x, *(u32x4 *)(dst + step) = y;
+}
+
+// Whether that kernel takes the call; lu: log2 of a head's units.
+template <typename T> bool rotary_wide(const RotaryArgs &a, int &lu) {
+  constexpr int E = RotaryPiece<T>::E;
+  uint64_t bits = (uintptr_t)a.angles;
+  const bool cache = a.slots != nullptr;
+  for (int i = 0; i < 3; ++i)
+    if (a.heads[i] > 0) {
+      bits |= (uintptr_t)a.src[i] | (uintptr_t)a.out[i] | (uint64_t)(a.src_t[i] | a.src_h[i]);
+      if (cache && i > 0) bits |= (uint64_t)(a.dst_p | a.dst_t | a.dst_h);
+    }
+  lu = 31 - __builtin_clz((unsigned)(a.D / (2 * E)));
+  return (bits & 15) == 0 && a.rot % (2 * E) == 0 && (int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) << lu < 1 << 21;
+}
+
+template <typename T, bool PAIRS, bool CACHE> void rotary_launch(const RotaryArgs &a, int lu, hipStream_t st) {
+  const int64_t units = a.rows * ((int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) << lu);
+  rotary_wide_kernel<T, PAIRS, CACHE><<<dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st>>>(a, lu);
+}
+
 template <typename T> void rotary_t(const RotaryArgs &a, bool pairs, hipStream_t st) {
+  int lu = 0;
+  if (rotary_wide<T>(a, lu)) {
+    if (a.slots != nullptr) {
+      if (pairs) rotary_launch<T, true, true>(a, lu, st);
+      else rotary_launch<T, false, true>(a, lu, st);
+    } else if (pairs) rotary_launch<T, true, false>(a, lu, st);
+    else rotary_launch<T, false, false>(a, lu, st);
+    return;
+  }
   if (pairs) rotary_kernel<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
   else rotary_kernel<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
 }
@@ -101,6 +207,8 @@ int rotary_check(const sigattn_rotary *r) {
   if (r->rows < 0 || r->rows > INT32_MAX / 2 || r->q_heads < 0 || r->kv_heads < 0 || r->q_heads > 65535 ||
       r->kv_heads > 65535 || r->num_positions > INT32_MAX)
     return SIGATTN_ERR_SHAPE;
+  // (Workgroups of 256 units of 16 columns at least.)
+  if (r->rows > 0 && (r->q_heads + 2 * r->kv_heads) * r->D > ((int64_t)1 << 42) / r->rows) return SIGATTN_ERR_SHAPE;
   if (r->rot_dim < 2 || r->rot_dim > r->D || r->rot_dim % 2 != 0 || r->num_positions < 1) return SIGATTN_ERR_ROTARY;
   const int64_t strides[4] = {r->q_stride_t, r->q_stride_h, r->k_stride_t, r->k_stride_h};
   for (int64_t s : strides)
