@@ -19,26 +19,12 @@ namespace sigattn {
 // queries, take one 32-key block of every tile each, and their accumulators
 // are added at the end (launch_bwd_dq_mfma says where).
 // A learned bias by relative position (P::kRel): WIN places of the head's line are
-// staged with each tile, and dS is summed by relative position.  A 32x32 block of
-// scores whose places all lie beyond the line's end adds to one sum per lane.  Any
-// other goes through LDS eight keys at a time, written so that a place's scores (a
-// diagonal's) are neighbours: a lane reads those of its place, sums them and
-// adds the sum to a line of the wave's own, which no other lane or wave touches, so
-// every addition has its order.  (LDS atomics, no two lanes of an instruction on
-// one place, took about 100 cycles each: bf16 H=12 D=64, 16 sequences of 101 .. 1001
-// reach 128, 262 us instead of 74.)
+// staged with each tile, and dS is summed by relative position (PlaceSums).
 template <class P, int WK> constexpr int dq_window() { return P::kRel ? 128 / WK + 64 : 0; }
 template <int D, bool SCOREMOD, int WIN = 0> struct DqLds {
   uint16_t k[2][64 * D], v[2][64 * D];
   float c[WIN > 0 ? 2 * WIN : (SCOREMOD ? 2 * 64 : 4)];
 };
-// Floats of a wave's line: a block's places on either side of the ends; and of the
-// piece of LDS that its diagonals go through, [39 places][8 keys] in rows of 12
-// (so that a row's two 16-byte reads meet no other lane's banks).
-constexpr int kNearMargin = 64, kSkewRow = 12, kSkew = 39 * kSkewRow;
-__host__ __device__ constexpr int near_places(int reach) { return 2 * reach + 2 * kNearMargin; }
-__host__ __device__ constexpr int near_floats(int reach) { return 4 * (near_places(reach) + kSkew); }
-
 template <typename T, int D, int WK, bool CAUSAL, bool SCOREMOD, class P = KParams>
 __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, SCOREMOD, dq_window<P, WK>()> &lds,
                                             float *near = nullptr) {
@@ -135,42 +121,8 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
   const int kv_stride_bytes = (int)(p.sk_t * 2);
 
   [[maybe_unused]] const int win0 = BM - (w % NG) * 32 - l32 + 4 * hi;  // this lane's place of the tile's key 0
-  [[maybe_unused]] float beyond[2] = {0.0f, 0.0f};
-  [[maybe_unused]] bool sums = false;
-  [[maybe_unused]] float *mine = near, *skew = near;  // relative position 0 of the wave's line; its piece
-  if constexpr (REL) {
-    sums = p.part != nullptr;
-    mine += w * near_places(p.reach) + p.reach + kNearMargin;
-    skew += 4 * near_places(p.reach) + w * kSkew;
-    if (sums)
-      for (int i = tid; i < near_floats(p.reach); i += 256) near[i] = 0.0f;
-  }
-  // dS of a block whose first key lies `off` after the wave's first query.
-  [[maybe_unused]] auto add_places = [&](const float (&ds)[16], int off) SIGATTN_INLINE {
-    if constexpr (REL) {
-      if (off + 31 <= -p.reach || off - 31 >= p.reach) {
-        float x = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x += ds[i];
-        if (off < 0) beyond[0] += x;
-        else beyond[1] += x;
-        return;
-      }
-      float *to = skew + (31 + 4 * hi - l32) * kSkewRow + 4 * hi;
-      float x = 0.0f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {  // keys 8g .. 8g + 7, places 8g - 31 .. 8g + 7 from `off` on
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[j * (kSkewRow + 1)] = ds[4 * g + j];
-        const int row = lane - 8 * g;
-        const float *from = skew + min(max(row, 0), 38) * kSkewRow;
-        const f32x4 u = *(const f32x4 *)from, v = *(const f32x4 *)(from + 4);
-        const float y = ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
-        x += row >= 0 && row <= 38 ? y : 0.0f;
-      }
-      mine[off - 31 + lane] += x;
-    }
-  };
+  [[maybe_unused]] PlaceSums sums;
+  if constexpr (REL) sums.init(p, near, w, tid);
 
   // dS of one 32-key block into eight packed words.
   auto ds_block = [&](const f32x16 &s, const f32x16 &dp, int st, int kl, int kbase, uint32_t *out,
@@ -204,7 +156,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
       }
     }
     if constexpr (REL) {
-      if (sums) add_places(ds, kbase - qw);
+      sums.add(ds, kbase - qw, l32, hi);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = Elem<T>::pack(ds[2 * i], ds[2 * i + 1]);
@@ -248,7 +200,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
       creg = key < Lk ? -(bias + p.score_mod[p.mod_base(b) + key0 + key]) * kLog2e : 0.0f;
     }
     if constexpr (REL) {
-      if (tid < WIN) creg = -(bias + rel_at(p, h, n0 + tid - q0 - BM)) * kLog2e;
+      if (tid < WIN) creg = rel_at(p, h, n0 + tid - q0 - BM);
     }
   };
   auto issue = [&](int st, int n0) SIGATTN_INLINE {
@@ -261,7 +213,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
     wait_dma();
     if (SCOREMOD && tid < BN) sC[ST * BN + tid] = creg;
     if constexpr (REL) {
-      if (tid < WIN) sC[ST * WIN + tid] = creg;
+      if (tid < WIN) sC[ST * WIN + tid] = -(bias + creg) * kLog2e;
     }
     __syncthreads();
     if (it + 1 < ntiles) {
@@ -283,32 +235,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
   }
 
   if constexpr (REL) {
-    if (sums && q0 < Lq) {  // (no such block: its place may be another's)
-      // The four waves' lines, in their order; what lies on either side of the
-      // ends goes to these, as do the waves' sums per lane.
-      const int n = near_places(p.reach), places = p.places();
-      __shared__ float ends[4][2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = wave_sum(beyond[e]);
-        if (lane == 0) ends[w][e] = x;
-      }
-      __syncthreads();
-      float *row = p.part_row(b, qb, h);
-      const auto all = [&](int i) SIGATTN_INLINE { return ((near[i] + near[n + i]) + near[2 * n + i]) + near[3 * n + i]; };
-      const auto end = [&](int e) SIGATTN_INLINE { return ((ends[0][e] + ends[1][e]) + ends[2][e]) + ends[3][e]; };
-      if (w < 2) {
-        // Wave 0: places up to the lower end, wave 1: from the upper one on.
-        const float x = wave_sum(all(w == 0 ? lane + 1 : kNearMargin + places - 1 + lane));
-        if (places > 1 && lane == 0) row[w == 0 ? 0 : places - 1] = x + end(w);
-        if (places == 1 && lane == 0 && w == 0) {
-          float y = x + end(0) + end(1);
-          for (int i = 1; i < kNearMargin; ++i) y += all(kNearMargin + i);
-          row[0] = y;
-        }
-      }
-      for (int i = tid + 1; i < places - 1; i += 256) row[i] = all(kNearMargin + i);
-    }
+    if (q0 < Lq) sums.finish(p, near, b, qb, h, w, tid);  // (no other block: its place may be another's)
   }
 
   if constexpr (WK == 2) {
@@ -539,14 +466,13 @@ __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<
   [[maybe_unused]] const int win0 = BN - w * 32 - l32 + 4 * hi;  // this lane's place of the tile's query 0
   auto store_c = [&](int t) SIGATTN_INLINE {
     if constexpr (REL) {
-      if (tid < WIN) lds.c[t % NST * WIN + tid] = creg;
+      if (tid < WIN) lds.c[t % NST * WIN + tid] = -(bias + creg) * kLog2e;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   };
   auto issue = [&](int st, int t) SIGATTN_INLINE {
     if constexpr (REL) {
-      if (tid < WIN)
-        creg = -(bias + rel_at(p, hq + (int)hs.head_of_tile(t), k0 + BN - mstart - hs.tile(t) * BMQ - tid)) * kLog2e;
+      if (tid < WIN) creg = rel_at(p, hq + (int)hs.head_of_tile(t), k0 + BN - mstart - hs.tile(t) * BMQ - tid);
     }
     const int64_t at = (int64_t)mstart * p.sq_t + hs.head_of_tile(t) * p.sq_h;
     dma.issue(sQ[st], Qb + at, q_stride_bytes, hs.tile(t) * BMQ, mend - mstart);

@@ -294,7 +294,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     [[maybe_unused]] const int win0 = WIN - 64 - slot * QW - l32 + 4 * hi;  // this lane's place of the tile's key 0
     auto load_c = [&](int n0) SIGATTN_INLINE {
       if constexpr (REL) {
-        if (tid < WIN) creg = -(bias + rel_at(p, h, n0 + tid - q0 - BM)) * kLog2e;
+        if (tid < WIN) creg = rel_at(p, h, n0 + tid - q0 - BM);
       }
       if (SCOREMOD && tid < BN) {
         const int key = n0 + tid;
@@ -308,7 +308,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     auto store_c = [&](int t) SIGATTN_INLINE {
       if (SCOREMOD && tid < BN) sC[(t % NST) * BN + tid] = creg;
       if constexpr (REL) {
-        if (tid < WIN) sC[(t % NST) * WIN + tid] = creg;
+        if (tid < WIN) sC[(t % NST) * WIN + tid] = -(bias + creg) * kLog2e;
       }
     };
     auto issue = [&](int st, int t) SIGATTN_INLINE {

@@ -9,16 +9,22 @@
 
 namespace sigattn {
 
-// Values and sums are rows of 2 reach + 1 places, place reach + d for relative
-// position d = key - query.  The caller's table may reach further than any two
-// tokens of a call lie apart: `reach` is then what those need.
+// Values and sums by relative position d = key - query, -reach .. reach.  The
+// caller's table may reach further than any two tokens of a call lie apart: `reach`
+// is then what those need.  A head's line of values has kRelPad places more on either
+// side (the ends' values), so that of a block of 32 keys or queries the first
+// place is all that is clamped.
+constexpr int kRelPad = 64;
+__host__ __device__ constexpr int line_places(int reach) { return 2 * (reach + kRelPad) + 1; }
+
 struct RelParams : KParams {
   static constexpr bool kRel = true;
-  const float *line;  // [H, places]
+  const float *line;  // [H, line_places(reach)]
   int reach;
   // dQ kernels: sums of dS of each (query block of part_rows rows, query head),
-  // [part_slots(), H, places].  Blocks of batch b follow one another from slot
-  // first row / part_rows + b on, which leaves none without a place of its own.
+  // [part_slots(), H, places()], place reach + d.  Blocks of batch b follow one
+  // another from slot first row / part_rows + b on, which leaves none without a
+  // place of its own.
   float *part;        // nullptr: no sums
   int part_rows;
 
@@ -30,46 +36,42 @@ struct RelParams : KParams {
   }
 };
 
-// Over a paged cache: query i of n at position L - n + i (forward only).  A lane of
-// the matrix kernels has a column, so a head and a position of its own: it reads the
-// values of a 32-key block itself, from a line with kRelPad places more on either
-// side, so that the block's first place is all that is clamped.  Blocks that lie
-// beyond the line's end for every lane, nearly all of a long context, cost nothing:
-// their value is the lane's constant.
-constexpr int kRelPad = 64;
+// Over a paged cache: query i of n at position L - n + i (forward only).
 struct PagedRelParams : PagedParams {
   static constexpr bool kRel = true;
-  const float *line;  // [H, 2 reach + 1 + 2 kRelPad], places from the padding's first
+  const float *line;
   int reach;
-
-  __device__ __forceinline__ const float *row(int h) const {
-    return line + (int64_t)h * (2 * reach + 1 + 2 * kRelPad) + kRelPad + reach;
-  }
 };
+
+// Place 0 of query head h's line, and its value at relative position d.
+template <class P> __device__ __forceinline__ const float *rel_row(const P &p, int h) {
+  return p.line + (int64_t)h * line_places(p.reach) + kRelPad + p.reach;
+}
+template <class P> __device__ __forceinline__ float rel_at(const P &p, int h, int d) {
+  if constexpr (P::kRel) return rel_row(p, h)[min(max(d, -p.reach), p.reach)];
+  else return 0.0f;
+}
 
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-// What a lane's scores have added beyond scale, times -log2(e), block by block.
+// What a lane's column of scores has added beyond scale, times -log2(e), a block of
+// 32 rows at a time, for kernels whose lanes read it themselves.  Blocks that lie
+// beyond the line's end for every lane, nearly all of a long context, cost nothing:
+// their value is the lane's constant.
 struct RelColumn {
   const float *row;  // relative position 0
   float nbl, ends[2];
-  int reach, pos;    // the query's position, from the chunk's first key
-  __device__ __forceinline__ void init(const PagedRelParams &p, int h, int position, float bias) {
-    row = p.row(h), reach = p.reach, pos = position;
+  int reach, pos;    // the column's position
+  template <class P> __device__ __forceinline__ void init(const P &p, int h, int position, float bias) {
+    row = rel_row(p, h), reach = p.reach, pos = position;
     nbl = -bias * kLog2e;
     ends[0] = __builtin_fmaf(row[-reach], -kLog2e, nbl), ends[1] = __builtin_fmaf(row[reach], -kLog2e, nbl);
   }
-  // The 32-key block from key `first` on, 16 keys of this half of the wave; `n` of
-  // them (2 or 16) are wanted.
+  // Rows are keys from position `first` on: 16 (or the first 2) of this half of the wave.
   template <int N> __device__ __forceinline__ void block(int first, int hi, float (&c)[N]) const {
     const int d = first - pos;  // of the block's first key
     const bool before = d + 31 <= -reach, after = d >= reach;
-    if (__all(before || after)) {
-      const float x = before ? ends[0] : ends[1];
-#pragma unroll
-      for (int i = 0; i < N; ++i) c[i] = x;
-      return;
-    }
+    if (__all(before || after)) return fill(before, c);
     const float *at = row + min(max(d, -reach - 32), reach) + 4 * hi;
 #pragma unroll
     for (int g = 0; g < (N + 3) / 4; ++g) {
@@ -79,14 +81,97 @@ struct RelColumn {
         if (4 * g + j < N) c[4 * g + j] = __builtin_fmaf(v[j], -kLog2e, nbl);
     }
   }
+  template <int N> __device__ __forceinline__ void fill(bool before, float (&c)[N]) const {
+    const float x = before ? ends[0] : ends[1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = x;
+  }
 };
 
-// Value of query head h at relative position d.
-template <class P> __device__ __forceinline__ float rel_at(const P &p, int h, int d) {
-  if constexpr (P::kRel && P::kPaged) return p.row(h)[min(max(d, -p.reach), p.reach)];
-  else if constexpr (P::kRel) return p.line[(int64_t)h * (2 * p.reach + 1) + p.reach + min(max(d, -p.reach), p.reach)];
-  else return 0.0f;
-}
+// dS by relative position, of a dQ workgroup of four waves.  A 32x32 block of scores
+// (lane: query, accumulator rows: keys) whose places all lie beyond the line's end
+// adds to one sum per lane.  Any other goes through LDS eight keys at a time,
+// written so that a place's scores (a diagonal's) are neighbours: a lane reads those
+// of its place, sums them and adds the sum to a line of the wave's own, which no
+// other lane or wave touches, so every addition has its order.  (LDS atomics, no two
+// lanes of an instruction on one place, took about 100 cycles each: bf16 H=12 D=64, 16
+// sequences of 101 .. 1001, reach 128, 262 us instead of 74; 55 without the bias.)
+// LDS: the waves' lines, a block's places more on either side of the ends, then the
+// pieces that diagonals go through, [39 places][8 keys] in rows of 12 (so that a
+// row's two 16-byte reads meet no other lane's banks).
+constexpr int kNearMargin = 64, kSkewRow = 12, kSkew = 39 * kSkewRow;
+__host__ __device__ constexpr int near_places(int reach) { return 2 * reach + 2 * kNearMargin; }
+__host__ __device__ constexpr int near_floats(int reach) { return 4 * (near_places(reach) + kSkew); }
+
+struct PlaceSums {
+  float beyond[2] = {0.0f, 0.0f};
+  float *mine, *skew;  // relative position 0 of the wave's line; its piece
+  int reach;
+  bool on;
+
+  // A barrier follows before the first add() or finish().
+  __device__ __forceinline__ void init(const RelParams &p, float *near, int w, int tid) {
+    on = p.part != nullptr, reach = p.reach;
+    mine = near + w * near_places(reach) + reach + kNearMargin;
+    skew = near + 4 * near_places(reach) + w * kSkew;
+    beyond[0] = beyond[1] = 0.0f;
+    if (on)
+      for (int i = tid; i < near_floats(reach); i += 256) near[i] = 0.0f;
+  }
+  // A block whose first key lies `off` (a multiple of 32) after the wave's first query.
+  __device__ __forceinline__ void add(const float (&ds)[16], int off, int l32, int hi) {
+    if (!on) return;
+    if (off + 31 <= -reach || off - 31 >= reach) {
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x += ds[i];
+      if (off < 0) beyond[0] += x;
+      else beyond[1] += x;
+      return;
+    }
+    const int lane = l32 + 32 * hi;
+    float *to = skew + (31 + 4 * hi - l32) * kSkewRow + 4 * hi;
+    float x = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {  // keys 8g .. 8g + 7, places 8g - 31 .. 8g + 7 from `off` on
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j * (kSkewRow + 1)] = ds[4 * g + j];
+      const int row = lane - 8 * g;
+      const float *from = skew + min(max(row, 0), 38) * kSkewRow;
+      const f32x4 u = *(const f32x4 *)from, v = *(const f32x4 *)(from + 4);
+      const float y = ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
+      x += row >= 0 && row <= 38 ? y : 0.0f;
+    }
+    mine[off - 31 + lane] += x;
+  }
+  // The four waves' lines, in their order, to the block's row of p.part; what lies on
+  // either side of the ends goes to these, as do the waves' sums per lane.
+  __device__ __forceinline__ void finish(const RelParams &p, const float *near, int b, int blk, int h, int w, int tid) {
+    if (!on) return;
+    const int n = near_places(reach), places = p.places(), lane = tid & 63;
+    __shared__ float ends[4][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = wave_sum(beyond[e]);
+      if (lane == 0) ends[w][e] = x;
+    }
+    __syncthreads();
+    float *row = p.part_row(b, blk, h);
+    const auto all = [&](int i) SIGATTN_INLINE { return ((near[i] + near[n + i]) + near[2 * n + i]) + near[3 * n + i]; };
+    const auto end = [&](int e) SIGATTN_INLINE { return ((ends[0][e] + ends[1][e]) + ends[2][e]) + ends[3][e]; };
+    if (w < 2) {
+      // Wave 0: places up to the lower end, wave 1: from the upper one on.
+      const float x = wave_sum(all(w == 0 ? lane + 1 : kNearMargin + places - 1 + lane));
+      if (places > 1 && lane == 0) row[w == 0 ? 0 : places - 1] = x + end(w);
+      if (places == 1 && lane == 0 && w == 0) {
+        float y = x + end(0) + end(1);
+        for (int i = 1; i < kNearMargin; ++i) y += all(kNearMargin + i);
+        row[0] = y;
+      }
+    }
+    for (int i = tid + 1; i < places - 1; i += 256) row[i] = all(kNearMargin + i);
+  }
+};
 
 // The learned table: [buckets, H] of `dtype` (enum sigattn_dtype), and the bucket
 // of each relative position -max_distance .. max_distance.
@@ -94,9 +179,6 @@ struct RelTable {
   const void *table;
   const int32_t *bucket;
   int dtype, buckets, max_distance, H, reach;
-  int pad;  // places of the lines before -reach and after reach
-
-  __host__ __device__ __forceinline__ int places() const { return 2 * (reach + pad) + 1; }
 };
 
 // The host's side: the caller's table for H heads and two lengths (reach: no two
@@ -114,10 +196,10 @@ inline RelTable rel_table(const sigattn_rel_bias *r, int64_t H, int64_t Tq, int6
   return t;
 }
 inline int64_t rel_line_bytes(const RelTable &t) {
-  return ((int64_t)t.H * t.places() * (int64_t)sizeof(float) + 255) / 256 * 256;
+  return ((int64_t)t.H * line_places(t.reach) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
-// line [H, places] from the table.
+// line [H, line_places(reach)] from the table.
 void launch_rel_line(const RelTable &t, float *line, hipStream_t st);
 // The table's gradient (`grad`, the table's type) from the dQ kernels' sums in
 // p.part (nullptr: zeros); sums: [H, 2 reach + 1] floats of scratch.
@@ -138,6 +220,14 @@ constexpr int kGenericRows = 64;
 void launch_rel_fwd_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
 void launch_rel_dq_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
 void launch_rel_dkdv_generic(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+// fp32 (launch_fwd_f32 and so on), D in {32, 64, 128} (16 as 32).
+void launch_rel_fwd_f32(const RelParams &p, int D, bool causal, hipStream_t st);
+int rel_dq_rows_f32(const RelParams &p, int D, bool causal);
+void launch_rel_dq_f32(const RelParams &p, int D, bool causal, hipStream_t st);
+void launch_rel_dkdv_f32(const RelParams &p, int D, bool causal, hipStream_t st);
+void launch_paged_rel_f32(const PagedRelParams &p, int units, int D, bool causal, hipStream_t st);
+void launch_paged_rel_decode_f32(const PagedRelParams &p, int units, int D, bool causal, hipStream_t st);
+
 // MFMA kernels over a paged cache, as launch_paged_fwd, launch_paged_decode and
 // launch_paged_mixed (paged.h).
 void launch_paged_rel_fwd(const PagedRelParams &p, int units, int dtype, int D, bool causal, hipStream_t st);

@@ -14,9 +14,9 @@ __device__ __forceinline__ bool inside(const RelTable &t, int u) { return u >= 0
 
 // One thread per place.  A few KB: bound by its launch.
 template <typename T> __global__ __launch_bounds__(256) void rel_line_kernel(const RelTable t, float *line) {
-  const int place = blockIdx.x * 256 + threadIdx.x, places = t.places(), h = blockIdx.y;
+  const int place = blockIdx.x * 256 + threadIdx.x, places = line_places(t.reach), h = blockIdx.y;
   if (place >= places) return;
-  const int u = bucket_of(t, min(max(place - t.pad, 0), 2 * t.reach));
+  const int u = bucket_of(t, min(max(place - kRelPad, 0), 2 * t.reach));
   float x = 0.0f;
   if (inside(t, u)) {
     const int64_t at = (int64_t)u * t.H + h;
@@ -97,7 +97,7 @@ template <class F> void by_type(int dtype, F &&f) {
 
 void launch_rel_line(const RelTable &t, float *line, hipStream_t st) {
   if (t.H == 0) return;
-  const dim3 grid((unsigned)((t.places() + 255) / 256), (unsigned)t.H);
+  const dim3 grid((unsigned)((line_places(t.reach) + 255) / 256), (unsigned)t.H);
   by_type(t.dtype, [&](auto *x) {
     rel_line_kernel<std::remove_pointer_t<decltype(x)>><<<grid, dim3(256), 0, st>>>(t, line);
   });

@@ -16,8 +16,9 @@ RelParams rel_params(const sigattn_problem *p, const RelTable &t, void *line) {
 }
 
 int64_t rel_part_bytes(const sigattn_problem *p, const RelTable &t) {
-  // (Blocks of 64 rows, the shortest; a multiple of 256 bytes.)
-  return ((p->rows_q / kGenericRows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
+  // (The shortest blocks' rows; a multiple of 256 bytes.)
+  const int rows = p->dtype == SIGATTN_F32 ? 32 : kGenericRows;
+  return ((p->rows_q / rows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
 RelParams rel_kv_items(const RelParams &k) {
@@ -28,13 +29,8 @@ RelParams rel_kv_items(const RelParams &k) {
 
 // The learned bias's table as far as the cache's sequences reach.
 RelTable rel_table_of(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
-  RelTable t = rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q, p->max_pages * p->page_size);
-  t.pad = kRelPad;
-  return t;
+  return rel_table(r, p->H, p->max_seqlen_q < p->rows_q ? p->max_seqlen_q : p->rows_q, p->max_pages * p->page_size);
 }
-
-// The matrix kernels with the bias: f16 / bf16.
-bool paged_mfma(const sigattn_paged_problem *p, const void *out) { return p->dtype != SIGATTN_F32 && use_mfma(p, out); }
 
 }  // namespace
 
@@ -76,11 +72,13 @@ int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *o
   (void)hipGetLastError();
   launch_rel_line(t, (float *)workspace, st);
   const void *ptrs[4] = {p->q, p->k, p->v, out};
-  if (use_mfma(p, ptrs, 4)) {
+  const bool f32 = use_f32_mfma(p, ptrs, 4);
+  if (f32 || use_mfma(p, ptrs, 4)) {
     GapAxis gq, gk;
     gap_axes(p, out, nullptr, nullptr, gq, gk);
     use_gaps(k, gq, gk);
-    launch_rel_fwd_mfma(k, p->dtype, mfma_head_dim(p), p->causal != 0, st);
+    if (f32) launch_rel_fwd_f32(k, mfma_head_dim(p), p->causal != 0, st);
+    else launch_rel_fwd_mfma(k, p->dtype, mfma_head_dim(p), p->causal != 0, st);
     return launch_status();
   }
   zero_packed_gaps(p, out, nullptr, nullptr, st);
@@ -93,7 +91,7 @@ size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_r
   const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
   // (Pointers are not known yet: aligned rows, as everywhere.)
   const void *none[1] = {nullptr};
-  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0)).bytes);
+  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
 }
 
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
@@ -115,7 +113,8 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
   k.dk = dk;
   k.dv = dv;
   const void *ptrs[7] = {p->q, p->k, p->v, dout, dq, dk, dv};
-  const bool mfma = use_mfma(p, ptrs, 7) && p->Tq > 0 && p->Tk > 0, causal = p->causal != 0;
+  const bool f32 = use_f32_mfma(p, ptrs, 7), causal = p->causal != 0;
+  const bool mfma = (f32 || use_mfma(p, ptrs, 7)) && p->Tq > 0 && p->Tk > 0;
   const int D = mfma ? mfma_head_dim(p) : (int)p->D;
   (void)hipGetLastError();
   if (!mfma) zero_packed_gaps(p, dq, dk, dv, st);
@@ -131,13 +130,18 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     const HeadSplit hs = head_split(p, mfma);
     k.qsplit = hs.n;
     k.kv_part = (float *)(parts + rel_part_bytes(p, t));
-    k.part_rows = rel_dq_rows(k, D, causal);
+    k.part_rows = f32 ? rel_dq_rows_f32(k, D, causal) : rel_dq_rows(k, D, causal);
     RelParams kq = k;
     GapAxis gq, gk;
     gap_axes(p, dq, dk, dv, gq, gk);
     use_gaps(kq, gq, gk);
-    launch_rel_dq_mfma(kq, p->dtype, D, causal, st);
-    launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, st);
+    if (f32) {
+      launch_rel_dq_f32(kq, D, causal, st);
+      launch_rel_dkdv_f32(rel_kv_items(k), D, causal, st);
+    } else {
+      launch_rel_dq_mfma(kq, p->dtype, D, causal, st);
+      launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, st);
+    }
   } else {
     k.part_rows = kGenericRows;
     launch_rel_dq_generic(k, p->dtype, D, causal, st);
@@ -159,7 +163,7 @@ int sigattn_paged_rel_check(const sigattn_paged_problem *p, const sigattn_rel_bi
 
 size_t sigattn_paged_rel_fwd_workspace_bytes(const sigattn_paged_problem *p, const sigattn_rel_bias *r) {
   if (sigattn_paged_rel_check(p, r) != SIGATTN_OK || p->rows_q == 0 || p->H == 0 || p->B == 0) return 0;
-  const size_t plan = paged_mfma(p, nullptr) ? make_plan(p, make_params(p, nullptr), kernel_dim(p)).bytes : 0;
+  const size_t plan = use_mfma(p, nullptr) ? make_plan(p, make_params(p, nullptr), kernel_dim(p)).bytes : 0;
   return (size_t)rel_line_bytes(rel_table_of(p, r)) + plan;
 }
 
@@ -172,7 +176,7 @@ int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias
   const RelTable t = rel_table_of(p, r);
   PagedRelParams k{};
   (PagedParams &)k = make_params(p, out);
-  const bool mfma = paged_mfma(p, out), causal = p->causal != 0;
+  const bool mfma = use_mfma(p, out), causal = p->causal != 0;
   const int D = kernel_dim(p);
   PagedPlan pl;
   if (mfma) pl = make_plan(p, k, D);
@@ -188,7 +192,10 @@ int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias
   }
   run_plan(p, k, pl, (char *)workspace + rel_line_bytes(t), out, st,
            [&](const PagedRelParams &first, int nf, const PagedRelParams &kd, int nd) {
+             const bool f32 = p->dtype == SIGATTN_F32;
              if (nf > 0 && nd > 0) launch_paged_rel_mixed(first, nf, kd, nd, p->dtype, D, causal, st);
+             else if (nd > 0 && f32) launch_paged_rel_decode_f32(first, nd, D, causal, st);
+             else if (f32) launch_paged_rel_f32(first, nf, D, causal, st);
              else if (nd > 0) launch_paged_rel_decode(first, nd, p->dtype, D, causal, st);
              else launch_paged_rel_fwd(first, nf, p->dtype, D, causal, st);
            });
