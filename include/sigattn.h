@@ -387,7 +387,7 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
  * Packed problems (both axes) without score_mod.
  */
 #define SIGATTN_REL_MAX_DISTANCE 2048
-#define SIGATTN_REL_MAX_BUCKETS 65536
+#define SIGATTN_REL_MAX_BUCKETS 4096
 typedef struct sigattn_rel_bias {
   int32_t dtype;          /* enum sigattn_dtype of the table and its gradient */
   int32_t num_buckets;
@@ -400,6 +400,9 @@ int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r);
 /*
  * Forward and backward with that bias.  Both need their workspace (16-byte
  * aligned, used until the call's kernels finish; SIGATTN_ERR_WORKSPACE without it).
+ * The forward leaves in its own what the table is at each relative position;
+ * given as `line` to the backward of the same problem, it is not read from the
+ * table again (NULL: it is).
  * `dtable` is the table's gradient, [num_buckets, H] of its type, written whole:
  * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed).
  * Deterministic.
@@ -408,8 +411,8 @@ size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_r
 int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
                     size_t workspace_bytes, void *stream);
 size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
-int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
-                    void *dtable, void *workspace, size_t workspace_bytes, void *stream);
+int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
+                    void *dk, void *dv, void *dtable, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * sigattn_paged_fwd with that bias; query i of n new tokens sits at position

@@ -79,7 +79,7 @@ def test_far_reaches(R, dtype, D):
     check(make([2150, 70], [2150, 70], 1, 1, D, DT[dtype], 40, R, seed=R), False)
 
 
-@pytest.mark.parametrize("num", [1, 2, 255, 256, 257, 700])
+@pytest.mark.parametrize("num", [1, 2, 255, 256, 257, 700, 4096])
 def test_numbers_of_buckets(num):
     check(make([150, 40], [150, 40], 2, 1, 32, torch.float16, num, 200, seed=num), False)
 

@@ -403,7 +403,7 @@ const char *sigattn_strerror(int status) {
       return "workspace too small for the call or not 16-byte aligned";
     case SIGATTN_ERR_KV_HEADS: return "kv_heads must divide H, and fewer than H need packed sequences";
     case SIGATTN_ERR_REL_BIAS:
-      return "relative bias: needs packed sequences without score_mod, max_distance up to 2048 and 1 to 65536 buckets";
+      return "relative bias: needs packed sequences without score_mod, max_distance up to 2048 and 1 to 4096 buckets";
     case SIGATTN_ERR_ROTARY: return "rotary embedding: rot_dim must be even, at most D, and positions not none";
     case SIGATTN_ERR_SCRATCH:
       return "problem needs more than the fixed scratch buffer of sigattn_fwd_noalloc";

@@ -28,24 +28,30 @@ template <typename T> __global__ __launch_bounds__(256) void rel_line_kernel(con
 
 // sums[h][place] of all query blocks: 64 places a workgroup, 16 shares of the
 // slots (in turn), added in their order.  Which slots hold a block is found for
-// 1024 of them at a time, a thread each.
-constexpr int kShares = 16;
+// 1024 of them at a time, a thread each, from the batches' first slots in LDS
+// (kFirst of them; a larger batch's come from its offsets).
+constexpr int kShares = 16, kFirst = 1024;
 __global__ __launch_bounds__(64 * kShares) void rel_sums_kernel(const RelParams p, float *sums) {
   __shared__ float got[kShares][64];
   __shared__ bool held[64 * kShares];
+  __shared__ int64_t first[kFirst];
   const int h = blockIdx.y, lane = threadIdx.x & 63, share = threadIdx.x >> 6, places = p.places();
   const int place = blockIdx.x * 64 + lane;
   const int64_t slots = p.part != nullptr ? p.part_slots() : 0;
+  const bool kept = p.B <= kFirst;
+  if (kept && (int)threadIdx.x < p.B) first[threadIdx.x] = p.first_slot(threadIdx.x);
+  __syncthreads();
+  const auto first_slot = [&](int b) SIGATTN_INLINE { return kept ? first[b] : p.first_slot(b); };
   float x = 0.0f;
   for (int64_t s0 = 0; s0 < slots; s0 += 64 * kShares) {
     const int64_t mine = s0 + threadIdx.x;
     int lo = 0, hi = p.B - 1;  // the last batch that begins at or before the slot
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (p.first_slot(mid) <= mine) lo = mid;
+      if (first_slot(mid) <= mine) lo = mid;
       else hi = mid - 1;
     }
-    const int64_t blk = mine - p.first_slot(lo);
+    const int64_t blk = mine - first_slot(lo);
     __syncthreads();
     held[threadIdx.x] = blk >= 0 && blk * p.part_rows < p.len_q(lo);
     __syncthreads();
@@ -63,27 +69,25 @@ __global__ __launch_bounds__(64 * kShares) void rel_sums_kernel(const RelParams 
   sums[(int64_t)h * places + place] = x;
 }
 
-// grad[u][h] = the sum over the places of bucket u, in their order.  A workgroup per
-// head; `shares` threads a bucket, each a run of places, added in order.
-template <typename T> __global__ __launch_bounds__(256) void rel_grad_kernel(const RelTable t, const float *sums, T *grad) {
-  __shared__ float got[256];
-  const int h = blockIdx.x, places = 2 * t.reach + 1, per = min(t.buckets, 256), shares = 256 / per;
-  const int share = threadIdx.x / per, run = (places + shares - 1) / shares;
-  const float *row = sums + (int64_t)h * places;
-  for (int u0 = 0; u0 < t.buckets; u0 += per) {
-    const int u = u0 + (int)threadIdx.x - share * per;
+// grad[u][h] = the sum over the places of bucket u.  A workgroup per head keeps the
+// sums and their buckets in LDS; a wave per bucket, its lanes' places added in order
+// and the lanes' sums by wave_sum.
+constexpr int kGradWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(64 * kGradWaves) void rel_grad_kernel(const RelTable t, const float *sums, T *grad) {
+  extern __shared__ float row[];  // [places] sums, then their buckets
+  const int h = blockIdx.x, places = 2 * t.reach + 1, lane = threadIdx.x & 63;
+  int *bucket = (int *)row + places;
+  for (int i = threadIdx.x; i < places; i += 64 * kGradWaves)
+    row[i] = sums[(int64_t)h * places + i], bucket[i] = bucket_of(t, i);
+  __syncthreads();
+  for (int u = threadIdx.x >> 6; u < t.buckets; u += kGradWaves) {
     float x = 0.0f;
-    if (share < shares && u < t.buckets)
-      for (int i = share * run; i < min(places, (share + 1) * run); ++i)
-        if (bucket_of(t, i) == u) x += row[i];
-    got[threadIdx.x] = x;
-    __syncthreads();
-    if (share == 0 && u < t.buckets) {
-      for (int s = 1; s < shares; ++s) x += got[s * per + threadIdx.x];
-      if constexpr (sizeof(T) == 4) grad[(int64_t)u * t.H + h] = x;
-      else ((uint16_t *)grad)[(int64_t)u * t.H + h] = Elem<T>::from_f32(x);
-    }
-    __syncthreads();
+    for (int i = lane; i < places; i += 64) x += bucket[i] == u ? row[i] : 0.0f;
+    x = wave_sum(x);
+    if (lane != 0) continue;
+    if constexpr (sizeof(T) == 4) grad[(int64_t)u * t.H + h] = x;
+    else ((uint16_t *)grad)[(int64_t)u * t.H + h] = Elem<T>::from_f32(x);
   }
 }
 
@@ -109,7 +113,7 @@ void launch_rel_grad(const RelTable &t, const RelParams &p, float *sums, void *g
   rel_sums_kernel<<<grid, dim3(64 * kShares), 0, st>>>(p, sums);
   by_type(t.dtype, [&](auto *x) {
     using T = std::remove_pointer_t<decltype(x)>;
-    rel_grad_kernel<T><<<dim3((unsigned)t.H), dim3(256), 0, st>>>(t, sums, (T *)grad);
+    rel_grad_kernel<T><<<dim3((unsigned)t.H), dim3(64 * kGradWaves), 8 * p.places(), st>>>(t, sums, (T *)grad);
   });
 }
 

@@ -7,7 +7,7 @@ using namespace sigattn;
 
 namespace {
 
-RelParams rel_params(const sigattn_problem *p, const RelTable &t, void *line) {
+RelParams rel_params(const sigattn_problem *p, const RelTable &t, const void *line) {
   RelParams k{};
   (KParams &)k = make_params(p);
   k.line = (const float *)line;
@@ -94,8 +94,8 @@ size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_r
   return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
 }
 
-int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *dout, void *dq, void *dk, void *dv,
-                    void *dtable, void *workspace, size_t workspace_bytes, void *stream) {
+int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
+                    void *dk, void *dv, void *dtable, void *workspace, size_t workspace_bytes, void *stream) {
   const int rc = sigattn_rel_check(p, r);
   if (rc != SIGATTN_OK) return rc;
   if (p->H == 0) return SIGATTN_OK;
@@ -106,7 +106,7 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < sigattn_rel_bwd_workspace_bytes(p, r))
     return SIGATTN_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
-  RelParams k = rel_params(p, t, workspace);
+  RelParams k = rel_params(p, t, line != nullptr ? line : workspace);
   float *sums = (float *)((char *)workspace + rel_line_bytes(t));
   k.dout = dout;
   k.dq = dq;
@@ -123,7 +123,7 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
     return launch_status();
   }
-  launch_rel_line(t, (float *)workspace, st);
+  if (line == nullptr) launch_rel_line(t, (float *)workspace, st);
   char *parts = (char *)workspace + 2 * rel_line_bytes(t);
   if (dtable != nullptr) k.part = (float *)parts;
   if (mfma) {

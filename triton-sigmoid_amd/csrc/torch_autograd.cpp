@@ -306,7 +306,6 @@ struct RelNode : public torch::autograd::Function<RelNode> {
                         const Tensor &buckets, const Tensor &bias, const Tensor &scale, const Tensor &cu_q,
                         const Tensor &cu_k, int64_t max_q, int64_t max_k, bool causal) {
     const Layout lay{Tensor(), Tensor(), cu_q, cu_k, max_q, max_k};
-    ctx->save_for_backward({q, k, v, table, buckets, bias, scale, cu_q, cu_k});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["max_q"] = max_q;
     ctx->saved_data["max_k"] = max_k;
@@ -317,6 +316,8 @@ struct RelNode : public torch::autograd::Function<RelNode> {
     const int64_t nbytes = (int64_t)g_api.rel_fwd_workspace_bytes(&p, &r);
     const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
     check_rc(g_api.rel_fwd(&p, &r, out.data_ptr(), ws.data_ptr(), nbytes, stream_of(q.device())), "sigattn_rel_fwd");
+    // (The workspace now holds the lines, which the backward reads too.)
+    ctx->save_for_backward({q, k, v, table, buckets, bias, scale, cu_q, cu_k, ws});
     return out;
   }
 
@@ -338,7 +339,7 @@ struct RelNode : public torch::autograd::Function<RelNode> {
     const sigattn_rel_bias r = make_rel(table, buckets);
     const int64_t nbytes = (int64_t)g_api.rel_bwd_workspace_bytes(&p, &r);
     const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
-    check_rc(g_api.rel_bwd(&p, &r, dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
+    check_rc(g_api.rel_bwd(&p, &r, saved[9].data_ptr(), dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
                            want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes, stream_of(q.device())),
              "sigattn_rel_bwd");
     differentiable_once(result);

@@ -173,7 +173,7 @@ class SigattnRotary(ctypes.Structure):
 
 # Farthest relative position and most buckets of the learned bias
 # (SIGATTN_REL_MAX_DISTANCE, SIGATTN_REL_MAX_BUCKETS).
-REL_MAX_DISTANCE, REL_MAX_BUCKETS = 2048, 65536
+REL_MAX_DISTANCE, REL_MAX_BUCKETS = 2048, 4096
 
 # Largest batch of sigattn_paged_plan (SIGATTN_PLAN_MAX_BATCH).
 PLAN_MAX_BATCH = 8192
@@ -216,7 +216,7 @@ SIGNATURES = {
     "sigattn_rel_bwd_workspace_bytes": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)],
                                         ctypes.c_size_t),
     "sigattn_rel_bwd": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias), _c_vp, _c_vp, _c_vp, _c_vp,
-                         _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
+                         _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
     "sigattn_paged_rel_check": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias)], _c_i32),
     "sigattn_paged_rel_fwd_workspace_bytes": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias)],
                                               ctypes.c_size_t),
@@ -761,7 +761,7 @@ def backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seql
     def run(stream):
         nbytes = int(lib.sigattn_rel_bwd_workspace_bytes(ctypes.byref(pr), ctypes.byref(r)))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
-        _raise(lib.sigattn_rel_bwd(ctypes.byref(pr), ctypes.byref(r), _ptr(dO), _ptr(dQ), _ptr(dK), _ptr(dV),
+        _raise(lib.sigattn_rel_bwd(ctypes.byref(pr), ctypes.byref(r), None, _ptr(dO), _ptr(dQ), _ptr(dK), _ptr(dV),
                                    _ptr(dtable), ws.data_ptr(), nbytes, stream), "sigattn_rel_bwd")
 
     _on_device(Q.device, run)
