@@ -405,16 +405,12 @@ int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r);
  * table again (NULL: it is).
  * `dtable` is the table's gradient, [num_buckets, H] of its type, written whole:
  * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed).
- * Deterministic.  At head_dim 128 in f16 / bf16, max_distance (or the longest
- * sequence) up to 320, a workspace of sigattn_rel_bwd_two_pass_bytes(p, r)
- * (0: no such form) runs the two-pass backward (sigattn_bwd_ws); `dtable` is then
- * the sum of dS as dK and dQ take it, rounded to the I/O dtype.
+ * Deterministic.
  */
 size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
 int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
                     size_t workspace_bytes, void *stream);
 size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
-size_t sigattn_rel_bwd_two_pass_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
                     void *dk, void *dv, void *dtable, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -5,9 +5,7 @@ term is then a matrix).
 The table's gradient is a sum of dS as the kernels hold it in fp32, before any
 rounding to the I/O dtype: each dS is off by reference64's share of it without that
 rounding, the sum of a bucket by (longest chain of additions) e of the sum of their
-sizes, and it is rounded once to the table's dtype.  At head_dim 128 in 16 bits, where
-the two-pass backward sums what it stored, each dS is off by half a step of the I/O
-dtype more (u of it + tiny).
+sizes, and it is rounded once to the table's dtype.
 """
 
 import math
@@ -68,8 +66,6 @@ def packed_rel(q, k, v, do, table, buckets, cu_q, cu_k, causal, bias=None):
             if do is None:
                 continue
             ds, eds = grad_of_scores(*heads, add, causal)
-            if q.shape[2] == 128 and dtype != torch.float32:
-                eds = eds + torch.where(ds != 0, u * (ds.abs() + eds) + tiny, 0.0)
             at = torch.where(bucket >= 0, bucket, table.shape[0]).flatten()
             for to, what in ((out["dtable"][0], ds), (out["dtable"][1], eds), (size, ds.abs())):
                 col = torch.zeros(table.shape[0] + 1, dtype=torch.float64, device=dev)

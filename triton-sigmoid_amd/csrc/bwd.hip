@@ -535,6 +535,238 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_pair_kernel(const KParams p) 
   }
 }
 
+// ---------------------------------------------------------------------------
+// dQ of the two-pass backward: dQ = dS · K · scale from the dS tiles the dK/dV
+// kernel stored (DsLayout), with no recomputation of S, P or dP.
+// Workgroup = NW waves x 64 queries (two 32-query column blocks per wave);
+// keys stream in stages of KB 32-key blocks through an NST-stage LDS ring:
+// the K rows (shared by the waves) and each wave's own dS tiles (its two
+// query blocks x KB key blocks), all by direct global->LDS copies issued
+// NST-1 stages ahead, so about (NST-1) x (32 KB x KB dS + K) per CU is in
+// flight against HBM latency.
+//   dQᵀ[d, q] += Kᵀ[d, key] · dSᵀ[key, q]
+// A = Kᵀ via ds_read_b64_tr_b16 from the row-major K rows; B = dSᵀ via
+// ds_read_b64_tr_b16 from the dS tile, which the copy lays out key-major
+// (64 bytes per key: its four 16-byte pieces (g-pair c, query half h) at
+// slot 2c + h), so lane (query n, k-slot h) receives keys 16ks + 4h + {0..3}
+// and 16ks + 8 + 4h + {0..3} -- the same key order as the Kᵀ read.
+// Per 32 keys a wave reads 4 KB of dS and runs 16 MFMAs: the kernel is bound
+// by HBM bandwidth.
+// ---------------------------------------------------------------------------
+#ifndef SIGATTN_DQDS_NT
+#define SIGATTN_DQDS_NT 1
+#endif
+constexpr bool kDqDsNT = SIGATTN_DQDS_NT != 0;
+
+// Waves per SIMD of the kernel's resident workgroups (its register budget).
+template <int D, int NW, int KB, int NST> constexpr int dq_ds_waves_per_simd() {
+  const int occ = 163840 / (NST * (32 * KB * D + NW * 2 * KB * DsLayout::kTileElems) * 2);
+  return occ * NW / 4 > 1 ? occ * NW / 4 : 1;
+}
+
+template <typename T, int D, bool CAUSAL, int NW, int KB, int NST>
+__global__ __launch_bounds__(64 * NW, (dq_ds_waves_per_simd<D, NW, KB, NST>())) void bwd_dq_ds_kernel(
+    const KParams p) {
+  constexpr int BM = 64 * NW, BN = 32 * KB;
+  constexpr int NDB = D / 32;
+  constexpr int TE = DsLayout::kTileElems;
+  constexpr int KI = BN * D / 8 / 64 / NW;  // K-row copy instructions per wave and stage
+  constexpr int NI = KI + 4 * KB;           // copy instructions per wave and stage
+  constexpr int PF = NST - 1;               // stages in flight ahead of the one computed
+  // Resident workgroups per CU, by the LDS ring's size (160 KB per CU).
+  constexpr int OCC = 163840 / (NST * (BN * D + NW * 2 * KB * TE) * 2);
+  static_assert(KI >= 1 && (NST - 2) * NI < 64 && OCC >= 1, "stage shape");
+
+  __shared__ __attribute__((aligned(16))) uint16_t sK[NST][BN * D];
+  __shared__ __attribute__((aligned(16))) uint16_t sS[NST][NW * 2 * KB * TE];
+
+  const int wg = gap_prologue<2>(p, sK);  // packed layouts: leading gap-zeroing workgroups
+  if (wg < 0) return;
+  int b, h, qblk;
+  if (p.ragged() && p.B <= 64) {
+    const auto lq = [&](int i) SIGATTN_INLINE { return p.len_q(i); };
+    const auto lk = [&](int i) SIGATTN_INLINE { return p.len_k(i); };
+    const WorkItem it = CAUSAL ? WorkOrder::by_level(wg, p.B, p.H, lq, BM, p.nblk, true, p.ncu, OCC)
+                               : WorkOrder::by_stream(wg, p.B, p.H, lq, BM, p.nblk, lk);
+    b = it.b, h = it.h, qblk = it.blk;
+  } else {
+    const int BH = p.B * p.H;
+    int bh;
+    dense_item(wg, BH, p.nblk, !CAUSAL, bh, qblk);
+    if (CAUSAL) qblk = p.nblk - 1 - qblk;  // heaviest query blocks first
+    b = bh / p.H, h = bh % p.H;
+  }
+  const int Lq = p.len_q(b);
+  const int Lk = p.len_k(b);
+  // Padding item: its zero rows as part of one contiguous span (see zero_row_span).
+  if (qblk * BM >= Lq && p.q_rows_contiguous(D)) {
+    zero_row_span((uint16_t *)p.dq + (int64_t)b * p.sq_b, p.sq_t, qblk * BM, min(qblk * BM + BM, p.Tq), h,
+                  p.H, threadIdx.x, 64 * NW);
+    return;
+  }
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const int q0 = qblk * BM;
+  const int qbw = q0 / 32 + 2 * w;  // the wave's two query blocks: qbw, qbw + 1
+  const int nqb_valid = (Lq + 31) / 32, nkb_valid = (Lk + 31) / 32;
+
+  const int64_t qoff = p.q_base(b, h);
+  const int64_t koff = p.k_base(b, h);
+  const uint16_t *Kb = (const uint16_t *)p.k + koff;
+  uint16_t *dQb = (uint16_t *)p.dq + qoff;
+  const uint16_t *ds_bh = p.ds + ((int64_t)b * p.H + h) * DsLayout::per_bh(p.ds_nqb, p.ds_nkb, CAUSAL) * TE;
+
+  int nend = Lk;
+  if (CAUSAL) nend = min(nend, min(q0 + BM, Lq));
+  if (q0 >= Lq) nend = 0;
+  const int ntiles = (nend + BN - 1) / BN;
+
+  // Tile (query block qb, key block kb) was stored by the dK/dV pass.
+  auto tile_ok = [&](int qb, int kb) SIGATTN_INLINE {
+    return qb < nqb_valid && kb < nkb_valid && (!CAUSAL || kb <= qb);
+  };
+
+  TileOffsets<D> to;
+  to.init(lane);
+  DmaPlan<BN, D, NW> dma;
+  dma.init(w, lane);
+  const int kv_stride_bytes = (int)(p.sk_t * 2);
+
+  // Copy of a dS tile: instruction i fills keys 16i .. 16i+15 (1 KB); lane
+  // j lands at key 16i + j/4, slot j%4 = (g-pair c, half h) and fetches
+  // piece c of the stored lane 32h + key (at 1024 c + 16 (32h + key)).
+  uint32_t soff[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 16 * i + lane / 4, s = lane % 4;
+    soff[i] = (uint32_t)((s >> 1) * 1024 + 16 * ((s & 1) * 32 + key));
+  }
+  // dSᵀ operand read: lane (group g16, s = 4e + m) reads key 16ks + 4h + e
+  // (+8 for the second half), queries 4M .. 4M+3 with M = 4(g16 & 1) + m.
+  int boff;
+  {
+    const int g16 = lane >> 4, s = lane & 15, e = s >> 2, m = s & 3, hh = g16 >> 1;
+    boff = 32 * (4 * hh + e) + 8 * (2 * (g16 & 1) + (m & 1)) + 4 * (m >> 1);
+  }
+  auto ld_ds = [&](const uint16_t *tile, int ks) SIGATTN_INLINE {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    const uint16_t *base = tile + 512 * ks + boff;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)base);
+    const s16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4 *)(base + 256));
+    const u32x2 lo = __builtin_bit_cast(u32x2, a);
+    const u32x2 hv = __builtin_bit_cast(u32x2, c);
+    return (u32x4){lo.x, lo.y, hv.x, hv.y};
+  };
+  // LDS slot of the wave's tile (column block cb, key block kl of the stage).
+  auto ds_slot = [&](int st, int cb, int kl) SIGATTN_INLINE {
+    return &sS[st][((4 * w + 2 * cb) * KB + 2 * kl) * TE / 2];
+  };
+
+  auto issue = [&](int st, int u) SIGATTN_INLINE {
+    dma.issue(sK[st], Kb, kv_stride_bytes, u * BN, Lk);
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+#pragma unroll
+      for (int kl = 0; kl < KB; ++kl) {
+        const int qb = qbw + cb, kb = KB * u + kl;
+        // Tiles the dK/dV pass did not store are replaced by tile 0 of this
+        // (batch, head) (in bounds; their products are skipped).
+        const int64_t ti = tile_ok(qb, kb) ? DsLayout::tile(qb, kb, p.ds_nqb, CAUSAL) : 0;
+        const uint16_t *src = ds_bh + ti * TE;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint16_t *dst = ds_slot(st, cb, kl) + 512 * i;
+          const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+          // dS is read once: non-temporal loads keep it from displacing the
+          // K rows the other workgroups of this (batch, head) re-read.
+          if constexpr (kDqDsNT)
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                         :
+                         : "v"(soff[i]), "s"(src), "{m0}"(m0)
+                         : "memory");
+          else
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                         :
+                         : "v"(soff[i]), "s"(src), "{m0}"(m0)
+                         : "memory");
+        }
+      }
+    }
+  };
+
+  f32x16 acc[2][NDB];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) acc[c][d] = zero16();
+
+  // Every MFMA runs on every stage: a tile the dK/dV pass did not store
+  // enters as a zero operand (the K rows are finite, so it adds exactly 0).
+  // Branching around the products instead makes the compiler copy all the
+  // accumulators at every join.
+  auto compute = [&](int st, int u) SIGATTN_INLINE {
+#pragma unroll
+    for (int kl = 0; kl < KB; ++kl) {
+      const int kb = KB * u + kl;
+      const bool ok0 = tile_ok(qbw, kb), ok1 = tile_ok(qbw + 1, kb);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int ks = 2 * kl + j;
+        u32x4 b0 = ld_ds(ds_slot(st, 0, kl), j);
+        u32x4 b1 = ld_ds(ds_slot(st, 1, kl), j);
+        b0 = ok0 ? b0 : zero4();
+        b1 = ok1 ? b1 : zero4();
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const u32x4 a = ld_tr<D>(sK[st], to, ks, db);
+          acc[0][db] = Elem<T>::mfma(a, b0, acc[0][db]);
+          acc[1][db] = Elem<T>::mfma(a, b1, acc[1][db]);
+        }
+      }
+    }
+  };
+
+#pragma unroll
+  for (int u = 0; u < PF; ++u)
+    if (u < ntiles) issue(u, u);
+  for (int u = 0; u < ntiles; ++u) {
+    // Wait for this wave's copies of stage u (the later stages' copies may
+    // stay in flight), then for every wave's.
+    wait_vm_steps<NI, PF - 1>(min(ntiles - 1 - u, PF - 1));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // The stage the copy fills last held stage u-1, which every wave has
+    // finished reading (they all passed the barrier above after computing it).
+    if (u + PF < ntiles) issue((u + PF) % NST, u + PF);
+    compute(u % NST, u);
+  }
+
+  const float scale = *p.scale;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int my_q = q0 + 64 * w + 32 * c + l32;
+    if (my_q < p.q_rows_out(Lq)) {
+      uint16_t *row = dQb + (int64_t)my_q * p.sq_t;
+      const bool valid = my_q < Lq;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d0 = db * 32 + 8 * g + 4 * hi;
+          u32x2 o;
+          o.x = Elem<T>::pack(acc[c][db][4 * g] * scale, acc[c][db][4 * g + 1] * scale);
+          o.y = Elem<T>::pack(acc[c][db][4 * g + 2] * scale, acc[c][db][4 * g + 3] * scale);
+          if (!valid) o = (u32x2){0u, 0u};
+          *(u32x2 *)(row + d0) = o;
+        }
+      }
+    }
+  }
+}
+
 template <int ROWBLK, typename Launch>
 static void launch_rows(const KParams &kp, int rows, Launch &&launch) {
   KParams p = kp;
@@ -644,8 +876,8 @@ static void bwd_dq_ds_t(const KParams &kp, bool causal, hipStream_t st) {
     if (SIGATTN_DQDS_SMALL_GRID && NW128 == 8 && wide < kp.ncu) {
       launch_rows<256>(kp, kp.Tq, [&](const KParams &p, dim3 grid) {
         grid.x += (unsigned)(p.ngap[0] + p.ngap[1]);
-        if (causal) bwd_dq_ds_kernel<T, D, true, 4, 1, 3, KParams><<<grid, 256, 0, st>>>(p);
-        else bwd_dq_ds_kernel<T, D, false, 4, 1, 3, KParams><<<grid, 256, 0, st>>>(p);
+        if (causal) bwd_dq_ds_kernel<T, D, true, 4, 1, 3><<<grid, 256, 0, st>>>(p);
+        else bwd_dq_ds_kernel<T, D, false, 4, 1, 3><<<grid, 256, 0, st>>>(p);
       });
       return;
     }
@@ -657,11 +889,11 @@ static void bwd_dq_ds_t(const KParams &kp, bool causal, hipStream_t st) {
     // divide over 8 waves' copies), 6-stage ring.
     grid.x += (unsigned)(p.ngap[0] + p.ngap[1]);
     if constexpr (D == 128) {
-      if (causal) bwd_dq_ds_kernel<T, D, true, NW128, 1, NST128, KParams><<<grid, 64 * NW128, 0, st>>>(p);
-      else bwd_dq_ds_kernel<T, D, false, NW128, 1, NST128, KParams><<<grid, 64 * NW128, 0, st>>>(p);
+      if (causal) bwd_dq_ds_kernel<T, D, true, NW128, 1, NST128><<<grid, 64 * NW128, 0, st>>>(p);
+      else bwd_dq_ds_kernel<T, D, false, NW128, 1, NST128><<<grid, 64 * NW128, 0, st>>>(p);
     } else {
-      if (causal) bwd_dq_ds_kernel<T, D, true, 4, 1, 6, KParams><<<grid, 256, 0, st>>>(p);
-      else bwd_dq_ds_kernel<T, D, false, 4, 1, 6, KParams><<<grid, 256, 0, st>>>(p);
+      if (causal) bwd_dq_ds_kernel<T, D, true, 4, 1, 6><<<grid, 256, 0, st>>>(p);
+      else bwd_dq_ds_kernel<T, D, false, 4, 1, 6><<<grid, 256, 0, st>>>(p);
     }
   });
 }

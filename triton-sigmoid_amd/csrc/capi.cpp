@@ -338,6 +338,13 @@ void use_range_split(KParams &k, const RangeSplit &r, void *ws) {
   k.rs_part = (float *)((char *)ws + r.cnt_bytes);
 }
 
+// Two-pass backward: bytes of dS tiles (DsLayout) per head, over all batches.
+int64_t ds_bytes_per_head(const sigattn_problem *p) {
+  const int64_t nqb = cdiv(p->Tq, 32), nkb = cdiv(p->Tk, 32);
+  const int64_t tiles = p->causal != 0 ? nqb * (nqb + 1) / 2 : nqb * nkb;
+  return p->B * tiles * 2048;
+}
+
 // The sub-problem of heads [h0, h0 + nh), whole groups: every tensor is
 // [.., H, D] with its own head stride, so the heads are a pointer offset away; bias,
 // score_mod and the sequence lengths are per batch and stay as they are.

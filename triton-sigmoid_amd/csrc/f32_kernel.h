@@ -219,7 +219,7 @@ __device__ __forceinline__ void dq_full(const P &p, const Item &w_, float *lds, 
   F32RowReads<D> rr;
   rr.init(l32, hi);
   const int stride_bytes = (int)(p.sk_t * 4);
-  [[maybe_unused]] PlaceSums<FW> sums;  // from nothing again
+  [[maybe_unused]] PlaceSums sums;  // from nothing again
   if constexpr (P::kRel) sums.init(p, near, w, tid);
   for (int t = 0; t < ntiles; ++t) {
     float *tK = lds + (t & 1) * 2 * FB * D, *tV = tK + FB * D, *tC = lds + 4 * FB * D + (t & 1) * FB;
@@ -748,7 +748,7 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dq_f32_
   to.init(lane);
   Tiles st;
   [[maybe_unused]] const int win0 = FB * wt + 4 * hi + RB - (myq - it.row0);  // as in the forward
-  [[maybe_unused]] PlaceSums<FW> sums;
+  [[maybe_unused]] PlaceSums sums;
   if constexpr (P::kRel) sums.init(p, near, w, tid);
   float creg = 0.0f;
   auto load = [&](int t) SIGATTN_INLINE {
@@ -962,7 +962,7 @@ template <class P, class F> void by_terms(const P &p, bool causal, F &&f) {
 
 // LDS of the dQ kernel's PlaceSums.
 template <class P> size_t rel_near_bytes(const P &p) {
-  if constexpr (P::kRel && !P::kPaged) return p.part != nullptr ? near_floats(p.reach, FW) * sizeof(float) : 0;
+  if constexpr (P::kRel && !P::kPaged) return p.part != nullptr ? near_floats(p.reach) * sizeof(float) : 0;
   else return 0;
 }
 

@@ -96,13 +96,6 @@ inline bool use_f32_mfma(const sigattn_problem *p, const void *const *ptrs, int 
 // kernels (KParams::dmem = 16).
 inline int mfma_head_dim(const sigattn_problem *p) { return p->D == 16 ? 32 : (int)p->D; }
 
-// Two-pass backward: bytes of dS tiles (DsLayout) per head, over all batches.
-inline int64_t ds_bytes_per_head(const sigattn_problem *p) {
-  const int64_t nqb = cdiv(p->Tq, 32), nkb = cdiv(p->Tk, 32);
-  const int64_t tiles = p->causal != 0 ? nqb * (nqb + 1) / 2 : nqb * nkb;
-  return p->B * tiles * 2048;
-}
-
 // Head split of grouped dK/dV items (KParams::qsplit).  Items are K / V heads
 // times key blocks, a group's queries long each: with few of them the GPU
 // waits for the last.  The fewest parts, up to a head each, that make two

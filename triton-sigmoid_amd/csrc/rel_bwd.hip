@@ -16,10 +16,10 @@ __global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelParams p) {
   if (wg >= 0) bwd_dq_body<T, D, WK, CAUSAL, false, RelParams>(p, wg, lds, near);
 }
 
-template <typename T, int D, bool CAUSAL, bool DSOUT, bool GROUPED>
+template <typename T, int D, bool CAUSAL, bool GROUPED>
 __global__ __launch_bounds__(256, (D <= 64 ? 2 : 1)) void rel_dkdv_kernel(const RelParams p) {
   __shared__ __attribute__((aligned(16))) DkdvLds<D, dkdv_window<RelParams>()> lds;
-  bwd_dkdv_body<T, D, CAUSAL, false, DSOUT, GROUPED, RelParams>(p, blockIdx.x, lds);
+  bwd_dkdv_body<T, D, CAUSAL, false, false, GROUPED, RelParams>(p, blockIdx.x, lds);
 }
 
 template <typename T, int D, int WK> void dq_w(const RelParams &kp, bool causal, hipStream_t st) {
@@ -27,7 +27,7 @@ template <typename T, int D, int WK> void dq_w(const RelParams &kp, bool causal,
   p.part_rows = 128 / WK;
   p.nblk = (p.Tq + p.part_rows - 1) / p.part_rows;
   const dim3 grid((unsigned)(p.nblk * p.B * p.H + p.ngap[0] + p.ngap[1]));
-  const size_t line = p.part != nullptr ? near_floats(p.reach, 4) * sizeof(float) : 0;
+  const size_t line = p.part != nullptr ? near_floats(p.reach) * sizeof(float) : 0;
   if (causal) rel_dq_kernel<T, D, WK, true><<<grid, 256, line, st>>>(p);
   else rel_dq_kernel<T, D, WK, false><<<grid, 256, line, st>>>(p);
 }
@@ -37,17 +37,17 @@ bool dq_pairs(const RelParams &p, int D, bool causal) {
   return D <= 64 && dq_wave_pairs((int64_t)p.B * p.H, p.Tq, p.Tk, causal, p.ragged(), p.ncu);
 }
 
-template <typename T, int D, bool DSOUT> void dkdv_t(const RelParams &kp, bool causal, hipStream_t st) {
+template <typename T, int D> void dkdv_t(const RelParams &kp, bool causal, hipStream_t st) {
   RelParams p = kp;
   p.nblk = (p.Tk + 127) / 128;
   dim3 grid((unsigned)(p.nblk * p.B * p.H));
   if (p.qgroup > 1) {
     if (p.qsplit > 1) grid.x *= (unsigned)p.qsplit;
-    if (causal) rel_dkdv_kernel<T, D, true, DSOUT, true><<<grid, 256, 0, st>>>(p);
-    else rel_dkdv_kernel<T, D, false, DSOUT, true><<<grid, 256, 0, st>>>(p);
+    if (causal) rel_dkdv_kernel<T, D, true, true><<<grid, 256, 0, st>>>(p);
+    else rel_dkdv_kernel<T, D, false, true><<<grid, 256, 0, st>>>(p);
   } else {
-    if (causal) rel_dkdv_kernel<T, D, true, DSOUT, false><<<grid, 256, 0, st>>>(p);
-    else rel_dkdv_kernel<T, D, false, DSOUT, false><<<grid, 256, 0, st>>>(p);
+    if (causal) rel_dkdv_kernel<T, D, true, false><<<grid, 256, 0, st>>>(p);
+    else rel_dkdv_kernel<T, D, false, false><<<grid, 256, 0, st>>>(p);
   }
 }
 
@@ -76,35 +76,11 @@ void launch_rel_dq_mfma(const RelParams &p, int dtype, int D, bool causal, hipSt
   });
 }
 
-void launch_rel_dkdv_mfma(const RelParams &p, int dtype, int D, bool causal, bool dsout, hipStream_t st) {
+void launch_rel_dkdv_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st) {
   by_type(dtype, D, [&](auto *t, auto d) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int DD = decltype(d)::value;
-    if constexpr (DD == 128) {
-      if (dsout) return dkdv_t<T, DD, true>(p, causal, st);
-    }
-    dkdv_t<T, DD, false>(p, causal, st);
+    dkdv_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(p, causal, st);
   });
   launch_add_parts(p, dtype, st);
-}
-
-// Three stages of the ring, where the kernel without the bias has four, leave the
-// sums by position their LDS (27 KB at a reach of 128).
-template <typename T> static void dq_ds_t(const RelParams &kp, bool causal, hipStream_t st) {
-  constexpr int NW = kRelDsRows / 64, NST = 3;
-  constexpr int ring = NST * (32 * 128 + NW * 2 * DsLayout::kTileElems) * 2;
-  static_assert(ring + near_floats(kRelDsReach, NW) * 4 + 256 <= 163840, "LDS");
-  RelParams p = kp;
-  p.nblk = (p.Tq + kRelDsRows - 1) / kRelDsRows;
-  const dim3 grid((unsigned)(p.nblk * p.B * p.H + p.ngap[0] + p.ngap[1])), block(64 * NW);
-  const size_t line = p.part != nullptr ? near_floats(p.reach, NW) * sizeof(float) : 0;
-  if (causal) bwd_dq_ds_kernel<T, 128, true, NW, 1, NST, RelParams><<<grid, block, line, st>>>(p);
-  else bwd_dq_ds_kernel<T, 128, false, NW, 1, NST, RelParams><<<grid, block, line, st>>>(p);
-}
-
-void launch_rel_dq_ds_mfma(const RelParams &p, int dtype, bool causal, hipStream_t st) {
-  if (dtype == kBF16) dq_ds_t<__bf16>(p, causal, st);
-  else dq_ds_t<_Float16>(p, causal, st);
 }
 
 }  // namespace sigattn

@@ -94,13 +94,6 @@ size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_r
   return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
 }
 
-size_t sigattn_rel_bwd_two_pass_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
-  if (sigattn_rel_check(p, r) != SIGATTN_OK || p->D != 128 || p->Tq == 0 || p->Tk == 0 || p->B == 0 || p->H == 0) return 0;
-  const void *none[1] = {nullptr};
-  if (!use_mfma(p, none, 0) || rel_table(r, p->H, p->Tq, p->Tk).reach > kRelDsReach) return 0;
-  return sigattn_rel_bwd_workspace_bytes(p, r) + (size_t)(ds_bytes_per_head(p) * p->H);
-}
-
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
                     void *dk, void *dv, void *dtable, void *workspace, size_t workspace_bytes, void *stream) {
   const int rc = sigattn_rel_check(p, r);
@@ -137,27 +130,17 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     const HeadSplit hs = head_split(p, mfma);
     k.qsplit = hs.n;
     k.kv_part = (float *)(parts + rel_part_bytes(p, t));
-    const size_t two_pass = f32 ? 0 : sigattn_rel_bwd_two_pass_bytes(p, r);
-    const bool dsout = two_pass > 0 && workspace_bytes >= two_pass;
-    if (dsout) {
-      k.ds = (uint16_t *)(parts + rel_part_bytes(p, t) + hs.bytes);
-      k.ds_nqb = (int)cdiv(p->Tq, 32);
-      k.ds_nkb = (int)cdiv(p->Tk, 32);
-    }
-    k.part_rows = dsout ? kRelDsRows : f32 ? rel_dq_rows_f32(k, D, causal) : rel_dq_rows(k, D, causal);
+    k.part_rows = f32 ? rel_dq_rows_f32(k, D, causal) : rel_dq_rows(k, D, causal);
     RelParams kq = k;
     GapAxis gq, gk;
     gap_axes(p, dq, dk, dv, gq, gk);
     use_gaps(kq, gq, gk);
-    if (dsout) {
-      launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, true, st);
-      launch_rel_dq_ds_mfma(kq, p->dtype, causal, st);
-    } else if (f32) {
+    if (f32) {
       launch_rel_dq_f32(kq, D, causal, st);
       launch_rel_dkdv_f32(rel_kv_items(k), D, causal, st);
     } else {
       launch_rel_dq_mfma(kq, p->dtype, D, causal, st);
-      launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, false, st);
+      launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, st);
     }
   } else {
     k.part_rows = kGenericRows;

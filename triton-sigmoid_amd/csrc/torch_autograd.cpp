@@ -68,7 +68,6 @@ struct Api {
   decltype(&sigattn_rel_fwd_workspace_bytes) rel_fwd_workspace_bytes = nullptr;
   decltype(&sigattn_rel_fwd) rel_fwd = nullptr;
   decltype(&sigattn_rel_bwd_workspace_bytes) rel_bwd_workspace_bytes = nullptr;
-  decltype(&sigattn_rel_bwd_two_pass_bytes) rel_bwd_two_pass_bytes = nullptr;
   decltype(&sigattn_rel_bwd) rel_bwd = nullptr;
   decltype(&sigattn_paged_rel_fwd_workspace_bytes) paged_rel_fwd_workspace_bytes = nullptr;
   decltype(&sigattn_paged_rel_fwd) paged_rel_fwd = nullptr;
@@ -195,9 +194,6 @@ int64_t two_pass_bytes(const sigattn_problem &p, int64_t limit, int dev) {
   if (heads == 0 || grid < compute_units(dev)) return 0;
   return heads * per_head;
 }
-
-// _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB.
-int64_t default_limit(int64_t H, int64_t Hkv) { return (int64_t)(H == Hkv ? 2048 : 8192) << 20; }
 
 struct SigattnNode : public torch::autograd::Function<SigattnNode> {
   static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
@@ -341,13 +337,8 @@ struct RelNode : public torch::autograd::Function<RelNode> {
     const c10::DeviceGuard guard(q.device());
     const sigattn_problem p = make_problem(q, k, v, saved[5], Tensor(), saved[6], lay, ctx->saved_data["causal"].toBool());
     const sigattn_rel_bias r = make_rel(table, buckets);
-    int64_t nbytes = (int64_t)g_api.rel_bwd_two_pass_bytes(&p, &r);
-    Tensor ws;
-    if (nbytes > 0 && nbytes <= default_limit(q.size(1), k.size(1))) ws = workspace(nbytes, q);
-    if (!ws.defined()) {
-      nbytes = (int64_t)g_api.rel_bwd_workspace_bytes(&p, &r);
-      ws = at::empty({nbytes}, q.options().dtype(at::kByte));
-    }
+    const int64_t nbytes = (int64_t)g_api.rel_bwd_workspace_bytes(&p, &r);
+    const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
     check_rc(g_api.rel_bwd(&p, &r, saved[9].data_ptr(), dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
                            want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes, stream_of(q.device())),
              "sigattn_rel_bwd");
@@ -380,11 +371,6 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
     ctx->save_for_backward({positions, angles});
     ctx->saved_data["pairs"] = pairs;
     ctx->saved_data["inverse"] = inverse;
-    return run(q, k, positions, angles, pairs, inverse);
-  }
-
-  static tensor_list run(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &angles, bool pairs,
-                         bool inverse) {
     const c10::DeviceGuard guard(q.device());
     const Tensor a = unit_stride(q), b = unit_stride(k);
     const Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
@@ -397,10 +383,8 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
 
   static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const bool pairs = ctx->saved_data["pairs"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
-    const tensor_list g = at::GradMode::is_enabled()
-                              ? RotaryNode::apply(grads[0], grads[1], saved[0], saved[1], pairs, inverse)
-                              : run(grads[0], grads[1], saved[0], saved[1], pairs, inverse);
+    const tensor_list g = RotaryNode::apply(grads[0], grads[1], saved[0], saved[1], ctx->saved_data["pairs"].toBool(),
+                                            !ctx->saved_data["inverse"].toBool());
     return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -614,7 +598,7 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
              "sigattn_default_bias");
   }
   if (rel) return py::cast(RelNode::apply(q, k, v, table, buckets, bias, st, cq, ck, mq, mk, is_causal.ptr() == Py_True));
-  const int64_t limit = default_limit(H, Hkv);
+  const int64_t limit = (int64_t)(H == Hkv ? 2048 : 8192) << 20;  // _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB
   return py::cast(SigattnNode::apply(q, k, v, bias, sm.defined() ? std::optional<Tensor>(sm) : std::nullopt, st,
                                      std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
 }
@@ -850,7 +834,6 @@ void bind(const py::dict &fns, const std::vector<int64_t> &two_pass_dims, int64_
   bind_one(api.rel_fwd_workspace_bytes, fns, "sigattn_rel_fwd_workspace_bytes");
   bind_one(api.rel_fwd, fns, "sigattn_rel_fwd");
   bind_one(api.rel_bwd_workspace_bytes, fns, "sigattn_rel_bwd_workspace_bytes");
-  bind_one(api.rel_bwd_two_pass_bytes, fns, "sigattn_rel_bwd_two_pass_bytes");
   bind_one(api.rel_bwd, fns, "sigattn_rel_bwd");
   bind_one(api.paged_rel_fwd_workspace_bytes, fns, "sigattn_paged_rel_fwd_workspace_bytes");
   bind_one(api.paged_rel_fwd, fns, "sigattn_paged_rel_fwd");
