@@ -429,7 +429,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
             // With three stages (four when a region is a tile) the copy below
             // refills the stage this region's Vᵀ operands came from: every
             // wave's reads of it complete first.
-            if constexpr (NST == 3 || WK == 2 || REL) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if constexpr (NST == 3 || WK == 2 || REL || SCOREMOD) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -541,7 +541,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
       if (u < ntiles) {
         wait_dma();
         store_c(u);
-        if constexpr (NST == 3 || WK == 2 || REL) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (NST == 3 || WK == 2 || REL || SCOREMOD) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
