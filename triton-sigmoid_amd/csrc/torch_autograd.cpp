@@ -371,6 +371,11 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
     ctx->save_for_backward({positions, angles});
     ctx->saved_data["pairs"] = pairs;
     ctx->saved_data["inverse"] = inverse;
+    return run(q, k, positions, angles, pairs, inverse);
+  }
+
+  static tensor_list run(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &angles, bool pairs,
+                         bool inverse) {
     const c10::DeviceGuard guard(q.device());
     const Tensor a = unit_stride(q), b = unit_stride(k);
     const Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
@@ -383,8 +388,10 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
 
   static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const tensor_list g = RotaryNode::apply(grads[0], grads[1], saved[0], saved[1], ctx->saved_data["pairs"].toBool(),
-                                            !ctx->saved_data["inverse"].toBool());
+    const bool pairs = ctx->saved_data["pairs"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
+    const tensor_list g = at::GradMode::is_enabled()
+                              ? RotaryNode::apply(grads[0], grads[1], saved[0], saved[1], pairs, inverse)
+                              : run(grads[0], grads[1], saved[0], saved[1], pairs, inverse);
     return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
