@@ -304,6 +304,41 @@ def test_empty_calls():
             assert g.shape == t.shape and not g.any()
 
 
+@pytest.mark.parametrize("D, dtype", [(64, "bf16"), (128, "f16"), (32, "f32")])
+def test_bindings_alike(monkeypatch, D, dtype):
+    args = make([300, 1, 77], [300, 1, 77], 4, 2, D, DT[dtype], 16, 60, seed=D)
+    node = run(*args, True)
+    monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    python = run(*args, True)
+    assert all(torch.equal(node[x], python[x]) for x in node)
+
+
+@pytest.mark.parametrize("binding", ["node", "python"])
+def test_gradients_have_none_of_their_own(monkeypatch, binding):
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    q, k, v, do, table, buckets, cu, _ = make([50], [50], 2, 2, 64, torch.bfloat16, 8, 20)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    o = ts.sigmoid_attention_varlen(*leaves[:3], ints(cu), ints(cu), 50, 50, bias_table=table, bias_buckets=buckets)
+    grads = torch.autograd.grad(o, leaves, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        sum(g.float().sum() for g in grads).backward()
+
+
+def test_more_sequences_than_the_sums_keep():
+    r = random.Random(6)
+    lens = [r.choice((0, 1, 2, r.randint(1, 12))) for _ in range(1300)]
+    check(make(lens, lens, 1, 1, 32, torch.bfloat16, 10, 9, seed=6), True)
+
+
+@pytest.mark.parametrize("f", [(1e-13, 1e12, 1e30, 1e-30), (1.0, 1.0, 1e-15, 1e-14), (1e10, 1e-10, 1e15, 1e10)])
+def test_fp32_values_far_from_one(f):
+    """What three bf16 parts cannot hold takes the fp32 instruction, the sums by position too."""
+    q, k, v, do, table, buckets, cu, _ = make([140, 33], [140, 33], 2, 1, 64, torch.float32, 12, 40)
+    q, k, v, do = (x * y for x, y in zip((q, k, v, do), f))
+    check((q, k, v, do, table, buckets, cu, cu), True)
+
+
 # --- over a paged cache ---------------------------------------------------------------
 
 def check_paged(ctx, new, H, Hkv, D, dtype, ps=16, num=16, R=40, causal=True, bias=None, mq="longest", seed=0,
@@ -465,3 +500,53 @@ def test_what_was_trained_is_served():
                                                bias_buckets=buckets))
         at += step
     assert_within(torch.cat(rows), want)
+
+
+def test_paged_streams_and_two_calls_at_once():
+    g = torch.Generator().manual_seed(1)
+    kc, vc = (randn(g, 40, 16, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    table, cu = torch.arange(40, dtype=I32, device="cuda").view(4, 10), ints([0, 1, 2, 3, 4])
+    buckets = torch.randint(0, 16, (201,), generator=g).to(I32).cuda()
+    calls = [(randn(g, 4, 8, 64, dtype=torch.bfloat16), randn(g, 16, 8, dtype=torch.bfloat16), ints(x))
+             for x in ([100, 3, 64, 160], [1, 160, 17, 33])]
+
+    def one(q, values, lens):
+        return ts.sigmoid_attention_paged(q, kc, vc, table, lens, cu, 1, is_causal=True, bias_table=values,
+                                          bias_buckets=buckets)
+
+    want = [one(*c) for c in calls]
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(one(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [90, 1]])
+def test_paged_bindings_alike(monkeypatch, new):
+    args = [300, 40], new, 8, 2, 64, torch.bfloat16
+    node = check_paged(*args, seed=9)
+    monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    assert torch.equal(node, check_paged(*args, seed=9))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [70, 1]])
+def test_paged_offsets_beyond_31_bits(new):
+    """A cache of more than 2^31 values: the same rows at its front and at its end."""
+    pages, ps, Hkv, D = 2 ** 31 // (16 * 2 * 128) + 40, 16, 2, 128
+    kc, vc = (torch.empty(pages, ps, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(2)
+    for c in (kc, vc):
+        c[:20] = randn(g, 20, ps, Hkv, D, dtype=torch.bfloat16)
+        c[-20:] = c[:20]
+    q, values = randn(g, sum(new), 8, D, dtype=torch.bfloat16), randn(g, 16, 8, dtype=torch.bfloat16)
+    buckets = torch.randint(0, 16, (101,), generator=g).to(I32).cuda()
+    front = torch.arange(20, dtype=I32, device="cuda").view(2, 10)
+    near, far = (ts.sigmoid_attention_paged(q, kc, vc, t, ints([160, 101]), ints(offsets(new)), max(new), is_causal=True,
+                                            bias_table=values, bias_buckets=buckets)
+                 for t in (front, front + (pages - 20)))
+    assert torch.equal(near, far) and near.any()

@@ -270,3 +270,52 @@ def test_scores_depend_on_the_difference_alone():
         rows.append(ts.sigmoid_attention_paged(a, kc, vc, plan.block_table, plan.seq_lens, plan.cu_seqlens, step,
                                                is_causal=True, sigmoid_bias=-2.0))
     assert (torch.cat(rows) - base).abs().max() <= 2 * bound
+
+
+def test_slots_beyond_31_bits():
+    """A cache of more than 2^31 values: rows at its end as at its front."""
+    pages, ps, Hkv, D, N = 2 ** 31 // (16 * 2 * 128) + 4, 16, 2, 128, 40
+    g = torch.Generator().manual_seed(4)
+    kc, vc = (torch.empty(pages, ps, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q, k, v = (randn(g, N, h, D, dtype=torch.bfloat16) for h in (4, Hkv, Hkv))
+    pos, angles = torch.arange(N, dtype=torch.int32, device="cuda"), ts.rotary_table(N, D, device="cuda")
+    slots = torch.arange(N, dtype=torch.int32, device="cuda")
+    for first in (0, pages * ps - N):
+        ts.paged_cache_write_rotary(q, k, v, kc, vc, slots + first, pos, angles)
+    for c in (kc, vc):
+        rows = c.view(-1, Hkv, D)
+        assert torch.equal(rows[:N], rows[-N:])
+    assert torch.equal(vc.view(-1, Hkv, D)[-N:], v)
+
+
+@pytest.mark.parametrize("D, pairs", [(64, False), (128, True), (16, False)])
+def test_bindings_alike(monkeypatch, D, pairs):
+    g = torch.Generator().manual_seed(5)
+    q, k, dq, dk = (randn(g, 100, h, D, dtype=torch.bfloat16) for h in (6, 2, 6, 2))
+    pos, angles = torch.arange(100, dtype=torch.int32, device="cuda"), ts.rotary_table(128, D, device="cuda")
+
+    def both():
+        a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+        out = ts.rotary_embedding(a, b, pos, angles, pairs)
+        return (*out, *torch.autograd.grad(out, (a, b), (dq, dk)))
+
+    node = both()
+    monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    assert all(torch.equal(x, y) for x, y in zip(node, both()))
+
+
+def test_streams_and_two_calls_at_once():
+    g = torch.Generator().manual_seed(6)
+    angles = ts.rotary_table(4096, 64, device="cuda")
+    pos = torch.arange(4000, dtype=torch.int32, device="cuda")
+    calls = [tuple(randn(g, 4000, h, 64, dtype=torch.float16) for h in (8, 2)) for _ in range(2)]
+    want = [ts.rotary_embedding(*c, pos, angles) for c in calls]
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(ts.rotary_embedding(*c, pos, angles))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))

@@ -206,6 +206,19 @@ def _varlen_rel_backward(ctx, dO):
 sigmoid_attn_varlen_rel_fwd_op.register_autograd(_varlen_rel_backward, setup_context=_varlen_rel_setup_context)
 
 
+class _Final(torch.autograd.Function):
+    """Gradients that have none of their own: a backward through them is an error,
+    whatever took part in them (the C++ node's says the same)."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice a function that was marked with @once_differentiable")
+
+
 class _VarlenRelEager(torch.autograd.Function):
     """Eager path of sigmoid_attention_varlen with the learned bias."""
 
@@ -218,11 +231,14 @@ class _VarlenRelEager(torch.autograd.Function):
                                  sm_scale, is_causal)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dO):
         Q, K, V, table, buckets, cu_seqlens_k, cu_seqlens_q, bias, sm_scale = ctx.saved_tensors
         grads = _capi.backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k, bias,
                                    table, buckets, sm_scale, ctx.is_causal, ctx.needs_input_grad[3])
+        if torch.is_grad_enabled():
+            there = [g for g in grads if g is not None]
+            final = iter(_Final.apply(*(g.detach().requires_grad_() for g in there)))
+            grads = [g if g is None else next(final) for g in grads]
         return (*grads, *(None,) * 8)
 
 
