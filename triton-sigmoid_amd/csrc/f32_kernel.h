@@ -707,17 +707,14 @@ __global__ __launch_bounds__(64 * FW, (fwd_f32_occupancy<D, WK>())) void fwd_f32
 }
 
 // dQ = (dP ⊙ P ⊙ (1 - P)) · K · scale with dP = dO · Vᵀ; keys streamed.
+// near: P::kRel, LDS of PlaceSums.
 template <int D, bool CAUSAL, bool SCOREMOD, int WK, class P>
-__global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dq_f32_kernel(const P p) {
+__device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[maybe_unused]] float *near) {
   constexpr int NKS = D / 16, NDB = D / 32, TR = FB * WK, RB = FB * FW / WK, WIN = TR + RB;
   using Tiles = SplitTiles<D, TR>;
-  __shared__ __attribute__((aligned(16))) float lds[lds_floats<D, WK>() + (P::kRel ? WIN : SCOREMOD ? 2 * TR : 0)];
   uint16_t *tiles = (uint16_t *)lds;
   float *sC = lds + lds_floats<D, WK>();
-  extern __shared__ __attribute__((aligned(16))) float near[];  // P::kRel: PlaceSums
 
-  const int wg = gap_prologue<4>(p, lds);  // packed layouts: leading gap-zeroing workgroups
-  if (wg < 0) return;
   const Item it = item_of<WK, CAUSAL, true>(p, wg, bwd_f32_occupancy<D, WK>());
   const int b = it.b, h = it.h;
   const int Lq = p.len_q(b), Lk = p.len_k(b);
@@ -810,14 +807,13 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dq_f32_
 
 // dV = Pᵀ · dO and dK = dSᵀ · Q · scale; queries streamed.
 template <int D, bool CAUSAL, bool SCOREMOD, int WK, class P>
-__global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f32_kernel(const P p) {
+__device__ __forceinline__ void dkdv_f32_body(const P &p, int block, float *lds) {
   constexpr int NKS = D / 16, NDB = D / 32, TR = FB * WK, RB = FB * FW / WK, WIN = TR + RB;
   using Tiles = SplitTiles<D, TR>;
-  __shared__ __attribute__((aligned(16))) float lds[lds_floats<D, WK>() + (P::kRel ? WIN : 0)];
   uint16_t *tiles = (uint16_t *)lds;
   [[maybe_unused]] float *sC = lds + lds_floats<D, WK>();
 
-  const int nparts = p.qsplit > 1 ? p.qsplit : 1, wg = (int)blockIdx.x / nparts, part = (int)blockIdx.x - wg * nparts;
+  const int nparts = p.qsplit > 1 ? p.qsplit : 1, wg = block / nparts, part = block - wg * nparts;
   const Item it = item_of<WK, CAUSAL, false>(p, wg, bwd_f32_occupancy<D, WK>());
   const int b = it.b, h = it.h;
   const int Lq = p.len_q(b), Lk = p.len_k(b);
@@ -919,6 +915,25 @@ __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f3
     store_row<D>((float *)p.dk + koff + (int64_t)myk * p.sk_t, dka, scale, kok, hi, half);
     store_row<D>((float *)p.dv + koff + (int64_t)myk * p.sk_t, dva, 1.0f, kok, hi, half);
   }
+}
+
+// LDS of a workgroup: the tiles, and the additive terms' windows or double-buffered columns.
+template <int D, int WK, class P> constexpr int window_floats(int columns) {
+  return lds_floats<D, WK>() + (P::kRel ? FB * WK + FB * FW / WK : columns);
+}
+
+template <int D, bool CAUSAL, bool SCOREMOD, int WK, class P>
+__global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dq_f32_kernel(const P p) {
+  __shared__ __attribute__((aligned(16))) float lds[window_floats<D, WK, P>(SCOREMOD ? 2 * FB * WK : 0)];
+  extern __shared__ __attribute__((aligned(16))) float near[];
+  const int wg = gap_prologue<4>(p, lds);  // packed layouts: leading gap-zeroing workgroups
+  if (wg >= 0) dq_f32_body<D, CAUSAL, SCOREMOD, WK, P>(p, wg, lds, near);
+}
+
+template <int D, bool CAUSAL, bool SCOREMOD, int WK, class P>
+__global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void dkdv_f32_kernel(const P p) {
+  __shared__ __attribute__((aligned(16))) float lds[window_floats<D, WK, P>(0)];
+  dkdv_f32_body<D, CAUSAL, SCOREMOD, WK, P>(p, (int)blockIdx.x, lds);
 }
 
 // Waves per row group.  Every workgroup streams its rows' whole range, so a

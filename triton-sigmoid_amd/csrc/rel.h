@@ -213,6 +213,8 @@ void launch_rel_fwd_mfma(const RelParams &p, int dtype, int D, bool causal, hipS
 int rel_dq_rows(const RelParams &p, int D, bool causal);
 void launch_rel_dq_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
 void launch_rel_dkdv_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st);
+// Both in one launch; false (and nothing launched) where two are better.
+bool launch_rel_bwd_mfma(const RelParams &pq, const RelParams &pk, int dtype, int D, bool causal, hipStream_t st);
 
 // Portable kernels (launch.h); the dQ one fills RelParams::part, in blocks of
 // kGenericRows rows.
@@ -225,6 +227,9 @@ void launch_rel_fwd_f32(const RelParams &p, int D, bool causal, hipStream_t st);
 int rel_dq_rows_f32(const RelParams &p, int D, bool causal);
 void launch_rel_dq_f32(const RelParams &p, int D, bool causal, hipStream_t st);
 void launch_rel_dkdv_f32(const RelParams &p, int D, bool causal, hipStream_t st);
+// Both in one launch; false (and nothing launched) where their workgroups differ or
+// the sums by position would leave dK/dV fewer of them per CU.
+bool launch_rel_bwd_f32(const RelParams &pq, const RelParams &pk, int D, bool causal, hipStream_t st);
 void launch_paged_rel_f32(const PagedRelParams &p, int units, int D, bool causal, hipStream_t st);
 void launch_paged_rel_decode_f32(const PagedRelParams &p, int units, int D, bool causal, hipStream_t st);
 

@@ -1,5 +1,7 @@
 // The recompute backward's kernels (bwd_kernel.h) with the learned bias by relative
 // position: dQ, which also sums dS by relative position, and dK/dV.
+#include <algorithm>
+
 #include "bwd_kernel.h"
 #include "launch.h"
 #include "rel.h"
@@ -30,6 +32,50 @@ template <typename T, int D, int WK> void dq_w(const RelParams &kp, bool causal,
   const size_t line = p.part != nullptr ? near_floats(p.reach) * sizeof(float) : 0;
   if (causal) rel_dq_kernel<T, D, WK, true><<<grid, 256, line, st>>>(p);
   else rel_dq_kernel<T, D, WK, false><<<grid, 256, line, st>>>(p);
+}
+
+// Both kernels in one launch (D <= 64): the first nkv workgroups (after dQ's gap
+// rows) are dK/dV's.
+template <typename T, int D, int WK, bool CAUSAL, bool GROUPED>
+__global__ __launch_bounds__(256, 2) void rel_bwd_kernel(const RelParams pq, const RelParams pk, int nkv) {
+  using Dq = DqLds<D, false, dq_window<RelParams, WK>()>;
+  using Dkdv = DkdvLds<D, dkdv_window<RelParams>()>;
+  __shared__ unsigned long long gap_lds[2];
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // a Dkdv, or a Dq and its sums
+  const int wg = gap_prologue<2>(pq, gap_lds);
+  if (wg < 0) return;
+  if (wg < nkv) bwd_dkdv_body<T, D, CAUSAL, false, false, GROUPED, RelParams>(pk, wg, *(Dkdv *)lds);
+  else bwd_dq_body<T, D, WK, CAUSAL, false, RelParams>(pq, wg - nkv, *(Dq *)lds, lds + sizeof(Dq) / 4);
+}
+
+// Where that pays: as long as either kernel alone leaves CUs idle for much of its
+// time, and two workgroups still fit a CU beside the sums' lines.  Forward + backward,
+// us, two launches / one, 128-row workgroups of both per CU: H=8 D=64 sequence
+// of 128 0.06, 39.5 / 32.2; four of 512 1, 60.3 / 47.8 (causal 59.7 / 47.9); two of
+// 1001 H=12 1.5, 112 / 105; eight of 512 2, 73.3 / 73.1; four of 1024 H=16 4, 150
+// / 152 (causal 110 / 108); sixteen of 101 .. 1001 H=12 12, 234 / 232 (D=32 175 / 185;
+// causal D=64 171 / 168, D=32 134 / 139); causal, eight of 2048 8, 271 / 296 (dQ misses
+// its third workgroup per CU).
+template <int D, int WK> bool one_launch(const RelParams &p, bool causal) {
+  const int64_t n = (int64_t)p.B * p.H * ((p.Tq + 127) / 128 + (p.Tk + 127) / 128);
+  const size_t dq = sizeof(DqLds<D, false, dq_window<RelParams, WK>()>) + (p.part != nullptr ? near_floats(p.reach) * 4 : 0);
+  return n <= (causal ? 4 : 2) * (int64_t)p.ncu && dq <= 79 * 1024;
+}
+
+template <typename T, int D, int WK>
+void bwd_w(const RelParams &kq, const RelParams &kk, bool causal, hipStream_t st) {
+  RelParams pq = kq, pk = kk;
+  pq.part_rows = 128 / WK;
+  pq.nblk = (pq.Tq + pq.part_rows - 1) / pq.part_rows;
+  pk.nblk = (pk.Tk + 127) / 128;
+  const bool grouped = pk.qgroup > 1;
+  const int nkv = pk.nblk * pk.B * pk.H * (grouped && pk.qsplit > 1 ? pk.qsplit : 1);
+  const dim3 grid((unsigned)(nkv + pq.nblk * pq.B * pq.H + pq.ngap[0] + pq.ngap[1]));
+  const size_t dq = sizeof(DqLds<D, false, dq_window<RelParams, WK>()>) + (pq.part != nullptr ? near_floats(pq.reach) * 4 : 0);
+  const size_t lds = std::max(dq, sizeof(DkdvLds<D, dkdv_window<RelParams>()>));
+  const auto go = [&](auto c, auto g) { rel_bwd_kernel<T, D, WK, c.value, g.value><<<grid, 256, lds, st>>>(pq, pk, nkv); };
+  if (causal) grouped ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  else grouped ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 // Pairs of waves as without the bias.
@@ -81,6 +127,23 @@ void launch_rel_dkdv_mfma(const RelParams &p, int dtype, int D, bool causal, hip
     dkdv_t<std::remove_pointer_t<decltype(t)>, decltype(d)::value>(p, causal, st);
   });
   launch_add_parts(p, dtype, st);
+}
+
+bool launch_rel_bwd_mfma(const RelParams &pq, const RelParams &pk, int dtype, int D, bool causal, hipStream_t st) {
+  bool done = false;
+  by_type(dtype, D, [&](auto *t, auto d) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int DD = decltype(d)::value;
+    if constexpr (DD <= 64) {
+      const auto go = [&](auto wk) {
+        if ((done = one_launch<DD, wk.value>(pq, causal))) bwd_w<T, DD, wk.value>(pq, pk, causal, st);
+      };
+      if (dq_pairs(pq, DD, causal)) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 1>{});
+    }
+  });
+  if (done) launch_add_parts(pk, dtype, st);
+  return done;
 }
 
 }  // namespace sigattn

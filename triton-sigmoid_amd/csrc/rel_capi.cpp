@@ -135,12 +135,15 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     GapAxis gq, gk;
     gap_axes(p, dq, dk, dv, gq, gk);
     use_gaps(kq, gq, gk);
-    if (f32) {
+    const RelParams kk = rel_kv_items(k);
+    if (f32 ? launch_rel_bwd_f32(kq, kk, D, causal, st) : launch_rel_bwd_mfma(kq, kk, p->dtype, D, causal, st)) {
+      // one launch
+    } else if (f32) {
       launch_rel_dq_f32(kq, D, causal, st);
-      launch_rel_dkdv_f32(rel_kv_items(k), D, causal, st);
+      launch_rel_dkdv_f32(kk, D, causal, st);
     } else {
       launch_rel_dq_mfma(kq, p->dtype, D, causal, st);
-      launch_rel_dkdv_mfma(rel_kv_items(k), p->dtype, D, causal, st);
+      launch_rel_dkdv_mfma(kk, p->dtype, D, causal, st);
     }
   } else {
     k.part_rows = kGenericRows;

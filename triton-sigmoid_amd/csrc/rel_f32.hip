@@ -11,6 +11,22 @@ template <class F> void by_dim(int D, F &&f) {
   else f(std::integral_constant<int, 32>{});
 }
 
+// Both kernels in one launch: the first nkv workgroups (after dQ's gap rows) are
+// dK/dV's.  Forward + backward, us, two launches / one: five sequences of up to 777
+// H=8 D=32, reach 300, 109 / 100; one of 128 D=64 50.1 / 37.6; eight of up to 1024
+// H=12 D=64 444 / 429; causal, eight of up to 2048 H=16 Hkv=4 999 / 920; D=128 H=8
+// Hkv=2, four of up to 1000 494 / 462, causal, eight of up to 2000 1295 / 1121.
+template <int D, bool CAUSAL, int WK>
+__global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void rel_bwd_f32_kernel(const RelParams pq,
+                                                                                         const RelParams pk, int nkv) {
+  __shared__ __attribute__((aligned(16))) float lds[window_floats<D, WK, RelParams>(0)];
+  extern __shared__ __attribute__((aligned(16))) float near[];
+  const int wg = gap_prologue<4>(pq, lds);
+  if (wg < 0) return;
+  if (wg < nkv) dkdv_f32_body<D, CAUSAL, false, WK, RelParams>(pk, wg, lds);
+  else dq_f32_body<D, CAUSAL, false, WK, RelParams>(pq, wg - nkv, lds, near);
+}
+
 }  // namespace
 
 void launch_rel_fwd_f32(const RelParams &p, int D, bool causal, hipStream_t st) {
@@ -34,6 +50,30 @@ void launch_rel_dkdv_f32(const RelParams &p, int D, bool causal, hipStream_t st)
   k.part = nullptr;  // dQ's
   by_dim(D, [&](auto d) { dkdv_t<d.value>(k, causal, st); });
   launch_add_parts(p, kF32, st);
+}
+
+bool launch_rel_bwd_f32(const RelParams &kq, const RelParams &kk, int D, bool causal, hipStream_t st) {
+  bool done = false;
+  RelParams kv = kk;
+  kv.part = nullptr;
+  by_dim(D, [&](auto d) {
+    by_waves<d.value>(kq, kq.Tq, kq.Tk, causal, [&](auto wq, const RelParams &pq, int64_t nq) {
+      by_waves<d.value>(kv, kv.Tk, kv.Tq, causal, [&](auto wk, const RelParams &pk, int64_t nk) {
+        if constexpr (wq.value == wk.value) {
+          constexpr int WK = wk.value;
+          const size_t near = rel_near_bytes(pq);
+          if (bwd_f32_occupancy<d.value, WK>() * (window_floats<d.value, WK, RelParams>(0) * 4 + near + 256) > 163840) return;
+          const int64_t nkv = nk * (pk.qsplit > 1 ? pk.qsplit : 1);
+          done = true;
+          const dim3 grid((unsigned)(nq + nkv + pq.ngap[0] + pq.ngap[1])), block(64 * FW);
+          if (causal) rel_bwd_f32_kernel<d.value, true, WK><<<grid, block, near, st>>>(pq, pk, (int)nkv);
+          else rel_bwd_f32_kernel<d.value, false, WK><<<grid, block, near, st>>>(pq, pk, (int)nkv);
+        }
+      });
+    });
+  });
+  if (done) launch_add_parts(kv, kF32, st);
+  return done;
 }
 
 void launch_paged_rel_f32(const PagedRelParams &p, int units, int D, bool causal, hipStream_t st) {
