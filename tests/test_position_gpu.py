@@ -9,7 +9,7 @@ import torch
 
 import triton_sigmoid as ts
 from reference64 import assert_within, one_head
-from reference64_rel import line_of, packed_rel
+from reference64_rel import grad_of_scores, line_of, packed_rel
 
 pytestmark = pytest.mark.gpu
 DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
@@ -329,6 +329,20 @@ def test_more_sequences_than_the_sums_keep():
     r = random.Random(6)
     lens = [r.choice((0, 1, 2, r.randint(1, 12))) for _ in range(1300)]
     check(make(lens, lens, 1, 1, 32, torch.bfloat16, 10, 9, seed=6), True)
+
+
+def test_fp32_sums_do_not_drift():
+    """Four million dS of either sign in one bucket: what each may be off by adds up as
+    its square where it has no preferred sign (six standard deviations; each within its
+    bound), beside what all share: the fp32 bias and additive term, 2^-20 of the sum."""
+    n = 2000
+    q, k, v, do, table, buckets, cu, _ = make([n], [n], 2, 2, 32, torch.float32, 1, 0, seed=8)
+    got = run(q, k, v, do, table, buckets, cu, cu, False)["dtable"].double()
+    for h in range(2):
+        add = (table.double()[0, h] - math.log(n)).expand(n, n)
+        ds, err = grad_of_scores(q[:, h], k[:, h], v[:, h], do[:, h], add, False)
+        bound = 6 * err.square().sum().sqrt() + 2.0 ** -20 * ds.sum().abs()
+        assert (got[0, h] - ds.sum()).abs() <= bound
 
 
 @pytest.mark.parametrize("f", [(1e-13, 1e12, 1e30, 1e-30), (1.0, 1.0, 1e-15, 1e-14), (1e10, 1e-10, 1e15, 1e10)])

@@ -738,6 +738,17 @@ __device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[ma
   u32x4 qf[3][NKS], of[3][NKS];
   load_split_row<D>(qf, (const float *)p.q + qoff + (int64_t)myq * p.sq_t, hi, myq < Lq, half);
   load_split_row<D>(of, (const float *)p.dout + qoff + (int64_t)myq * p.sq_t, hi, myq < Lq, half);
+  // P::kRel: dO of every other query enters negated, and so do its dP, dS and dQ.  The
+  // matrix cores' sums end below the exact ones by 2^-25 of their size on average,
+  // which sums of dS by position, millions of either sign, would add up (error of the
+  // table's gradient 1.1e-6, 3.7e-7 so: five sequences of up to 777, H=8 D=32).
+  [[maybe_unused]] const float sgn = P::kRel && (l32 & 1) ? -1.0f : 1.0f;
+  if constexpr (P::kRel) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int k = 0; k < NKS; ++k) of[i][k] ^= l32 & 1 ? 0x80008000u : 0u;
+  }
   f32x16 acc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc[db] = zero16();
@@ -784,7 +795,7 @@ __device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[ma
       for (int i = 0; i < 16; ++i)
         if (8 * (i / 4) + i % 4 >= lim) ds[i] = 0.0f;
     }
-    if constexpr (P::kRel) sums.add(ds, k0 - qw, l32, hi);
+    if constexpr (P::kRel) sums.add(ds, k0 - qw, l32, hi, sgn);
     row3<D, Tiles::PART>(acc, tiles, to, 2 * wt, ds);
   }
   add_waves<NDB, WK>(acc, lds, w, lane);
@@ -802,7 +813,7 @@ __device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[ma
     if (it.row0 < Lq) sums.finish(p, near, b, it.row0 / p.part_rows, h, w, tid);
   }
   if (wt == 0 && myq < p.q_rows_out(Lq))
-    store_row<D>((float *)p.dq + qoff + (int64_t)myq * p.sq_t, acc, scale, myq < Lq, hi, half);
+    store_row<D>((float *)p.dq + qoff + (int64_t)myq * p.sq_t, acc, P::kRel ? scale * sgn : scale, myq < Lq, hi, half);
 }
 
 // dV = Pᵀ · dO and dK = dSᵀ · Q · scale; queries streamed.

@@ -118,15 +118,16 @@ struct PlaceSums {
     if (on)
       for (int i = tid; i < near_floats(reach); i += 256) near[i] = 0.0f;
   }
-  // A block whose first key lies `off` (a multiple of 32) after the wave's first query.
-  __device__ __forceinline__ void add(const float (&ds)[16], int off, int l32, int hi) {
+  // A block whose first key lies `off` (a multiple of 32) after the wave's first query;
+  // sgn: what the lane's dS are to be times.
+  __device__ __forceinline__ void add(const float (&ds)[16], int off, int l32, int hi, float sgn = 1.0f) {
     if (!on) return;
     if (off + 31 <= -reach || off - 31 >= reach) {
       float x = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x += ds[i];
-      if (off < 0) beyond[0] += x;
-      else beyond[1] += x;
+      if (off < 0) beyond[0] = __builtin_fmaf(x, sgn, beyond[0]);
+      else beyond[1] = __builtin_fmaf(x, sgn, beyond[1]);
       return;
     }
     const int lane = l32 + 32 * hi;
@@ -135,7 +136,7 @@ struct PlaceSums {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {  // keys 8g .. 8g + 7, places 8g - 31 .. 8g + 7 from `off` on
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[j * (kSkewRow + 1)] = ds[4 * g + j];
+      for (int j = 0; j < 4; ++j) to[j * (kSkewRow + 1)] = ds[4 * g + j] * sgn;
       const int row = lane - 8 * g;
       const float *from = skew + min(max(row, 0), 38) * kSkewRow;
       const f32x4 u = *(const f32x4 *)from, v = *(const f32x4 *)(from + 4);
