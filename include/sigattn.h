@@ -384,7 +384,8 @@ int sigattn_paged_fwd(const sigattn_paged_problem *p, void *out, void *workspace
  * of query i and key j of a sequence gets table[buckets[max_distance + d], h], d = j - i
  * clamped to [-max_distance, max_distance] and h the query head, beside scale
  * and bias.  Buckets outside [0, num_buckets) add nothing and get no gradient.
- * Packed problems (both axes) without score_mod.
+ * Packed problems (both axes) without score_mod; sigattn_problem.bias may be NULL
+ * here: -log(key length) of each sequence (sigattn_default_bias), with no launch of its own.
  */
 #define SIGATTN_REL_MAX_DISTANCE 2048
 #define SIGATTN_REL_MAX_BUCKETS 4096
@@ -402,7 +403,7 @@ int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r);
  * aligned, used until the call's kernels finish; SIGATTN_ERR_WORKSPACE without it).
  * The forward leaves in its own what the table is at each relative position;
  * given as `line` to the backward of the same problem, it is not read from the
- * table again (NULL: it is).
+ * table again (NULL: it is), nor the default bias made again.
  * `dtable` is the table's gradient, [num_buckets, H] of its type, written whole:
  * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed).
  * Deterministic.

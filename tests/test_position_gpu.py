@@ -313,6 +313,25 @@ def test_bindings_alike(monkeypatch, D, dtype):
     assert all(torch.equal(node[x], python[x]) for x in node)
 
 
+@pytest.mark.parametrize("D, dtype", [(64, "bf16"), (128, "f16"), (32, "f32")])
+def test_the_library_makes_the_default_bias(monkeypatch, D, dtype):
+    """A problem without one: in the forward, and in a backward that has no lines either."""
+    from triton_sigmoid import _capi
+
+    monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    args = make([300, 0, 77], [200, 5, 77], 4, 2, D, DT[dtype], 16, 60, seed=D)
+    given, problem = run(*args, True), _capi._problem
+
+    def without(*a, **k):
+        p = problem(*a, **k)
+        p.bias = None
+        return p
+
+    monkeypatch.setattr(_capi, "_problem", without)
+    made = run(*args, True)
+    assert all(torch.equal(given[x], made[x]) for x in given)
+
+
 @pytest.mark.parametrize("binding", ["node", "python"])
 def test_gradients_have_none_of_their_own(monkeypatch, binding):
     if binding == "python":

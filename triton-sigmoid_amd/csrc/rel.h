@@ -182,6 +182,10 @@ struct RelTable {
   int dtype, buckets, max_distance, H, reach;
 };
 
+__device__ __forceinline__ int bucket_of(const RelTable &t, int place) {
+  return t.bucket[t.max_distance + place - t.reach];
+}
+
 // The host's side: the caller's table for H heads and two lengths (reach: no two
 // tokens lie further apart), and the bytes of its lines.
 inline bool rel_table_ok(const sigattn_rel_bias *r) {
@@ -200,8 +204,9 @@ inline int64_t rel_line_bytes(const RelTable &t) {
   return ((int64_t)t.H * line_places(t.reach) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
-// line [H, line_places(reach)] from the table.
-void launch_rel_line(const RelTable &t, float *line, hipStream_t st);
+// line [H, line_places(reach)] from the table, and bias [B] (nullptr: not wanted), the
+// default one of the key sequences.
+void launch_rel_line(const RelTable &t, float *line, const int32_t *cu_k, int64_t B, float *bias, hipStream_t st);
 // The table's gradient (`grad`, the table's type) from the dQ kernels' sums in
 // p.part (nullptr: zeros); sums: [H, 2 reach + 1] floats of scratch.
 void launch_rel_grad(const RelTable &t, const RelParams &p, float *sums, void *grad, hipStream_t st);

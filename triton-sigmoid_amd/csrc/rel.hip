@@ -1,30 +1,10 @@
-// The learned bias by relative position outside the attention kernels: a line of
-// values per head from the table, and the table's gradient from their sums.
+// The gradient of the learned bias's table from the dQ kernels' sums by relative
+// position (the lines of values that the kernels read: bias.hip).
 #include "launch.h"
 #include "rel.h"
 
 namespace sigattn {
 namespace {
-
-__device__ __forceinline__ int bucket_of(const RelTable &t, int place) {
-  return t.bucket[t.max_distance + place - t.reach];
-}
-// (Buckets outside the table add nothing and get nothing.)
-__device__ __forceinline__ bool inside(const RelTable &t, int u) { return u >= 0 && u < t.buckets; }
-
-// One thread per place.  A few KB: bound by its launch.
-template <typename T> __global__ __launch_bounds__(256) void rel_line_kernel(const RelTable t, float *line) {
-  const int place = blockIdx.x * 256 + threadIdx.x, places = line_places(t.reach), h = blockIdx.y;
-  if (place >= places) return;
-  const int u = bucket_of(t, min(max(place - kRelPad, 0), 2 * t.reach));
-  float x = 0.0f;
-  if (inside(t, u)) {
-    const int64_t at = (int64_t)u * t.H + h;
-    if constexpr (sizeof(T) == 4) x = ((const float *)t.table)[at];
-    else x = Elem<T>::to_f32(((const uint16_t *)t.table)[at]);
-  }
-  line[(int64_t)h * places + place] = x;
-}
 
 // sums[h][place] of all query blocks: 64 places a workgroup, 16 shares of the
 // slots (in turn), added in their order.  Which slots hold a block is found for
@@ -98,14 +78,6 @@ template <class F> void by_type(int dtype, F &&f) {
 }
 
 }  // namespace
-
-void launch_rel_line(const RelTable &t, float *line, hipStream_t st) {
-  if (t.H == 0) return;
-  const dim3 grid((unsigned)((line_places(t.reach) + 255) / 256), (unsigned)t.H);
-  by_type(t.dtype, [&](auto *x) {
-    rel_line_kernel<std::remove_pointer_t<decltype(x)>><<<grid, dim3(256), 0, st>>>(t, line);
-  });
-}
 
 void launch_rel_grad(const RelTable &t, const RelParams &p, float *sums, void *grad, hipStream_t st) {
   if (t.H == 0 || t.buckets == 0) return;

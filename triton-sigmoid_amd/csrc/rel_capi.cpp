@@ -7,12 +7,24 @@ using namespace sigattn;
 
 namespace {
 
+// What the line's launch leaves: the lines, then (without a bias of the caller's) the
+// sequences' default ones.
+int64_t rel_head_bytes(const sigattn_problem *p, const RelTable &t) {
+  return rel_line_bytes(t) + (p->bias == nullptr ? (p->B * (int64_t)sizeof(float) + 255) / 256 * 256 : 0);
+}
+
 RelParams rel_params(const sigattn_problem *p, const RelTable &t, const void *line) {
   RelParams k{};
   (KParams &)k = make_params(p);
   k.line = (const float *)line;
+  if (p->bias == nullptr) k.bias = (const float *)((const char *)line + rel_line_bytes(t));
   k.reach = t.reach;
   return k;
+}
+
+void make_line(const sigattn_problem *p, const RelTable &t, void *to, hipStream_t st) {
+  launch_rel_line(t, (float *)to, p->cu_seqlens_k, p->B,
+                  p->bias == nullptr ? (float *)((char *)to + rel_line_bytes(t)) : nullptr, st);
 }
 
 int64_t rel_part_bytes(const sigattn_problem *p, const RelTable &t) {
@@ -37,9 +49,11 @@ RelTable rel_table_of(const sigattn_paged_problem *p, const sigattn_rel_bias *r)
 extern "C" {
 
 int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r) {
-  const int rc = sigattn_check(p);
+  if (p == nullptr || r == nullptr) return SIGATTN_ERR_NULL_ARG;
+  sigattn_problem with_bias = *p;
+  if (p->bias == nullptr) with_bias.bias = p->scale;  // (its own: any pointer)
+  const int rc = sigattn_check(&with_bias);
   if (rc != SIGATTN_OK) return rc;
-  if (r == nullptr) return SIGATTN_ERR_NULL_ARG;
   if (r->dtype != SIGATTN_F16 && r->dtype != SIGATTN_BF16 && r->dtype != SIGATTN_F32) return SIGATTN_ERR_DTYPE;
   if (!rel_table_ok(r) || p->score_mod != nullptr || p->cu_seqlens_q == nullptr || p->cu_seqlens_k == nullptr)
     return SIGATTN_ERR_REL_BIAS;
@@ -49,7 +63,7 @@ int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r) {
 }
 
 size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
-  return sigattn_rel_check(p, r) == SIGATTN_OK ? (size_t)rel_line_bytes(rel_table(r, p->H, p->Tq, p->Tk)) : 0;
+  return sigattn_rel_check(p, r) == SIGATTN_OK ? (size_t)rel_head_bytes(p, rel_table(r, p->H, p->Tq, p->Tk)) : 0;
 }
 
 int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
@@ -65,12 +79,12 @@ int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *o
     return launch_status();
   }
   const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
-  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < rel_line_bytes(t))
+  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < rel_head_bytes(p, t))
     return SIGATTN_ERR_WORKSPACE;
   RelParams k = rel_params(p, t, workspace);
   k.out = out;
   (void)hipGetLastError();
-  launch_rel_line(t, (float *)workspace, st);
+  make_line(p, t, workspace, st);
   const void *ptrs[4] = {p->q, p->k, p->v, out};
   const bool f32 = use_f32_mfma(p, ptrs, 4);
   if (f32 || use_mfma(p, ptrs, 4)) {
@@ -91,7 +105,7 @@ size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_r
   const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
   // (Pointers are not known yet: aligned rows, as everywhere.)
   const void *none[1] = {nullptr};
-  return (size_t)(2 * rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
+  return (size_t)(rel_head_bytes(p, t) + rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
 }
 
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
@@ -107,7 +121,7 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     return SIGATTN_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
   RelParams k = rel_params(p, t, line != nullptr ? line : workspace);
-  float *sums = (float *)((char *)workspace + rel_line_bytes(t));
+  float *sums = (float *)((char *)workspace + rel_head_bytes(p, t));
   k.dout = dout;
   k.dq = dq;
   k.dk = dk;
@@ -123,8 +137,8 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     if (dtable != nullptr) launch_rel_grad(t, k, sums, dtable, st);
     return launch_status();
   }
-  if (line == nullptr) launch_rel_line(t, (float *)workspace, st);
-  char *parts = (char *)workspace + 2 * rel_line_bytes(t);
+  if (line == nullptr) make_line(p, t, workspace, st);
+  char *parts = (char *)sums + rel_line_bytes(t);
   if (dtable != nullptr) k.part = (float *)parts;
   if (mfma) {
     const HeadSplit hs = head_split(p, mfma);
@@ -188,7 +202,7 @@ int sigattn_paged_rel_fwd(const sigattn_paged_problem *p, const sigattn_rel_bias
   const hipStream_t st = (hipStream_t)stream;
   k.line = (const float *)workspace, k.reach = t.reach;
   (void)hipGetLastError();
-  launch_rel_line(t, (float *)workspace, st);
+  launch_rel_line(t, (float *)workspace, nullptr, 0, nullptr, st);
   if (!mfma) {
     launch_paged_rel_generic(k, p->dtype, (int)p->D, causal, st);
     return launch_status();

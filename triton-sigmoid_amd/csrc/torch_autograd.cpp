@@ -1,5 +1,6 @@
 // Eager autograd node of the public APIs (sigmoid_attention,
-// sigmoid_attention_padded, sigmoid_attention_varlen), in C++, and the short
+// sigmoid_attention_padded, sigmoid_attention_varlen), in C++, those of the
+// learned bias by relative position and of rotary embedding, and the short
 // ways of eager calls with canonical arguments into the library.
 //
 // The reference builds its eager path from torch.autograd.Function-style
@@ -303,9 +304,10 @@ sigattn_rel_bias make_rel(const Tensor &table, const Tensor &buckets) {
 // sigmoid_attention_varlen with the learned bias, at least one sequence and one row.
 struct RelNode : public torch::autograd::Function<RelNode> {
   static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table,
-                        const Tensor &buckets, const Tensor &bias, const Tensor &scale, const Tensor &cu_q,
+                        const Tensor &buckets, const std::optional<Tensor> &own_bias, const Tensor &scale, const Tensor &cu_q,
                         const Tensor &cu_k, int64_t max_q, int64_t max_k, bool causal) {
     const Layout lay{Tensor(), Tensor(), cu_q, cu_k, max_q, max_k};
+    const Tensor bias = own_bias.value_or(Tensor());  // none: the library's default
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["max_q"] = max_q;
     ctx->saved_data["max_k"] = max_k;
@@ -598,13 +600,14 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
   if (own_bias) {
     bias = Quick::constant(B, bias_value, at::kFloat, dev);
     if (!bias.defined()) return no;
-  } else {
+  } else if (!rel) {  // (with it, the launch of its lines makes them)
     bias = at::empty({B}, q.options().dtype(at::kFloat).requires_grad(false));
     check_rc(g_api.default_bias(nullptr, static_cast<const int32_t *>(ck.data_ptr()), B,
                                 static_cast<float *>(bias.data_ptr()), stream),
              "sigattn_default_bias");
   }
-  if (rel) return py::cast(RelNode::apply(q, k, v, table, buckets, bias, st, cq, ck, mq, mk, is_causal.ptr() == Py_True));
+  if (rel) return py::cast(RelNode::apply(q, k, v, table, buckets, own_bias ? std::optional<Tensor>(bias) : std::nullopt, st, cq, ck, mq, mk,
+                                      is_causal.ptr() == Py_True));
   const int64_t limit = (int64_t)(H == Hkv ? 2048 : 8192) << 20;  // _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB
   return py::cast(SigattnNode::apply(q, k, v, bias, sm.defined() ? std::optional<Tensor>(sm) : std::nullopt, st,
                                      std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
