@@ -304,6 +304,14 @@ def test_empty_calls():
             assert g.shape == t.shape and not g.any()
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("R", [140, 150, 600, 1100, 1200])
+def test_128_columns_and_the_room_for_sums(R, causal):
+    """Workgroups of four waves, of eight where longer lines leave room for those alone, and of four again."""
+    lens = [1250, 257, 0, 33]
+    check(make(lens, lens, 1, 1, 128, torch.bfloat16, 40, R, seed=R), causal)
+
+
 @pytest.mark.parametrize("D, dtype", [(64, "bf16"), (128, "f16"), (32, "f32")])
 def test_bindings_alike(monkeypatch, D, dtype):
     args = make([300, 1, 77], [300, 1, 77], 4, 2, D, DT[dtype], 16, 60, seed=D)

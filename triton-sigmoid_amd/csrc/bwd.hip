@@ -19,6 +19,8 @@
 // with the MFMA chains of the next; the dQ kernel (two waves per SIMD) relies
 // on the second wave for that overlap.  Rows past seq_lens are fetched as
 // copies of the last valid row (in bounds) and masked on boundary tiles.
+// Their bodies are in bwd_kernel.h, shared with the learned bias by relative
+// position (rel_bwd.hip).
 #include <type_traits>
 
 #include "bwd_kernel.h"

@@ -20,16 +20,17 @@ namespace sigattn {
 // are added at the end (launch_bwd_dq_mfma says where).
 // A learned bias by relative position (P::kRel): WIN places of the head's line are
 // staged with each tile, and dS is summed by relative position (PlaceSums).
-template <class P, int WK> constexpr int dq_window() { return P::kRel ? 128 / WK + 64 : 0; }
+template <class P, int WK, int NW = 4> constexpr int dq_window() { return P::kRel ? 32 * NW / WK + 64 : 0; }
 template <int D, bool SCOREMOD, int WIN = 0> struct DqLds {
   uint16_t k[2][64 * D], v[2][64 * D];
   float c[WIN > 0 ? 2 * WIN : (SCOREMOD ? 2 * 64 : 4)];
 };
-template <typename T, int D, int WK, bool CAUSAL, bool SCOREMOD, class P = KParams>
-__device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, SCOREMOD, dq_window<P, WK>()> &lds,
+// (NW waves; eight only with P::kRel at D = 128.)
+template <typename T, int D, int WK, bool CAUSAL, bool SCOREMOD, class P = KParams, int NW = 4>
+__device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, SCOREMOD, dq_window<P, WK, NW>()> &lds,
                                             float *near = nullptr) {
-  constexpr int NG = 4 / WK, BM = 32 * NG, BN = 64;
-  constexpr int WIN = dq_window<P, WK>();
+  constexpr int NG = NW / WK, BM = 32 * NG, BN = 64;
+  constexpr int WIN = dq_window<P, WK, NW>();
   constexpr bool REL = P::kRel;
   constexpr int NKS = D / 16, NDB = D / 32;
   auto &sK = lds.k;
@@ -47,7 +48,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
     const auto lq = [&](int i) SIGATTN_INLINE { return p.len_q(i); };
     const auto lk = [&](int i) SIGATTN_INLINE { return p.len_k(i); };
     const WorkItem it = CAUSAL ? WorkOrder::by_level(wg, p.B, p.H, lq, BM, p.nblk, true, p.ncu,
-                                                     D <= 64 ? 3 : 2)
+                                                     D <= 64 ? 3 : 8 / NW)
                                : WorkOrder::by_stream(wg, p.B, p.H, lq, BM, p.nblk, lk);
     b = it.b, h = it.h, qb = it.blk;
   } else {
@@ -70,7 +71,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
   // Padding item: its zero rows as part of one contiguous span (see zero_row_span).
   if (qb * BM >= Lq && p.q_rows_contiguous(half ? 16 : D)) {
     zero_row_span((uint16_t *)p.dq + (int64_t)b * p.sq_b, p.sq_t, qb * BM, min(qb * BM + BM, p.Tq), h, p.H,
-                  threadIdx.x, 256);
+                  threadIdx.x, 64 * NW);
     return;
   }
 
@@ -116,12 +117,12 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
   TileOffsets<D> to;
   to.init(lane);
   if constexpr (WK == 2) to.advance(32 * wt);  // this wave's half of every tile
-  DmaPlan<BN, D, 4> dma;
+  DmaPlan<BN, D, NW> dma;
   dma.init(w, lane, half);
   const int kv_stride_bytes = (int)(p.sk_t * 2);
 
   [[maybe_unused]] const int win0 = BM - (w % NG) * 32 - l32 + 4 * hi;  // this lane's place of the tile's key 0
-  [[maybe_unused]] PlaceSums sums;
+  [[maybe_unused]] PlaceSums<NW> sums;
   if constexpr (REL) sums.init(p, near, w, tid);
 
   // dS of one 32-key block into eight packed words.

@@ -219,7 +219,7 @@ __device__ __forceinline__ void dq_full(const P &p, const Item &w_, float *lds, 
   F32RowReads<D> rr;
   rr.init(l32, hi);
   const int stride_bytes = (int)(p.sk_t * 4);
-  [[maybe_unused]] PlaceSums sums;  // from nothing again
+  [[maybe_unused]] PlaceSums<FW> sums;  // from nothing again
   if constexpr (P::kRel) sums.init(p, near, w, tid);
   for (int t = 0; t < ntiles; ++t) {
     float *tK = lds + (t & 1) * 2 * FB * D, *tV = tK + FB * D, *tC = lds + 4 * FB * D + (t & 1) * FB;
@@ -756,7 +756,7 @@ __device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[ma
   to.init(lane);
   Tiles st;
   [[maybe_unused]] const int win0 = FB * wt + 4 * hi + RB - (myq - it.row0);  // as in the forward
-  [[maybe_unused]] PlaceSums sums;
+  [[maybe_unused]] PlaceSums<FW> sums;
   if constexpr (P::kRel) sums.init(p, near, w, tid);
   float creg = 0.0f;
   auto load = [&](int t) SIGATTN_INLINE {

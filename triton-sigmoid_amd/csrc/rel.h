@@ -88,7 +88,7 @@ struct RelColumn {
   }
 };
 
-// dS by relative position, of a dQ workgroup of four waves.  A 32x32 block of scores
+// dS by relative position, of a dQ workgroup of NW waves.  A 32x32 block of scores
 // (lane: query, accumulator rows: keys) whose places all lie beyond the line's end
 // adds to one sum per lane.  Any other goes through LDS eight keys at a time,
 // written so that a place's scores (a diagonal's) are neighbours: a lane reads those
@@ -101,9 +101,9 @@ struct RelColumn {
 // row's two 16-byte reads meet no other lane's banks).
 constexpr int kNearMargin = 64, kSkewRow = 12, kSkew = 39 * kSkewRow;
 __host__ __device__ constexpr int near_places(int reach) { return 2 * reach + 2 * kNearMargin; }
-__host__ __device__ constexpr int near_floats(int reach) { return 4 * (near_places(reach) + kSkew); }
+__host__ __device__ constexpr int near_floats(int reach, int waves = 4) { return waves * (near_places(reach) + kSkew); }
 
-struct PlaceSums {
+template <int NW> struct PlaceSums {
   float beyond[2] = {0.0f, 0.0f};
   float *mine, *skew;  // relative position 0 of the wave's line; its piece
   int reach;
@@ -113,10 +113,10 @@ struct PlaceSums {
   __device__ __forceinline__ void init(const RelParams &p, float *near, int w, int tid) {
     on = p.part != nullptr, reach = p.reach;
     mine = near + w * near_places(reach) + reach + kNearMargin;
-    skew = near + 4 * near_places(reach) + w * kSkew;
+    skew = near + NW * near_places(reach) + w * kSkew;
     beyond[0] = beyond[1] = 0.0f;
     if (on)
-      for (int i = tid; i < near_floats(reach); i += 256) near[i] = 0.0f;
+      for (int i = tid; i < near_floats(reach, NW); i += 64 * NW) near[i] = 0.0f;
   }
   // A block whose first key lies `off` (a multiple of 32) after the wave's first query;
   // sgn: what the lane's dS are to be times.
@@ -145,12 +145,12 @@ struct PlaceSums {
     }
     mine[off - 31 + lane] += x;
   }
-  // The four waves' lines, in their order, to the block's row of p.part; what lies on
+  // The waves' lines, in their order, to the block's row of p.part; what lies on
   // either side of the ends goes to these, as do the waves' sums per lane.
   __device__ __forceinline__ void finish(const RelParams &p, const float *near, int b, int blk, int h, int w, int tid) {
     if (!on) return;
     const int n = near_places(reach), places = p.places(), lane = tid & 63;
-    __shared__ float ends[4][2];
+    __shared__ float ends[NW][2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float x = wave_sum(beyond[e]);
@@ -158,8 +158,18 @@ struct PlaceSums {
     }
     __syncthreads();
     float *row = p.part_row(b, blk, h);
-    const auto all = [&](int i) SIGATTN_INLINE { return ((near[i] + near[n + i]) + near[2 * n + i]) + near[3 * n + i]; };
-    const auto end = [&](int e) SIGATTN_INLINE { return ((ends[0][e] + ends[1][e]) + ends[2][e]) + ends[3][e]; };
+    const auto all = [&](int i) SIGATTN_INLINE {
+      float x = near[i];
+#pragma unroll
+      for (int v = 1; v < NW; ++v) x += near[v * n + i];
+      return x;
+    };
+    const auto end = [&](int e) SIGATTN_INLINE {
+      float x = ends[0][e];
+#pragma unroll
+      for (int v = 1; v < NW; ++v) x += ends[v][e];
+      return x;
+    };
     if (w < 2) {
       // Wave 0: places up to the lower end, wave 1: from the upper one on.
       const float x = wave_sum(all(w == 0 ? lane + 1 : kNearMargin + places - 1 + lane));
@@ -170,7 +180,7 @@ struct PlaceSums {
         row[0] = y;
       }
     }
-    for (int i = tid + 1; i < places - 1; i += 256) row[i] = all(kNearMargin + i);
+    for (int i = tid + 1; i < places - 1; i += 64 * NW) row[i] = all(kNearMargin + i);
   }
 };
 

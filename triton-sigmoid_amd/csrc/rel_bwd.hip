@@ -1,5 +1,11 @@
 // The recompute backward's kernels (bwd_kernel.h) with the learned bias by relative
-// position: dQ, which also sums dS by relative position, and dK/dV.
+// position: dQ, which also sums dS by relative position, and dK/dV.  The lines' windows
+// are staged as in the forward.  bf16, us, with / without the bias: 16 sequences of 101
+// .. 1001 H=12 D=64 dK/dV 83 / 78, dQ 73 / 55 (62 without the sums: near the diagonal
+// they are a third of a block's arithmetic); causal, 3 of 1500 .. 4096 H=16 Hkv=4
+// D=128 dK/dV 419 / 428 (storing dS, in pairs of waves), dQ 327 (300 without the sums) / 184 from the stored
+// dS.  No two-pass form: what is stored is rounded, and so would be what the table's
+// gradient sums (906 -> 843 us a step, error 1e-6 -> 0.0024).
 #include <algorithm>
 
 #include "bwd_kernel.h"
@@ -9,13 +15,13 @@
 namespace sigattn {
 namespace {
 
-template <typename T, int D, int WK, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void rel_dq_kernel(const RelParams p) {
-  __shared__ __attribute__((aligned(16))) DqLds<D, false, dq_window<RelParams, WK>()> lds;
+template <typename T, int D, int WK, bool CAUSAL, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void rel_dq_kernel(const RelParams p) {
+  __shared__ __attribute__((aligned(16))) DqLds<D, false, dq_window<RelParams, WK, NW>()> lds;
   __shared__ unsigned long long gap_lds[2];
-  extern __shared__ __attribute__((aligned(16))) float near[];  // the four waves' lines and pieces
+  extern __shared__ __attribute__((aligned(16))) float near[];  // the waves' lines and pieces
   const int wg = gap_prologue<2>(p, gap_lds);
-  if (wg >= 0) bwd_dq_body<T, D, WK, CAUSAL, false, RelParams>(p, wg, lds, near);
+  if (wg >= 0) bwd_dq_body<T, D, WK, CAUSAL, false, RelParams, NW>(p, wg, lds, near);
 }
 
 template <typename T, int D, bool CAUSAL, bool GROUPED>
@@ -24,14 +30,25 @@ __global__ __launch_bounds__(256, (D <= 64 ? 2 : 1)) void rel_dkdv_kernel(const 
   bwd_dkdv_body<T, D, CAUSAL, false, false, GROUPED, RelParams>(p, blockIdx.x, lds);
 }
 
-template <typename T, int D, int WK> void dq_w(const RelParams &kp, bool causal, hipStream_t st) {
+template <typename T, int D, int WK, int NW = 4> void dq_w(const RelParams &kp, bool causal, hipStream_t st) {
   RelParams p = kp;
-  p.part_rows = 128 / WK;
+  p.part_rows = 32 * NW / WK;
   p.nblk = (p.Tq + p.part_rows - 1) / p.part_rows;
   const dim3 grid((unsigned)(p.nblk * p.B * p.H + p.ngap[0] + p.ngap[1]));
-  const size_t line = p.part != nullptr ? near_floats(p.reach) * sizeof(float) : 0;
-  if (causal) rel_dq_kernel<T, D, WK, true><<<grid, 256, line, st>>>(p);
-  else rel_dq_kernel<T, D, WK, false><<<grid, 256, line, st>>>(p);
+  const size_t line = p.part != nullptr ? near_floats(p.reach, NW) * sizeof(float) : 0;
+  if (causal) rel_dq_kernel<T, D, WK, true, NW><<<grid, 64 * NW, line, st>>>(p);
+  else rel_dq_kernel<T, D, WK, false, NW><<<grid, 64 * NW, line, st>>>(p);
+}
+
+// At D = 128 two workgroups of four waves share a CU as long as their sums' lines fit
+// beside the tiles, up to a reach of 143.  Beyond, one of eight waves holds as many, in
+// twice the queries per copied tile (up to 1139, then four alone).  Causal step of 3
+// sequences of 1500 .. 4096 H=16 Hkv=4, us by reach: 140 720, 150 719, 300 747, 1000 769, 1300
+// 893 (four waves alone at 150: dQ 500 instead of 330).
+bool dq_eight_waves(const RelParams &p, int D) {
+  constexpr size_t tiles = 4 * 64 * 128 * 2, cu = 163840 - 512;
+  const size_t four = tiles + 2 * 192 * 4 + near_floats(p.reach, 4) * 4, eight = tiles + 2 * 320 * 4 + near_floats(p.reach, 8) * 4;
+  return D == 128 && p.part != nullptr && 2 * four > cu && eight <= cu;
 }
 
 // Both kernels in one launch (D <= 64): the first nkv workgroups (after dQ's gap
@@ -109,7 +126,9 @@ template <class F> void by_type(int dtype, int D, F &&f) {
 
 }  // namespace
 
-int rel_dq_rows(const RelParams &p, int D, bool causal) { return dq_pairs(p, D, causal) ? 64 : 128; }
+int rel_dq_rows(const RelParams &p, int D, bool causal) {
+  return dq_pairs(p, D, causal) ? 64 : dq_eight_waves(p, D) ? 256 : 128;
+}
 
 void launch_rel_dq_mfma(const RelParams &p, int dtype, int D, bool causal, hipStream_t st) {
   by_type(dtype, D, [&](auto *t, auto d) {
@@ -117,6 +136,8 @@ void launch_rel_dq_mfma(const RelParams &p, int dtype, int D, bool causal, hipSt
     constexpr int DD = decltype(d)::value;
     if constexpr (DD <= 64) {
       if (dq_pairs(p, DD, causal)) return dq_w<T, DD, 2>(p, causal, st);
+    } else if (dq_eight_waves(p, DD)) {
+      return dq_w<T, DD, 1, 8>(p, causal, st);
     }
     dq_w<T, DD, 1>(p, causal, st);
   });

@@ -1,4 +1,7 @@
-// The fp32 kernels (f32_kernel.h) with the learned bias by relative position.
+// The fp32 kernels (f32_kernel.h) with the learned bias by relative position, its
+// windows of the lines beside the split tiles in LDS.  us, with / without: five sequences of up
+// to 777 H=8 D=32, reach 300, forward 25.5 / 23.6, dK/dV 34 / 31.3, dQ 35.5 / 27.2
+// (30.5 without the sums by position).
 #include "f32_kernel.h"
 #include "rel.h"
 

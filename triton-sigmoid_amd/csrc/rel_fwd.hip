@@ -1,4 +1,11 @@
-// The forward kernel (fwd_kernel.h) with the learned bias by relative position.
+// The forward kernel (fwd_kernel.h) with the learned bias by relative position:
+// sigmoid(q·k·scale + bias + line[k - q]).  A tile of 64 keys meets a block of BM
+// queries at BM + 63 relative positions, so BM + 64 values of the line go to LDS with
+// each tile, a thread one of them, loaded a tile ahead; a lane (a query) reads the
+// sixteen of its accumulator, four in a row at a time.  The scores' fma takes them
+// where it takes the bias without the line: the sigmoid's arithmetic bounds D = 64, the
+// matrix cores D = 128, as without (us, with / without: bf16 16 sequences of 101 .. 1001
+// H=12 D=64 46 / 45; causal, 3 of 1500 .. 4096 H=16 Hkv=4 D=128 201 / 205).
 #include "fwd_kernel.h"
 #include "launch.h"
 #include "rel.h"

@@ -1,4 +1,11 @@
 // The matrix kernels over a paged cache with the learned bias by relative position.
+// Each lane reads what its column (a query head's token) adds (RelColumn): a
+// block's columns are of several heads, whose windows in LDS would be as many.  A block
+// of keys beyond the line's end for every column costs a comparison: us, with /
+// without, 16 requests on 1024 .. 8191 H=32 Hkv=8 D=128 43.9 / 42.4, bound by HBM; 24
+// requests, four of them prompts, H=12 Hkv=4 D=64 40.3 / 37.1; two chunks of 1024 on 5000 ..
+// 12000 H=32 Hkv=8 D=128 351 / 313, where the columns' 32 registers leave the
+// products' operands a read-ahead of 8 instead of 16.
 #include "launch.h"
 #include "paged_launch.h"
 #include "rel.h"

@@ -35,7 +35,8 @@ __device__ __forceinline__ void turn_pair(float a, float b, float cs, float sn, 
 }
 
 // Any strides, alignment and rot_dim: a workgroup per row, a thread per pair (or two
-// copied columns).
+// copied columns); bound by its narrow loads (bf16 16384 rows H=32 Hkv=8 D=128 384 us
+// forward and backward, where the other kernel takes 119).
 template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const int64_t t = blockIdx.x;
   const int half = a.rot / 2, dh = a.D / 2;
