@@ -352,6 +352,29 @@ def test_gradients_have_none_of_their_own(monkeypatch, binding):
         sum(g.float().sum() for g in grads).backward()
 
 
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("bf16", 32), ("f32", 32), ("f32", 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_infinite_keys_reach_no_sum_through_rows_that_are_not_there(dtype, D, causal):
+    """A key of +-inf has sigmoids of 0 and 1, so dS = 0: the pairs of a key block with
+    the rows that fill up a sequence's last block of queries are no pairs."""
+    n, R, at = 37, 12, 33
+    q, k, v, do, table, buckets, cu, _ = make([n], [n], 2, 2, D, DT[dtype], 2 * R + 1, R, seed=D)
+    buckets = torch.arange(2 * R + 1, dtype=I32, device="cuda")
+    k[at, :, 3] = math.inf
+    got = run(q, k, v, do, table, buckets, cu, cu, causal)["dtable"].double()
+    finite, u = torch.where(torch.isfinite(k), k, 0.0), torch.finfo(table.dtype).eps / 2
+    pos = torch.arange(n, device="cuda")
+    d = pos[None] - pos[:, None]
+    for h in range(2):
+        line, place = line_of(table, buckets, h, d)
+        ds, err = grad_of_scores(q[:, h], finite[:, h], v[:, h], do[:, h], line - math.log(n), causal)
+        ds[:, at] = err[:, at] = 0.0
+        want, bound, size = (torch.zeros(2 * R + 1, dtype=torch.float64, device="cuda").index_add_(0, place.flatten(), x.flatten())
+                             for x in (ds, err, ds.abs()))
+        bound = bound + 300 * 2.0 ** -24 * size  # (fewer additions than that)
+        assert ((got[:, h] - want).abs() <= bound + u * (want.abs() + bound) + torch.finfo(table.dtype).tiny).all()
+
+
 def test_more_sequences_than_the_sums_keep():
     r = random.Random(6)
     lens = [r.choice((0, 1, 2, r.randint(1, 12))) for _ in range(1300)]

@@ -153,7 +153,7 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = kbase + 8 * (i / 4) + 4 * hi + (i % 4);
-        if (key >= Lk || (CAUSAL && key > my_q)) ds[i] = 0.0f;
+        if (key >= Lk || (CAUSAL && key > my_q) || (REL && my_q >= Lq)) ds[i] = 0.0f;
       }
     }
     if constexpr (REL) {
@@ -222,7 +222,8 @@ __device__ __forceinline__ void bwd_dq_body(const P &p, const int wg, DqLds<D, S
       issue(ST ^ 1, n0 + BN);
     }
     if (!CAUSAL || n0 + (WK == 2 ? 32 * wt : 0) <= qw + 31) {
-      tile_step(ST, n0, (n0 + BN > Lk) || (CAUSAL && n0 + BN - 1 > qw));
+      // (REL: rows past the last query have dS = 0 too, whatever a key holds: 0 * inf is none.)
+      tile_step(ST, n0, (n0 + BN > Lk) || (CAUSAL && n0 + BN - 1 > qw) || (REL && qw + 32 > Lq));
     }
   };
 

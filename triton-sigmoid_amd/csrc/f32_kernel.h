@@ -244,7 +244,7 @@ __device__ __forceinline__ void dq_full(const P &p, const Item &w_, float *lds, 
       if constexpr (P::kRel) c = -(bias + rel_at(p, h, k0 + kr - myq)) * kLog2e;
       const float pr = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, c)), u = pr * dp[i];
       ds[i] = __builtin_fmaf(-pr, u, u);
-      if (k0 + kr >= Lk || (CAUSAL && k0 + kr > myq)) ds[i] = 0.0f;
+      if (k0 + kr >= Lk || (CAUSAL && k0 + kr > myq) || (P::kRel && myq >= rows)) ds[i] = 0.0f;
     }
     if constexpr (P::kRel) sums.add(ds, k0 - qw, l32, hi);
     row_product<D>(acc, tK, ds, rr);
@@ -789,8 +789,10 @@ __device__ __forceinline__ void dq_f32_body(const P &p, int wg, float *lds, [[ma
       const float pr = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, c)), u = pr * dp[i];
       ds[i] = __builtin_fmaf(-pr, u, u);  // dP·P·(1 - P)
     }
-    if (k0 + FB > Lk || (CAUSAL && k0 + FB - 1 > qw)) {
-      const int lim = (CAUSAL ? min(Lk, myq + 1) : Lk) - k0 - 4 * hi;
+    if (k0 + FB > Lk || (CAUSAL && k0 + FB - 1 > qw) || (P::kRel && qw + FB > Lq)) {
+      // (P::kRel: rows past the last query have dS = 0 too, whatever a key holds: 0 * inf is none.)
+      const int keys = P::kRel && myq >= Lq ? 0 : (CAUSAL ? min(Lk, myq + 1) : Lk);
+      const int lim = keys - k0 - 4 * hi;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (8 * (i / 4) + i % 4 >= lim) ds[i] = 0.0f;
