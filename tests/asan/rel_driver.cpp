@@ -336,7 +336,9 @@ void empty_calls() {
         EXPECT(sigattn_rel_fwd(&p, &r, kO, kWs, sigattn_rel_fwd_workspace_bytes(&p, &r), nullptr) == SIGATTN_OK);
         EXPECT(sigattn_rel_bwd(&p, &r, nullptr, kDo, kDq, kDk, kDv, kTable, kWs, sigattn_rel_bwd_workspace_bytes(&p, &r),
                                nullptr) == SIGATTN_OK);
-        EXPECT(find("rel_grad_kernel") != nullptr);
+        // (The sums' kernel finds every batch's first slot by dividing by the rows of a block.)
+        const Kernel *sums = find("rel_sums_kernel");
+        EXPECT(find("rel_grad_kernel") != nullptr && sums != nullptr && sums->p.part_rows > 0);
       }
 }
 

@@ -19,6 +19,7 @@ RelParams rel_params(const sigattn_problem *p, const RelTable &t, const void *li
   k.line = (const float *)line;
   if (p->bias == nullptr) k.bias = (const float *)((const char *)line + rel_line_bytes(t));
   k.reach = t.reach;
+  k.part_rows = kGenericRows;  // of calls without blocks of queries too, which divide by it
   return k;
 }
 
@@ -160,7 +161,6 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
       launch_rel_dkdv_mfma(kk, p->dtype, D, causal, st);
     }
   } else {
-    k.part_rows = kGenericRows;
     launch_rel_dq_generic(k, p->dtype, D, causal, st);
     if (p->Tk > 0) launch_rel_dkdv_generic(rel_kv_items(k), p->dtype, D, causal, st);
   }
