@@ -405,6 +405,26 @@ void rotary() {
       EXPECT(g_kernels.size() == (r.q_heads + r.kv_heads > 0 ? 1u : 0u));
     }
   }
+  // As many rows as the check lets through, on 16-byte boundaries and off them.
+  for (const int dtype : {SIGATTN_BF16, SIGATTN_F32})
+    for (const int64_t heads : {1, 40, 65535})
+      for (const int64_t D : {16, 128})
+        for (const int64_t odd : {0, 1}) {
+          sigattn_rotary r;
+          std::memset(&r, 0, sizeof r);
+          r.dtype = dtype, r.D = r.rot_dim = D, r.q_heads = heads, r.num_positions = 9;
+          r.q_stride_t = heads * D + odd, r.q_stride_h = D;
+          r.q = kQ, r.q_out = kO, r.positions = (int32_t *)at(12), r.angles = (float *)at(13);
+          r.rows = std::min<int64_t>(INT32_MAX / 2, (int64_t(1) << 42) / (heads * D));
+          g_kernels.clear();
+          EXPECT(sigattn_rotary_apply(&r, nullptr) == SIGATTN_OK && g_kernels.size() == 1);
+          const int64_t columns = dtype == SIGATTN_F32 ? 8 : 16;  // of a thread
+          const dim3 g = g_kernels[0].grid;
+          if (!odd) EXPECT((int64_t)g.x * g.y * 256 >= r.rows * heads * D / columns);
+          r.rows = r.rows + 1;
+          g_kernels.clear();
+          EXPECT(sigattn_rotary_apply(&r, nullptr) == SIGATTN_ERR_SHAPE && g_kernels.empty());
+        }
 }
 
 }  // namespace

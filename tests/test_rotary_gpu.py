@@ -319,3 +319,35 @@ def test_streams_and_two_calls_at_once():
                 got.append(ts.rotary_embedding(*c, pos, angles))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))
+
+
+@pytest.mark.parametrize("off", [0, 1])
+def test_more_rows_than_a_launch_has_workgroups(off):
+    """2^24 rows and more, on 16-byte boundaries and off them: each as its copy among a few."""
+    N, D, g = 2 ** 24 + 300, 16, torch.Generator().manual_seed(off)
+    few = randn(g, 4099, 1, D, dtype=torch.bfloat16)
+    at, angles = torch.arange(4099, dtype=I32, device="cuda"), tables(5000, D)
+    q = torch.empty(N * D + off, dtype=torch.bfloat16, device="cuda")[off:].view(N, 1, D)
+    rows = torch.arange(N, device="cuda") % 4099
+    q.copy_(few[rows])
+    got, _ = ts.rotary_embedding(q, few[:1].expand(N, 1, D), rows.to(I32), angles)
+    want, _ = ts.rotary_embedding(few, few, at, angles)
+    assert torch.equal(got, want[rows])
+
+
+def test_more_units_than_a_launch_has_threads():
+    """2^32 pieces and more (of an expanded query, whose copy is 137 GB): as in calls of a few rows."""
+    N, H, D = 2 ** 23 + 70, 64, 128
+    if torch.cuda.mem_get_info()[0] < 180 << 30:
+        pytest.skip("not enough free memory")
+    g = torch.Generator().manual_seed(0)
+    q, k = randn(g, 1, H, D, dtype=torch.bfloat16), randn(g, 1, 1, D, dtype=torch.bfloat16)
+    angles, at = tables(1000, D), (torch.arange(N, device="cuda") % 1000).to(I32)
+    got, keys = ts.rotary_embedding(q.expand(N, H, D), k.expand(N, 1, D), at, angles)
+    want, want_keys = ts.rotary_embedding(q.expand(1000, H, D), k.expand(1000, 1, D), at[:1000].contiguous(), angles)
+    for first in (0, 2 ** 22, 2 ** 23 - 1000, 2 ** 23, N - 500):
+        n = min(1000, N - first)
+        assert torch.equal(got[first:first + n], want[at[first:first + n].long()]), first
+    assert torch.equal(keys, want_keys[at.long()])
+    del got
+    torch.cuda.empty_cache()

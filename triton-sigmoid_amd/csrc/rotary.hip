@@ -36,9 +36,10 @@ __device__ __forceinline__ void turn_pair(float a, float b, float cs, float sn, 
 
 // Any strides, alignment and rot_dim: a workgroup per row, a thread per pair (or two
 // copied columns); bound by its narrow loads (bf16 16384 rows H=32 Hkv=8 D=128 384 us
-// forward and backward, where the other kernel takes 119).
-template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
-  const int64_t t = blockIdx.x;
+// forward and backward, where the other kernel takes 119).  A launch has fewer than 2^32
+// threads: a workgroup goes on to the row kRotaryRows behind its own.
+constexpr int64_t kRotaryRows = 1 << 20;
+template <typename T, bool PAIRS> __device__ __forceinline__ void rotary_row(const RotaryArgs &a, const int64_t t) {
   const int half = a.rot / 2, dh = a.D / 2;
   const int pos = min(max(a.positions[t], 0), a.num_positions - 1);
   const float *row = a.angles + (int64_t)pos * a.rot;
@@ -70,11 +71,15 @@ template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_
     rot_st<T>(dst, x, u), rot_st<T>(dst, y, w);
   }
 }
+template <typename T, bool PAIRS> __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+  for (int64_t t = blockIdx.x; t < a.rows; t += kRotaryRows) rotary_row<T, PAIRS>(a, t);
+}
 
 // Rows on 16-byte boundaries: a thread's unit is two 16-byte pieces, E pairs
 // of columns (pieces of the two halves, or neighbours), or two pieces to copy.
 // Units of all rows and heads follow one another; the quotient by a row's units is
-// exact in fp32 (a workgroup's span and a row's units lie below 2^22).  Bound by
+// exact in fp32 (a workgroup's span and a row's units lie below 2^22).  The grid's second
+// dimension counts kRotarySlice workgroups each (fewer than 2^32 threads in the first).  Bound by
 // memory, at the rate of a large copy (5.1 TB/s): bf16 16384 rows H=32 Hkv=8 D=128
 // (337 MB) 60.6 us, 5.6 TB/s, fp16 16383 rows H=16 Hkv=8 D=64 into a cache 23.6 us;
 // 64 rows into a cache 3.4 us.  (Two units a thread 62.0 and 23.7, four 69.3 and
@@ -91,13 +96,14 @@ template <typename T> struct RotaryPiece {
   }
 };
 
+constexpr int64_t kRotarySlice = 1 << 23;
 template <typename T, bool PAIRS, bool CACHE>
 __global__ __launch_bounds__(256) void rotary_wide_kernel(const RotaryArgs a, const int lu) {
   using Piece = RotaryPiece<T>;
   constexpr int E = Piece::E;
   const int half = a.rot / 2;
   const int n = (a.heads[0] + a.heads[1] + a.heads[2]) << lu;  // units of a row, 1 << lu of a head
-  const int64_t base = (int64_t)blockIdx.x * 256, row0 = base / n;
+  const int64_t base = (blockIdx.y * kRotarySlice + blockIdx.x) * 256, row0 = base / n;
   const int i = (int)(base - row0 * n) + (int)threadIdx.x, q = (int)(((float)i + 0.5f) * (1.0f / (float)n));
   const int64_t t = row0 + q;
   if (t >= a.rows) return;
@@ -158,8 +164,10 @@ template <typename T> bool rotary_wide(const RotaryArgs &a, int &lu) {
 }
 
 template <typename T, bool PAIRS, bool CACHE> void rotary_launch(const RotaryArgs &a, int lu, hipStream_t st) {
-  const int64_t units = a.rows * ((int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) << lu);
-  rotary_wide_kernel<T, PAIRS, CACHE><<<dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st>>>(a, lu);
+  const int64_t units = a.rows * ((int64_t)(a.heads[0] + a.heads[1] + a.heads[2]) << lu), groups = (units + 255) / 256;
+  const int64_t slices = (groups + kRotarySlice - 1) / kRotarySlice;
+  const dim3 grid((unsigned)(slices > 1 ? kRotarySlice : groups), (unsigned)slices);
+  rotary_wide_kernel<T, PAIRS, CACHE><<<grid, dim3(256), 0, st>>>(a, lu);
 }
 
 template <typename T> void rotary_t(const RotaryArgs &a, bool pairs, hipStream_t st) {
@@ -172,8 +180,9 @@ template <typename T> void rotary_t(const RotaryArgs &a, bool pairs, hipStream_t
     else rotary_launch<T, false, false>(a, lu, st);
     return;
   }
-  if (pairs) rotary_kernel<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
-  else rotary_kernel<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, st>>>(a);
+  const dim3 grid((unsigned)(a.rows < kRotaryRows ? a.rows : kRotaryRows));
+  if (pairs) rotary_kernel<T, true><<<grid, dim3(256), 0, st>>>(a);
+  else rotary_kernel<T, false><<<grid, dim3(256), 0, st>>>(a);
 }
 
 int rotary_run(const sigattn_rotary *r, bool cache, hipStream_t st) {
@@ -208,7 +217,7 @@ int rotary_check(const sigattn_rotary *r) {
   if (r->rows < 0 || r->rows > INT32_MAX / 2 || r->q_heads < 0 || r->kv_heads < 0 || r->q_heads > 65535 ||
       r->kv_heads > 65535 || r->num_positions > INT32_MAX)
     return SIGATTN_ERR_SHAPE;
-  // (Workgroups of 256 units of 16 columns at least.)
+  // (Units of 16 columns, in fp32 8, in workgroups of 256: 2^8 slices at most.)
   if (r->rows > 0 && (r->q_heads + 2 * r->kv_heads) * r->D > ((int64_t)1 << 42) / r->rows) return SIGATTN_ERR_SHAPE;
   if (r->rot_dim < 2 || r->rot_dim > r->D || r->rot_dim % 2 != 0 || r->num_positions < 1) return SIGATTN_ERR_ROTARY;
   const int64_t strides[4] = {r->q_stride_t, r->q_stride_h, r->k_stride_t, r->k_stride_h};
