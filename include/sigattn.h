@@ -405,13 +405,16 @@ int sigattn_rel_check(const sigattn_problem *p, const sigattn_rel_bias *r);
  * given as `line` to the backward of the same problem, it is not read from the
  * table again (NULL: it is), nor the default bias made again.
  * `dtable` is the table's gradient, [num_buckets, H] of its type, written whole:
- * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed).
+ * fp32 sums of the fp32 dS in a fixed order, rounded once (NULL: not computed, and
+ * sigattn_rel_bwd_frozen_workspace_bytes is enough: without the sums of each block of
+ * queries, B + rows_q / 64 (fp32 below D = 128: 32) lines of every head).
  * Deterministic.
  */
 size_t sigattn_rel_fwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
 int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *out, void *workspace,
                     size_t workspace_bytes, void *stream);
 size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
+size_t sigattn_rel_bwd_frozen_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r);
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
                     void *dk, void *dv, void *dtable, void *workspace, size_t workspace_bytes, void *stream);
 

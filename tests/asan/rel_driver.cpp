@@ -235,8 +235,8 @@ void training(const sigattn_problem &p, const sigattn_rel_bias &r, bool mfma, bo
 
   for (const bool lines : {false, true}) {
     g_kernels.clear(), g_parts = 0;
-    n = sigattn_rel_bwd_workspace_bytes(&p, &r);
-    EXPECT(sigattn_rel_bwd(&p, &r, lines ? kLine : nullptr, kDo, kDq, kDk, kDv, with_table ? kTable : nullptr, kWs, n,
+    n = (with_table ? sigattn_rel_bwd_workspace_bytes : sigattn_rel_bwd_frozen_workspace_bytes)(&p, &r);
+    EXPECT(n > 0 && sigattn_rel_bwd(&p, &r, lines ? kLine : nullptr, kDo, kDq, kDk, kDv, with_table ? kTable : nullptr, kWs, n,
                            nullptr) == SIGATTN_OK);
     spans.clear();
     const Kernel *made = find("rel_line_kernel"), *one = find("rel_bwd"), *sums = find("rel_sums_kernel"),

@@ -216,6 +216,27 @@ def test_rel_calls_need_their_workspace():
     assert lib.sigattn_paged_rel_fwd(pp, r, FAKE, None, 0, None) == -10
 
 
+@pytest.mark.parametrize("dtype, D, rows", [(_capi.BF16, 64, 64), (_capi.BF16, 128, 64), (_capi.F32, 64, 32),
+                                            (_capi.F32, 128, 64)])
+def test_workspaces_with_and_without_a_gradient_of_the_table(dtype, D, rows):
+    """A sum per block of queries, head and position; a call that wants none pays for none."""
+    lib, N, H, R = _capi.load_library(), 65536, 32, 2048
+    p = _problem(dtype=dtype, D=D, B=4, Tq=N, Tk=N, rows_q=N, rows_k=N, H=H, kv_heads=H, q_stride_t=H * D, q_stride_h=D,
+                 k_stride_t=H * D, k_stride_h=D)
+    r = _rel(max_distance=R)
+    parts = (N // rows + 4) * H * (2 * R + 1) * 4
+    full = lib.sigattn_rel_bwd_workspace_bytes(ctypes.byref(p), ctypes.byref(r))
+    frozen = lib.sigattn_rel_bwd_frozen_workspace_bytes(ctypes.byref(p), ctypes.byref(r))
+    line = lib.sigattn_rel_fwd_workspace_bytes(ctypes.byref(p), ctypes.byref(r))
+    assert frozen == line < 1 << 20
+    assert parts <= full - frozen - line <= parts + 256
+    assert lib.sigattn_rel_bwd(ctypes.byref(p), ctypes.byref(r), None, FAKE, FAKE, FAKE, FAKE, None, FAKE, frozen - 1,
+                               None) == -10
+    assert lib.sigattn_rel_bwd(ctypes.byref(p), ctypes.byref(r), None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, frozen,
+                               None) == -10
+    assert lib.sigattn_rel_bwd_frozen_workspace_bytes(None, ctypes.byref(r)) == 0
+
+
 def _rotary(**kw):
     r = _set(_capi.SigattnRotary(), dtype=_capi.BF16, rows=3, q_heads=4, kv_heads=2, D=64, rot_dim=64, num_positions=9,
              q_stride_t=256, q_stride_h=64, k_stride_t=128, k_stride_h=64, cache_stride_p=2048, cache_stride_t=128,

@@ -232,6 +232,27 @@ def test_a_table_without_gradient(frozen):
         assert torch.equal(full[x], y)
 
 
+@pytest.mark.parametrize("binding", ["node", "python"])
+def test_a_table_without_gradient_takes_no_room_for_one(monkeypatch, binding):
+    if binding == "python":
+        monkeypatch.setenv("SIGATTN_EAGER_BINDING", "python")
+    n, H, R = 4096, 8, 2048
+    q, k, v, do, table, buckets, cu, _ = make([n], [n], H, H, 64, torch.bfloat16, 8, R)
+    sums = n // 64 * H * (2 * R + 1) * 4
+    peak = {}
+    for frozen in (True, False):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        t = table.clone().requires_grad_(not frozen)
+        o = ts.sigmoid_attention_varlen(*leaves, ints(cu), ints(cu), n, n, bias_table=t, bias_buckets=buckets)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(o, leaves + ([] if frozen else [t]), do)
+        peak[frozen] = torch.cuda.max_memory_allocated() - before
+        del o, got
+    assert peak[False] >= sums > 2 ** 23 and peak[True] < 3 * q.numel() * 2 + 2 ** 21
+
+
 def test_captured_step_replays():
     q, k, v, do, table, buckets, cu, _ = make([300, 170, 64], [300, 170, 64], 4, 2, 64, torch.bfloat16, 32, 100)
     leaves = [t.requires_grad_() for t in (q, k, v, table)]

@@ -29,9 +29,26 @@ void make_line(const sigattn_problem *p, const RelTable &t, void *to, hipStream_
 }
 
 int64_t rel_part_bytes(const sigattn_problem *p, const RelTable &t) {
-  // (The shortest blocks' rows; a multiple of 256 bytes.)
-  const int rows = p->dtype == SIGATTN_F32 ? 32 : kGenericRows;
+  // (The shortest blocks' rows: whether the portable kernel's are taken depends on pointers
+  // that a query of the size does not have.  A multiple of 256 bytes.)
+  const int rows = p->dtype == SIGATTN_F32 && p->D < 128 ? 32 : kGenericRows;
   return ((p->rows_q / rows + p->B) * p->H * (2 * t.reach + 1) * (int64_t)sizeof(float) + 255) / 256 * 256;
+}
+
+// The backward's workspace: what the line's launch leaves, then (grad: a gradient of the
+// table) the sums over blocks and those of each block, then grouped heads' parts.
+struct RelSpace {
+  int64_t sums, part, kv_part, bytes;
+};
+RelSpace rel_space(const sigattn_problem *p, const RelTable &t, bool grad) {
+  RelSpace s;
+  s.sums = rel_head_bytes(p, t);
+  s.part = s.sums + (grad ? rel_line_bytes(t) : 0);
+  s.kv_part = s.part + (grad ? rel_part_bytes(p, t) : 0);
+  // (Pointers are not known to a query: aligned rows, as everywhere.)
+  const void *none[1] = {nullptr};
+  s.bytes = s.kv_part + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes;
+  return s;
 }
 
 RelParams rel_kv_items(const RelParams &k) {
@@ -103,10 +120,12 @@ int sigattn_rel_fwd(const sigattn_problem *p, const sigattn_rel_bias *r, void *o
 
 size_t sigattn_rel_bwd_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
   if (sigattn_rel_check(p, r) != SIGATTN_OK) return 0;
-  const RelTable t = rel_table(r, p->H, p->Tq, p->Tk);
-  // (Pointers are not known yet: aligned rows, as everywhere.)
-  const void *none[1] = {nullptr};
-  return (size_t)(rel_head_bytes(p, t) + rel_line_bytes(t) + rel_part_bytes(p, t) + head_split(p, use_mfma(p, none, 0) || use_f32_mfma(p, none, 0)).bytes);
+  return (size_t)rel_space(p, rel_table(r, p->H, p->Tq, p->Tk), true).bytes;
+}
+
+size_t sigattn_rel_bwd_frozen_workspace_bytes(const sigattn_problem *p, const sigattn_rel_bias *r) {
+  if (sigattn_rel_check(p, r) != SIGATTN_OK) return 0;
+  return (size_t)rel_space(p, rel_table(r, p->H, p->Tq, p->Tk), false).bytes;
 }
 
 int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const void *line, const void *dout, void *dq,
@@ -118,11 +137,12 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
   if ((p->rows_q > 0 && (dq == nullptr || dout == nullptr)) ||
       (p->rows_k > 0 && (dk == nullptr || dv == nullptr)))
     return SIGATTN_ERR_NULL_ARG;
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < sigattn_rel_bwd_workspace_bytes(p, r))
+  const RelSpace space = rel_space(p, t, dtable != nullptr);
+  if (workspace == nullptr || !aligned16(workspace) || (int64_t)workspace_bytes < space.bytes)
     return SIGATTN_ERR_WORKSPACE;
   const hipStream_t st = (hipStream_t)stream;
   RelParams k = rel_params(p, t, line != nullptr ? line : workspace);
-  float *sums = (float *)((char *)workspace + rel_head_bytes(p, t));
+  float *sums = (float *)((char *)workspace + space.sums);
   k.dout = dout;
   k.dq = dq;
   k.dk = dk;
@@ -139,12 +159,11 @@ int sigattn_rel_bwd(const sigattn_problem *p, const sigattn_rel_bias *r, const v
     return launch_status();
   }
   if (line == nullptr) make_line(p, t, workspace, st);
-  char *parts = (char *)sums + rel_line_bytes(t);
-  if (dtable != nullptr) k.part = (float *)parts;
+  if (dtable != nullptr) k.part = (float *)((char *)workspace + space.part);
   if (mfma) {
     const HeadSplit hs = head_split(p, mfma);
     k.qsplit = hs.n;
-    k.kv_part = (float *)(parts + rel_part_bytes(p, t));
+    k.kv_part = (float *)((char *)workspace + space.kv_part);
     k.part_rows = f32 ? rel_dq_rows_f32(k, D, causal) : rel_dq_rows(k, D, causal);
     RelParams kq = k;
     GapAxis gq, gk;

@@ -69,6 +69,7 @@ struct Api {
   decltype(&sigattn_rel_fwd_workspace_bytes) rel_fwd_workspace_bytes = nullptr;
   decltype(&sigattn_rel_fwd) rel_fwd = nullptr;
   decltype(&sigattn_rel_bwd_workspace_bytes) rel_bwd_workspace_bytes = nullptr;
+  decltype(&sigattn_rel_bwd_frozen_workspace_bytes) rel_bwd_frozen_workspace_bytes = nullptr;
   decltype(&sigattn_rel_bwd) rel_bwd = nullptr;
   decltype(&sigattn_paged_rel_fwd_workspace_bytes) paged_rel_fwd_workspace_bytes = nullptr;
   decltype(&sigattn_paged_rel_fwd) paged_rel_fwd = nullptr;
@@ -339,7 +340,8 @@ struct RelNode : public torch::autograd::Function<RelNode> {
     const c10::DeviceGuard guard(q.device());
     const sigattn_problem p = make_problem(q, k, v, saved[5], Tensor(), saved[6], lay, ctx->saved_data["causal"].toBool());
     const sigattn_rel_bias r = make_rel(table, buckets);
-    const int64_t nbytes = (int64_t)g_api.rel_bwd_workspace_bytes(&p, &r);
+    const int64_t nbytes =
+        (int64_t)(want_table ? g_api.rel_bwd_workspace_bytes(&p, &r) : g_api.rel_bwd_frozen_workspace_bytes(&p, &r));
     const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
     check_rc(g_api.rel_bwd(&p, &r, saved[9].data_ptr(), dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
                            want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes, stream_of(q.device())),
@@ -844,6 +846,7 @@ void bind(const py::dict &fns, const std::vector<int64_t> &two_pass_dims, int64_
   bind_one(api.rel_fwd_workspace_bytes, fns, "sigattn_rel_fwd_workspace_bytes");
   bind_one(api.rel_fwd, fns, "sigattn_rel_fwd");
   bind_one(api.rel_bwd_workspace_bytes, fns, "sigattn_rel_bwd_workspace_bytes");
+  bind_one(api.rel_bwd_frozen_workspace_bytes, fns, "sigattn_rel_bwd_frozen_workspace_bytes");
   bind_one(api.rel_bwd, fns, "sigattn_rel_bwd");
   bind_one(api.paged_rel_fwd_workspace_bytes, fns, "sigattn_paged_rel_fwd_workspace_bytes");
   bind_one(api.paged_rel_fwd, fns, "sigattn_paged_rel_fwd");

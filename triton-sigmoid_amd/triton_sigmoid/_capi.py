@@ -215,6 +215,8 @@ SIGNATURES = {
                          _c_vp], _c_i32),
     "sigattn_rel_bwd_workspace_bytes": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)],
                                         ctypes.c_size_t),
+    "sigattn_rel_bwd_frozen_workspace_bytes": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias)],
+                                               ctypes.c_size_t),
     "sigattn_rel_bwd": ([ctypes.POINTER(SigattnProblem), ctypes.POINTER(SigattnRelBias), _c_vp, _c_vp, _c_vp, _c_vp,
                          _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_vp], _c_i32),
     "sigattn_paged_rel_check": ([ctypes.POINTER(SigattnPagedProblem), ctypes.POINTER(SigattnRelBias)], _c_i32),
@@ -272,7 +274,8 @@ _AUTOGRAD_FNS = ("sigattn_strerror", "sigattn_fwd_workspace_bytes", "sigattn_fwd
                  "sigattn_bwd_workspace_bytes", "sigattn_bwd_ws", "sigattn_bwd_split_workspace_bytes",
                  "sigattn_bwd_split", "sigattn_default_bias", "sigattn_paged_plan", "sigattn_paged_write",
                  "sigattn_paged_fwd_workspace_bytes", "sigattn_paged_fwd", "sigattn_rel_fwd_workspace_bytes",
-                 "sigattn_rel_fwd", "sigattn_rel_bwd_workspace_bytes", "sigattn_rel_bwd",
+                 "sigattn_rel_fwd", "sigattn_rel_bwd_workspace_bytes", "sigattn_rel_bwd_frozen_workspace_bytes",
+                 "sigattn_rel_bwd",
                  "sigattn_paged_rel_fwd_workspace_bytes", "sigattn_paged_rel_fwd", "sigattn_rotary_apply",
                  "sigattn_paged_write_rotary")
 _autograd = None  # the bound module, or False after a failed import
@@ -759,7 +762,8 @@ def backward_rel(Q, K, V, dO, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seql
                   packed=_packed_dims(Q, K, cu_q, cu_k, max_seqlen_q, max_seqlen_k))
 
     def run(stream):
-        nbytes = int(lib.sigattn_rel_bwd_workspace_bytes(ctypes.byref(pr), ctypes.byref(r)))
+        need = lib.sigattn_rel_bwd_workspace_bytes if want_table else lib.sigattn_rel_bwd_frozen_workspace_bytes
+        nbytes = int(need(ctypes.byref(pr), ctypes.byref(r)))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         _raise(lib.sigattn_rel_bwd(ctypes.byref(pr), ctypes.byref(r), None, _ptr(dO), _ptr(dQ), _ptr(dK), _ptr(dV),
                                    _ptr(dtable), ws.data_ptr(), nbytes, stream), "sigattn_rel_bwd")
