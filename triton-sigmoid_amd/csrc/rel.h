@@ -103,6 +103,13 @@ constexpr int kNearMargin = 64, kSkewRow = 12, kSkew = 39 * kSkewRow;
 __host__ __device__ constexpr int near_places(int reach) { return 2 * reach + 2 * kNearMargin; }
 __host__ __device__ constexpr int near_floats(int reach, int waves = 4) { return waves * (near_places(reach) + kSkew); }
 
+// What the wave's lanes wrote to LDS before is what its lanes read behind this.  The
+// hardware keeps a wave's LDS accesses in order, so no instruction comes of it.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int NW> struct PlaceSums {
   float beyond[2] = {0.0f, 0.0f};
   float *mine, *skew;  // relative position 0 of the wave's line; its piece
@@ -137,11 +144,13 @@ template <int NW> struct PlaceSums {
     for (int g = 0; g < 4; ++g) {  // keys 8g .. 8g + 7, places 8g - 31 .. 8g + 7 from `off` on
 #pragma unroll
       for (int j = 0; j < 4; ++j) to[j * (kSkewRow + 1)] = ds[4 * g + j] * sgn;
+      wave_order();
       const int row = lane - 8 * g;
       const float *from = skew + min(max(row, 0), 38) * kSkewRow;
       const f32x4 u = *(const f32x4 *)from, v = *(const f32x4 *)(from + 4);
       const float y = ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
       x += row >= 0 && row <= 38 ? y : 0.0f;
+      wave_order();
     }
     mine[off - 31 + lane] += x;
   }
