@@ -333,6 +333,51 @@ def test_128_columns_and_the_room_for_sums(R, causal):
     check(make(lens, lens, 1, 1, 128, torch.bfloat16, 40, R, seed=R), causal)
 
 
+# Where dQ at D = 128 takes workgroups of eight waves: reaches 159 .. 1190.
+@pytest.mark.parametrize("dtype, R", [("bf16", 158), ("bf16", 159), ("f16", 159), ("bf16", 1190), ("f16", 1190),
+                                      ("bf16", 1191)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_128_columns_on_either_side_of_eight_waves(dtype, R, causal):
+    lens = [1250, 0, 33] if R > 1000 else [500, 0, 33]  # (a line reaches no further than the longest)
+    check(make(lens, lens, 2, 1, 128, DT[dtype], 400, R, seed=R), causal)
+
+
+@pytest.mark.parametrize("H, Hkv", [(3, 1), (8, 8), (12, 4), (16, 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_eight_waves_and_grouped_heads(H, Hkv, dtype):
+    lens = [180, 300, 37, 257]
+    check(make(lens, lens, H, Hkv, 128, DT[dtype], 16, 170, seed=H), True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_eight_waves_and_many_sequences(dtype):
+    r = random.Random(9)
+    lens = [200, 290] + [r.choice((0, 1, 3, r.randint(1, 90))) for _ in range(100)]
+    for causal in (False, True):
+        check(make(lens, lens, 2, 1, 128, DT[dtype], 10, 180, seed=7), causal)
+    check(make(lens, lens[::-1], 2, 1, 128, DT[dtype], 10, 180, seed=8), False)
+
+
+@pytest.mark.parametrize("dtype, D, R", [("bf16", 128, 200), ("f16", 128, 200), ("bf16", 64, 200), ("f32", 128, 200),
+                                         ("f32", 32, 200)])
+def test_far_reaches_and_rows_outside_every_sequence(dtype, D, R):
+    q, k, v, do, table, buckets, cu, _ = make([210, 300], [210, 300], 2, 1, D, DT[dtype], 8, R, first=70, rest=70)
+    got = run(q, k, v, do, table, buckets, cu, cu, True, mq=280, mk=280)
+    cut = [70, 280, 560]  # the second sequence to 280 rows; its default bias is the whole one's
+    want = packed_rel(q[:560], k[:560], v[:560], do[:560], table, buckets, cut, cut, True, [-math.log(210), -math.log(300)])
+    for x in ("o", "dq", "dk", "dv"):
+        assert_within(got[x][:560], want[x], x)
+        assert not got[x][560:].any() and not got[x][:70].any(), x
+    assert_within(got["dtable"], want["dtable"], "dtable")
+
+
+@pytest.mark.parametrize("lens, H, R, causal", [([300, 290], 2, 300, True), ([600], 3, 1000, False),
+                                                ([1800, 70], 1, 2048, True)])
+def test_fp32_far_reaches_at_128_columns(lens, H, R, causal):
+    """The longest leave room for the tiles of one wave to 32 rows instead of two."""
+    check(make(lens, lens, H, 1, 128, torch.float32, 40, R, seed=R), causal)
+
+
 @pytest.mark.parametrize("D, dtype", [(64, "bf16"), (128, "f16"), (32, "f32")])
 def test_bindings_alike(monkeypatch, D, dtype):
     args = make([300, 1, 77], [300, 1, 77], 4, 2, D, DT[dtype], 16, 60, seed=D)

@@ -41,10 +41,10 @@ template <typename T, int D, int WK, int NW = 4> void dq_w(const RelParams &kp, 
 }
 
 // At D = 128 two workgroups of four waves share a CU as long as their sums' lines fit
-// beside the tiles, up to a reach of 143.  Beyond, one of eight waves holds as many, in
-// twice the queries per copied tile (up to 1139, then four alone).  Causal step of 3
-// sequences of 1500 .. 4096 H=16 Hkv=4, us by reach: 140 720, 150 719, 300 747, 1000 769, 1300
-// 893 (four waves alone at 150: dQ 500 instead of 330).
+// beside the tiles, up to a reach of 158.  Beyond, one of eight waves holds as many, in
+// twice the queries per copied tile (up to 1190, then four alone).  dQ of the causal step of 3
+// sequences of 1500 .. 4096 H=16 Hkv=4, us by reach: four waves 140 327, 150 308, 158 306;
+// eight 160 327, 300 327, 1100 345, 1190 347; four alone 1200 515.
 bool dq_eight_waves(const RelParams &p, int D) {
   constexpr size_t tiles = 4 * 64 * 128 * 2, cu = 163840 - 512;
   const size_t four = tiles + 2 * 192 * 4 + near_floats(p.reach, 4) * 4, eight = tiles + 2 * 320 * 4 + near_floats(p.reach, 8) * 4;
