@@ -461,6 +461,34 @@ def test_fp32_sums_do_not_drift():
         assert (got[0, h] - ds.sum()).abs() <= bound
 
 
+def test_fp32_sums_would_show_a_drift():
+    """Sixty-four million dS of either sign in one bucket, with a bound that a drift of
+    2^-27 of each dP to one side would be twice of (what the matrix cores' truncations add
+    up to here: 9.1e-5 when nothing was done about it, 6e-8 now).  What has no preferred
+    sign adds up as its square.  A truncation to 24 bits leaves 2^-23 / sqrt(12) of its value
+    about the mean, three of them, of partial sums up to |dO|·|V|, 2^-24 of those: dP; of
+    |q|·|k| scale: S, whose sum with the bias and the table's value is rounded once more; P is
+    off by 2^-21.  Then the additions: 16 dS, and a lane's running sum of the keys before.
+    Six standard deviations, and 2^-18 of the sum for what all share (the rounded bias
+    and table)."""
+    n, D = 8000, 32
+    q, k, v, do, table, buckets, cu, _ = make([n], [n], 1, 1, D, torch.float32, 1, 0, seed=8)
+    got = run(q, k, v, do, table, buckets, cu, cu, False)["dtable"].double()[0, 0]
+    q, k, v, do = (t[:, 0].double() for t in (q, k, v, do))
+    e, scale = 2.0 ** -24, 1.0 / math.sqrt(D)
+    s = q @ k.t().contiguous() * scale + (table.double()[0, 0] - math.log(n))
+    p = torch.sigmoid(s)
+    w, dp = p * (1.0 - p), do @ v.t().contiguous()
+    ds = w * dp
+    var = (e * w * (do.abs() @ v.abs().t().contiguous())).square().sum()
+    var += (e * ds * (q.abs() @ k.abs().t().contiguous() * scale + s.abs())).square().sum()
+    var += (2.0 ** -21 * ds).square().sum()
+    var += (e * ds.cumsum(1)[:, 31::32]).square().sum() * 2 + (16 * e * ds).square().sum()
+    bound = 6 * var.sqrt() + 2.0 ** -18 * ds.sum().abs()
+    assert 2.0 ** -27 * (w * dp.abs()).sum() >= 2 * bound
+    assert (got - ds.sum()).abs() <= bound
+
+
 @pytest.mark.parametrize("f", [(1e-13, 1e12, 1e30, 1e-30), (1.0, 1.0, 1e-15, 1e-14), (1e10, 1e-10, 1e15, 1e10)])
 def test_fp32_values_far_from_one(f):
     """What three bf16 parts cannot hold takes the fp32 instruction, the sums by position too."""
