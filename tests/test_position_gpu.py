@@ -634,6 +634,39 @@ def test_paged_captured_step_replays():
         assert torch.equal(got, step())
 
 
+@pytest.mark.parametrize("dtype, D", [("bf16", 128), ("f16", 64), ("bf16", 32), ("f32", 128), ("f32", 32)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("new", [[1, 1], [90, 40], [90, 1]])
+def test_paged_values_of_positions_that_hold_no_key(dtype, D, causal, new):
+    """NaN at relative positions that lie behind every sequence: no pair's, so of no consequence."""
+    g, R, ctx = torch.Generator().manual_seed(4), 200, (37, 71)
+    lens = [c + n for c, n in zip(ctx, new)]
+    kc, vc = (randn(g, 24, 16, 2, D, dtype=DT[dtype]) for _ in range(2))
+    q, values = randn(g, sum(new), 4, D, dtype=DT[dtype]), randn(g, 2 * R + 1, 4, dtype=DT[dtype])
+    table, buckets = torch.arange(24, dtype=I32, device="cuda").view(2, 12), torch.arange(2 * R + 1, dtype=I32, device="cuda")
+    first = 1 if causal else max(new)  # the nearest position that no pair has
+
+    def attend(t):
+        return ts.sigmoid_attention_paged(q, kc, vc, table, ints(lens), ints(offsets(new)), max(new), is_causal=causal,
+                                          bias_table=t, bias_buckets=buckets)
+
+    want = attend(values)
+    values[R + first:] = math.nan
+    assert torch.equal(attend(values), want) and want.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 32), ("f32", 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_values_of_positions_that_hold_no_pair(dtype, D, causal):
+    lens, R = [37, 70], 200
+    q, k, v, do, table, _, cu, _ = make(lens, lens, 2, 1, D, DT[dtype], 2 * R + 1, R)
+    buckets = torch.arange(2 * R + 1, dtype=I32, device="cuda")
+    want = run(q, k, v, do, table, buckets, cu, cu, causal)
+    table[R + (1 if causal else 70):] = table[:R - 69] = math.nan
+    got = run(q, k, v, do, table, buckets, cu, cu, causal)
+    assert all(torch.equal(got[x], want[x]) and want[x].isfinite().all() for x in want)
+
+
 def test_what_was_trained_is_served():
     """A sequence in one training-shaped call, and token by token over a paged cache."""
     g = torch.Generator().manual_seed(8)

@@ -1068,7 +1068,8 @@ __global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const P p) {
   const int l32 = lane & 31, hi = lane >> 5;
   const int cols = un.Lq * p.G, keys = un.k1 - un.k0;
   const int q0 = un.qb * BM, qw = q0 + 32 * w, myq = qw + l32;
-  // Keys of the chunk that column c sees.
+  // Keys of the chunk that column c sees (the others have zero V rows, but what the
+  // learned bias holds there may be NaN).
   const auto seen = [&](int c) SIGATTN_INLINE { return CAUSAL ? un.Lk - un.Lq + c / p.G + 1 - un.k0 : keys; };
   const int nend = min(keys, max(seen(min(q0 + BM, cols) - 1), 0));
   const int wend = qw < cols ? min(nend, seen(min(qw + 32, cols) - 1)) : 0;  // of this wave's columns
@@ -1129,7 +1130,7 @@ __global__ __launch_bounds__(64 * FW, 2) void paged_f32_kernel(const P p) {
     for (int i = 0; i < 16; ++i)
       pr[i] = sigmoid_from_neg_log2(
           __builtin_fmaf(s[i], nsl, P::kRel ? c[i] : SCOREMOD ? tC[8 * (i / 4) + 4 * hi + i % 4] : nbl));
-    if (CAUSAL && k0 + FB > all_see) {
+    if ((CAUSAL || P::kRel) && k0 + FB > all_see) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (k0 + 8 * (i / 4) + 4 * hi + i % 4 >= lim) pr[i] = 0.0f;
@@ -1164,7 +1165,8 @@ __global__ __launch_bounds__(64 * FW, 1) void paged_f32_decode_kernel(const P p)
   const int cols = un.Lq * p.G, keys = un.k1 - un.k0, ntiles = (keys + FB - 1) / FB;
   const int tok = l32 / p.G, head = un.hk * p.G + l32 - tok * p.G;
   // Keys of the chunk that this lane's token sees, and that every token sees.
-  const int lim = un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0, all_see = un.Lk - un.Lq + 1 - un.k0;
+  const int lim = CAUSAL ? un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0 : keys;
+  const int all_see = CAUSAL ? un.Lk - un.Lq + 1 - un.k0 : keys;
   const float bias = p.bias_of(un.Lk), nsl = -p.fscale * kLog2e, nbl = -bias * kLog2e;
   const int64_t row0 = packed_first(p.cu_q, p.rows_q, un.b);
   const uint16_t *Kb = (const uint16_t *)((const float *)p.k + (int64_t)un.hk * p.sk_h);
@@ -1221,7 +1223,7 @@ __global__ __launch_bounds__(64 * FW, 1) void paged_f32_decode_kernel(const P p)
     float pr[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) pr[i] = sigmoid_from_neg_log2(__builtin_fmaf(s[i], nsl, c[i]));
-    if (CAUSAL && k0 + FB > all_see) {
+    if ((CAUSAL || P::kRel) && k0 + FB > all_see) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (k0 + 8 * (i / 4) + 4 * hi + i % 4 >= lim) pr[i] = 0.0f;

@@ -334,7 +334,8 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
     // Block g needs element masks when it crosses seq_lens_k or the diagonal of
     // this wave's first query.
     auto needs_mask = [&](int g) SIGATTN_INLINE {
-      if constexpr (PAGED) return CAUSAL && 32 * g + 32 > all_see;
+      // (Keys past a chunk's have zero V rows, but what the learned bias holds there may be NaN.)
+      if constexpr (PAGED) return CAUSAL ? 32 * g + 32 > all_see : P::kRel && 32 * g + 32 > Lk;
       return (32 * g + 32 > Lk) || (CAUSAL && 32 * g + 31 > qw);
     };
     // Zeroes the P entries of block g whose key lies before 0 (pipeline fill),

@@ -69,7 +69,8 @@ __device__ __forceinline__ void paged_decode_body(const P &p, const int wg, Deco
     for (int ks = 0; ks < NKS; ++ks) qf[ks] = ok && !(half && ks > 0) ? *(const u32x4 *)(qrow + 16 * ks) : zero4();
   }
   // Keys of the chunk that this lane's token sees, and that every token sees.
-  const int lim = un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0, all_see = un.Lk - un.Lq + 1 - un.k0;
+  const int lim = CAUSAL ? un.Lk - un.Lq + min(tok, un.Lq - 1) + 1 - un.k0 : keys;
+  const int all_see = CAUSAL ? un.Lk - un.Lq + 1 - un.k0 : keys;
 
   [[maybe_unused]] RelColumn rc;
   if constexpr (P::kRel) {
@@ -141,14 +142,15 @@ __device__ __forceinline__ void paged_decode_body(const P &p, const int wg, Deco
     }
 
     // P words: accumulator element e of lane (l32, hi) is key
-    // kb + 8(e/4) + 4hi + e%4 of column l32.  Keys past the chunk have zero V rows.
+    // kb + 8(e/4) + 4hi + e%4 of column l32.  Keys past the chunk have zero V rows (but
+    // what the learned bias holds there may be NaN).
     const int kb = KB * i;
     uint32_t pk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       pk[e] = Elem<T>::pack(sigmoid_from_neg_log2(__builtin_fmaf(sc[2 * e], nsl, c[2 * e])),
                             sigmoid_from_neg_log2(__builtin_fmaf(sc[2 * e + 1], nsl, c[2 * e + 1])));
-    if (CAUSAL && kb + KB > all_see) {
+    if ((CAUSAL || P::kRel) && kb + KB > all_see) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int key = kb + 8 * (e / 2) + 4 * hi + 2 * (e % 2);
