@@ -6,6 +6,7 @@ from fractions import Fraction
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import triton_sigmoid as ts
 from triton_sigmoid import _capi
@@ -145,6 +146,18 @@ def test_rotary_write_refusals(kw, error, match):
     args.update(kw)
     with pytest.raises(error, match=match):
         ts.paged_cache_write_rotary(**args)
+
+
+@pytest.mark.parametrize("name", ["query", "key", "value", "key_cache", "value_cache", "angles"])
+def test_tangents_are_not_written(name):
+    args = dict(query=torch.zeros(5, 4, 16), key=torch.zeros(5, 2, 16), value=torch.zeros(5, 2, 16),
+                key_cache=torch.zeros(3, 16, 2, 16), value_cache=torch.zeros(3, 16, 2, 16),
+                slot_mapping=torch.zeros(5, dtype=torch.int32), positions=torch.zeros(5, dtype=torch.int32),
+                angles=torch.zeros(9, 16))
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            ts.paged_cache_write_rotary(**args)
 
 
 # --- C ABI -----------------------------------------------------------------------------

@@ -242,7 +242,7 @@ def rotary_embedding(
 # --- rotary embedding on the way into the cache -----------------------------------
 
 def _write_rotary(query, key, value, key_cache, value_cache, slot_mapping, positions, angles, interleaved):
-    _no_tangent("paged_cache_write_rotary", query, key, value, key_cache, value_cache)
+    _no_tangent("paged_cache_write_rotary", query, key, value, key_cache, value_cache, angles)
     lib = _capi.load_library()
     _capi._check_device(key_cache)
     dev = key_cache.device
