@@ -655,6 +655,62 @@ def test_paged_values_of_positions_that_hold_no_key(dtype, D, causal, new):
     assert torch.equal(attend(values), want) and want.isfinite().all()
 
 
+def _f16_bound(q, k, add, *vectors):
+    """P v (and, of a second one, its transpose times do) of one head in 64 bits, and the bounds with
+    P rounded to 11 bits however small it is (to 2^-37 below 2^-26): reference64's, without
+    what rounding next to zero costs."""
+    D, u, e = q.shape[1], 2.0 ** -11, 2.0 ** -24
+    q, k = q.double(), k.double()
+    p = torch.sigmoid(q @ k.t().contiguous() / math.sqrt(D) + add)
+    share = (D + 8) * e * (q.abs() @ k.abs().t().contiguous() / math.sqrt(D) + add.abs()) + 2.0 ** -21
+    off = p * (share + u) + 2.0 ** -37 * (p < 2.0 ** -26)
+    out = []
+    for x in vectors:
+        val, err = p @ x.double(), off @ x.double().abs() + (p.shape[1] + 2) * e * (p @ x.double().abs())
+        out.append((val, err + u * (val.abs() + err) + 2.0 ** -25))
+        p, off = p.t().contiguous(), off.t().contiguous()
+    return out
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("odd", [False, True])
+def test_f16_sigmoids_next_to_zero(D, odd):
+    """Long contexts have sigmoids near one over their length, and less with negative values:
+    below 2^-14 fp16 has fewer bits of them."""
+    g, n, value = torch.Generator().manual_seed(D), 800, -8.0
+    q, k, v = (randn(g, n * 2 * D + odd, dtype=torch.float16)[odd:].view(n, 2, D) for _ in range(3))
+    v.mul_(4096)  # (so that an output's own rounding is no matter)
+    table, buckets, cu = torch.full((1, 2), value, device="cuda"), ints([0]), ints([0, n])
+    do = randn(g, n, 2, D, dtype=torch.float16) * 4096
+    got = ts.sigmoid_attention_varlen(q, k, v.requires_grad_(), cu, cu, n, n, bias_table=table, bias_buckets=buckets)
+    dv = torch.autograd.grad(got, v, do)[0]
+    add = torch.full((), value - math.log(n), dtype=torch.float64, device="cuda")
+    for h in range(2):
+        o, dv_h = _f16_bound(q[:, h], k[:, h], add, v.detach()[:, h], do[:, h])
+        assert_within(got[:, h], o)
+        assert_within(dv[:, h], dv_h)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("new", [[1, 1], [70, 1], [70, 100]])
+@pytest.mark.parametrize("odd", [False, True])
+def test_paged_f16_sigmoids_next_to_zero(D, new, odd):
+    g, ctx, value = torch.Generator().manual_seed(D), (700, 2900), -7.0
+    lens = [c + n for c, n in zip(ctx, new)]
+    kc, vc = (randn(g, 400, 16, 2, D + odd, dtype=torch.float16)[..., :D] for _ in range(2))
+    vc.mul_(4096)
+    q = randn(g, sum(new), 4, D, dtype=torch.float16)
+    pages = torch.arange(400, dtype=I32, device="cuda").view(2, 200)
+    got = ts.sigmoid_attention_paged(q, kc, vc, pages, ints(lens), ints(offsets(new)), max(new),
+                                     bias_table=torch.full((1, 4), value, device="cuda"), bias_buckets=ints([0]))
+    for b, (n, L, first) in enumerate(zip(new, lens, offsets(new))):
+        rows = [c[200 * b: 200 * b + 200].reshape(3200, 2, D)[:L] for c in (kc, vc)]
+        add = torch.full((), value - math.log(L), dtype=torch.float64, device="cuda")
+        for h in range(4):
+            o, = _f16_bound(q[first:first + n, h], rows[0][:, h // 2], add, rows[1][:, h // 2])
+            assert_within(got[first:first + n, h], o)
+
+
 @pytest.mark.parametrize("dtype, D", [("bf16", 64), ("f16", 128), ("f32", 32), ("f32", 128)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_values_of_positions_that_hold_no_pair(dtype, D, causal):

@@ -350,6 +350,7 @@ template <typename T, int D, bool CAUSAL, bool SCOREMOD, bool DSOUT, bool GROUPE
 __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<D, dkdv_window<P>()> &lds) {
   constexpr int WIN = dkdv_window<P>();
   constexpr bool REL = P::kRel;
+  constexpr int PB = p_bits<T, P>();
   static_assert(!(DSOUT && GROUPED), "two-pass backward of grouped heads: D = 128 only");
   constexpr int BN = 128;                 // keys per workgroup (32 per wave)
   constexpr int BMQ = 64;                 // queries per LDS tile (two 32-query blocks)
@@ -651,7 +652,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<
         for (int x = 0; x < 2; ++x) t[x] = pr[x] * acc_read(pacc[1 - SL][2 * e + x]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) ds[x] = __builtin_fmaf(-pr[x], t[x], t[x]);
-        pw[1 - SL][e] = Elem<T>::pack(pr[0], pr[1]);
+        if constexpr (PB > 0) pw[1 - SL][e] = Elem<T>::pack(pr[0] * (1 << PB), pr[1] * (1 << PB));
+        else pw[1 - SL][e] = Elem<T>::pack(pr[0], pr[1]);
         dw[1 - SL][e] = Elem<T>::pack(ds[0], ds[1]);
         asm volatile("" : "+v"(pw[1 - SL][e]), "+v"(dw[1 - SL][e]));
       }
@@ -713,6 +715,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<
           p.rs_part + (int64_t)ritem * p.rsplit * (2 * BN * D), p.rs_cnt + ritem, rchunk, p.rsplit, w, lane))
     return;
 
+  if constexpr (PB > 0) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) dva[db] *= 1.0f / (1 << PB);
+  }
   if (GROUPED && nparts > 1) {
     if (kok) store_part<NDB>(p, part, b, my_k, h, dka, 0, scale, hi, half), store_part<NDB>(p, part, b, my_k, h, dva, 1, 1.0f, hi, half);
     return;

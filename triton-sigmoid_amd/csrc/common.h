@@ -492,6 +492,20 @@ __device__ __forceinline__ float sigmoid_from_neg_log2(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x));
 }
 
+// 2^E times that.
+template <int E> __device__ __forceinline__ float sigmoid_times_2(float x) {
+  if constexpr (E == 0) return sigmoid_from_neg_log2(x);
+  constexpr float s = 1.0f / (1 << E);
+  return __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(x), s, s));
+}
+
+// With a learned bias P enters its products in fp16 as 2^12 P, and their sums are scaled
+// back: fp16 has its 11 bits from 2^-14 on only, and a P near one over the length of a
+// long context, less where the learned value is negative, is smaller (contexts of 700 ..
+// 2900 keys with a value of -7: 2 % off).  2^12 P is 4096 at most, and exact where P was.
+// (dS stays as it is: it grows with dO, which a loss scale moves.)
+template <typename T, class P> constexpr int p_bits() { return P::kRel && std::is_same<T, _Float16>::value ? 12 : 0; }
+
 // Element-type traits: MFMA call and fp32 -> element conversions (RNE).
 template <typename T> struct Elem;
 

@@ -100,6 +100,7 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
   constexpr int WIN = fwd_window<P, NWV, NCB, WK>();
   constexpr bool REL = WIN > 0;
   constexpr bool LANE_REL = P::kRel && P::kPaged;  // each lane reads its column's (RelColumn)
+  constexpr int PB = p_bits<T, P>();
   static_assert(!(REL && SCOREMOD) && (!REL || (NCB == 1 && WIN <= 64 * NWV)), "terms");
   static_assert(!PAGED || WK == 1, "pairs of waves: contiguous keys only");
   // NWV waves per workgroup (8: two per SIMD), NCB 32-query column blocks each.
@@ -460,8 +461,14 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
         for (int wd = step * NWD / NSTEP; wd < (step + 1) * NWD / NSTEP; ++wd) {
           {
             const int cb = wd / 8, e = wd % 8;
-            const float a0 = __builtin_amdgcn_rcpf(1.0f + ea[0]);
-            const float a1 = __builtin_amdgcn_rcpf(1.0f + ea[1]);
+            float a0, a1;  // 2^PB P
+            if constexpr (PB == 0) {
+              a0 = __builtin_amdgcn_rcpf(1.0f + ea[0]);
+              a1 = __builtin_amdgcn_rcpf(1.0f + ea[1]);
+            } else {
+              a0 = __builtin_amdgcn_rcpf(__builtin_fmaf(ea[0], 1.0f / (1 << PB), 1.0f / (1 << PB)));
+              a1 = __builtin_amdgcn_rcpf(__builtin_fmaf(ea[1], 1.0f / (1 << PB), 1.0f / (1 << PB)));
+            }
             pn[cb][e] = Elem<T>::pack(a0, a1);
             asm volatile("" : "+v"(pn[cb][e]));
           }
@@ -564,6 +571,12 @@ __device__ __forceinline__ void fwd_mfma_body(const P &p, const int wg, FwdTiles
                                        rchunk, p.rsplit, w, lane))
       return;
 
+    if constexpr (PB > 0) {
+#pragma unroll
+      for (int c = 0; c < NCB; ++c)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) acc[c][db] *= 1.0f / (1 << PB);
+    }
     if constexpr (PAGED) {
       paged_store<T, D, NCB>(p, un, acc, myq0, myq0 - q0, BM, wg, hi, half);
       return;

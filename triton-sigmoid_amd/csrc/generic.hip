@@ -27,6 +27,12 @@ __device__ __forceinline__ float sigmoid_of(float s, float scale, float c) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
+// P as the matrix kernels round it.
+template <typename T, class P> __device__ __forceinline__ float round_p(float x) {
+  constexpr float s = 1 << p_bits<T, P>();
+  return round_to<T>(x * s) * (1.0f / s);
+}
+
 constexpr int GB = kGenericRows;  // rows per block (one per thread)
 constexpr int GT = 32;  // tile length along the walked sequence
 
@@ -76,7 +82,7 @@ __global__ __launch_bounds__(GB) void fwd_generic_kernel(const P p) {
       if constexpr (P::kRel) c = bias + rel_at(p, h, key - q);
       float pr = sigmoid_of(s, scale, c);
       if (CAUSAL && key > q) pr = 0.0f;
-      pr = round_to<T>(pr);
+      pr = round_p<T, P>(pr);
 #pragma unroll
       for (int d = 0; d < D; ++d) acc[d] = __builtin_fmaf(pr, sV[j][d], acc[d]);
     }
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(GB) void dkdv_generic_kernel(const P p) {
         const float t = pr * dp;
         float ds = __builtin_fmaf(-pr, t, t);
         if (CAUSAL && key > q) { pr = 0.0f; ds = 0.0f; }
-        pr = round_to<T>(pr);
+        pr = round_p<T, P>(pr);
         ds = round_to<T>(ds);
 #pragma unroll
         for (int d = 0; d < D; ++d) {

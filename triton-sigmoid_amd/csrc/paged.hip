@@ -203,7 +203,8 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(const P p) {
         for (int d = 0; d < D; ++d) s = __builtin_fmaf(sq[d], ld_elem<T>(p.k, row + d), s);
         float c = bias + (p.score_mod ? p.score_mod[b * p.mod_stride + key] : 0.0f);
         if constexpr (P::kRel) c = bias + rel_at(p, h, key - (Lk - Lq + (int)(r - first)));
-        pr = round_to<T>(sigmoid_from_neg_log2(-__builtin_fmaf(s, p.fscale, c) * kLog2e));
+        constexpr int PB = p_bits<T, P>();
+        pr = round_to<T>(sigmoid_times_2<PB>(-__builtin_fmaf(s, p.fscale, c) * kLog2e)) * (1.0f / (1 << PB));
       }
     }
     sp[tid] = pr;

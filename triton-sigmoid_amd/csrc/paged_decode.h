@@ -38,7 +38,7 @@ template <typename T, int D, int NW, bool CAUSAL, bool SCOREMOD, class P>
 __device__ __forceinline__ void paged_decode_body(const P &p, const int wg, DecodeTiles<D, NW> &sK,
                                                   DecodeTiles<D, NW> &sV, DecodeTerms<NW, SCOREMOD> &sM) {
   constexpr int KB = 32;  // keys per block
-  constexpr int NKS = D / 16, NDB = D / 32;
+  constexpr int NKS = D / 16, NDB = D / 32, PB = p_bits<T, P>();
   static_assert(kDecodeCols == 32, "a column a lane");
   using Dma = PagedDma<KB, D, 1, true>;
   constexpr int NI = Dma::NI;                  // copy instructions per block of V
@@ -148,8 +148,8 @@ __device__ __forceinline__ void paged_decode_body(const P &p, const int wg, Deco
     uint32_t pk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      pk[e] = Elem<T>::pack(sigmoid_from_neg_log2(__builtin_fmaf(sc[2 * e], nsl, c[2 * e])),
-                            sigmoid_from_neg_log2(__builtin_fmaf(sc[2 * e + 1], nsl, c[2 * e + 1])));
+      pk[e] = Elem<T>::pack(sigmoid_times_2<PB>(__builtin_fmaf(sc[2 * e], nsl, c[2 * e])),
+                            sigmoid_times_2<PB>(__builtin_fmaf(sc[2 * e + 1], nsl, c[2 * e + 1])));
     if ((CAUSAL || P::kRel) && kb + KB > all_see) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -172,6 +172,10 @@ __device__ __forceinline__ void paged_decode_body(const P &p, const int wg, Deco
     }
   }
 
+  if constexpr (PB > 0) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) acc[0][db] *= 1.0f / (1 << PB);
+  }
   paged_store<T, D, 1>(p, un, acc, l32, l32, kDecodeCols, unit, hi, half);
 }
 
