@@ -38,8 +38,9 @@ int g_fail = 0, g_cus = 256;
 
 // Addresses that are never dereferenced, far apart.
 char *at(int i) { return reinterpret_cast<char *>(uintptr_t(i + 1) << 40); }
-char *const kQ = at(0), *const kK = at(1), *const kV = at(2), *const kDo = at(3), *const kDq = at(4), *const kDk = at(5),
-            *const kDv = at(6), *const kWs = at(7), *const kO = at(8), *const kTable = at(9), *const kLine = at(10);
+char *const kQ = at(0), *const kK = at(1), *const kV = at(2), *const kDo = at(3), *const kDq = at(4),
+            *const kDk = at(5), *const kDv = at(6), *const kWs = at(7), *const kO = at(8), *const kTable = at(9),
+            *const kLine = at(10);
 
 std::map<const void *, std::string> &names() {
   static std::map<const void *, std::string> m;
@@ -100,8 +101,8 @@ void **__hipRegisterFatBinary(const void *) {
   return &none;
 }
 void __hipUnregisterFatBinary(void **) {}
-void __hipRegisterFunction(void **, const void *host, char *, const char *name, unsigned, void *, void *, void *, void *,
-                           int *) {
+void __hipRegisterFunction(void **, const void *host, char *, const char *name, unsigned, void *, void *, void *,
+                           void *, int *) {
   names()[host] = name;
 }
 void __hipRegisterVar(void **, void *, char *, const char *, int, size_t, int, int) {}
@@ -236,8 +237,9 @@ void training(const sigattn_problem &p, const sigattn_rel_bias &r, bool mfma, bo
   for (const bool lines : {false, true}) {
     g_kernels.clear(), g_parts = 0;
     n = (with_table ? sigattn_rel_bwd_workspace_bytes : sigattn_rel_bwd_frozen_workspace_bytes)(&p, &r);
-    EXPECT(n > 0 && sigattn_rel_bwd(&p, &r, lines ? kLine : nullptr, kDo, kDq, kDk, kDv, with_table ? kTable : nullptr, kWs, n,
-                           nullptr) == SIGATTN_OK);
+    void *const to = with_table ? kTable : nullptr;
+    EXPECT(n > 0 && sigattn_rel_bwd(&p, &r, lines ? kLine : nullptr, kDo, kDq, kDk, kDv, to, kWs, n, nullptr) ==
+                        SIGATTN_OK);
     spans.clear();
     const Kernel *made = find("rel_line_kernel"), *one = find("rel_bwd"), *sums = find("rel_sums_kernel"),
                  *grad = find("rel_grad_kernel"), *dq = one != nullptr ? one : find("dq_"),
@@ -276,7 +278,6 @@ void training(const sigattn_problem &p, const sigattn_rel_bias &r, bool mfma, bo
     apart(spans, kWs, n);
     // Too little, or off its alignment: refused, and nothing launched.
     g_kernels.clear();
-    void *const to = with_table ? kTable : nullptr;
     EXPECT(sigattn_rel_bwd(&p, &r, nullptr, kDo, kDq, kDk, kDv, to, kWs, n - 1, nullptr) == SIGATTN_ERR_WORKSPACE);
     EXPECT(sigattn_rel_bwd(&p, &r, nullptr, kDo, kDq, kDk, kDv, to, kWs + 8, n, nullptr) == SIGATTN_ERR_WORKSPACE);
     EXPECT(g_kernels.empty());
@@ -334,8 +335,8 @@ void empty_calls() {
         if (sigattn_rel_check(&p, &r) != SIGATTN_OK) continue;
         g_kernels.clear();
         EXPECT(sigattn_rel_fwd(&p, &r, kO, kWs, sigattn_rel_fwd_workspace_bytes(&p, &r), nullptr) == SIGATTN_OK);
-        EXPECT(sigattn_rel_bwd(&p, &r, nullptr, kDo, kDq, kDk, kDv, kTable, kWs, sigattn_rel_bwd_workspace_bytes(&p, &r),
-                               nullptr) == SIGATTN_OK);
+        const size_t n = sigattn_rel_bwd_workspace_bytes(&p, &r);
+        EXPECT(sigattn_rel_bwd(&p, &r, nullptr, kDo, kDq, kDk, kDv, kTable, kWs, n, nullptr) == SIGATTN_OK);
         // (The sums' kernel finds every batch's first slot by dividing by the rows of a block.)
         const Kernel *sums = find("rel_sums_kernel");
         EXPECT(find("rel_grad_kernel") != nullptr && sums != nullptr && sums->p.part_rows > 0);

@@ -638,7 +638,8 @@ __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<
         const int e = last ? pp : (win + 1) * PPW + pp;
         const f32x16 &sv = last ? sacc[SL] : sacc[1 - SL];
         nx[pp][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc_read(sv[2 * e]), nsl, last ? cn[2 * pp] : c[2 * e]));
-        nx[pp][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc_read(sv[2 * e + 1]), nsl, last ? cn[2 * pp + 1] : c[2 * e + 1]));
+        nx[pp][1] = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(acc_read(sv[2 * e + 1]), nsl, last ? cn[2 * pp + 1] : c[2 * e + 1]));
       }
 #pragma unroll
       for (int pp = 0; pp < PPW; ++pp) {
@@ -720,7 +721,10 @@ __device__ __forceinline__ void bwd_dkdv_body(const P &p, const int id, DkdvLds<
     for (int db = 0; db < NDB; ++db) dva[db] *= 1.0f / (1 << PB);
   }
   if (GROUPED && nparts > 1) {
-    if (kok) store_part<NDB>(p, part, b, my_k, h, dka, 0, scale, hi, half), store_part<NDB>(p, part, b, my_k, h, dva, 1, 1.0f, hi, half);
+    if (kok) {
+      store_part<NDB>(p, part, b, my_k, h, dka, 0, scale, hi, half);
+      store_part<NDB>(p, part, b, my_k, h, dva, 1, 1.0f, hi, half);
+    }
     return;
   }
   if (my_k < p.k_rows_out(Lk)) {

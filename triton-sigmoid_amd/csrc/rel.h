@@ -262,8 +262,8 @@ void launch_paged_rel_decode_f32(const PagedRelParams &p, int units, int D, bool
 // launch_paged_mixed (paged.h).
 void launch_paged_rel_fwd(const PagedRelParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
 void launch_paged_rel_decode(const PagedRelParams &p, int units, int dtype, int D, bool causal, hipStream_t st);
-void launch_paged_rel_mixed(const PagedRelParams &pf, int nf, const PagedRelParams &pd, int nd, int dtype, int D, bool causal,
-                            hipStream_t st);
+void launch_paged_rel_mixed(const PagedRelParams &pf, int nf, const PagedRelParams &pd, int nd, int dtype, int D,
+                            bool causal, hipStream_t st);
 void launch_paged_rel_generic(const PagedRelParams &p, int dtype, int D, bool causal, hipStream_t st);
 
 }  // namespace sigattn

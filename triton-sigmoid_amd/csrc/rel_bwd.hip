@@ -3,9 +3,10 @@
 // are staged as in the forward.  bf16, us, with / without the bias: 16 sequences of 101
 // .. 1001 H=12 D=64 dK/dV 83 / 78, dQ 73 / 55 (62 without the sums: near the diagonal
 // they are a third of a block's arithmetic); causal, 3 of 1500 .. 4096 H=16 Hkv=4
-// D=128 dK/dV 419 / 428 (storing dS, in pairs of waves), dQ 327 (300 without the sums) / 184 from the stored
-// dS.  No two-pass form: what is stored is rounded, and so would be what the table's
-// gradient sums (906 -> 843 us a step, error 1e-6 -> 0.0024).
+// D=128 dK/dV 419 / 428 (storing dS, in pairs of waves), dQ 327 (300 without the sums) /
+// 184 from the stored dS.  No two-pass form: what is stored is rounded, and so would be
+// what the table's gradient sums (906 -> 843 us a step, error 1e-6 -> 0.0024).  Calls without
+// that gradient take the same kernels, without the sums.
 #include <algorithm>
 
 #include "bwd_kernel.h"
@@ -47,7 +48,8 @@ template <typename T, int D, int WK, int NW = 4> void dq_w(const RelParams &kp, 
 // eight 160 327, 300 327, 1100 345, 1190 347; four alone 1200 515.
 bool dq_eight_waves(const RelParams &p, int D) {
   constexpr size_t tiles = 4 * 64 * 128 * 2, cu = 163840 - 512;
-  const size_t four = tiles + 2 * 192 * 4 + near_floats(p.reach, 4) * 4, eight = tiles + 2 * 320 * 4 + near_floats(p.reach, 8) * 4;
+  const size_t four = tiles + 2 * 192 * 4 + near_floats(p.reach, 4) * 4;
+  const size_t eight = tiles + 2 * 320 * 4 + near_floats(p.reach, 8) * 4;
   return D == 128 && p.part != nullptr && 2 * four > cu && eight <= cu;
 }
 
@@ -66,17 +68,19 @@ __global__ __launch_bounds__(256, 2) void rel_bwd_kernel(const RelParams pq, con
 }
 
 // Where that pays: as long as either kernel alone leaves CUs idle for much of its
-// time, and two workgroups still fit a CU beside the sums' lines.  Forward + backward,
-// us, two launches / one, 128-row workgroups of both per CU: H=8 D=64 sequence
-// of 128 0.06, 39.5 / 32.2; four of 512 1, 60.3 / 47.8 (causal 59.7 / 47.9); two of
-// 1001 H=12 1.5, 112 / 105; eight of 512 2, 73.3 / 73.1; four of 1024 H=16 4, 150
-// / 152 (causal 110 / 108); sixteen of 101 .. 1001 H=12 12, 234 / 232 (D=32 175 / 185;
-// causal D=64 171 / 168, D=32 134 / 139); causal, eight of 2048 8, 271 / 296 (dQ misses
+// time, and two workgroups still fit a CU beside the sums' lines.  Captured steps
+// (forward and backward, bf16, reach 128), us, two launches / one, by 128-row workgroups of
+// both per CU: H=8 D=64 sequence of 128 0.06, 39.8 / 32.3; four of 512 1, 61 / 51 (causal
+// 60 / 48); two of 1001 H=12 1.5, 96 / 85; eight of 512 2, 71 / 72; four of 1024 H=16 4, 150
+// / 150 (causal 110 / 107); sixteen of 101 .. 1001 H=12 12, 235 / 233 (D=32 176 / 187;
+// causal D=64 171 / 170, D=32 138 / 141); causal, eight of 2048 H=8 8, 266 / 292 (dQ misses
 // its third workgroup per CU).
+template <int D, int WK> size_t dq_lds(const RelParams &p) {
+  return sizeof(DqLds<D, false, dq_window<RelParams, WK>()>) + (p.part != nullptr ? near_floats(p.reach) * 4 : 0);
+}
 template <int D, int WK> bool one_launch(const RelParams &p, bool causal) {
   const int64_t n = (int64_t)p.B * p.H * ((p.Tq + 127) / 128 + (p.Tk + 127) / 128);
-  const size_t dq = sizeof(DqLds<D, false, dq_window<RelParams, WK>()>) + (p.part != nullptr ? near_floats(p.reach) * 4 : 0);
-  return n <= (causal ? 4 : 2) * (int64_t)p.ncu && dq <= 79 * 1024;
+  return n <= (causal ? 4 : 2) * (int64_t)p.ncu && dq_lds<D, WK>(p) <= 79 * 1024;
 }
 
 template <typename T, int D, int WK>
@@ -88,9 +92,10 @@ void bwd_w(const RelParams &kq, const RelParams &kk, bool causal, hipStream_t st
   const bool grouped = pk.qgroup > 1;
   const int nkv = pk.nblk * pk.B * pk.H * (grouped && pk.qsplit > 1 ? pk.qsplit : 1);
   const dim3 grid((unsigned)(nkv + pq.nblk * pq.B * pq.H + pq.ngap[0] + pq.ngap[1]));
-  const size_t dq = sizeof(DqLds<D, false, dq_window<RelParams, WK>()>) + (pq.part != nullptr ? near_floats(pq.reach) * 4 : 0);
-  const size_t lds = std::max(dq, sizeof(DkdvLds<D, dkdv_window<RelParams>()>));
-  const auto go = [&](auto c, auto g) { rel_bwd_kernel<T, D, WK, c.value, g.value><<<grid, 256, lds, st>>>(pq, pk, nkv); };
+  const size_t lds = std::max(dq_lds<D, WK>(pq), sizeof(DkdvLds<D, dkdv_window<RelParams>()>));
+  const auto go = [&](auto c, auto g) {
+    rel_bwd_kernel<T, D, WK, c.value, g.value><<<grid, 256, lds, st>>>(pq, pk, nkv);
+  };
   if (causal) grouped ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
   else grouped ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }

@@ -1,7 +1,7 @@
 // The fp32 kernels (f32_kernel.h) with the learned bias by relative position, its
-// windows of the lines beside the split tiles in LDS.  us, with / without: five sequences of up
-// to 777 H=8 D=32, reach 300, forward 25.5 / 23.6, dK/dV 34 / 31.3, dQ 35.5 / 27.2
-// (30.5 without the sums by position).
+// windows of the lines beside the split tiles in LDS.  us, with / without: five sequences
+// of 1 .. 777 H=8 D=32, reach 300, forward 25.5 / 23.6, dK/dV 34 / 31.3, dQ 35.5 / 27.2
+// (30.5 without the sums by position); dQ and dK/dV in one launch 50 .. 58.
 #include "f32_kernel.h"
 #include "rel.h"
 
@@ -15,10 +15,10 @@ template <class F> void by_dim(int D, F &&f) {
 }
 
 // Both kernels in one launch: the first nkv workgroups (after dQ's gap rows) are
-// dK/dV's.  Forward + backward, us, two launches / one: five sequences of up to 777
-// H=8 D=32, reach 300, 109 / 100; one of 128 D=64 50.1 / 37.6; eight of up to 1024
-// H=12 D=64 444 / 429; causal, eight of up to 2048 H=16 Hkv=4 999 / 920; D=128 H=8
-// Hkv=2, four of up to 1000 494 / 462, causal, eight of up to 2000 1295 / 1121.
+// dK/dV's.  Captured steps (forward and backward), us, two launches / one: five sequences
+// of 1 .. 777 H=8 D=32, reach 300, 110 / 101; one of 128 H=8 D=64 50 / 37; eight of 256 ..
+// 1024 H=12 D=64 440 / 390; causal, eight of 512 .. 2048 H=16 Hkv=4 D=64 1266 / 1110; D=128
+// H=8 Hkv=2, four of 250 .. 1000 484 / 438, causal, eight of 500 .. 2000 1328 / 1150.
 template <int D, bool CAUSAL, int WK>
 __global__ __launch_bounds__(64 * FW, (bwd_f32_occupancy<D, WK>())) void rel_bwd_f32_kernel(const RelParams pq,
                                                                                          const RelParams pk, int nkv) {
@@ -65,7 +65,8 @@ bool launch_rel_bwd_f32(const RelParams &kq, const RelParams &kk, int D, bool ca
         if constexpr (wq.value == wk.value) {
           constexpr int WK = wk.value;
           const size_t near = rel_near_bytes(pq);
-          if (bwd_f32_occupancy<d.value, WK>() * (window_floats<d.value, WK, RelParams>(0) * 4 + near + 256) > 163840) return;
+          const size_t tiles = window_floats<d.value, WK, RelParams>(0) * 4;
+          if (bwd_f32_occupancy<d.value, WK>() * (tiles + near + 256) > 163840) return;
           const int64_t nkv = nk * (pk.qsplit > 1 ? pk.qsplit : 1);
           done = true;
           const dim3 grid((unsigned)(nq + nkv + pq.ngap[0] + pq.ngap[1])), block(64 * FW);

@@ -24,7 +24,10 @@ void fwd_w(const RelParams &kp, bool causal, hipStream_t st) {
   else fwd_mfma_kernel<T, D, NWV, 1, WK, false, false, RelParams><<<grid, block, 0, st>>>(p);
 }
 
-// Waves and pairs of them as without the bias.
+// Pairs of waves as without the bias.  Not its 64 queries a wave of large grids at D = 64:
+// their windows would be 320 places a tile for 256 threads.  Without that form a wave reads
+// each tile for 32 queries; us, with / without the bias, H=16 D=64: one sequence of 8192 353 / 317
+// (causal 189 / 169), four 1295 / 1115 (causal 703 / 613), two of 4096 187 / 164.
 template <typename T, int D> void fwd_t(const RelParams &p, bool causal, hipStream_t st) {
   if constexpr (D <= 64) {
     if (fwd_wave_pairs(p)) return fwd_w<T, D, 4, 2>(p, causal, st);

@@ -92,7 +92,8 @@ template <typename T> struct RotaryPiece {
   }
   static __device__ __forceinline__ u32x4 put(const float (&x)[E]) {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(u32x4, (f32x4){x[0], x[1], x[2], x[3]});
-    else return (u32x4){Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]), Elem<T>::pack(x[6], x[7])};
+    else return (u32x4){Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
+                        Elem<T>::pack(x[6], x[7])};
   }
 };
 
@@ -121,8 +122,8 @@ __global__ __launch_bounds__(256) void rotary_wide_kernel(const RotaryArgs a, co
   if (CACHE && which > 0) {
     const int32_t slot = a.slots[t];
     if (slot < 0 || slot >= a.num_slots) return;
-    dst = (which == 1 ? a.out[1] : a.out[2]) + (int64_t)(slot >> a.lp) * a.dst_p + (slot & ((1 << a.lp) - 1)) * a.dst_t +
-          h * a.dst_h + at;
+    dst = (which == 1 ? a.out[1] : a.out[2]) + (int64_t)(slot >> a.lp) * a.dst_p +
+          (slot & ((1 << a.lp) - 1)) * a.dst_t + h * a.dst_h + at;
   } else {
     dst = (which == 0 ? a.out[0] : a.out[1]) + t * (which == 0 ? a.out_t[0] : a.out_t[1]) +
           (int64_t)h * a.D * sizeof(T) + at;

@@ -305,8 +305,8 @@ sigattn_rel_bias make_rel(const Tensor &table, const Tensor &buckets) {
 // sigmoid_attention_varlen with the learned bias, at least one sequence and one row.
 struct RelNode : public torch::autograd::Function<RelNode> {
   static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table,
-                        const Tensor &buckets, const std::optional<Tensor> &own_bias, const Tensor &scale, const Tensor &cu_q,
-                        const Tensor &cu_k, int64_t max_q, int64_t max_k, bool causal) {
+                        const Tensor &buckets, const std::optional<Tensor> &own_bias, const Tensor &scale,
+                        const Tensor &cu_q, const Tensor &cu_k, int64_t max_q, int64_t max_k, bool causal) {
     const Layout lay{Tensor(), Tensor(), cu_q, cu_k, max_q, max_k};
     const Tensor bias = own_bias.value_or(Tensor());  // none: the library's default
     ctx->saved_data["causal"] = causal;
@@ -338,13 +338,15 @@ struct RelNode : public torch::autograd::Function<RelNode> {
     result[0] = at::empty_like(q), result[1] = at::empty_like(k), result[2] = at::empty_like(v);
     if (want_table) result[3] = at::empty_like(table);
     const c10::DeviceGuard guard(q.device());
-    const sigattn_problem p = make_problem(q, k, v, saved[5], Tensor(), saved[6], lay, ctx->saved_data["causal"].toBool());
+    const bool causal = ctx->saved_data["causal"].toBool();
+    const sigattn_problem p = make_problem(q, k, v, saved[5], Tensor(), saved[6], lay, causal);
     const sigattn_rel_bias r = make_rel(table, buckets);
     const int64_t nbytes =
         (int64_t)(want_table ? g_api.rel_bwd_workspace_bytes(&p, &r) : g_api.rel_bwd_frozen_workspace_bytes(&p, &r));
     const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte));
-    check_rc(g_api.rel_bwd(&p, &r, saved[9].data_ptr(), dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(), result[2].data_ptr(),
-                           want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes, stream_of(q.device())),
+    check_rc(g_api.rel_bwd(&p, &r, saved[9].data_ptr(), dout.data_ptr(), result[0].data_ptr(), result[1].data_ptr(),
+                           result[2].data_ptr(), want_table ? result[3].data_ptr() : nullptr, ws.data_ptr(), nbytes,
+                           stream_of(q.device())),
              "sigattn_rel_bwd");
     differentiable_once(result);
     return result;
@@ -352,7 +354,8 @@ struct RelNode : public torch::autograd::Function<RelNode> {
 };
 
 // The rotary struct over rows [N, heads, D] of any strides but the last.
-sigattn_rotary make_rotary(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &angles, bool pairs) {
+sigattn_rotary make_rotary(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &angles,
+                           bool pairs) {
   sigattn_rotary r;
   std::memset(&r, 0, sizeof(r));
   r.dtype = dtype_code(q);
@@ -608,8 +611,10 @@ py::object quick_varlen(const py::object &query, const py::object &key, const py
                                 static_cast<float *>(bias.data_ptr()), stream),
              "sigattn_default_bias");
   }
-  if (rel) return py::cast(RelNode::apply(q, k, v, table, buckets, own_bias ? std::optional<Tensor>(bias) : std::nullopt, st, cq, ck, mq, mk,
-                                      is_causal.ptr() == Py_True));
+  if (rel) {
+    const auto own = own_bias ? std::optional<Tensor>(bias) : std::nullopt;
+    return py::cast(RelNode::apply(q, k, v, table, buckets, own, st, cq, ck, mq, mk, is_causal.ptr() == Py_True));
+  }
   const int64_t limit = (int64_t)(H == Hkv ? 2048 : 8192) << 20;  // _capi._WS_DEFAULT_MB, _WS_DEFAULT_GROUPED_MB
   return py::cast(SigattnNode::apply(q, k, v, bias, sm.defined() ? std::optional<Tensor>(sm) : std::nullopt, st,
                                      std::nullopt, std::nullopt, is_causal.ptr() == Py_True, limit, cq, ck, mq, mk));
@@ -741,7 +746,8 @@ py::object quick_paged(const py::object &query, const py::object &key_cache, con
     const sigattn_rel_bias r = make_rel(learned, buckets);
     const int64_t nbytes = (int64_t)g_api.paged_rel_fwd_workspace_bytes(&p, &r);
     const Tensor ws = at::empty({nbytes}, q.options().dtype(at::kByte).requires_grad(false));
-    check_rc(g_api.paged_rel_fwd(&p, &r, out.data_ptr(), ws.data_ptr(), nbytes, stream_of(dev)), "sigattn_paged_rel_fwd");
+    check_rc(g_api.paged_rel_fwd(&p, &r, out.data_ptr(), ws.data_ptr(), nbytes, stream_of(dev)),
+             "sigattn_paged_rel_fwd");
     return py::cast(out);
   }
   const Tensor ws = workspace((int64_t)g_api.paged_fwd_workspace_bytes(&p), q);  // without it: unsplit
@@ -774,8 +780,8 @@ py::object quick_rotary(const py::object &query, const py::object &key, const py
   const py::object no = py::none();
   Tensor q, k, at, table;
   if (!Quick::usable() || !Quick::strided(query, q) || !Quick::strided(key, k) || !PyBool_Check(interleaved.ptr()) ||
-      (q.dim() != 3 && q.dim() != 4) || k.dim() != q.dim() || !Quick::float_type(q) || k.scalar_type() != q.scalar_type() ||
-      !q.is_cuda() || k.device() != q.device() || !Quick::gfx950(q.device().index()) || q.size(-1) != k.size(-1) ||
+      (q.dim() != 3 && q.dim() != 4) || k.dim() != q.dim() || !Quick::float_type(q) ||
+      k.scalar_type() != q.scalar_type() || !q.is_cuda() || k.device() != q.device() || !Quick::gfx950(q.device().index()) || q.size(-1) != k.size(-1) ||
       !rotary_dim(q.size(-1)) || q._fw_grad(0).defined() || k._fw_grad(0).defined())
     return no;
   for (int64_t i = 0; i + 2 < q.dim(); ++i)
@@ -792,8 +798,9 @@ py::object quick_rotary(const py::object &query, const py::object &key, const py
 }
 
 py::object quick_write_rotary(const py::object &query, const py::object &key, const py::object &value,
-                              const py::object &key_cache, const py::object &value_cache, const py::object &slot_mapping,
-                              const py::object &positions, const py::object &angles, const py::object &interleaved) {
+                              const py::object &key_cache, const py::object &value_cache,
+                              const py::object &slot_mapping, const py::object &positions, const py::object &angles,
+                              const py::object &interleaved) {
   const py::object no = py::none();
   Tensor q, k, v, kc, vc, slots, at, table;
   if (!Quick::usable() || !quick_caches(key_cache, value_cache, kc, vc) || !Quick::strided(query, q) ||
@@ -801,8 +808,9 @@ py::object quick_write_rotary(const py::object &query, const py::object &key, co
     return no;
   const at::Device dev = kc.device();
   const at::ScalarType type = kc.scalar_type();
-  if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || k.strides() != v.strides() || q.scalar_type() != type ||
-      k.scalar_type() != type || v.scalar_type() != type || q.device() != dev || k.device() != dev || v.device() != dev ||
+  if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || k.strides() != v.strides() ||
+      q.scalar_type() != type || k.scalar_type() != type || v.scalar_type() != type || q.device() != dev ||
+      k.device() != dev || v.device() != dev ||
       q.size(0) != k.size(0) || q.size(2) != k.size(2) || k.size(1) != kc.size(2) || k.size(2) != kc.size(3) ||
       !rotary_dim(k.size(2)) || !Quick::ints(slot_mapping, slots, 1, dev) || slots.size(0) != k.size(0) ||
       !quick_angles(positions, angles, k.size(0), k.size(2), dev, at, table) || at.dim() != 1 ||

@@ -27,7 +27,8 @@ LIB_PATH = PKG_DIR / "libsigattn.so"
 BUILD_DIR = ROOT / "_build"
 
 SOURCES = ["fwd.hip", "bwd.hip", "decode.hip", "f32.hip", "generic.hip", "bias.hip", "paged.hip",
-           "paged_fwd.hip", "paged_decode.hip", "rel.hip", "rel_fwd.hip", "rel_bwd.hip", "rel_paged.hip", "rel_f32.hip", "rotary.hip",
+           "paged_fwd.hip", "paged_decode.hip", "rel.hip", "rel_fwd.hip", "rel_bwd.hip", "rel_paged.hip", "rel_f32.hip",
+           "rotary.hip",
            "capi.cpp", "paged_capi.cpp", "rel_capi.cpp"]
 SOURCE_FLAGS = {"bias.hip": ["-ffp-contract=off"]}  # see the file
 ARCH = "gfx950"

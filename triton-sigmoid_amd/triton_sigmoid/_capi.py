@@ -282,7 +282,7 @@ _autograd = None  # the bound module, or False after a failed import
 # The node's entries for eager calls with canonical arguments (None until the
 # node is bound): the call's result, or None where it does not take it.
 quick = None
-quick_module = None  # the module with quick_varlen, quick_plan, quick_write, quick_paged, quick_rotary, quick_write_rotary
+quick_module = None  # the module with quick_varlen, quick_plan, quick_write, quick_paged, quick_rotary and so on
 
 
 def autograd_node():
