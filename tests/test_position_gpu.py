@@ -447,6 +447,39 @@ def test_more_sequences_than_the_sums_keep():
     check(make(lens, lens, 1, 1, 32, torch.bfloat16, 10, 9, seed=6), True)
 
 
+def test_more_sums_than_31_bits_count():
+    """2^31 sums of blocks and more: a batch's gradients are its sequences' in smaller batches, and
+    the table's is the sum of theirs (fp32 sums of as many terms, in another order)."""
+    n, B, H, D, R = 4096, 264, 64, 16, 2048
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("not enough free memory")
+    assert n * B // 128 * H * (2 * R + 1) > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn(n * B, H, D, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(4))
+    table, buckets = torch.zeros(40, H, device="cuda"), torch.randint(0, 40, (2 * R + 1,), generator=g, device="cuda")
+
+    def grads(first, count):
+        at = slice(first * n, (first + count) * n)
+        leaves = [t[at].requires_grad_() for t in (q, k, v)] + [table.clone().requires_grad_()]
+        cu = torch.arange(count + 1, dtype=I32, device="cuda") * n
+        o = ts.sigmoid_attention_varlen(*leaves[:3], cu, cu, n, n, is_causal=True, bias_table=leaves[3],
+                                        bias_buckets=buckets.to(I32))
+        return torch.autograd.grad(o, leaves, do[at])
+
+    *whole, dtable = grads(0, B)
+    parts = torch.zeros(40, H, dtype=torch.float64, device="cuda")
+    for first, count in ((0, 100), (100, 100), (200, 64)):
+        *some, t = grads(first, count)
+        parts += t.double()
+        for x, y in zip(whole, some):
+            assert torch.equal(x[first * n:(first + count) * n], y)
+    # dS have either sign, so running sums stay near the result S's size / sqrt(100) (a bucket's
+    # places) and their rounding adds up as its square: 8448 blocks x 100 places of 2^-24 S / 10,
+    # 6e-6 S.  The last 258 blocks, those past 2^31, make up a share of sqrt(3 %) of S.
+    assert (dtable.double() - parts).abs().max() <= 2.0 ** -12 * parts.abs().max()
+    assert dtable.abs().min() > 0
+
+
 def test_fp32_sums_do_not_drift():
     """Four million dS of either sign in one bucket: what each may be off by adds up as
     its square where it has no preferred sign (six standard deviations; each within its
